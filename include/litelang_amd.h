@@ -141,6 +141,51 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
                          int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                          int64_t max_input_len, float sm_scale, int dtype, hipStream_t stream);
 
+/* ---------------------------------------------- attention over a window
+ * The two calls above for contexts of which only the last `window` tokens and
+ * the first `sinks` ones are kept: a query at position p sees the keys n <= p
+ * with n > p - window (its own included) or n < sinks. window >= 1, sinks >= 0
+ * (both may exceed the length). No counterpart in the reference (whose configs'
+ * use_sliding_window it does not read).
+ * No entry of the slot table is read but those of keys that some query of the
+ * request's call sees, so the tokens between the sinks and the window may have
+ * left the cache and their entries may hold anything. Keys and values that one
+ * query of the call sees and another does not must be finite. Sums and softmax
+ * statistics are fp32. */
+
+/* ll_prefill_attention under a window. Requests whose b_seq_len is not above
+ * their b_shared_seq_len have no query rows; rows of `out` that no request
+ * owns are left as they were. */
+int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h,
+                                const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
+                                const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
+                                void* out, int64_t out_stride_tok, int64_t out_stride_h,
+                                const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                                const void* b_req_idx, int req_idx_i64, const void* b_start_loc,
+                                int start_loc_i64, const void* b_seq_len, int seq_len_i64,
+                                const void* b_shared_seq_len, int shared_i64, int64_t batch,
+                                int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                int64_t max_input_len, int64_t window, int64_t sinks,
+                                float sm_scale, int dtype, hipStream_t stream);
+
+/* ll_decode_attention under a window: the query is the token at b_seq_len - 1,
+ * so its keys are one list, the sinks and the last `window` tokens. Sequences
+ * of length 0 give zero rows. The workspace (0 bytes where the list is not
+ * split) needs no initialisation and nothing in it lasts beyond the call. */
+int64_t ll_window_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                  int64_t head_dim, int64_t max_len_in_batch,
+                                                  int64_t window, int64_t sinks);
+int ll_window_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                               const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
+                               const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
+                               const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                               const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
+                               int seq_len_i64, void* out, int64_t out_stride_b,
+                               int64_t out_stride_h, int64_t batch, int64_t q_heads,
+                               int64_t kv_heads, int64_t head_dim, int64_t max_len_in_batch,
+                               int64_t window, int64_t sinks, float sm_scale, int dtype,
+                               void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 /* ------------------------------------------------------------- elementwise */
 
 /* RMSNorm over rows: out = (x / sqrt(mean(x^2) + eps)) * gamma in fp32.
@@ -171,6 +216,41 @@ int ll_rope_kv_scatter(void* qkv, int64_t qkv_row_stride, int64_t ntok, int64_t 
                        int64_t table_row_stride, int cs_dtype, const int32_t* slots,
                        void* pool_layer, int64_t pool_slot_stride, int64_t pool_head_stride,
                        int dtype, hipStream_t stream);
+
+/* Rotary positions from the frequencies (rotary.hip): the first rotary_dim
+ * elements of every head are pairs, (i, i + rotary_dim/2) or, interleaved,
+ * (2i, 2i + 1); pair i of a token at position p turns by p * inv_freq[i] and
+ * is scaled by `factor` (1, or the attention factor of scaled frequencies).
+ * The elements behind rotary_dim are copied. Angles are fp64, the rest fp32
+ * with one rounding. positions [ntok] int32 or int64 (below 2^31), inv_freq
+ * [rotary_dim/2] fp32; head_dim at most 1024, rotary_dim even. The outputs may
+ * be the inputs (same strides), but not otherwise overlap them. No counterpart
+ * in the reference, whose rotation is ll_rotary_emb's. */
+int ll_rope_positions(const void* q, int64_t q_stride_tok, int64_t q_stride_h, void* q_out,
+                      int64_t q_out_stride_tok, int64_t q_out_stride_h, int64_t q_heads,
+                      const void* k, int64_t k_stride_tok, int64_t k_stride_h, void* k_out,
+                      int64_t k_out_stride_tok, int64_t k_out_stride_h, int64_t k_heads,
+                      const void* positions, int positions_i64, const float* inv_freq,
+                      int64_t rotary_dim, int interleaved, float factor, int64_t ntok,
+                      int64_t head_dim, int dtype, hipStream_t stream);
+
+/* The attention's input in one pass over the projection output qkv
+ * [ntok, (q_heads + 2 kv_heads) * head_dim]: every q and k head is normalised,
+ * x / sqrt(mean(x^2) + eps) * gamma (gammas [head_dim] in `dtype`; a null one:
+ * no norm of those heads), and rotated as in ll_rope_positions; q goes to q_out
+ * (which may be qkv itself), k and the plain v to pool_layer[slots[t]], K heads
+ * first. A slot outside [0, pool_slots) is a padded token: its K and V are not
+ * stored. slots of one call must differ. fp32 with one rounding. No
+ * counterpart in the reference (ll_rope_kv_scatter without norms). */
+int ll_qk_norm_rope_kv_scatter(const void* qkv, int64_t qkv_row_stride, int64_t ntok,
+                               int64_t q_heads, int64_t kv_heads, int64_t head_dim, void* q_out,
+                               int64_t q_out_stride_tok, int64_t q_out_stride_h,
+                               const void* q_gamma, const void* k_gamma, float eps,
+                               const void* positions, int positions_i64, const float* inv_freq,
+                               int64_t rotary_dim, int interleaved, float factor,
+                               const int32_t* slots, void* pool_layer, int64_t pool_slot_stride,
+                               int64_t pool_head_stride, int64_t pool_slots, int dtype,
+                               hipStream_t stream);
 
 /* pool[slots[t], h, :] = src[t, h, :] (plain KV write, no RoPE).
  * Replaces the index_put of transformer_layer.py:143 when K is already rotated. */
@@ -238,6 +318,34 @@ int ll_argmax_status(const void* x, int64_t x_row_stride, int64_t M, int64_t N, 
  * stack and computes (slot, row, col) exactly as the reference does. */
 int ll_assign_slots(int32_t* req_to_tokens, int64_t req_to_tokens_stride, const int32_t* slots,
                     const int32_t* rows, const int32_t* cols, int64_t n, hipStream_t stream);
+
+/* Slot maps of a batch, built on the device (slot_maps.hip). Request b sits in
+ * row b_req_idx[b] of the slot table, holds b_cached_len[b] tokens and gets
+ * b_seq_len[b] - b_cached_len[b] new ones, at the positions in between. With
+ * pages of page_size tokens its first ceil(cached / page_size) pages are in
+ * block_table[row] (page_size 1: no block table, a page is a slot); the
+ * pages that the new tokens need beyond those are free_pages[0], [1], ... in
+ * batch order, and slot = page * page_size + position % page_size.
+ * Written: slots and positions of the new tokens, request after request,
+ * b_start_loc (its first new token), last_rows (its last one, -1 for a request
+ * without), req_to_tokens and block_table at the new entries alone, and counts
+ * = {new tokens, pages taken, error}. The error word is 0, or with nothing but
+ * counts written the sum of: 1 a length outside 0 <= cached <= len <= max_len
+ * (or the block table), 2 a row outside the table or two requests with new
+ * tokens on one row, 4 more new tokens than max_tokens, 8 than free pages.
+ * Entries past the new tokens are left as they were. At most 8192 requests and
+ * 2^18 table rows; pages and slots are int32. Replaces, for lengths that live
+ * on the device, the host construction of PageCache.alloc_token_idxs
+ *   (litelang/models/cache.py:225-249) and of RunnerBatch's start offsets and
+ * positions (litelang/models/runner_batch.py:88-265). */
+int ll_build_slot_maps(const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
+                       int seq_len_i64, const void* b_cached_len, int cached_len_i64,
+                       int64_t batch, const int32_t* free_pages, int64_t n_free, int64_t page_size,
+                       int32_t* block_table, int64_t block_table_stride, int64_t block_table_cols,
+                       int32_t* req_to_tokens, int64_t req_to_tokens_stride, int64_t req_rows,
+                       int64_t max_len, int32_t* slots, int32_t* positions, int64_t max_tokens,
+                       int32_t* b_start_loc, int32_t* last_rows, int32_t* counts,
+                       hipStream_t stream);
 
 /* ------------------------------------------------------------------- GEMM */
 

@@ -42,6 +42,19 @@ SIGNATURES = {
     "ll_prefill_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64,
                                    P, I32, P, I32, P, I32, P, I32, I64, I64, I64, I64, I64, F32,
                                    I32, P]),
+    "ll_window_prefill_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P,
+                                          I64, P, I32, P, I32, P, I32, P, I32, I64, I64, I64, I64,
+                                          I64, I64, I64, F32, I32, P]),
+    "ll_window_decode_attention_workspace_size": (I64, [I64] * 7),
+    "ll_window_decode_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, P, I32, P,
+                                         I32, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, F32,
+                                         I32, P, I64, P]),
+    "ll_rope_positions": (I32, [P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P,
+                                I32, P, I64, I32, F32, I64, I64, I32, P]),
+    "ll_qk_norm_rope_kv_scatter": (I32, [P, I64, I64, I64, I64, I64, P, I64, I64, P, P, F32, P, I32,
+                                         P, I64, I32, F32, P, P, I64, I64, I64, I32, P]),
+    "ll_build_slot_maps": (I32, [P, I32, P, I32, P, I32, I64, P, I64, I64, P, I64, I64, P, I64, I64,
+                                 I64, P, P, I64, P, P, P, P]),
     "ll_rmsnorm": (I32, [P, I64, P, I64, P, P, I64, I64, I64, F32, I32, P]),
     "ll_rotary_emb": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, P, I64, I64, I64, I32,
                             I32, P]),

@@ -125,7 +125,24 @@ struct DecodeArgs {
   const int32_t* new_slots;  // [B] pool slot of each sequence's new token
   // optional quantisation of the output rows for the next int8 projection
   int8_t* qout; int64_t ldq; float* qscale; const float* qstatic;
+  // windowed forms: visible tokens n >= len - window or n < sinks (both <= 2^30)
+  int window, sinks;
 };
+
+// The visible tokens of a sequence of len tokens under a window with sinks, as
+// one list of n: entry j is token j below `sinks`, else token j + skip. One
+// query sees them all, so that attention over the list needs no mask, and no
+// table entry of another token is read.
+struct WindowList {
+  int64_t n;
+  int sinks;
+  int64_t skip;
+};
+__device__ __forceinline__ WindowList window_list(int64_t len, int window, int sinks) {
+  const int64_t low = len - window;
+  if (low <= sinks) return {len, 0, 0};
+  return {len - (low - sinks), sinks, low - sinks};
+}
 
 // Partial kinds of the fused RoPE kernels (template MODE): 1 = fp32 partials
 // from at most kRopeF32Splits splits, summed by one fixed, branch-free set of
@@ -974,7 +991,7 @@ __global__ __launch_bounds__(1024) void decode_attn_combine_quant_kernel(DecodeA
 // One 64-lane workgroup per (sequence, query head); tokens are spread over the
 // lanes for q.k, the head dim over the lanes for p.v. Used for fp32 and for
 // shapes the MFMA path does not cover; exactness, not speed, is its purpose.
-template <typename T>
+template <typename T, bool WIN>
 __global__ __launch_bounds__(64) void decode_attn_generic_kernel(DecodeArgs a, int D, float sm_scale) {
   const int b = blockIdx.y;
   const int h = blockIdx.x;
@@ -986,6 +1003,11 @@ __global__ __launch_bounds__(64) void decode_attn_generic_kernel(DecodeArgs a, i
   int64_t* ss = (int64_t*)(ps + 64);  // [64]
   int64_t len = ll_load_idx(a.seq_len, b, a.len64);
   if (len > a.max_len) len = a.max_len;
+  WindowList wl = {0, 0, 0};
+  if constexpr (WIN) {
+    wl = window_list(len, a.window, a.sinks);
+    len = wl.n;
+  }
   const int64_t rid = ll_load_idx(a.req_idx, b, a.req64);
   const T* qp = (const T*)a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
   for (int d = lane; d < D; d += 64) qs[d] = ll_to_f32(qp[d]);
@@ -1000,7 +1022,7 @@ __global__ __launch_bounds__(64) void decode_attn_generic_kernel(DecodeArgs a, i
     float s = -INFINITY;
     int64_t slot = 0;
     if (t < len) {
-      slot = a.r2t[rid * a.r2t_s + t];
+      slot = a.r2t[rid * a.r2t_s + (WIN && t >= wl.sinks ? t + wl.skip : t)];
       const T* kr = kb + slot * a.k_st;
       float dot = 0.f;
       for (int d = 0; d < D; ++d) dot += qs[d] * (ll_to_f32(kr[d]) * sm_scale);
@@ -1359,26 +1381,32 @@ extern "C" int64_t ll_decode_attention_workspace_size(int64_t batch, int64_t q_h
   return workspace_bytes_for(batch, q_heads, kv_heads, head_dim, max_len_in_batch);
 }
 
-extern "C" int ll_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h,
-                                   const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
-                                   const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
-                                   const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
-                                   const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
-                                   int seq_len_i64, void* out, int64_t out_stride_b,
-                                   int64_t out_stride_h, int64_t batch, int64_t q_heads,
-                                   int64_t kv_heads, int64_t head_dim, int64_t max_len_in_batch,
-                                   float sm_scale, int dtype, void* workspace,
-                                   int64_t workspace_bytes, hipStream_t stream) {
+namespace {
+
+// Both entry points with a q tensor: win false is the whole context (window
+// and sinks unused).
+int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                     const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
+                     const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
+                     const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                     const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
+                     int seq_len_i64, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                     int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                     int64_t max_len_in_batch, bool win, int64_t window, int64_t sinks,
+                     float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream) {
+  if (win && batch == 0) return LL_OK;  // (an empty tensor has no address)
   LL_CHECK_ARG(q && k_cache && v_cache && req_to_tokens && b_req_idx && b_seq_len && out,
-               "ll_decode_attention: null pointer");
+               "%s: null pointer", fn);
   LL_CHECK_ARG(kv_heads > 0 && q_heads % kv_heads == 0,
-               "ll_decode_attention: q_heads %lld not a multiple of kv_heads %lld",
-               (long long)q_heads, (long long)kv_heads);
-  LL_CHECK_ARG(head_dim > 0 && head_dim <= 256, "ll_decode_attention: head_dim %lld unsupported",
+               "%s: q_heads %lld not a multiple of kv_heads %lld", fn, (long long)q_heads, (long long)kv_heads);
+  LL_CHECK_ARG(head_dim > 0 && head_dim <= 256, "%s: head_dim %lld unsupported", fn,
                (long long)head_dim);
   LL_CHECK_ARG(max_len_in_batch >= 0 && max_len_in_batch <= INT32_MAX,
-               "ll_decode_attention: max_len_in_batch %lld out of range",
+               "%s: max_len_in_batch %lld out of range", fn,
                (long long)max_len_in_batch);
+  LL_CHECK_ARG(!win || (window >= 1 && sinks >= 0), "%s: window %lld (min 1), sinks %lld (min 0)", fn,
+               (long long)window, (long long)sinks);
   if (batch == 0) return LL_OK;
   DecodeArgs a = {};
   a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h;
@@ -1394,24 +1422,78 @@ extern "C" int ll_decode_attention(const void* q, int64_t q_stride_b, int64_t q_
   a.slots_cap = 0;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.part_acc = nullptr; a.part_ml = nullptr;
+  // (token indices are below 2^31, so a larger window or count sees as much)
+  a.window = (int)std::min<int64_t>(window, 1 << 30);
+  a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
 
   const bool mfma_ok = (dtype == LL_BF16 || dtype == LL_F16) && (head_dim == 128 || head_dim == 64) &&
                        a.G <= 16 && (q_stride_h % 8 == 0) && (q_stride_b % 8 == 0) &&
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  if (!mfma_ok) {
+  if (!mfma_ok || win) {
+    LL_CHECK_ARG(!win || batch <= 65535, "%s: more than 65535 requests", fn);
     a.nsplit = 1;
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 8;
     return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-      hipLaunchKernelGGL((decode_attn_generic_kernel<T>), dim3((unsigned)q_heads, (unsigned)batch),
-                         dim3(64), shm, stream, a, (int)head_dim, sm_scale);
+      const dim3 grid((unsigned)q_heads, (unsigned)batch);
+      if (win)
+        hipLaunchKernelGGL((decode_attn_generic_kernel<T, true>), grid, dim3(64), shm, stream, a,
+                           (int)head_dim, sm_scale);
+      else
+        hipLaunchKernelGGL((decode_attn_generic_kernel<T, false>), grid, dim3(64), shm, stream, a,
+                           (int)head_dim, sm_scale);
       LL_RETURN_LAUNCH();
     });
   }
 
   return launch_mfma(a, head_dim, dtype, false, max_len_in_batch, workspace, workspace_bytes,
                      stream);
+}
+
+}  // namespace
+
+extern "C" int ll_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                   const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
+                                   const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
+                                   const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                                   const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
+                                   int seq_len_i64, void* out, int64_t out_stride_b,
+                                   int64_t out_stride_h, int64_t batch, int64_t q_heads,
+                                   int64_t kv_heads, int64_t head_dim, int64_t max_len_in_batch,
+                                   float sm_scale, int dtype, void* workspace,
+                                   int64_t workspace_bytes, hipStream_t stream) {
+  return decode_attention("ll_decode_attention", q, q_stride_b, q_stride_h, k_cache, k_stride_tok,
+                          k_stride_head, v_cache, v_stride_tok, v_stride_head, req_to_tokens,
+                          req_to_tokens_stride, b_req_idx, req_idx_i64, b_seq_len, seq_len_i64, out,
+                          out_stride_b, out_stride_h, batch, q_heads, kv_heads, head_dim,
+                          max_len_in_batch, false, 0, 0, sm_scale, dtype, workspace,
+                          workspace_bytes, stream);
+}
+
+extern "C" int ll_window_decode_attention(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v_cache, int64_t v_stride_tok,
+    int64_t v_stride_head, const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+    const void* b_req_idx, int req_idx_i64, const void* b_seq_len, int seq_len_i64, void* out,
+    int64_t out_stride_b, int64_t out_stride_h, int64_t batch, int64_t q_heads, int64_t kv_heads,
+    int64_t head_dim, int64_t max_len_in_batch, int64_t window, int64_t sinks, float sm_scale,
+    int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  return decode_attention("ll_window_decode_attention", q, q_stride_b, q_stride_h, k_cache,
+                          k_stride_tok, k_stride_head, v_cache, v_stride_tok, v_stride_head,
+                          req_to_tokens, req_to_tokens_stride, b_req_idx, req_idx_i64, b_seq_len,
+                          seq_len_i64, out, out_stride_b, out_stride_h, batch, q_heads, kv_heads,
+                          head_dim, max_len_in_batch, true, window, sinks, sm_scale, dtype,
+                          workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t ll_window_decode_attention_workspace_size(int64_t batch, int64_t q_heads,
+                                                             int64_t kv_heads, int64_t head_dim,
+                                                             int64_t max_len_in_batch,
+                                                             int64_t window, int64_t sinks) {
+  (void)batch, (void)q_heads, (void)kv_heads, (void)head_dim, (void)max_len_in_batch, (void)window,
+      (void)sinks;
+  return 0;
 }
 
 // ---------------------------------------------------------------- no-allocation variant

@@ -113,7 +113,20 @@ struct PrefillArgs {
   int nblk, B, KVH;  // MFMA path: query-row blocks per request, requests, KV heads
   float scale_log2;
   float sm_scale;
+  int window, sinks;  // windowed forms: visible keys n > p - window or n < sinks (both <= 2^30)
 };
+
+// The keys that any query at positions first .. first + rows - 1 sees, causal
+// limit aside: [0, sinks) and [low, ...). Where the two meet they are one
+// range from 0, given as (0, 0).
+struct WindowRange {
+  int sinks, low;
+};
+__device__ __forceinline__ WindowRange window_range(int64_t first, int window, int sinks) {
+  const int64_t low = first - window + 1;
+  if (low <= sinks) return {0, 0};
+  return {sinks, (int)low};
+}
 
 template <int D> struct FaGeom {
   static constexpr int ROWB = D * 2;            // bytes of a K or V row
@@ -605,7 +618,10 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
 }
 
 // Generic path: one wave per (query row, head), keys spread over the lanes.
-template <typename T>
+// WIN: only the keys of the row's window and the sinks, taken as one list
+// (index j is key j below the sinks, else j + skip), so that no table entry of
+// another key is read.
+template <typename T, bool WIN>
 __global__ __launch_bounds__(64) void prefill_attn_generic_kernel(PrefillArgs a, int D) {
   const int64_t m_row = blockIdx.x;
   const int h = blockIdx.y;
@@ -624,7 +640,14 @@ __global__ __launch_bounds__(64) void prefill_attn_generic_kernel(PrefillArgs a,
   const T* qp = (const T*)a.q + (start + m_row) * a.q_st + (int64_t)h * a.q_sh;
   for (int d = lane; d < D; d += 64) qs[d] = ll_to_f32(qp[d]);
   __syncthreads();
-  const int64_t kv_end = min(L, m_row + S + 1);
+  int64_t kv_end = min(L, m_row + S + 1);
+  int64_t nsink = 0, skip = 0;
+  if constexpr (WIN) {
+    const WindowRange r = window_range(m_row + S, a.window, a.sinks);
+    nsink = r.sinks;
+    skip = r.low - r.sinks;
+    kv_end -= skip;
+  }
   const int nd = (D + 63) / 64;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
@@ -635,7 +658,7 @@ __global__ __launch_bounds__(64) void prefill_attn_generic_kernel(PrefillArgs a,
     float s = -INFINITY;
     int slot = 0;
     if (t < kv_end) {
-      slot = a.r2t[rid * a.r2t_s + t];
+      slot = a.r2t[rid * a.r2t_s + (WIN && t >= nsink ? t + skip : t)];
       const T* kr = kb + (int64_t)slot * a.k_st;
       float dot = 0.f;
       for (int d = 0; d < D; ++d) dot += qs[d] * ll_to_f32(kr[d]);
@@ -666,29 +689,28 @@ __global__ __launch_bounds__(64) void prefill_attn_generic_kernel(PrefillArgs a,
   }
 }
 
-}  // namespace
-
-extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h,
-                                    const void* k_cache, int64_t k_stride_tok,
-                                    int64_t k_stride_head, const void* v_cache,
-                                    int64_t v_stride_tok, int64_t v_stride_head, void* out,
-                                    int64_t out_stride_tok, int64_t out_stride_h,
-                                    const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
-                                    const void* b_req_idx, int req_idx_i64,
-                                    const void* b_start_loc, int start_loc_i64,
-                                    const void* b_seq_len, int seq_len_i64,
-                                    const void* b_shared_seq_len, int shared_i64, int64_t batch,
-                                    int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                    int64_t max_input_len, float sm_scale, int dtype,
-                                    hipStream_t stream) {
+// Both entry points: win false is the whole context (window and sinks unused).
+int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64_t q_stride_h,
+                      const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
+                      const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head, void* out,
+                      int64_t out_stride_tok, int64_t out_stride_h, const int32_t* req_to_tokens,
+                      int64_t req_to_tokens_stride, const void* b_req_idx, int req_idx_i64,
+                      const void* b_start_loc, int start_loc_i64, const void* b_seq_len,
+                      int seq_len_i64, const void* b_shared_seq_len, int shared_i64, int64_t batch,
+                      int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_input_len,
+                      bool win, int64_t window, int64_t sinks, float sm_scale, int dtype,
+                      hipStream_t stream) {
+  if (win && batch == 0) return LL_OK;  // (an empty tensor has no address)
   LL_CHECK_ARG(q && k_cache && v_cache && out && req_to_tokens && b_req_idx && b_start_loc &&
                    b_seq_len,
-               "ll_prefill_attention: null pointer");
+               "%s: null pointer", fn);
   LL_CHECK_ARG(kv_heads > 0 && q_heads % kv_heads == 0,
-               "ll_prefill_attention: q_heads %lld not a multiple of kv_heads %lld",
-               (long long)q_heads, (long long)kv_heads);
+               "%s: q_heads %lld not a multiple of kv_heads %lld", fn, (long long)q_heads, (long long)kv_heads);
   LL_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0,
-               "ll_prefill_attention: head_dim %lld unsupported", (long long)head_dim);
+               "%s: head_dim %lld unsupported", fn, (long long)head_dim);
+  // window 1 sees the query's own token alone: no row is left without a key
+  LL_CHECK_ARG(!win || (window >= 1 && sinks >= 0), "%s: window %lld (min 1), sinks %lld (min 0)", fn,
+               (long long)window, (long long)sinks);
   if (batch == 0 || max_input_len <= 0) return LL_OK;
   PrefillArgs a;
   a.q = q; a.q_st = q_stride_tok; a.q_sh = q_stride_h;
@@ -702,6 +724,9 @@ extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
   a.shared = b_shared_seq_len; a.shared64 = shared_i64;
   a.H = (int)q_heads; a.G = (int)(q_heads / kv_heads);
   a.sm_scale = sm_scale;
+  // (token indices are below 2^31, so a larger window or count sees as much)
+  a.window = (int)std::min<int64_t>(window, 1 << 30);
+  a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
   a.scale_log2 = sm_scale * 1.4426950408889634f;
 
   const bool mfma_ok = (dtype == LL_BF16 || dtype == LL_F16) && (head_dim == 128 || head_dim == 64) &&
@@ -709,12 +734,17 @@ extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  if (!mfma_ok) {
+  if (!mfma_ok || win) {
+    LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535, "%s: more than 65535 heads or requests", fn);
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 4;
     return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-      hipLaunchKernelGGL((prefill_attn_generic_kernel<T>),
-                         dim3((unsigned)max_input_len, (unsigned)q_heads, (unsigned)batch), dim3(64),
-                         shm, stream, a, (int)head_dim);
+      const dim3 grid((unsigned)max_input_len, (unsigned)q_heads, (unsigned)batch);
+      if (win)
+        hipLaunchKernelGGL((prefill_attn_generic_kernel<T, true>), grid, dim3(64), shm, stream, a,
+                           (int)head_dim);
+      else
+        hipLaunchKernelGGL((prefill_attn_generic_kernel<T, false>), grid, dim3(64), shm, stream, a,
+                           (int)head_dim);
       LL_RETURN_LAUNCH();
     });
   }
@@ -726,8 +756,7 @@ extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
   a.KVH = (int)kv_heads;
   const int64_t units = (int64_t)a.nblk * batch * kv_heads;
   const int64_t nv = (int64_t)ll_cdiv(units, 8) * 8 * ll_cdiv(a.G, 8 / wph);  // work items
-  LL_CHECK_ARG(nv < ((int64_t)1 << 31), "ll_prefill_attention: %lld work items (max 2^31 - 1)",
-               (long long)nv);
+  LL_CHECK_ARG(nv < ((int64_t)1 << 31), "%s: %lld work items (max 2^31 - 1)", fn, (long long)nv);
   // persistent grid: one workgroup per CU (the LDS ring takes the whole CU),
   // a multiple of 16 so that the head groups of a (row block, request, KV
   // head) share an XCD on the reversed passes too; more when the items
@@ -763,4 +792,44 @@ extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
     if (head_dim == 128) launch(_Float16{}, D128{}); else launch(_Float16{}, D64{});
   }
   LL_RETURN_LAUNCH();
+}
+
+}  // namespace
+
+extern "C" int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h,
+                                    const void* k_cache, int64_t k_stride_tok,
+                                    int64_t k_stride_head, const void* v_cache,
+                                    int64_t v_stride_tok, int64_t v_stride_head, void* out,
+                                    int64_t out_stride_tok, int64_t out_stride_h,
+                                    const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                                    const void* b_req_idx, int req_idx_i64,
+                                    const void* b_start_loc, int start_loc_i64,
+                                    const void* b_seq_len, int seq_len_i64,
+                                    const void* b_shared_seq_len, int shared_i64, int64_t batch,
+                                    int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                    int64_t max_input_len, float sm_scale, int dtype,
+                                    hipStream_t stream) {
+  return prefill_attention("ll_prefill_attention", q, q_stride_tok, q_stride_h, k_cache,
+                           k_stride_tok, k_stride_head, v_cache, v_stride_tok, v_stride_head, out,
+                           out_stride_tok, out_stride_h, req_to_tokens, req_to_tokens_stride,
+                           b_req_idx, req_idx_i64, b_start_loc, start_loc_i64, b_seq_len,
+                           seq_len_i64, b_shared_seq_len, shared_i64, batch, q_heads, kv_heads,
+                           head_dim, max_input_len, false, 0, 0, sm_scale, dtype, stream);
+}
+
+extern "C" int ll_window_prefill_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_h, const void* k_cache,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v_cache, int64_t v_stride_tok,
+    int64_t v_stride_head, void* out, int64_t out_stride_tok, int64_t out_stride_h,
+    const int32_t* req_to_tokens, int64_t req_to_tokens_stride, const void* b_req_idx,
+    int req_idx_i64, const void* b_start_loc, int start_loc_i64, const void* b_seq_len,
+    int seq_len_i64, const void* b_shared_seq_len, int shared_i64, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t head_dim, int64_t max_input_len, int64_t window, int64_t sinks,
+    float sm_scale, int dtype, hipStream_t stream) {
+  return prefill_attention("ll_window_prefill_attention", q, q_stride_tok, q_stride_h, k_cache,
+                           k_stride_tok, k_stride_head, v_cache, v_stride_tok, v_stride_head, out,
+                           out_stride_tok, out_stride_h, req_to_tokens, req_to_tokens_stride,
+                           b_req_idx, req_idx_i64, b_start_loc, start_loc_i64, b_seq_len,
+                           seq_len_i64, b_shared_seq_len, shared_i64, batch, q_heads, kv_heads,
+                           head_dim, max_input_len, true, window, sinks, sm_scale, dtype, stream);
 }

@@ -8,6 +8,7 @@ computes on the host; a missing library raises at import.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -44,6 +45,23 @@ def _dev(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
+
+
+def _here(*ts) -> None:
+    """Raises unless all of `ts` (None skipped) sit on the current device: a
+    launch goes to that device's stream."""
+    idx = None
+    for t in ts:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
+        if idx is None:
+            idx = torch._C._cuda_getDevice()
+        if at != idx:
+            raise ValueError(f"lite_lang_amd ops need tensors of the current device (cuda:{idx}), "
+                             f"got {t.device}")
 
 
 def _call(fn, rec, fields, name, ws_name, ws_at, t):
@@ -222,6 +240,77 @@ def prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_input_l
     return o
 
 
+def _window_checks(q, cache_k, cache_v, out, req_to_tokens, window, sinks):
+    D = q.shape[2]
+    assert cache_k.shape[-1] == D and cache_v.shape == cache_k.shape and out.shape == q.shape
+    assert q.shape[1] % cache_k.shape[1] == 0
+    assert q.dtype == cache_k.dtype == cache_v.dtype == out.dtype
+    assert q.stride(2) == 1 and cache_k.stride(2) == 1 and cache_v.stride(2) == 1
+    assert out.stride(2) == 1
+    assert req_to_tokens.dtype == torch.int32 and req_to_tokens.stride(1) == 1
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window {window} must be at least 1 and sinks {sinks} at least 0")
+
+
+def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_input_len,
+                             req_to_tokens, window, sinks=0, b_shared_seq_len=None, sm_scale=None):
+    """prefill_attention in which the query at position p sees the keys n <= p
+    with n > p - window or n < sinks. Slot-table entries of keys that no query
+    of the call sees are not read, so those tokens may have left the cache."""
+    _window_checks(q, k, v, o, req_to_tokens, window, sinks)
+    T, H, D = q.shape
+    B = b_seq_len.shape[0]
+    assert b_req_idx.shape == (B,) and b_start_loc.shape == (B,)
+    assert b_req_idx.is_contiguous() and b_start_loc.is_contiguous() and b_seq_len.is_contiguous()
+    sh_ptr, sh64 = 0, 0
+    if b_shared_seq_len is not None:
+        assert b_shared_seq_len.shape == (B,) and b_shared_seq_len.is_contiguous()
+        sh_ptr, sh64 = b_shared_seq_len.data_ptr(), _idx(b_shared_seq_len, "b_shared_seq_len")
+    _here(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, req_to_tokens, b_shared_seq_len)
+    if sm_scale is None:
+        sm_scale = 1.0 / (D ** 0.5)
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
+    rc = _L.ll_window_prefill_attention(
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+        o.data_ptr(), os_[0], os_[1], req_to_tokens.data_ptr(), req_to_tokens.stride(0),
+        b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
+        b_start_loc.data_ptr(), _idx(b_start_loc, "b_start_loc"),
+        b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), sh_ptr, sh64,
+        B, H, k.shape[1], D, int(max_input_len), int(window), int(sinks), float(sm_scale),
+        dtype_code(q), _stream(q))
+    _lib.check(rc, "ll_window_prefill_attention")
+    return o
+
+
+def window_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_batch, cache_k,
+                            cache_v, out, window, sinks=0, sm_scale=None):
+    """decode_attention over the last `window` tokens and the first `sinks` ones."""
+    _window_checks(q, cache_k, cache_v, out, req_to_tokens, window, sinks)
+    B, H, D = q.shape
+    KVH = cache_k.shape[1]
+    assert b_req_idx.shape == (B,) and b_seq_len.shape == (B,)
+    assert b_req_idx.is_contiguous() and b_seq_len.is_contiguous()
+    _here(q, req_to_tokens, b_req_idx, b_seq_len, cache_k, cache_v, out)
+    if sm_scale is None:
+        sm_scale = 1.0 / (D ** 0.5)
+    max_len, window, sinks = int(max_len_in_batch), int(window), int(sinks)
+    # A buffer of the call's own, not the stream's persistent workspace: under
+    # capture it comes from the graph's memory, so graphs replayed at the same
+    # time share nothing.
+    need = _L.ll_window_decode_attention_workspace_size(B, H, KVH, D, max_len, window, sinks)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    qs, ks, vs, os_ = q.stride(), cache_k.stride(), cache_v.stride(), out.stride()
+    rc = _L.ll_window_decode_attention(
+        q.data_ptr(), qs[0], qs[1], cache_k.data_ptr(), ks[0], ks[1], cache_v.data_ptr(), vs[0],
+        vs[1], req_to_tokens.data_ptr(), req_to_tokens.stride(0),
+        b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
+        b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), out.data_ptr(), os_[0], os_[1],
+        B, H, KVH, D, max_len, window, sinks, float(sm_scale), dtype_code(q),
+        ws.data_ptr() if ws is not None else None, need, _stream(q))
+    _lib.check(rc, "ll_window_decode_attention")
+    return out
+
+
 # ------------------------------------------------------------------ elementwise
 def rmsnorm(x, gamma, eps, residual=None, out=None):
     """out = rmsnorm(x [+ residual]) * gamma; with residual, x is updated in place."""
@@ -273,6 +362,136 @@ def rope_kv_scatter(qkv, q_heads, kv_heads, head_dim, positions, cos_table, sin_
                                pool_layer.stride(0), pool_layer.stride(1), dtype_code(qkv),
                                _stream(qkv))
     _lib.check(rc, "ll_rope_kv_scatter")
+
+
+def rope_frequencies(rotary_dim, theta=1e6, scaling=None, max_position=None, length=None):
+    """(inv_freq fp32 [rotary_dim/2] on the CPU, factor) of rope_positions and
+    qk_norm_rope_kv_scatter: theta^(-2i/rotary_dim), scaled for contexts beyond
+    the max_position tokens a model was trained on as a Hugging Face config's
+    `rope_scaling` dict says (rope_type or type; `original_max_position_embeddings`
+    in it takes max_position's place):
+
+    * default: none;
+    * linear: every frequency divided by `factor`;
+    * dynamic: theta grown so that the slowest pair's wavelength stretches with
+      `length`, the longest context served (none below max_position);
+    * yarn: pairs that turn more than beta_fast times within max_position keep
+      their frequency, those below beta_slow are divided by `factor`, a linear
+      ramp between; the factor 0.1 ln(factor) + 1 (or attention_factor);
+    * longrope: frequencies divided pair by pair by `long_factor`, or by
+      `short_factor` where `length` is given and within max_position."""
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError(f"rotary_dim {rotary_dim} must be even and positive")
+    sc = dict(scaling or {})
+    kind = sc.get("rope_type", sc.get("type", "default"))
+    orig = sc.get("original_max_position_embeddings") or max_position
+    if kind in ("dynamic", "yarn", "longrope") and not orig:
+        raise ValueError(f"rope scaling '{kind}' needs max_position")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    factor = 1.0
+    if kind == "dynamic":
+        s = float(sc["factor"])
+        grow = max(1.0, s * max(length or 0, orig) / orig - (s - 1.0))
+        if rotary_dim > 2:
+            theta = theta * grow ** (rotary_dim / (rotary_dim - 2))
+    f = float(theta) ** -i
+    if kind == "linear":
+        f = f / float(sc["factor"])
+    elif kind == "yarn":
+        s = float(sc["factor"])
+        # the (fractional) pair that turns t times within orig:
+        # orig * theta^(-2n/R) / 2 pi = t
+        ends = [rotary_dim * math.log(orig / (2 * math.pi * t)) / (2 * math.log(theta))
+                for t in (sc.get("beta_fast") or 32, sc.get("beta_slow") or 1)]
+        if sc.get("truncate", True):
+            ends = [math.floor(ends[0]), math.ceil(ends[1])]
+        low, high = max(ends[0], 0), min(ends[1], rotary_dim - 1)
+        n = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        stretch = ((n - low) / max(high - low, 1e-3)).clamp(0, 1)
+        f = f * (1 - stretch) + f / s * stretch
+        factor = sc.get("attention_factor")
+        if factor is None:
+            factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+    elif kind == "longrope":
+        ext = sc["short_factor"] if length is not None and length <= orig else sc["long_factor"]
+        if len(ext) != rotary_dim // 2:
+            raise ValueError(f"longrope: {len(ext)} factors for {rotary_dim // 2} pairs")
+        f = f / torch.tensor(ext, dtype=torch.float64)
+        s = sc.get("factor") or (max_position / orig if max_position else 1.0)
+        factor = sc.get("attention_factor")
+        if factor is None:
+            factor = 1.0 if s <= 1 else math.sqrt(1 + math.log(s) / math.log(orig))
+    elif kind not in ("default", "dynamic"):
+        raise ValueError(f"unknown rope scaling '{kind}'")
+    return f.to(torch.float32), float(factor)
+
+
+def _rope_checks(positions, inv_freq, T, D):
+    assert positions.shape == (T,) and positions.is_contiguous()
+    assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.ndim == 1
+    assert 2 * inv_freq.shape[0] <= D, "more rotated pairs than the head has"
+
+
+def rope_positions(q, k, positions, inv_freq, interleaved=False, factor=1.0, q_out=None,
+                   k_out=None):
+    """Rotates q [T, Hq, D] and k [T, Hk, D] (or k None) at positions [T], in
+    place or into q_out / k_out. Rotated are the first 2 * len(inv_freq)
+    elements of a head, as pairs (i, i + len(inv_freq)) or, interleaved,
+    (2i, 2i + 1); pair i by positions * inv_freq[i], scaled by factor (see
+    rope_frequencies)."""
+    q_out = q if q_out is None else q_out
+    k_out = k if k_out is None else k_out
+    T, Hq, D = q.shape
+    assert q.stride(2) == 1 and q_out.stride(2) == 1 and q_out.shape == q.shape
+    assert q_out.dtype == q.dtype
+    _rope_checks(positions, inv_freq, T, D)
+    kargs = (None, 0, 0, None, 0, 0, 0)
+    if k is not None:
+        assert k.shape[0] == T and k.shape[2] == D and k.dtype == q.dtype
+        assert k.stride(2) == 1 and k_out.stride(2) == 1
+        assert k_out.shape == k.shape and k_out.dtype == k.dtype
+        ks, kos = k.stride(), k_out.stride()
+        kargs = (k.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], k.shape[1])
+    _here(q, k, positions, inv_freq, q_out, k_out)
+    qs, qos = q.stride(), q_out.stride()
+    rc = _L.ll_rope_positions(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], Hq,
+                              *kargs, positions.data_ptr(), _idx(positions, "positions"),
+                              inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(bool(interleaved)),
+                              float(factor), T, D, dtype_code(q), _stream(q))
+    _lib.check(rc, "ll_rope_positions")
+    return q_out, k_out
+
+
+def qk_norm_rope_kv_scatter(qkv, q_heads, kv_heads, head_dim, q_gamma, k_gamma, eps, positions,
+                            inv_freq, slots, pool_layer, interleaved=False, factor=1.0,
+                            q_out=None):
+    """rope_kv_scatter with an RMSNorm of every q and k head before the rotation
+    (q_gamma, k_gamma [head_dim]; None: no norm) and rope_positions' rotation:
+    q into q_out [T, q_heads, head_dim] (None: in place in qkv), K and V to
+    pool_layer[slots]. A slot outside the pool marks a padded token, whose K and
+    V go nowhere. Returns q [T, q_heads, head_dim]."""
+    T, D = qkv.shape[0], head_dim
+    assert qkv.stride(1) == 1 and qkv.shape[1] == (q_heads + 2 * kv_heads) * D
+    if q_out is None:
+        q_out = qkv[:, : q_heads * D].view(T, q_heads, D)
+    assert q_out.shape == (T, q_heads, D) and q_out.stride(2) == 1 and q_out.dtype == qkv.dtype
+    assert slots.dtype == torch.int32 and slots.shape == (T,) and slots.is_contiguous()
+    assert pool_layer.shape[1:] == (2 * kv_heads, D) and pool_layer.stride(2) == 1
+    assert pool_layer.dtype == qkv.dtype
+    for g in (q_gamma, k_gamma):
+        assert g is None or (g.shape == (D,) and g.is_contiguous() and g.dtype == qkv.dtype)
+    _rope_checks(positions, inv_freq, T, D)
+    _here(qkv, q_gamma, k_gamma, positions, inv_freq, slots, pool_layer, q_out)
+    qos, ps = q_out.stride(), pool_layer.stride()
+    rc = _L.ll_qk_norm_rope_kv_scatter(
+        qkv.data_ptr(), qkv.stride(0), T, q_heads, kv_heads, D, q_out.data_ptr(), qos[0], qos[1],
+        q_gamma.data_ptr() if q_gamma is not None else None,
+        k_gamma.data_ptr() if k_gamma is not None else None, float(eps), positions.data_ptr(),
+        _idx(positions, "positions"), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
+        int(bool(interleaved)), float(factor), slots.data_ptr(), pool_layer.data_ptr(), ps[0],
+        ps[1], pool_layer.shape[0], dtype_code(qkv), _stream(qkv))
+    _lib.check(rc, "ll_qk_norm_rope_kv_scatter")
+    return q_out
 
 
 def kv_store(src, slots, pool):
@@ -523,6 +742,52 @@ def assign_slots(req_to_tokens, packed, n):
     rc = _L.ll_assign_slots(req_to_tokens.data_ptr(), req_to_tokens.stride(0), packed[0].data_ptr(),
                             packed[1].data_ptr(), packed[2].data_ptr(), n, _stream(req_to_tokens))
     _lib.check(rc, "ll_assign_slots")
+
+
+def build_slot_maps(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_tokens, slots,
+                    positions, b_start_loc, last_rows, counts, page_size=1, block_table=None):
+    """Slot maps of a batch from its lengths, in one launch and without a host
+    read: request b (row b_req_idx[b] of req_to_tokens) holds b_cached_len[b]
+    tokens and grows to b_seq_len[b]. The pages that takes come off free_pages
+    [0], [1], ... in batch order; page_size 1 is the token-granular pool, whose
+    slots are the pages; else block_table [rows, pages] int32 holds each
+    request's pages and gets the new ones.
+
+    Written, all int32: slots and positions [>= new tokens] of the new tokens,
+    request after request; b_start_loc and last_rows [B], the first and the
+    last new token of each request (-1 without); the new entries of
+    req_to_tokens; counts [3] = (new tokens, pages taken, error). The error
+    word is 0, or, with nothing but counts written, the sum of 1: a length out
+    of range, 2: a bad or repeated row, 4: more tokens than `slots` holds, 8:
+    too few free pages."""
+    B = b_req_idx.shape[0]
+    for t in (b_req_idx, b_seq_len, b_cached_len, b_start_loc, last_rows):
+        assert t.shape == (B,) and t.is_contiguous()
+    for t in (free_pages, req_to_tokens, slots, positions, b_start_loc, last_rows, counts):
+        assert t.dtype == torch.int32
+    assert free_pages.ndim == 1 and free_pages.is_contiguous()
+    assert slots.ndim == 1 and slots.is_contiguous()
+    assert positions.shape == slots.shape and positions.is_contiguous()
+    assert counts.shape == (3,) and counts.is_contiguous()
+    assert req_to_tokens.ndim == 2 and req_to_tokens.stride(1) == 1
+    if page_size < 1 or (page_size > 1 and block_table is None):
+        raise ValueError(f"page_size {page_size} needs a block table" if page_size > 1 else
+                         f"page_size {page_size} must be at least 1")
+    bt = (None, 0, 0)
+    if page_size > 1:
+        assert block_table.dtype == torch.int32 and block_table.ndim == 2
+        assert block_table.stride(1) == 1 and block_table.shape[0] == req_to_tokens.shape[0]
+        bt = (block_table.data_ptr(), block_table.stride(0), block_table.shape[1])
+    _here(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_tokens, slots, positions,
+          b_start_loc, last_rows, counts, block_table)
+    rc = _L.ll_build_slot_maps(
+        b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(),
+        _idx(b_seq_len, "b_seq_len"), b_cached_len.data_ptr(), _idx(b_cached_len, "b_cached_len"),
+        B, free_pages.data_ptr(), free_pages.shape[0], page_size, *bt, req_to_tokens.data_ptr(),
+        req_to_tokens.stride(0), req_to_tokens.shape[0], req_to_tokens.shape[1], slots.data_ptr(),
+        positions.data_ptr(), slots.shape[0], b_start_loc.data_ptr(), last_rows.data_ptr(),
+        counts.data_ptr(), _stream(counts))
+    _lib.check(rc, "ll_build_slot_maps")
 
 
 # ------------------------------------------------------------------ decode split-K path
