@@ -444,7 +444,10 @@ __device__ __forceinline__ void unit_merge_tail(const DecodeArgs& a, bool item, 
 // sequence's new slot appears in no other sequence's first seq_len entries
 // and in its own only within the last split (the decode step puts it at
 // seq_len - 1).
-// The split stage, for both kernels below. p_len .. idx64 are the fields of
+// Windowed (MODE 3): q is given and `len` counts the visible tokens, which the
+// slot-table reads take as one list (window_list); everything behind the slot
+// ids is the same.
+// The split stage, for the kernels below. p_len .. idx64 are the fields of
 // the first loads (lengths, request rows, positions, new slots, the grid
 // geometry); idx64: bit 0 lengths, bit 1 request rows, bit 2 positions are
 // int64; bit 3 the spread block mapping.
@@ -452,11 +455,12 @@ template <typename T, int D, int MODE>
 __device__ __forceinline__ void decode_attn_split_stage(
     const int32_t* __restrict__ p_len, const int32_t* __restrict__ p_rid,
     const int32_t* __restrict__ p_pos, const int32_t* __restrict__ p_nslot, int KVH, int nsplit,
-    int B, int idx64, const DecodeArgs& a) {
+    int B, int idx64, const DecodeArgs& a, int window = 0, int sinks = 0) {
   typedef typename Vec8<T>::type V8;
   typedef typename Vec4<T>::type V4;
   typedef TileGeom<D> TG;
-  constexpr bool ROPE = MODE != 0;  // q from the QKV partials (1: fp32, 2: any kind)
+  constexpr bool ROPE = MODE == 1 || MODE == 2;  // q from the QKV partials (1: fp32, 2: any kind)
+  constexpr bool WIN = MODE == 3;
   constexpr int DS = D / 32;  // k-steps of the S^T product
   constexpr int DB = D / 16;  // 16-wide d blocks of the output
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -472,7 +476,7 @@ __device__ __forceinline__ void decode_attn_split_stage(
   const int32_t len32 = p_len[(idx64 & 1) ? 2 * b : b];
   const int32_t rid32 = p_rid[(idx64 & 2) ? 2 * b : b];
   int32_t pos32 = 0, new_slot = 0;
-  if constexpr (MODE != 0) {
+  if constexpr (ROPE) {
     pos32 = p_pos[(idx64 & 4) ? 2 * b : b];
     new_slot = p_nslot[b];
   }
@@ -500,6 +504,11 @@ __device__ __forceinline__ void decode_attn_split_stage(
   // two dependent chains (length/row -> slots, position -> cos/sin) overlap.
   asm volatile("" ::"s"(len32), "s"(rid32), "s"(pos32), "s"(new_slot));  // the loads are in
   int64_t len = len32 > a.max_len ? a.max_len : len32;
+  WindowList wl = {0, 0, 0};
+  if constexpr (WIN) {
+    wl = window_list(len, window, sinks);
+    len = wl.n;
+  }
   const int64_t rid = rid32;
   const int32_t* slot_row = a.r2t + rid * a.r2t_s;
   const int ntiles = (int)((len + kTT - 1) / kTT);
@@ -527,7 +536,8 @@ __device__ __forceinline__ void decode_attn_split_stage(
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = (wave + kWaves * (4 * (r0 + u) + (lane >> 4))) * kTT + (lane & 15);
-      const int64_t t = min(tok0 + i, len > 0 ? len - 1 : (int64_t)0);  // always a valid entry
+      int64_t t = min(tok0 + i, len > 0 ? len - 1 : (int64_t)0);  // always a valid entry
+      if (WIN && t >= wl.sinks) t += wl.skip;
       sl[u] = slot_row[t];
     }
   };
@@ -891,6 +901,14 @@ __global__ __launch_bounds__(kWaves * 64) void decode_attn_dma_kernel(
   decode_attn_split_stage<T, D, 0>(p_len, p_rid, nullptr, nullptr, KVH, nsplit, B, idx64, a);
 }
 
+template <typename T, int D>
+__global__ __launch_bounds__(kWaves * 64) void decode_attn_window_kernel(
+    const int32_t* __restrict__ p_len, const int32_t* __restrict__ p_rid, int KVH, int nsplit,
+    int B, int idx64, int window, int sinks, DecodeArgs a) {
+  decode_attn_split_stage<T, D, 3>(p_len, p_rid, nullptr, nullptr, KVH, nsplit, B, idx64, a,
+                                   window, sinks);
+}
+
 // Fused RoPE variants: the argument block only (their q rebuild waits for the
 // positions' round trip either way, and preloaded arguments made the W8A8
 // decode step 7 us slower).
@@ -907,7 +925,9 @@ __global__ __launch_bounds__(kWaves * 64) void decode_attn_rope_kernel(DecodeArg
 // Separate merge kernels, for the shapes the split stage does not merge itself
 // (spread splits, more than kMergeUnits units, or a quantised row larger than
 // the tile rings): one wave per (sequence, head).
-template <typename T, int D>
+// CLEAR: the partial rows are left at zero, as every call leaves the workspace
+// that the same-launch merges poll (a windowed call's is its own).
+template <typename T, int D, bool CLEAR>
 __global__ __launch_bounds__(kCombWaves * 64) void decode_attn_combine_kernel(DecodeArgs a) {
   constexpr int DPL = D / 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -916,7 +936,7 @@ __global__ __launch_bounds__(kCombWaves * 64) void decode_attn_combine_kernel(De
   const int b = bh / a.H, h = bh - b * a.H;
   float o[DPL];
   combine_bh<D>(a, bh, lane, o);
-  clear_bh<D>(a, bh, lane);
+  if constexpr (CLEAR) clear_bh<D>(a, bh, lane);
   T* op = (T*)a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh;
 #pragma unroll
   for (int q = 0; q < DPL; ++q) op[lane + 64 * q] = ll_from_f32<T>(o[q]);
@@ -1224,11 +1244,23 @@ void launch_combine(const DecodeArgs& a, int dtype, hipStream_t stream) {
   }
   const dim3 cgrid((unsigned)((a.B * a.H + kCombWaves - 1) / kCombWaves));
   if (dtype == LL_BF16)
-    hipLaunchKernelGGL((decode_attn_combine_kernel<__bf16, D>), cgrid, dim3(kCombWaves * 64), 0,
-                       stream, a);
+    hipLaunchKernelGGL((decode_attn_combine_kernel<__bf16, D, true>), cgrid, dim3(kCombWaves * 64),
+                       0, stream, a);
   else
-    hipLaunchKernelGGL((decode_attn_combine_kernel<_Float16, D>), cgrid, dim3(kCombWaves * 64), 0,
-                       stream, a);
+    hipLaunchKernelGGL((decode_attn_combine_kernel<_Float16, D, true>), cgrid,
+                       dim3(kCombWaves * 64), 0, stream, a);
+}
+
+template <typename T, int D>
+void launch_window(const DecodeArgs& a, unsigned grid, size_t lds, hipStream_t stream) {
+  const int idx64 = (a.len64 ? 1 : 0) | (a.req64 ? 2 : 0) | 8;
+  hipLaunchKernelGGL((decode_attn_window_kernel<T, D>), dim3(grid), dim3(kWaves * 64), lds, stream,
+                     (const int32_t*)a.seq_len, (const int32_t*)a.req_idx, a.KVH, a.nsplit, a.B,
+                     idx64, a.window, a.sinks, a);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((decode_attn_combine_kernel<T, D, false>),
+                       dim3((unsigned)ll_cdiv((int64_t)a.B * a.H, kCombWaves)),
+                       dim3(kCombWaves * 64), 0, stream, a);
 }
 
 // Workspace layout when the sequences are split: [kMergeUnits split tickets]
@@ -1324,6 +1356,74 @@ int launch_mfma(DecodeArgs& a, int64_t head_dim, int dtype, bool rope, int64_t m
   LL_RETURN_LAUNCH();
 }
 
+// Visible tokens of a sequence, at most.
+int64_t window_bound(int64_t max_len, int64_t window, int64_t sinks) {
+  if (window >= max_len || sinks >= max_len - window) return max_len;
+  return window + sinks;
+}
+
+// Splits of a windowed call: always merged by a second launch, so that the
+// workspace needs no initial state, holds nothing between calls and may be
+// anyone's (two graphs in flight each have their own); spread over all XCDs.
+// The counts of choose_splits but where its same-launch merge set them (from a
+// sweep of 1-32 splits over 1-128 sequences, windows of 256-8192, 2 to 8 KV
+// heads of 128 and 64, in a graph; us per call):
+// * up to 24 tiles, three rounds of a workgroup's waves, the second launch
+//   costs more than it saves (1 x 260 visible tokens, 16/2 heads of 128: 1
+//   split 6.6, 3 7.3; 40 x 304: 7.5, with 2 9.4);
+// * at head_dim 64 so do 2 or 3 splits of any length: those come of many units
+//   (96 x 504, 8/2 heads: 8.2, with 2 11.4; 128 x 2052: 27.7 and 30.6);
+// * 8 splits merge as fast as 4, so that from 48 tiles they are worth their
+//   shorter streams where they fit one dispatch round (1 x 1028, 16/2: 7.9,
+//   with 4 8.6; 8/2 heads of 64: 6.9 and 7.3).
+int choose_window_splits(int64_t B, int64_t KVH, int64_t bound, int64_t head_dim) {
+  const int64_t tiles = (bound + kTT - 1) / kTT;
+  if (tiles <= 3 * kWaves) return 1;
+  const int min_ns = (int)((tiles * kTT + kMaxSplitTokens - 1) / kMaxSplitTokens);
+  const int ns = choose_splits((int)B, (int)KVH, bound, head_dim).ns;
+  if (head_dim == 64 && ns <= 3) return min_ns;
+  if (ns == 4 && tiles >= 48 && B * KVH * 8 <= 256 * split_wg_per_cu(head_dim)) return 8;
+  return ns;
+}
+
+int64_t window_workspace_bytes(int64_t parts, int64_t head_dim) {
+  return align256(parts * head_dim * 4) + parts * 2 * 4;  // partial acc, (m, l)
+}
+
+int launch_window_mfma(DecodeArgs& a, int64_t head_dim, int dtype, int64_t bound, void* workspace,
+                       int64_t workspace_bytes, hipStream_t stream) {
+  a.nsplit = choose_window_splits(a.B, a.KVH, bound, head_dim);
+  LL_CHECK_ARG((int64_t)a.B * a.H * a.nsplit <= INT32_MAX,
+               "window decode attention: %d sequences of %d heads in %d splits (max 2^31 - 1 rows)",
+               a.B, a.H, a.nsplit);
+  a.spread = 1;
+  a.merge_cnt = nullptr;
+  const int64_t parts = (int64_t)a.B * a.H * a.nsplit;
+  std::unique_lock<std::mutex> lock;
+  if (a.nsplit > 1) {
+    const int64_t need = window_workspace_bytes(parts, head_dim);
+    LL_CHECK_ARG(workspace != nullptr && workspace_bytes >= need,
+                 "window decode attention: workspace too small (need %lld bytes, got %lld)",
+                 (long long)need, (long long)workspace_bytes);
+    a.part_acc = (float*)workspace;
+    a.part_ml = (float*)((char*)workspace + align256(parts * head_dim * 4));
+    // no other thread's call on this workspace between the two launches
+    lock = std::unique_lock<std::mutex>(ll_workspace_mutex(workspace));
+  }
+  const int64_t tiles = (bound + kTT - 1) / kTT;
+  a.slots_cap = (int)((tiles + a.nsplit - 1) / a.nsplit) * kTT;
+  const unsigned grid = (unsigned)(a.units * a.nsplit);
+  const size_t extra = (size_t)a.slots_cap * 4;
+  if (head_dim == 128) {
+    if (dtype == LL_BF16) launch_window<__bf16, 128>(a, grid, TileGeom<128>::MAIN_B + extra, stream);
+    else launch_window<_Float16, 128>(a, grid, TileGeom<128>::MAIN_B + extra, stream);
+  } else {
+    if (dtype == LL_BF16) launch_window<__bf16, 64>(a, grid, TileGeom<64>::MAIN_B + extra, stream);
+    else launch_window<_Float16, 64>(a, grid, TileGeom<64>::MAIN_B + extra, stream);
+  }
+  LL_RETURN_LAUNCH();
+}
+
 // The XCD (hardware register XCC_ID) each workgroup runs on, for the premise
 // of the same-launch split merge: workgroup i of a grid runs on XCD
 // (i + r) mod 8 with one r for the whole launch.
@@ -1407,6 +1507,8 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
                (long long)max_len_in_batch);
   LL_CHECK_ARG(!win || (window >= 1 && sinks >= 0), "%s: window %lld (min 1), sinks %lld (min 0)", fn,
                (long long)window, (long long)sinks);
+  LL_CHECK_ARG(!win || (sm_scale > 0.f && sm_scale < INFINITY), "%s: sm_scale %g must be positive",
+               fn, (double)sm_scale);
   if (batch == 0) return LL_OK;
   DecodeArgs a = {};
   a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h;
@@ -1431,7 +1533,8 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  if (!mfma_ok || win) {
+  // (without a token the split stage would still read a table entry per sequence)
+  if (!mfma_ok || (win && max_len_in_batch == 0)) {
     LL_CHECK_ARG(!win || batch <= 65535, "%s: more than 65535 requests", fn);
     a.nsplit = 1;
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 8;
@@ -1447,6 +1550,9 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
     });
   }
 
+  if (win)
+    return launch_window_mfma(a, head_dim, dtype, window_bound(max_len_in_batch, window, sinks),
+                              workspace, workspace_bytes, stream);
   return launch_mfma(a, head_dim, dtype, false, max_len_in_batch, workspace, workspace_bytes,
                      stream);
 }
@@ -1491,9 +1597,12 @@ extern "C" int64_t ll_window_decode_attention_workspace_size(int64_t batch, int6
                                                              int64_t kv_heads, int64_t head_dim,
                                                              int64_t max_len_in_batch,
                                                              int64_t window, int64_t sinks) {
-  (void)batch, (void)q_heads, (void)kv_heads, (void)head_dim, (void)max_len_in_batch, (void)window,
-      (void)sinks;
-  return 0;
+  if (batch <= 0 || kv_heads <= 0 || max_len_in_batch <= 0 || window < 1 || sinks < 0 ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  const int ns = choose_window_splits(batch, kv_heads,
+                                      window_bound(max_len_in_batch, window, sinks), head_dim);
+  return ns > 1 ? window_workspace_bytes(batch * q_heads * ns, head_dim) : 0;
 }
 
 // ---------------------------------------------------------------- no-allocation variant

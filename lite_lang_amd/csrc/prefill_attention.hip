@@ -179,7 +179,12 @@ __device__ __forceinline__ int64_t fa_item_of_pass(int j, int P, int w) {
 // SGPRs at dispatch, so those loads do not wait for the argument block's
 // load. idx64: bit 0 lengths, 1 shared, 2 starts, 3 request rows are int64.
 // nv: virtual blocks (items, valid or not) of the launch.
-template <typename T, int D, int WPH>
+// WIN: windowed. An item's tiles are its sinks' (none where they meet its
+// window, whose range then starts at key 0) and then those of its window,
+// which starts at the first key that the item's first row sees, so that no
+// table entry below it is read. A wave leaves out the tiles in which none of
+// its rows sees a key, and masks those that some of its rows see in part.
+template <typename T, int D, int WPH, bool WIN>
 __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     const void* __restrict__ p_len, const void* __restrict__ p_shared,
     const void* __restrict__ p_start, const void* __restrict__ p_rid, int idx64, int nblk, int B,
@@ -203,6 +208,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // and head group, its first query row, key count and tile count). An item
   // is valid when its row block starts inside its request's query rows.
   int it_L = 0, it_S = 0, it_blk0 = 0, it_kvend = 1, it_nt = 0, it_kvh = 0, it_hp = 0;
+  int it_low = 0, it_sk = 0;  // WIN: first key of the window's tiles, sinks apart from them
   int64_t it_start = 0, it_rid = 0;
   bool it_ok = false;
   {
@@ -225,6 +231,12 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
         it_blk0 = (int)blk0;
         it_kvend = (int)min(L, blk0 + SH::BQ + S);  // keys of the item
         it_nt = (it_kvend + kBK - 1) / kBK;
+        if constexpr (WIN) {
+          const WindowRange r = window_range(blk0 + S, a.window, a.sinks);
+          it_low = r.low;
+          it_sk = r.sinks;
+          it_nt = (it_sk + kBK - 1) / kBK + (it_kvend - it_low + kBK - 1) / kBK;
+        }
         it_kvh = unit % KVH;
         it_hp = (int)(vb >> 3) % HP;
       }
@@ -252,6 +264,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   struct WaveItem {
     int64_t start;
     int h, row0, qlast, S, Lm1, kv_end;
+    int low, sk, nst;  // WIN: the item's window start, sinks apart from it, their tiles
     bool ok;
   };
   auto wave_item = [&](int k) -> WaveItem {
@@ -266,6 +279,11 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     r.S = S;
     r.Lm1 = L - 1;
     r.kv_end = (int)min((int64_t)L, (int64_t)r.row0 + SH::RW + S);
+    if constexpr (WIN) {
+      r.low = rl(it_low, k);
+      r.sk = rl(it_sk, k);
+      r.nst = (r.sk + kBK - 1) / kBK;
+    }
     return r;
   };
   // Q^T fragments (B operand: column = query row row0 + l32, clamped into the
@@ -305,6 +323,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // stays on the last item's last tile.
   struct SlotCursor {
     int k, u, nt, last_key;
+    int low, last_sink, nst;  // WIN
     const int32_t* row;
   };
   struct KvCursor {
@@ -317,6 +336,11 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     c.u = 0;
     c.nt = rl(it_nt, k);
     c.last_key = rl(it_kvend, k) - 1;
+    if constexpr (WIN) {
+      c.low = rl(it_low, k);
+      c.last_sink = rl(it_sk, k) - 1;
+      c.nst = (c.last_sink + kBK) / kBK;
+    }
     c.row = a.r2t + rl64(it_rid, k) * a.r2t_s;
   };
   auto kv_at = [&](KvCursor& c, int k) {
@@ -340,8 +364,13 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   };
   const int k_first = (int)__builtin_ctzll(items);
   // slot ids of cursor c's tile (keys 64 u + lane, clamped) -> ring entry x % NST
+  // (WIN: the window's tiles start at its first key, clamped likewise)
   auto slot_copy = [&](int x, const SlotCursor& c) {
-    dma4(c.row + min(c.u * kBK + lane, c.last_key), wslots + (x % NST) * (kBK * 4));
+    int key = min(c.u * kBK + lane, c.last_key);
+    if constexpr (WIN)
+      key = c.u < c.nst ? min(c.u * kBK + lane, c.last_sink)
+                        : min(c.low + (c.u - c.nst) * kBK + lane, c.last_key);
+    dma4(c.row + key, wslots + (x % NST) * (kBK * 4));
   };
   // this wave's K and V rows of cursor c's tile (slot ids in ring entry
   // x % NST) -> stage x % NST
@@ -370,7 +399,9 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       for (int qb = 0; qb < QB; ++qb) acc[db][qb] = (f32x16){};
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      m_run[qb] = -INFINITY;
+      // WIN: finite, so that a row that sees nothing of its wave's first tiles
+      // gets exp2(-inf - m) = 0 from them and a later tile's rescale is 0
+      m_run[qb] = WIN ? -3.402823466e38f : -INFINITY;
       l_run[qb] = 0.f;
     }
   };
@@ -404,7 +435,8 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // half-wave's keys in m_cand
   f32x16 sacc[2][QB];
   float m_cand[QB];
-  auto scores = [&](int t0, int buf) {
+  // (t0: the tile's first key; WIN: top is the last key of the tile's range)
+  auto scores = [&](int t0, int buf, int top) {
     const char* kl = smem + buf * FG::STAGE_B;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -427,19 +459,24 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     // the causal + length mask only where a key can pass the wave's first
     // row's limit (masked keys -> -inf), then the tile's row maxima in the
     // exp2 domain (finite: key 0 is visible to every row, scale_log2 > 0)
-    const bool need_mask = t0 + kBK - 1 > min(cur.row0 + cur.S, cur.Lm1);
+    const int last_row_low = cur.row0 + SH::RW - 1 + cur.S - a.window;  // below its window
+    const bool need_mask = WIN ? t0 + kBK - 1 > min(cur.row0 + cur.S, top) ||
+                                     (t0 <= last_row_low && t0 + kBK > a.sinks)
+                               : t0 + kBK - 1 > min(cur.row0 + cur.S, cur.Lm1);
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       if (need_mask) {
         // last key this row sees, relative to the tile (rows past the
         // request see every key of it)
-        const int lim = min(cur.row0 + 32 * qb + l32 + cur.S, cur.Lm1) - t0;
+        const int p = cur.row0 + 32 * qb + l32 + cur.S;
+        const int lim = min(p, WIN ? top : cur.Lm1) - t0;
+        const int below = p - a.window - t0, sink = a.sinks - t0;  // WIN
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = 32 * kb + 8 * (e >> 2) + 4 * hf + (e & 3);
-            if (key > lim) sacc[kb][qb][e] = -INFINITY;
+            if (key > lim || (WIN && key <= below && key >= sink)) sacc[kb][qb][e] = -INFINITY;
           }
       }
       float tmax = -INFINITY;
@@ -570,10 +607,23 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     kv_next(ck);
     slot_copy(x + 2 * NST - 2, cs);
     slot_next(cs);
-    const int t0 = cc_u * kBK, buf = x % NST;
-    const bool work = cur.ok && t0 < cur.kv_end;
+    const int buf = x % NST;
+    int t0 = cc_u * kBK, top = cur.Lm1;
+    bool work = cur.ok && t0 < cur.kv_end;
+    if constexpr (WIN) {
+      if (cc_u < cur.nst) {
+        top = cur.sk - 1;  // a sink tile: every row sees all of its keys
+        work = cur.ok;
+      } else {
+        // not where the causal limit or the wave's first row's window leaves
+        // the tile out, but where it holds sinks
+        t0 = cur.low + (cc_u - cur.nst) * kBK;
+        work = cur.ok && t0 < cur.kv_end &&
+               (t0 + kBK - 1 > cur.row0 + cur.S - a.window || t0 < a.sinks);
+      }
+    }
     const bool last = cc_u + 1 == cc_nt;
-    if (work) scores(t0, buf);
+    if (work) scores(t0, buf, top);
     if (last) {
       const int k2 = next_item(cc_k);
       if (k2 < 64) prefetch_q(wave_item(k2));
@@ -711,6 +761,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   // window 1 sees the query's own token alone: no row is left without a key
   LL_CHECK_ARG(!win || (window >= 1 && sinks >= 0), "%s: window %lld (min 1), sinks %lld (min 0)", fn,
                (long long)window, (long long)sinks);
+  LL_CHECK_ARG(!win || (sm_scale > 0.f && sm_scale < INFINITY), "%s: sm_scale %g must be positive",
+               fn, (double)sm_scale);
   if (batch == 0 || max_input_len <= 0) return LL_OK;
   PrefillArgs a;
   a.q = q; a.q_st = q_stride_tok; a.q_sh = q_stride_h;
@@ -734,7 +786,9 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  if (!mfma_ok || win) {
+  // (its rows are stored 8 bytes at a time)
+  const bool out_ok = out_stride_tok % 4 == 0 && out_stride_h % 4 == 0 && (uintptr_t)out % 8 == 0;
+  if (!mfma_ok || (win && !out_ok)) {
     LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535, "%s: more than 65535 heads or requests", fn);
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 4;
     return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
@@ -775,14 +829,17 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
     constexpr size_t lds = kStages * FaGeom<D>::STAGE_B + 8 * kStages * kBK * 4 + 8 * 256;
     const int idx64 = (a.len64 ? 1 : 0) | (a.shared64 ? 2 : 0) | (a.start64 ? 4 : 0) |
                       (a.req64 ? 8 : 0);
-    if (wph == 2)
-      hipLaunchKernelGGL((prefill_attn_fa_kernel<T, D, 2>), grid, block, lds, stream, a.seq_len,
-                         a.shared, a.start_loc, a.req_idx, idx64, a.nblk, a.B, a.KVH, a.G, (int)nv,
-                         a);
-    else
-      hipLaunchKernelGGL((prefill_attn_fa_kernel<T, D, 4>), grid, block, lds, stream, a.seq_len,
-                         a.shared, a.start_loc, a.req_idx, idx64, a.nblk, a.B, a.KVH, a.G, (int)nv,
-                         a);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, block, lds, stream, a.seq_len, a.shared, a.start_loc,
+                         a.req_idx, idx64, a.nblk, a.B, a.KVH, a.G, (int)nv, a);
+    };
+    if (wph == 2) {
+      if (win) go(prefill_attn_fa_kernel<T, D, 2, true>);
+      else go(prefill_attn_fa_kernel<T, D, 2, false>);
+    } else {
+      if (win) go(prefill_attn_fa_kernel<T, D, 4, true>);
+      else go(prefill_attn_fa_kernel<T, D, 4, false>);
+    }
   };
   typedef std::integral_constant<int, 128> D128;
   typedef std::integral_constant<int, 64> D64;

@@ -236,7 +236,7 @@ def _prefill_case(cuda, H, KVH, D, dtype, lens, before, window, sinks, seed=0, i
     q = (torch.randn(T, H, D, generator=g) * mag).to(dtype)
     qd = torch.zeros(T, H, D + pad, dtype=dtype, device=cuda)[..., :D]
     qd.copy_(q)
-    out = torch.full((T, H, D), 7.0, dtype=dtype, device=cuda)
+    out = torch.full((T, H, D + pad), 7.0, dtype=dtype, device=cuda)[..., :D]
     pd = pool.to(cuda)
     shared = None if not any(before) else _i32(before, cuda, idx)
     _ops().window_prefill_attention(qd, pd[:, :KVH], pd[:, KVH:], out, _i32(rids, cuda, idx),
