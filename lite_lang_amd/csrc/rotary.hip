@@ -45,7 +45,9 @@ __device__ __forceinline__ void rot_angle(int64_t pos, float inv_freq, float fac
   s *= factor;
 }
 
-// Any head_dim, rotary_dim and alignment: one wave per (token, head), a lane
+// Any head_dim, rotary_dim and alignment, for the shapes and strides that the
+// 16-byte form below does not take (24,000 tokens of 28/4 heads of 128: 247 us
+// against its 68): one wave per (token, head), a lane
 // per pair.
 template <typename T, bool INTER>
 __global__ __launch_bounds__(64) void rotary_kernel(RotArgs a) {
@@ -93,6 +95,226 @@ __global__ __launch_bounds__(64) void rotary_kernel(RotArgs a) {
     y[d] = g != nullptr ? ll_from_f32<T>(value(d)) : x[d];
 }
 
+// 16-byte form: a group of LPH lanes per head, 16 elements per lane (one "unit",
+// two chunks of 8 that hold its 8 pairs), D / 16 <= LPH units.
+// HBM-bound (a token's heads are read and written once), so what counts is
+// that nothing else shows: the angles, 60-odd instructions each in fp64 and
+// sincospif, are computed once per token and pair into LDS and shared by its
+// heads, while the first heads' loads are in flight; a workgroup takes TB
+// tokens so that there are enough heads to cover that. The norm's sum stays in
+// the LPH lanes of its head.
+template <typename T> struct alignas(16) Chunk { T v[8]; };
+
+// Stores go out non-temporally: nothing of this call reads them, and the lines
+// they would leave in the L2 have to be written back at its end anyway (24,000
+// tokens of 28/4 heads 81 -> 68 us, 2000 of 32/8 heads of 64 10.6 -> 7.9;
+// non-temporal loads gained 3-6% at 24,000 tokens and lost up to 30% at 4000,
+// whose rows the projection has just left on the memory side's cache).
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) {
+  constexpr int N = sizeof(c) / 16;
+  struct Words { u32x4 w[N]; };
+  const Words v = __builtin_bit_cast(Words, c);
+#pragma unroll
+  for (int i = 0; i < N; ++i) __builtin_nontemporal_store(v.w[i], (u32x4*)p + i);
+}
+
+constexpr int kRotThreads = 256;
+
+template <typename T, int LPH, bool INTER, bool NORM>
+__global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int TB, int heads_mul,
+                                                                 int heads_shift) {
+  extern __shared__ __attribute__((aligned(16))) float sh[];  // [TB][R/2] cos, then sin
+  typedef Chunk<T> C;
+  constexpr int kGroups = kRotThreads / LPH;
+  const int half = a.R / 2, heads = a.na + a.nb;
+  const int64_t t0 = (int64_t)blockIdx.x * TB;
+  const int nt = (int)min((int64_t)TB, a.ntok - t0);
+  const int items = nt * heads;
+  const int u = threadIdx.x % LPH;
+  const int units = a.D / 16, runits = a.R / 16;
+  const bool live = u < units;
+  // The chunks of unit u, such that neighbouring lanes read neighbouring
+  // chunks. Half layout: u and u + R / 16 hold pairs 8u .. 8u + 7, and the
+  // units behind R share its chunks out likewise; interleaved: u and u + D / 16,
+  // chunk c with pairs 4c .. 4c + 3.
+  const bool rot0 = INTER ? u < 2 * runits : u < runits;
+  const bool rot1 = INTER ? u + units < 2 * runits : rot0;
+  const int c0 = INTER || rot0 ? u : runits + u;
+  const int c1 = INTER ? u + units : rot0 ? u + runits : units + u;
+  const int p0 = INTER ? 4 * u : 8 * u, p1 = INTER ? 4 * (u + units) : 8 * u + 4;
+
+  struct Item {
+    C x0, x1;
+    T* y;       // null: not stored
+    int tok, kind;  // kind: 0 copied, 1 rotated head of a, 2 of b
+  };
+  auto load = [&](int i) {
+    Item it;
+    // i / heads by multiplication (exact for the items of a workgroup)
+    it.tok = (int)(((uint32_t)i * (uint32_t)heads_mul) >> heads_shift);
+    const int h = i - it.tok * heads;
+    const int64_t t = t0 + it.tok;
+    const bool isa = h < a.na;
+    const int hb = h - a.na;
+    const T* x = isa ? (const T*)a.a + t * a.a_st + (int64_t)h * a.a_sh
+                     : (const T*)a.b + t * a.b_st + (int64_t)hb * a.b_sh;
+    it.y = isa ? (T*)a.ao + t * a.ao_st + (int64_t)h * a.ao_sh
+               : (T*)a.bo + t * a.bo_st + (int64_t)hb * a.bo_sh;
+    if (!isa && a.slots != nullptr) {
+      const int64_t row = a.slots[t];
+      it.y = row >= 0 && row < a.nslots ? (T*)a.bo + row * a.bo_st + (int64_t)hb * a.bo_sh : nullptr;
+    }
+    it.kind = h < a.nrot ? (isa ? 1 : 2) : 0;
+    if (live) {
+      it.x0 = *(const C*)(x + 8 * c0);
+      it.x1 = *(const C*)(x + 8 * c1);
+    }
+    return it;
+  };
+  int i = threadIdx.x / LPH;
+  Item cur;
+  if (i < items) cur = load(i);
+  float* s_cos = sh;
+  float* s_sin = sh + TB * half;
+  for (int j = threadIdx.x; j < nt * half; j += kRotThreads) {
+    const int tok = j / half;
+    float c, s;
+    rot_angle(ll_load_idx(a.pos, t0 + tok, a.pos64), a.inv_freq[j - tok * half], a.factor, c, s);
+    s_cos[j] = c;
+    s_sin[j] = s;
+  }
+  __syncthreads();
+  // (the groups of a wave leave the loop together or one pass apart; a norm's
+  // shuffles stay inside a group)
+  for (; i < items; i += kGroups) {
+    Item next;
+    const bool more = i + kGroups < items;
+    if (more) next = load(i + kGroups);
+    if (cur.kind == 0) {
+      if (live && cur.y != nullptr) {
+        store_chunk(cur.y + 8 * c0, cur.x0);
+        store_chunk(cur.y + 8 * c1, cur.x1);
+      }
+    } else {
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = live ? ll_to_f32(cur.x0.v[e]) : 0.f;
+        x[8 + e] = live ? ll_to_f32(cur.x1.v[e]) : 0.f;
+      }
+      if constexpr (NORM) {
+        const T* g = (const T*)(cur.kind == 1 ? a.ga : a.gb);
+        if (g != nullptr) {
+          C g0, g1;
+          if (live) {
+            g0 = *(const C*)(g + 8 * c0);
+            g1 = *(const C*)(g + 8 * c1);
+          }
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
+#pragma unroll
+          for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+          const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = x[e] * r * ll_to_f32(g0.v[e]);
+            x[8 + e] = x[8 + e] * r * ll_to_f32(g1.v[e]);
+          }
+        }
+      }
+      if (live && cur.y != nullptr) {
+        float y[16];
+        const int at = cur.tok * half;
+        if constexpr (INTER) {
+          auto turn = [&](const float* z, float* w, bool rot, int p) {
+            if (rot) {
+              const f32x4 c = *(const f32x4*)(s_cos + at + p), s = *(const f32x4*)(s_sin + at + p);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[2 * e] = z[2 * e] * c[e] - z[2 * e + 1] * s[e];
+                w[2 * e + 1] = z[2 * e] * s[e] + z[2 * e + 1] * c[e];
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = z[e];
+            }
+          };
+          turn(x, y, rot0, p0);
+          turn(x + 8, y + 8, rot1, p1);
+        } else if (rot0) {
+          const f32x4 c4[2] = {*(const f32x4*)(s_cos + at + p0), *(const f32x4*)(s_cos + at + p1)};
+          const f32x4 s4[2] = {*(const f32x4*)(s_sin + at + p0), *(const f32x4*)(s_sin + at + p1)};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float c = c4[e >> 2][e & 3], s = s4[e >> 2][e & 3];
+            y[e] = x[e] * c - x[8 + e] * s;
+            y[8 + e] = x[e] * s + x[8 + e] * c;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] = x[e];
+        }
+        C o0, o1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          o0.v[e] = ll_from_f32<T>(y[e]);
+          o1.v[e] = ll_from_f32<T>(y[8 + e]);
+        }
+        store_chunk(cur.y + 8 * c0, o0);
+        store_chunk(cur.y + 8 * c1, o1);
+      }
+    }
+    if (more) cur = next;
+  }
+}
+
+template <typename T, int LPH>
+void launch_rotary_vec(const RotArgs& a, int interleaved, hipStream_t stream) {
+  const int heads = a.na + a.nb;
+  // tokens per workgroup: one until the grid fills the CUs eight times over,
+  // then up to 2 where a token's heads fill the workgroup's lanes, else 8
+  // (24,000 tokens, 28/4 heads of 128: 1 69.9 us, 2 68.0, 4 74.2, 8 80.1; 16/2
+  // heads with norms: 71.5, 57.3, 57.3, 55.5); LDS 32 KB at most
+  int tb = (int)std::min<int64_t>(heads * LPH >= kRotThreads ? 2 : 8,
+                                  std::max<int64_t>(1, a.ntok / 2048));
+  while (tb > 1 && tb * a.R * 4 > 32768) tb /= 2;
+  // i / heads = (i * mul) >> shift for i < tb * heads <= 2^19 / 8 * 8: with
+  // mul = ceil(2^shift / heads), exact while i * heads < 2^shift
+  int shift = 0;
+  while (((int64_t)1 << shift) < (int64_t)tb * heads * heads) ++shift;
+  const int mul = (int)((((int64_t)1 << shift) + heads - 1) / heads);
+  const unsigned grid = (unsigned)((a.ntok + tb - 1) / tb);
+  const size_t lds = (size_t)tb * a.R * 4;
+  const bool norm = a.ga != nullptr || a.gb != nullptr;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kRotThreads), lds, stream, a, tb, mul, shift);
+  };
+  if (norm) {
+    if (interleaved) go(rotary_vec_kernel<T, LPH, true, true>);
+    else go(rotary_vec_kernel<T, LPH, false, true>);
+  } else {
+    if (interleaved) go(rotary_vec_kernel<T, LPH, true, false>);
+    else go(rotary_vec_kernel<T, LPH, false, false>);
+  }
+}
+
+// Whether every head of the call can be read and written in 16-byte chunks.
+bool rotary_vec_ok(const RotArgs& a, int64_t es) {
+  if (a.D % 16 != 0 || a.D > 256 || a.R % 16 != 0) return false;
+  // (the division by multiplication holds for i * mul < 2^32)
+  const int64_t heads = a.na + a.nb;
+  if (8 * heads * heads >= (int64_t)1 << 24) return false;
+  int64_t strides = a.na ? a.a_st | a.a_sh | a.ao_st | a.ao_sh : 0;
+  uintptr_t at = a.na ? (uintptr_t)a.a | (uintptr_t)a.ao : 0;
+  if (a.nb) {
+    strides |= a.b_st | a.b_sh | a.bo_st | a.bo_sh;
+    at |= (uintptr_t)a.b | (uintptr_t)a.bo;
+  }
+  at |= (uintptr_t)a.ga | (uintptr_t)a.gb;
+  return (strides * es) % 16 == 0 && at % 16 == 0;
+}
+
 int launch_rotary(const char* fn, const RotArgs& a, int interleaved, int dtype,
                   hipStream_t stream) {
   LL_CHECK_ARG(a.D > 0 && a.D <= 1024 && a.R >= 0 && a.R <= a.D && a.R % 2 == 0,
@@ -101,7 +323,15 @@ int launch_rotary(const char* fn, const RotArgs& a, int interleaved, int dtype,
   if (a.na + a.nb == 0) return LL_OK;
   LL_CHECK_ARG(a.ntok < ((int64_t)1 << 31) && a.na + a.nb <= 65535,
                "%s: %lld tokens of %d heads unsupported", fn, (long long)a.ntok, a.na + a.nb);
+  const bool vec = rotary_vec_ok(a, dtype == LL_F32 ? 4 : 2);
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    if (vec) {
+      const int units = a.D / 16;
+      if (units <= 4) launch_rotary_vec<T, 4>(a, interleaved, stream);
+      else if (units <= 8) launch_rotary_vec<T, 8>(a, interleaved, stream);
+      else launch_rotary_vec<T, 16>(a, interleaved, stream);
+      LL_RETURN_LAUNCH();
+    }
     const dim3 grid((unsigned)a.ntok, (unsigned)(a.na + a.nb));
     if (interleaved)
       hipLaunchKernelGGL((rotary_kernel<T, true>), grid, dim3(64), 0, stream, a);
