@@ -769,6 +769,53 @@ typedef struct {
 } LLGemmCall;
 int64_t ll_call_gemm(const LLGemmCall* c);
 
+typedef struct {
+  int64_t q, q_stride_tok, q_stride_h, k_cache, k_stride_tok, k_stride_head, v_cache, v_stride_tok,
+      v_stride_head, out, out_stride_tok, out_stride_h, req_to_tokens, req_to_tokens_stride,
+      b_req_idx, req_idx_i64, b_start_loc, start_loc_i64, b_seq_len, seq_len_i64, b_shared_seq_len,
+      shared_i64, batch, q_heads, kv_heads, head_dim, max_input_len, window, sinks;
+  double sm_scale;
+  int64_t dtype, stream;
+} LLWindowPrefillAttentionCall;
+int64_t ll_call_window_prefill_attention(const LLWindowPrefillAttentionCall* c);
+
+typedef struct {
+  int64_t q, q_stride_b, q_stride_h, k_cache, k_stride_tok, k_stride_head, v_cache, v_stride_tok,
+      v_stride_head, req_to_tokens, req_to_tokens_stride, b_req_idx, req_idx_i64, b_seq_len,
+      seq_len_i64, out, out_stride_b, out_stride_h, batch, q_heads, kv_heads, head_dim,
+      max_len_in_batch, window, sinks;
+  double sm_scale;
+  int64_t dtype, workspace, workspace_bytes, stream;
+} LLWindowDecodeAttentionCall;
+int64_t ll_call_window_decode_attention(const LLWindowDecodeAttentionCall* c);
+
+typedef struct {
+  int64_t q, q_stride_tok, q_stride_h, q_out, q_out_stride_tok, q_out_stride_h, q_heads, k,
+      k_stride_tok, k_stride_h, k_out, k_out_stride_tok, k_out_stride_h, k_heads, positions,
+      positions_i64, inv_freq, rotary_dim, interleaved;
+  double factor;
+  int64_t ntok, head_dim, dtype, stream;
+} LLRopePositionsCall;
+int64_t ll_call_rope_positions(const LLRopePositionsCall* c);
+
+typedef struct {
+  int64_t qkv, qkv_row_stride, ntok, q_heads, kv_heads, head_dim, q_out, q_out_stride_tok,
+      q_out_stride_h, q_gamma, k_gamma;
+  double eps;
+  int64_t positions, positions_i64, inv_freq, rotary_dim, interleaved;
+  double factor;
+  int64_t slots, pool_layer, pool_slot_stride, pool_head_stride, pool_slots, dtype, stream;
+} LLQkNormRopeKvScatterCall;
+int64_t ll_call_qk_norm_rope_kv_scatter(const LLQkNormRopeKvScatterCall* c);
+
+typedef struct {
+  int64_t b_req_idx, req_idx_i64, b_seq_len, seq_len_i64, b_cached_len, cached_len_i64, batch,
+      free_pages, n_free, page_size, block_table, block_table_stride, block_table_cols,
+      req_to_tokens, req_to_tokens_stride, req_rows, max_len, slots, positions, max_tokens,
+      b_start_loc, last_rows, counts, stream;
+} LLBuildSlotMapsCall;
+int64_t ll_call_build_slot_maps(const LLBuildSlotMapsCall* c);
+
 #ifdef __cplusplus
 }
 #endif

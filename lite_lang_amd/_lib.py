@@ -24,6 +24,11 @@ RMSNORM_CALL = struct.Struct("=9qd2q")
 DECODE_ATTENTION_CALL = struct.Struct("=23qd4q")
 PREFILL_ATTENTION_CALL = struct.Struct("=27qd2q")
 GEMM_CALL = struct.Struct("=15q")
+WINDOW_PREFILL_ATTENTION_CALL = struct.Struct("=29qd2q")
+WINDOW_DECODE_ATTENTION_CALL = struct.Struct("=25qd4q")
+ROPE_POSITIONS_CALL = struct.Struct("=19qd4q")
+QK_NORM_ROPE_KV_SCATTER_CALL = struct.Struct("=11qd5qd7q")
+BUILD_SLOT_MAPS_CALL = struct.Struct("=24q")
 
 # name -> (restype, argtypes), mirroring include/litelang_amd.h
 SIGNATURES = {
@@ -144,6 +149,11 @@ SIGNATURES = {
     "ll_call_decode_attention": (I64, [ctypes.c_char_p]),
     "ll_call_prefill_attention": (I64, [ctypes.c_char_p]),
     "ll_call_gemm": (I64, [ctypes.c_char_p]),
+    "ll_call_window_prefill_attention": (I64, [ctypes.c_char_p]),
+    "ll_call_window_decode_attention": (I64, [ctypes.c_char_p]),
+    "ll_call_rope_positions": (I64, [ctypes.c_char_p]),
+    "ll_call_qk_norm_rope_kv_scatter": (I64, [ctypes.c_char_p]),
+    "ll_call_build_slot_maps": (I64, [ctypes.c_char_p]),
 }
 
 

@@ -128,6 +128,25 @@ __device__ __forceinline__ WindowRange window_range(int64_t first, int window, i
   return {sinks, (int)low};
 }
 
+// One step of a prefix operation over the lanes of a wave, by data-parallel
+// moves (a shuffle through LDS takes ten times as long): v of the lane that
+// CTRL names, `id` where there is none or ROWS leaves the row out.
+template <int CTRL, int ROWS> __device__ __forceinline__ int lane_move(int id, int v) {
+  return __builtin_amdgcn_update_dpp(id, v, CTRL, ROWS, 0xf, false);
+}
+// Inclusive prefix op over the 64 lanes: within rows of 16 (row_shr 1, 2, 4, 8),
+// then the last lane of a row into the next row, and of the first two rows
+// into the others (row_bcast 15 and 31).
+template <typename Op> __device__ __forceinline__ int lane_scan(int v, int id, Op op) {
+  v = op(v, lane_move<0x111, 0xf>(id, v));
+  v = op(v, lane_move<0x112, 0xf>(id, v));
+  v = op(v, lane_move<0x114, 0xf>(id, v));
+  v = op(v, lane_move<0x118, 0xf>(id, v));
+  v = op(v, lane_move<0x142, 0xa>(id, v));
+  v = op(v, lane_move<0x143, 0xc>(id, v));
+  return v;
+}
+
 template <int D> struct FaGeom {
   static constexpr int ROWB = D * 2;            // bytes of a K or V row
   static constexpr int CH = ROWB / 16;          // 16 B chunks per row
@@ -197,6 +216,12 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   constexpr int DB = D / 32;  // 32-row d blocks of O^T
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
+  auto rl = [&](int v, int k) -> int { return __builtin_amdgcn_readlane(v, k); };
+  auto shfl64 = [&](int64_t v, int k) -> int64_t {
+    const uint32_t lo = (uint32_t)__shfl((int)(uint64_t)v, k, 64);
+    const uint32_t hi = (uint32_t)__shfl((int)((uint64_t)v >> 32), k, 64);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+  };
   const int HP = (G + SH::HPW - 1) / SH::HPW;  // head groups per KV head
   const int P = (int)gridDim.x, w = (int)blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -211,7 +236,121 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   int it_low = 0, it_sk = 0;  // WIN: first key of the window's tiles, sinks apart from them
   int64_t it_start = 0, it_rid = 0;
   bool it_ok = false;
-  {
+  if constexpr (WIN) {
+    // The windowed form's items are those that exist, the costly first (a
+    // grid over all row blocks up to the longest length deals out the missing
+    // blocks of shorter requests and of cached prefixes along with the real
+    // ones: 5 x 4111 tokens, 60% cached, 28/4 heads: 70 tiles for the busiest
+    // workgroup, 54 so). 64 requests at a time, one per lane: the blocks whose
+    // window is whole, all alike in cost, request after request; then those
+    // nearer their context's start by level, the multiple of BQ that their
+    // first position is at or above, the highest level first.
+    const int64_t vb = fa_item_of_pass(lane, P, w);
+    const int ui = vb < nv ? ((int)(vb >> 3) / HP) * 8 + (int)(vb & 7) : 0;
+    const int want = vb < nv ? ui / KVH : INT32_MAX;  // the lane's (request, block) in that order
+    it_kvh = ui % KVH;
+    it_hp = vb < nv ? (int)(vb >> 3) % HP : 0;
+    const int lam = (a.window + SH::BQ - 1) / SH::BQ;  // level from which the window is whole
+    auto scan = [&](int v) { return lane_scan(v, 0, [](int x, int y) { return x + y; }); };
+    auto highest = [&](int v) {
+      return rl(lane_scan(v, INT32_MIN, [](int x, int y) { return max(x, y); }), 63);
+    };
+    // the first lane whose prefix sum exceeds v
+    auto find = [&](int incl, int v) {
+      int at = 0;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1)
+        if (__shfl(incl, at + o - 1, 64) <= v) at += o;
+      return min(at, 63);
+    };
+    int base = 0;  // (request, block)s listed so far
+    for (int c0 = 0; c0 < B; c0 += 64) {
+      const int b = min(c0 + lane, B - 1), nreq = min(B - c0, 64);
+      const int64_t Lb = ll_load_idx(p_len, b, idx64 & 1);
+      const int64_t Sb = p_shared ? ll_load_idx(p_shared, b, (idx64 >> 1) & 1) : 0;
+      const int64_t start_b = ll_load_idx(p_start, b, (idx64 >> 2) & 1);
+      const int64_t rid_b = ll_load_idx(p_rid, b, (idx64 >> 3) & 1);
+      const int L = (int)Lb, S = (int)Sb;
+      // its blocks, the levels of the first `ramp` of them, the number of whole ones
+      const int nb = lane < nreq && Lb > Sb ? (L - S + SH::BQ - 1) / SH::BQ : 0;
+      const int l0 = S / SH::BQ;
+      const int ramp = min(nb, max(0, lam - l0)), full = nb - ramp;
+      int src = -1, blk = 0;  // lane's request (as a lane number) and row block
+      if (nreq == 1) {  // one request: its blocks from the last
+        const int n = rl(nb, 0), rel = want - base;
+        if (rel >= 0 && rel < n) {
+          src = 0;
+          blk = n - 1 - rel;
+        }
+        base += n;
+      } else {
+        const int incl = scan(full);
+        const int total = rl(incl, 63), rel = want - base;
+        base += total;
+        if (total > 0) {
+          const int at = find(incl, rel);
+          const int before = __shfl(incl - full, at, 64), last = __shfl(nb, at, 64) - 1;
+          if (rel >= 0 && rel < total) {
+            src = at;
+            blk = last - (rel - before);
+          }
+        }
+        // levels 64 at a time, level hi - i in lane i: the requests that have
+        // it, as the prefix sum of +1 where a request's levels begin and -1
+        // behind their end (in the wave's slot ring, not in use yet)
+        int* edge = (int*)(smem + kStages * FG::STAGE_B + wave * (kStages * kBK * 4));
+        const int top = highest(ramp > 0 ? l0 + ramp - 1 : -1);
+        const int bot = -highest(ramp > 0 ? -l0 : -INT32_MAX);
+        for (int hi = top; hi >= bot; hi -= 64) {
+          const int i0 = hi - (l0 + ramp - 1), i1 = hi - l0 + 1;
+          edge[lane] = 0;
+          if (ramp > 0 && i1 > 0 && i0 < 64) {
+            atomicAdd(&edge[max(i0, 0)], 1);
+            if (i1 < 64) atomicAdd(&edge[i1], -1);
+          }
+          const int cnt = scan(edge[lane]), lincl = scan(cnt);
+          const int ltotal = rl(lincl, 63), lrel = want - base;
+          base += ltotal;
+          const bool mine = lrel >= 0 && lrel < ltotal;
+          uint64_t left = __builtin_amdgcn_ballot_w64(mine);
+          if (!left) continue;
+          const int at = find(lincl, lrel);
+          const int nth = lrel - __shfl(lincl - cnt, at, 64);  // of the requests with that level
+          while (left) {  // a workgroup's few items of these levels
+            const int i = (int)__builtin_ctzll(left);
+            left &= left - 1;
+            const int d = hi - rl(at, i) - l0;
+            const uint64_t has = __builtin_amdgcn_ballot_w64((unsigned)d < (unsigned)ramp);
+            const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
+                                                       __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+            const uint64_t it = __builtin_amdgcn_ballot_w64((unsigned)d < (unsigned)ramp &&
+                                                            rank == rl(nth, i));
+            const int r = (int)__builtin_ctzll(it);
+            if (lane == i) {
+              src = r;
+              blk = rl(d, r);
+            }
+          }
+        }
+      }
+      const int from = max(src, 0);
+      const int Lx = __shfl(L, from, 64), Sx = __shfl(S, from, 64);
+      const int64_t startx = shfl64(start_b, from), ridx = shfl64(rid_b, from);
+      if (src >= 0) {
+        it_ok = true;
+        it_L = Lx;
+        it_S = Sx;
+        it_start = startx;
+        it_rid = ridx;
+        it_blk0 = blk * SH::BQ;
+        it_kvend = (int)min((int64_t)Lx, (int64_t)it_blk0 + SH::BQ + Sx);
+        const WindowRange r = window_range((int64_t)it_blk0 + Sx, a.window, a.sinks);
+        it_low = r.low;
+        it_sk = r.sinks;
+        it_nt = (it_sk + kBK - 1) / kBK + (it_kvend - it_low + kBK - 1) / kBK;
+      }
+    }
+  } else {
     const int64_t vb = fa_item_of_pass(lane, P, w);  // vb >= nv for every pass past the last
     const int units = nblk * B * KVH;
     if (vb < nv && ((int)(vb >> 3) / HP) * 8 + (int)(vb & 7) < units) {
@@ -231,12 +370,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
         it_blk0 = (int)blk0;
         it_kvend = (int)min(L, blk0 + SH::BQ + S);  // keys of the item
         it_nt = (it_kvend + kBK - 1) / kBK;
-        if constexpr (WIN) {
-          const WindowRange r = window_range(blk0 + S, a.window, a.sinks);
-          it_low = r.low;
-          it_sk = r.sinks;
-          it_nt = (it_sk + kBK - 1) / kBK + (it_kvend - it_low + kBK - 1) / kBK;
-        }
         it_kvh = unit % KVH;
         it_hp = (int)(vb >> 3) % HP;
       }
@@ -252,7 +385,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     const uint64_t rest = k >= 63 ? 0 : items & (~(uint64_t)0 << (k + 1));
     return rest ? (int)__builtin_ctzll(rest) : 64;
   };
-  auto rl = [&](int v, int k) -> int { return __builtin_amdgcn_readlane(v, k); };
   auto rl64 = [&](int64_t v, int k) -> int64_t {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint64_t)v, k);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)((uint64_t)v >> 32), k);
@@ -476,7 +608,11 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = 32 * kb + 8 * (e >> 2) + 4 * hf + (e & 3);
-            if (key > lim || (WIN && key <= below && key >= sink)) sacc[kb][qb][e] = -INFINITY;
+            // (bitwise: with && and || the compiler branches around every
+            // element, 130 -> 122 us at 40 x 600, window 256, 16/2 heads)
+            bool hide = key > lim;
+            if constexpr (WIN) hide |= (key <= below) & (key >= sink);
+            sacc[kb][qb][e] = hide ? -INFINITY : sacc[kb][qb][e];
           }
       }
       float tmax = -INFINITY;
@@ -540,23 +676,39 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       }
     }
   };
-  // acc[db][qb][4 g + i] = O^T[d = 32 db + 8 g + 4 hf + i][query row0 + 32 qb + l32]
+  // acc[db][qb][4 g + i] = O^T[d = 32 db + 8 g + 4 hf + i][query row0 + 32 qb + l32].
+  // The halves of a row (lanes l and l + 32) swap 4-element groups, so that
+  // each stores 8 elements of it at a time: half the store instructions, whose
+  // 32 rows each take the memory path about 50 cycles (40 x 600, window 256,
+  // 16/2 heads: 122 -> 114 us; the same rows as whole lines through LDS: 118).
   auto store_rows = [&](const WaveItem& it) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int r = it.row0 + 32 * qb + l32;
-      if (r > it.qlast) continue;
+      if (r > it.qlast) continue;  // the same in both halves
       const float inv = 1.0f / (l_run[qb] + __shfl_xor(l_run[qb], 32, 64));
-      T* op = (T*)a.o + (it.start + r) * a.o_st + (int64_t)it.h * a.o_sh + 4 * hf;
+      T* op = (T*)a.o + (it.start + r) * a.o_st + (int64_t)it.h * a.o_sh + 8 * hf;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 y;
+        for (int g = 0; g < 4; g += 2) {
+          T4 y0, y1;  // d = 32 db + 8 g + 4 hf + i, and 8 further
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = ll_from_f32<T>(acc[db][qb][4 * g + i] * inv);
-          *(T4*)(op + 32 * db + 8 * g) = y;
+          for (int i = 0; i < 4; ++i) {
+            y0[i] = ll_from_f32<T>(acc[db][qb][4 * g + i] * inv);
+            y1[i] = ll_from_f32<T>(acc[db][qb][4 * g + 4 + i] * inv);
+          }
+          const U2 u0 = __builtin_bit_cast(U2, y0), u1 = __builtin_bit_cast(U2, y1);
+          u32x4 w;  // lower half: d = 32 db + 8 g .. + 7, upper: 8 further
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const auto p = __builtin_amdgcn_permlane32_swap(u0[i], u1[i], false, false);
+            w[i] = p[0];
+            w[2 + i] = p[1];
+          }
+          *(u32x4*)(op + 32 * db + 8 * g) = w;
         }
     }
   };
@@ -786,8 +938,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  // (its rows are stored 8 bytes at a time)
-  const bool out_ok = out_stride_tok % 4 == 0 && out_stride_h % 4 == 0 && (uintptr_t)out % 8 == 0;
+  // (its rows are stored 16 bytes at a time; a causal call's may be anywhere)
+  const bool out_ok = out_stride_tok % 8 == 0 && out_stride_h % 8 == 0 && (uintptr_t)out % 16 == 0;
   if (!mfma_ok || (win && !out_ok)) {
     LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535, "%s: more than 65535 heads or requests", fn);
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 4;

@@ -8,6 +8,7 @@ computes on the host; a missing library raises at import.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -47,21 +48,19 @@ def _dev(*ts: torch.Tensor) -> None:
             raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
 
 
-def _here(*ts) -> None:
-    """Raises unless all of `ts` (None skipped) sit on the current device: a
-    launch goes to that device's stream."""
-    idx = None
+def _here(*ts) -> int:
+    """The current stream, after checking that all of `ts` (None skipped) sit on
+    the current device: a launch goes to that device's stream."""
+    idx = ts[0].get_device()
     for t in ts:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
-            raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
-        if idx is None:
-            idx = torch._C._cuda_getDevice()
-        if at != idx:
-            raise ValueError(f"lite_lang_amd ops need tensors of the current device (cuda:{idx}), "
-                             f"got {t.device}")
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"lite_lang_amd ops need tensors of one device (got {ts[0].device} "
+                             f"and {t.device})")
+    if idx < 0:
+        raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
+    if idx != torch._C._cuda_getDevice():
+        raise ValueError(f"lite_lang_amd ops run on the current device (got cuda:{idx} tensors)")
+    return _raw_stream(idx)
 
 
 def _call(fn, rec, fields, name, ws_name, ws_at, t):
@@ -241,15 +240,22 @@ def prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_input_l
 
 
 def _window_checks(q, cache_k, cache_v, out, req_to_tokens, window, sinks):
-    D = q.shape[2]
-    assert cache_k.shape[-1] == D and cache_v.shape == cache_k.shape and out.shape == q.shape
-    assert q.shape[1] % cache_k.shape[1] == 0
-    assert q.dtype == cache_k.dtype == cache_v.dtype == out.dtype
-    assert q.stride(2) == 1 and cache_k.stride(2) == 1 and cache_v.stride(2) == 1
-    assert out.stride(2) == 1
-    assert req_to_tokens.dtype == torch.int32 and req_to_tokens.stride(1) == 1
+    """Shapes and strides of a windowed call; returns what its record needs of them."""
+    shape, kshape, dt = q.shape, cache_k.shape, q.dtype
+    _, H, D = shape
+    assert kshape[2] == D and cache_v.shape == kshape and out.shape == shape
+    assert H % kshape[1] == 0
+    assert dt == cache_k.dtype and dt == cache_v.dtype and dt == out.dtype
+    qs, ks, vs, os_ = q.stride(), cache_k.stride(), cache_v.stride(), out.stride()
+    assert qs[2] == 1 and ks[2] == 1 and vs[2] == 1 and os_[2] == 1
+    ts = req_to_tokens.stride()
+    assert req_to_tokens.dtype == torch.int32 and ts[1] == 1
     if window < 1 or sinks < 0:
         raise ValueError(f"window {window} must be at least 1 and sinks {sinks} at least 0")
+    return shape, kshape[1], qs, ks, vs, os_, ts[0]
+
+
+_I62 = 1 << 62  # more than any length, and an int64 (a larger window or count sees as much)
 
 
 def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_input_len,
@@ -257,58 +263,61 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
     """prefill_attention in which the query at position p sees the keys n <= p
     with n > p - window or n < sinks. Slot-table entries of keys that no query
     of the call sees are not read, so those tokens may have left the cache."""
-    _window_checks(q, k, v, o, req_to_tokens, window, sinks)
-    T, H, D = q.shape
-    B = b_seq_len.shape[0]
-    assert b_req_idx.shape == (B,) and b_start_loc.shape == (B,)
+    (T, H, D), KVH, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window, sinks)
+    bs = b_seq_len.shape
+    assert len(bs) == 1 and b_req_idx.shape == bs and b_start_loc.shape == bs
     assert b_req_idx.is_contiguous() and b_start_loc.is_contiguous() and b_seq_len.is_contiguous()
     sh_ptr, sh64 = 0, 0
     if b_shared_seq_len is not None:
-        assert b_shared_seq_len.shape == (B,) and b_shared_seq_len.is_contiguous()
+        assert b_shared_seq_len.shape == bs and b_shared_seq_len.is_contiguous()
         sh_ptr, sh64 = b_shared_seq_len.data_ptr(), _idx(b_shared_seq_len, "b_shared_seq_len")
-    _here(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, req_to_tokens, b_shared_seq_len)
-    if sm_scale is None:
-        sm_scale = 1.0 / (D ** 0.5)
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), o.stride()
-    rc = _L.ll_window_prefill_attention(
+    stream = _here(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, req_to_tokens, b_shared_seq_len)
+    rc = _L.ll_call_window_prefill_attention(_lib.WINDOW_PREFILL_ATTENTION_CALL.pack(
         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-        o.data_ptr(), os_[0], os_[1], req_to_tokens.data_ptr(), req_to_tokens.stride(0),
+        o.data_ptr(), os_[0], os_[1], req_to_tokens.data_ptr(), ts,
         b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
         b_start_loc.data_ptr(), _idx(b_start_loc, "b_start_loc"),
         b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), sh_ptr, sh64,
-        B, H, k.shape[1], D, int(max_input_len), int(window), int(sinks), float(sm_scale),
-        dtype_code(q), _stream(q))
-    _lib.check(rc, "ll_window_prefill_attention")
+        bs[0], H, KVH, D, max_input_len, min(window, _I62), min(sinks, _I62),
+        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, dtype_code(q), stream))
+    if rc:
+        _lib.check(rc, "ll_window_prefill_attention")
     return o
 
 
 def window_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_batch, cache_k,
                             cache_v, out, window, sinks=0, sm_scale=None):
     """decode_attention over the last `window` tokens and the first `sinks` ones."""
-    _window_checks(q, cache_k, cache_v, out, req_to_tokens, window, sinks)
-    B, H, D = q.shape
-    KVH = cache_k.shape[1]
+    (B, H, D), KVH, qs, ks, vs, os_, ts = _window_checks(q, cache_k, cache_v, out, req_to_tokens,
+                                                         window, sinks)
     assert b_req_idx.shape == (B,) and b_seq_len.shape == (B,)
     assert b_req_idx.is_contiguous() and b_seq_len.is_contiguous()
-    _here(q, req_to_tokens, b_req_idx, b_seq_len, cache_k, cache_v, out)
-    if sm_scale is None:
-        sm_scale = 1.0 / (D ** 0.5)
-    max_len, window, sinks = int(max_len_in_batch), int(window), int(sinks)
-    # A buffer of the call's own, not the stream's persistent workspace: under
-    # capture it comes from the graph's memory, so graphs replayed at the same
-    # time share nothing.
-    need = _L.ll_window_decode_attention_workspace_size(B, H, KVH, D, max_len, window, sinks)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    qs, ks, vs, os_ = q.stride(), cache_k.stride(), cache_v.stride(), out.stride()
-    rc = _L.ll_window_decode_attention(
+    stream = _here(q, req_to_tokens, b_req_idx, b_seq_len, cache_k, cache_v, out)
+    window, sinks = min(window, _I62), min(sinks, _I62)
+    # Under capture a buffer of the call's own, from the graph's memory, so that
+    # graphs replayed at the same time share nothing; else the stream's.
+    need = _window_decode_bytes(B, H, KVH, D, max_len_in_batch, window, sinks)
+    ws = None
+    if need > 0:
+        if torch._C._cuda_isCurrentStreamCapturing():
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        else:
+            ws = workspace(q.device, "window_decode", need)
+    rc = _L.ll_call_window_decode_attention(_lib.WINDOW_DECODE_ATTENTION_CALL.pack(
         q.data_ptr(), qs[0], qs[1], cache_k.data_ptr(), ks[0], ks[1], cache_v.data_ptr(), vs[0],
-        vs[1], req_to_tokens.data_ptr(), req_to_tokens.stride(0),
-        b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
+        vs[1], req_to_tokens.data_ptr(), ts, b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
         b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), out.data_ptr(), os_[0], os_[1],
-        B, H, KVH, D, max_len, window, sinks, float(sm_scale), dtype_code(q),
-        ws.data_ptr() if ws is not None else None, need, _stream(q))
-    _lib.check(rc, "ll_window_decode_attention")
+        B, H, KVH, D, max_len_in_batch, window, sinks,
+        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, dtype_code(q),
+        0 if ws is None else ws.data_ptr(), need, stream))
+    if rc:
+        _lib.check(rc, "ll_window_decode_attention")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_decode_bytes(*shape):
+    return _L.ll_window_decode_attention_workspace_size(*shape)
 
 
 # ------------------------------------------------------------------ elementwise
@@ -427,9 +436,12 @@ def rope_frequencies(rotary_dim, theta=1e6, scaling=None, max_position=None, len
 
 
 def _rope_checks(positions, inv_freq, T, D):
+    """The rotated part of a head's D elements."""
     assert positions.shape == (T,) and positions.is_contiguous()
-    assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.ndim == 1
-    assert 2 * inv_freq.shape[0] <= D, "more rotated pairs than the head has"
+    (n,) = inv_freq.shape
+    assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
+    assert 2 * n <= D, "more rotated pairs than the head has"
+    return 2 * n
 
 
 def rope_positions(q, k, positions, inv_freq, interleaved=False, factor=1.0, q_out=None,
@@ -441,24 +453,23 @@ def rope_positions(q, k, positions, inv_freq, interleaved=False, factor=1.0, q_o
     rope_frequencies)."""
     q_out = q if q_out is None else q_out
     k_out = k if k_out is None else k_out
-    T, Hq, D = q.shape
-    assert q.stride(2) == 1 and q_out.stride(2) == 1 and q_out.shape == q.shape
-    assert q_out.dtype == q.dtype
-    _rope_checks(positions, inv_freq, T, D)
-    kargs = (None, 0, 0, None, 0, 0, 0)
+    shape, dt, qs, qos = q.shape, q.dtype, q.stride(), q_out.stride()
+    T, Hq, D = shape
+    assert qs[2] == 1 and qos[2] == 1 and q_out.shape == shape and q_out.dtype == dt
+    R = _rope_checks(positions, inv_freq, T, D)
+    kargs = (0, 0, 0, 0, 0, 0, 0)
     if k is not None:
-        assert k.shape[0] == T and k.shape[2] == D and k.dtype == q.dtype
-        assert k.stride(2) == 1 and k_out.stride(2) == 1
-        assert k_out.shape == k.shape and k_out.dtype == k.dtype
-        ks, kos = k.stride(), k_out.stride()
-        kargs = (k.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], k.shape[1])
-    _here(q, k, positions, inv_freq, q_out, k_out)
-    qs, qos = q.stride(), q_out.stride()
-    rc = _L.ll_rope_positions(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], Hq,
-                              *kargs, positions.data_ptr(), _idx(positions, "positions"),
-                              inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(bool(interleaved)),
-                              float(factor), T, D, dtype_code(q), _stream(q))
-    _lib.check(rc, "ll_rope_positions")
+        kshape, ks, kos = k.shape, k.stride(), k_out.stride()
+        assert kshape[0] == T and kshape[2] == D and k.dtype == dt and k_out.dtype == dt
+        assert ks[2] == 1 and kos[2] == 1 and k_out.shape == kshape
+        kargs = (k.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], kshape[1])
+    stream = _here(q, k, positions, inv_freq, q_out, k_out)
+    rc = _L.ll_call_rope_positions(_lib.ROPE_POSITIONS_CALL.pack(
+        q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], Hq, *kargs,
+        positions.data_ptr(), _idx(positions, "positions"), inv_freq.data_ptr(), R,
+        bool(interleaved), factor, T, D, dtype_code(q), stream))
+    if rc:
+        _lib.check(rc, "ll_rope_positions")
     return q_out, k_out
 
 
@@ -470,27 +481,28 @@ def qk_norm_rope_kv_scatter(qkv, q_heads, kv_heads, head_dim, q_gamma, k_gamma, 
     q into q_out [T, q_heads, head_dim] (None: in place in qkv), K and V to
     pool_layer[slots]. A slot outside the pool marks a padded token, whose K and
     V go nowhere. Returns q [T, q_heads, head_dim]."""
-    T, D = qkv.shape[0], head_dim
-    assert qkv.stride(1) == 1 and qkv.shape[1] == (q_heads + 2 * kv_heads) * D
+    T, width = qkv.shape
+    D, dt, xs = head_dim, qkv.dtype, qkv.stride()
+    assert xs[1] == 1 and width == (q_heads + 2 * kv_heads) * D
     if q_out is None:
-        q_out = qkv[:, : q_heads * D].view(T, q_heads, D)
-    assert q_out.shape == (T, q_heads, D) and q_out.stride(2) == 1 and q_out.dtype == qkv.dtype
+        q_out = qkv[:, : q_heads * D].unflatten(1, (q_heads, D))
+    qos, pshape, ps = q_out.stride(), pool_layer.shape, pool_layer.stride()
+    assert q_out.shape == (T, q_heads, D) and qos[2] == 1 and q_out.dtype == dt
     assert slots.dtype == torch.int32 and slots.shape == (T,) and slots.is_contiguous()
-    assert pool_layer.shape[1:] == (2 * kv_heads, D) and pool_layer.stride(2) == 1
-    assert pool_layer.dtype == qkv.dtype
+    assert pshape[1] == 2 * kv_heads and pshape[2] == D and ps[2] == 1 and pool_layer.dtype == dt
+    R = _rope_checks(positions, inv_freq, T, D)
+    gammas = []
     for g in (q_gamma, k_gamma):
-        assert g is None or (g.shape == (D,) and g.is_contiguous() and g.dtype == qkv.dtype)
-    _rope_checks(positions, inv_freq, T, D)
-    _here(qkv, q_gamma, k_gamma, positions, inv_freq, slots, pool_layer, q_out)
-    qos, ps = q_out.stride(), pool_layer.stride()
-    rc = _L.ll_qk_norm_rope_kv_scatter(
-        qkv.data_ptr(), qkv.stride(0), T, q_heads, kv_heads, D, q_out.data_ptr(), qos[0], qos[1],
-        q_gamma.data_ptr() if q_gamma is not None else None,
-        k_gamma.data_ptr() if k_gamma is not None else None, float(eps), positions.data_ptr(),
-        _idx(positions, "positions"), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
-        int(bool(interleaved)), float(factor), slots.data_ptr(), pool_layer.data_ptr(), ps[0],
-        ps[1], pool_layer.shape[0], dtype_code(qkv), _stream(qkv))
-    _lib.check(rc, "ll_qk_norm_rope_kv_scatter")
+        assert g is None or (g.shape == (D,) and g.is_contiguous() and g.dtype == dt)
+        gammas.append(0 if g is None else g.data_ptr())
+    stream = _here(qkv, q_gamma, k_gamma, positions, inv_freq, slots, pool_layer, q_out)
+    rc = _L.ll_call_qk_norm_rope_kv_scatter(_lib.QK_NORM_ROPE_KV_SCATTER_CALL.pack(
+        qkv.data_ptr(), xs[0], T, q_heads, kv_heads, D, q_out.data_ptr(), qos[0], qos[1], *gammas,
+        eps, positions.data_ptr(), _idx(positions, "positions"), inv_freq.data_ptr(), R,
+        bool(interleaved), factor, slots.data_ptr(), pool_layer.data_ptr(), ps[0], ps[1],
+        pshape[0], dtype_code(qkv), stream))
+    if rc:
+        _lib.check(rc, "ll_qk_norm_rope_kv_scatter")
     return q_out
 
 
@@ -760,34 +772,38 @@ def build_slot_maps(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_token
     word is 0, or, with nothing but counts written, the sum of 1: a length out
     of range, 2: a bad or repeated row, 4: more tokens than `slots` holds, 8:
     too few free pages."""
-    B = b_req_idx.shape[0]
+    bs, i32 = b_req_idx.shape, torch.int32
+    assert len(bs) == 1
     for t in (b_req_idx, b_seq_len, b_cached_len, b_start_loc, last_rows):
-        assert t.shape == (B,) and t.is_contiguous()
+        assert t.shape == bs and t.is_contiguous()
     for t in (free_pages, req_to_tokens, slots, positions, b_start_loc, last_rows, counts):
-        assert t.dtype == torch.int32
-    assert free_pages.ndim == 1 and free_pages.is_contiguous()
-    assert slots.ndim == 1 and slots.is_contiguous()
-    assert positions.shape == slots.shape and positions.is_contiguous()
-    assert counts.shape == (3,) and counts.is_contiguous()
-    assert req_to_tokens.ndim == 2 and req_to_tokens.stride(1) == 1
-    if page_size < 1 or (page_size > 1 and block_table is None):
-        raise ValueError(f"page_size {page_size} needs a block table" if page_size > 1 else
-                         f"page_size {page_size} must be at least 1")
-    bt = (None, 0, 0)
-    if page_size > 1:
-        assert block_table.dtype == torch.int32 and block_table.ndim == 2
-        assert block_table.stride(1) == 1 and block_table.shape[0] == req_to_tokens.shape[0]
-        bt = (block_table.data_ptr(), block_table.stride(0), block_table.shape[1])
-    _here(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_tokens, slots, positions,
-          b_start_loc, last_rows, counts, block_table)
-    rc = _L.ll_build_slot_maps(
+        assert t.dtype == i32
+    assert free_pages.ndim == 1 and slots.ndim == 1 and req_to_tokens.ndim == 2
+    n_free, n_tokens, (rows, cols) = free_pages.shape[0], slots.shape[0], req_to_tokens.shape
+    assert free_pages.is_contiguous() and slots.is_contiguous() and positions.is_contiguous()
+    assert positions.shape == (n_tokens,) and counts.shape == (3,) and counts.is_contiguous()
+    ts = req_to_tokens.stride()
+    assert ts[1] == 1
+    bt = (0, 0, 0)
+    if page_size != 1:
+        if page_size < 1:
+            raise ValueError(f"page_size {page_size} must be at least 1")
+        if block_table is None:
+            raise ValueError(f"page_size {page_size} needs a block table")
+        bshape, bstride = block_table.shape, block_table.stride()
+        assert block_table.dtype == i32 and len(bshape) == 2
+        assert bstride[1] == 1 and bshape[0] == rows
+        bt = (block_table.data_ptr(), bstride[0], bshape[1])
+    stream = _here(counts, b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_tokens, slots,
+                   positions, b_start_loc, last_rows, block_table)
+    rc = _L.ll_call_build_slot_maps(_lib.BUILD_SLOT_MAPS_CALL.pack(
         b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(),
         _idx(b_seq_len, "b_seq_len"), b_cached_len.data_ptr(), _idx(b_cached_len, "b_cached_len"),
-        B, free_pages.data_ptr(), free_pages.shape[0], page_size, *bt, req_to_tokens.data_ptr(),
-        req_to_tokens.stride(0), req_to_tokens.shape[0], req_to_tokens.shape[1], slots.data_ptr(),
-        positions.data_ptr(), slots.shape[0], b_start_loc.data_ptr(), last_rows.data_ptr(),
-        counts.data_ptr(), _stream(counts))
-    _lib.check(rc, "ll_build_slot_maps")
+        bs[0], free_pages.data_ptr(), n_free, page_size, *bt, req_to_tokens.data_ptr(), ts[0], rows,
+        cols, slots.data_ptr(), positions.data_ptr(), n_tokens, b_start_loc.data_ptr(),
+        last_rows.data_ptr(), counts.data_ptr(), stream))
+    if rc:
+        _lib.check(rc, "ll_build_slot_maps")
 
 
 # ------------------------------------------------------------------ decode split-K path
