@@ -99,6 +99,28 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// Wait until at most LEFT of this wave's LDS reads are in flight (they complete
+// in order); the values pass through the wait, as in ll_lds_wait_tie.
+template <int LEFT> __device__ __forceinline__ void lds_wait_tie(s16x4 (&v)[8]) {
+  asm volatile("s_waitcnt lgkmcnt(%8)"
+               : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]),
+                 "+v"(v[6]), "+v"(v[7])
+               : "n"(LEFT)
+               : "memory");
+}
+template <int LEFT> __device__ __forceinline__ void lds_wait_tie(s16x4 (&v)[4]) {
+  asm volatile("s_waitcnt lgkmcnt(%4)"
+               : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])
+               : "n"(LEFT)
+               : "memory");
+}
+// ll_lds_read_tr16 at a constant offset from an LDS address
+template <int OFF> __device__ __forceinline__ s16x4 lds_read_tr16_at(uint32_t at) {
+  s16x4 r;
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(r) : "v"(at), "n"(OFF) : "memory");
+  return r;
+}
+
 struct PrefillArgs {
   const void* q; int64_t q_st, q_sh;
   const void* k; int64_t k_st, k_sh;
@@ -510,13 +532,18 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     char* kl = smem + (x % NST) * FG::STAGE_B;
     char* vl = kl + FG::K_B;
     const int32_t* sl = (const int32_t*)(wslots + (x % NST) * (kBK * 4));
+    uint32_t slot[IPW];
+#pragma unroll
+    for (int i = 0; i < IPW; ++i) slot[i] = (uint32_t)sl[(wave * IPW + i) * RPI + dr];
+    // (a slot's row by one 32 x 32 -> 64 bit multiply-add: the launcher checks
+    // that a token's stride has 32 bits)
+    const uint32_t kst = (uint32_t)a.k_st * sizeof(T), vst = (uint32_t)a.v_st * sizeof(T);
 #pragma unroll
     for (int i = 0; i < IPW; ++i) {
       const int ii = wave * IPW + i;
       const int r = ii * RPI + dr;  // the LDS chunk position dp of row r holds chunk swz(dp, r)
-      const int64_t slot = sl[r];
-      dma16(c.kb + slot * a.k_st + 8 * FG::kswz(dp, r), kl + ii * 1024);
-      dma16(c.vb + slot * a.v_st + 8 * FG::vswz(dp, r), vl + ii * 1024);
+      dma16((const char*)c.kb + ((uint64_t)slot[i] * kst + 16 * FG::kswz(dp, r)), kl + ii * 1024);
+      dma16((const char*)c.vb + ((uint64_t)slot[i] * vst + 16 * FG::vswz(dp, r)), vl + ii * 1024);
     }
   };
 
@@ -574,19 +601,24 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) sacc[kb][qb] = (f32x16){};
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      V8 qf[QB], ka[2];
+    // the operands of a k-step are read while the step before it multiplies
+    auto k_read = [&](int s, V8 (&k)[2]) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = 32 * x + l32;
-        ka[x] = *(const V8*)(kl + r * FG::ROWB + FG::kswz(2 * s + hf, r) * 16);
+        k[x] = *(const V8*)(kl + r * FG::ROWB + FG::kswz(2 * s + hf, r) * 16);
       }
-      qf[0] = qreg[s];
+    };
+    V8 ka[2][2];
+    k_read(0, ka[0]);
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      if (s + 1 < DS) k_read(s + 1, ka[(s + 1) & 1]);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) sacc[kb][qb] = mfma32(ka[kb], qf[qb], sacc[kb][qb]);
+        for (int qb = 0; qb < QB; ++qb) sacc[kb][qb] = mfma32(ka[s & 1][kb], qreg[s], sacc[kb][qb]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     // the causal + length mask only where a key can pass the wave's first
     // row's limit (masked keys -> -inf), then the tile's row maxima in the
@@ -633,17 +665,36 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // transposing reads, the 16-lane group g = lane / 16 reading keys
   // 16 s + 4 (g / 2) + j / 4 (+ 8), d 32 db + 16 (g % 2) + 4 (j % 4) .. + 3
   const int tg = lane >> 4, tj = lane & 15;
-  // the two transposing reads of fragment (s, db): keys 16 s + 4 (g / 2) + j / 4
-  // and 8 keys further, d bytes 64 db + 32 (g % 2) + 8 (j % 4)
-  auto vfrag_reads = [&](const char* vl, int s, int db, s16x4& lo, s16x4& hi) {
-    const int key = 16 * s + 4 * (tg >> 1) + (tj >> 2);
+  // the lane's LDS address in a V tile of stage 0 of key step 0's first read for
+  // each d block: d bytes 64 db + 32 (g % 2) + 8 (j % 4) of key 4 (g / 2) + j / 4.
+  // The other reads are whole rows further, which the swizzle repeats every 4.
+  uint32_t vaddr[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    const int key = 4 * (tg >> 1) + (tj >> 2);
     const int dbyte = 64 * db + 32 * (tg & 1) + 8 * (tj & 3);
-    const int c = dbyte >> 4, off = dbyte & 15;
-    lo = ll_lds_read_tr16(vl + key * FG::ROWB + FG::vswz(c, key) * 16 + off);
-    hi = ll_lds_read_tr16(vl + (key + 8) * FG::ROWB + FG::vswz(c, key + 8) * 16 + off);
+    vaddr[db] = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)smem + FG::K_B +
+                key * FG::ROWB + FG::vswz(dbyte >> 4, key) * 16 + (dbyte & 15);
+  }
+  // the fragments of key step S, two reads per d block: keys 16 S + 4 (g / 2) + j / 4
+  // and 8 keys further
+  auto v_reads = [&](auto step, const uint32_t (&at)[DB], s16x4 (&v)[2 * DB]) {
+    constexpr int S0 = decltype(step)::value * 16 * FG::ROWB;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      v[2 * db] = lds_read_tr16_at<S0>(at[db]);
+      v[2 * db + 1] = lds_read_tr16_at<S0 + 8 * FG::ROWB>(at[db]);
+    }
   };
   auto accumulate = [&](int buf) {
-    const char* vl = smem + buf * FG::STAGE_B + FG::K_B;
+    // V fragments a key step ahead of their MFMAs, the first under the
+    // exponentials (the waits of reads and MFMAs in turn were a sixth of a
+    // tile's time)
+    uint32_t vat[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) vat[db] = vaddr[db] + buf * FG::STAGE_B;
+    s16x4 vr[2][2 * DB];
+    v_reads(std::integral_constant<int, 0>{}, vat, vr[0]);
     V8 pf[QB][4];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -661,20 +712,26 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       }
       l_run[qb] += psum;  // this half-wave's keys; the halves add up at the store
     }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      s16x4 vr[2 * DB];  // lo, hi of each d block
-#pragma unroll
-      for (int db = 0; db < DB; ++db) vfrag_reads(vl, s, db, vr[2 * db], vr[2 * db + 1]);
-      ll_lds_wait_tie(vr);
+    auto multiply = [&](int s, const s16x4 (&v)[2 * DB]) {
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         const V8 va = __builtin_bit_cast(
-            V8, __builtin_shufflevector(vr[2 * db], vr[2 * db + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+            V8, __builtin_shufflevector(v[2 * db], v[2 * db + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) acc[db][qb] = mfma32(va, pf[qb][s], acc[db][qb]);
       }
-    }
+    };
+    v_reads(std::integral_constant<int, 1>{}, vat, vr[1]);
+    lds_wait_tie<2 * DB>(vr[0]);
+    multiply(0, vr[0]);
+    v_reads(std::integral_constant<int, 2>{}, vat, vr[0]);
+    lds_wait_tie<2 * DB>(vr[1]);
+    multiply(1, vr[1]);
+    v_reads(std::integral_constant<int, 3>{}, vat, vr[1]);
+    lds_wait_tie<2 * DB>(vr[0]);
+    multiply(2, vr[0]);
+    lds_wait_tie<0>(vr[1]);
+    multiply(3, vr[1]);
   };
   // acc[db][qb][4 g + i] = O^T[d = 32 db + 8 g + 4 hf + i][query row0 + 32 qb + l32].
   // The halves of a row (lanes l and l + 32) swap 4-element groups, so that
@@ -755,10 +812,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       if (done.ok) store_rows(done);
       reset();
     }
-    kv_copy(x + NST - 1, ck);
-    kv_next(ck);
-    slot_copy(x + 2 * NST - 2, cs);
-    slot_next(cs);
     const int buf = x % NST;
     int t0 = cc_u * kBK, top = cur.Lm1;
     bool work = cur.ok && t0 < cur.kv_end;
@@ -776,6 +829,11 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     }
     const bool last = cc_u + 1 == cc_nt;
     if (work) scores(t0, buf, top);
+    // (behind the score MFMAs, which run on while the addresses are computed)
+    kv_copy(x + NST - 1, ck);
+    kv_next(ck);
+    slot_copy(x + 2 * NST - 2, cs);
+    slot_next(cs);
     if (last) {
       const int k2 = next_item(cc_k);
       if (k2 < 64) prefetch_q(wave_item(k2));
@@ -937,6 +995,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                        (q_stride_tok % 8 == 0) && (q_stride_h % 8 == 0) &&
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
+                       k_stride_tok >= 0 && k_stride_tok < ((int64_t)1 << 31) &&
+                       v_stride_tok >= 0 && v_stride_tok < ((int64_t)1 << 31) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
   // (its rows are stored 16 bytes at a time; a causal call's may be anywhere)
   const bool out_ok = out_stride_tok % 8 == 0 && out_stride_h % 8 == 0 && (uintptr_t)out % 16 == 0;

@@ -22,10 +22,14 @@ _IDX = {torch.int32: 0, torch.int64: 1}
 
 
 def dtype_code(t: torch.Tensor) -> int:
+    return _code(t.dtype)
+
+
+def _code(dt: torch.dtype) -> int:
     try:
-        return _DTYPES[t.dtype]
+        return _DTYPES[dt]
     except KeyError:
-        raise TypeError(f"unsupported dtype {t.dtype}") from None
+        raise TypeError(f"unsupported dtype {dt}") from None
 
 
 def _idx(t: torch.Tensor, name: str) -> int:
@@ -36,6 +40,8 @@ def _idx(t: torch.Tensor, name: str) -> int:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # by device index, without a Stream object
+_current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -48,17 +54,17 @@ def _dev(*ts: torch.Tensor) -> None:
             raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
 
 
-def _here(*ts) -> int:
-    """The current stream, after checking that all of `ts` (None skipped) sit on
-    the current device: a launch goes to that device's stream."""
-    idx = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != idx:
-            raise ValueError(f"lite_lang_amd ops need tensors of one device (got {ts[0].device} "
-                             f"and {t.device})")
+def _here(idx: int, *others: int) -> int:
+    """The current stream, given the device indices of a call's tensors, which
+    all have to be the current device: a launch goes to its stream. (Indices,
+    not tensors: an eager call's checks cost as much as its launch.)"""
+    for i in others:
+        if i != idx:
+            raise ValueError("lite_lang_amd ops need tensors of one device "
+                             f"(got devices {sorted({idx, *others})}, -1: the CPU)")
     if idx < 0:
         raise ValueError("lite_lang_amd ops need device tensors (got a CPU tensor)")
-    if idx != torch._C._cuda_getDevice():
+    if idx != _current_device():
         raise ValueError(f"lite_lang_amd ops run on the current device (got cuda:{idx} tensors)")
     return _raw_stream(idx)
 
@@ -252,7 +258,7 @@ def _window_checks(q, cache_k, cache_v, out, req_to_tokens, window, sinks):
     assert req_to_tokens.dtype == torch.int32 and ts[1] == 1
     if window < 1 or sinks < 0:
         raise ValueError(f"window {window} must be at least 1 and sinks {sinks} at least 0")
-    return shape, kshape[1], qs, ks, vs, os_, ts[0]
+    return shape, kshape[1], dt, qs, ks, vs, os_, ts[0]
 
 
 _I62 = 1 << 62  # more than any length, and an int64 (a larger window or count sees as much)
@@ -263,15 +269,18 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
     """prefill_attention in which the query at position p sees the keys n <= p
     with n > p - window or n < sinks. Slot-table entries of keys that no query
     of the call sees are not read, so those tokens may have left the cache."""
-    (T, H, D), KVH, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window, sinks)
+    (_, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window,
+                                                             sinks)
     bs = b_seq_len.shape
     assert len(bs) == 1 and b_req_idx.shape == bs and b_start_loc.shape == bs
     assert b_req_idx.is_contiguous() and b_start_loc.is_contiguous() and b_seq_len.is_contiguous()
-    sh_ptr, sh64 = 0, 0
+    dev, sh_ptr, sh64 = q.get_device(), 0, 0
     if b_shared_seq_len is not None:
         assert b_shared_seq_len.shape == bs and b_shared_seq_len.is_contiguous()
+        assert b_shared_seq_len.get_device() == dev
         sh_ptr, sh64 = b_shared_seq_len.data_ptr(), _idx(b_shared_seq_len, "b_shared_seq_len")
-    stream = _here(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, req_to_tokens, b_shared_seq_len)
+    stream = _here(dev, k.get_device(), v.get_device(), o.get_device(), b_req_idx.get_device(),
+                   b_start_loc.get_device(), b_seq_len.get_device(), req_to_tokens.get_device())
     rc = _L.ll_call_window_prefill_attention(_lib.WINDOW_PREFILL_ATTENTION_CALL.pack(
         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
         o.data_ptr(), os_[0], os_[1], req_to_tokens.data_ptr(), ts,
@@ -279,7 +288,7 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
         b_start_loc.data_ptr(), _idx(b_start_loc, "b_start_loc"),
         b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), sh_ptr, sh64,
         bs[0], H, KVH, D, max_input_len, min(window, _I62), min(sinks, _I62),
-        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, dtype_code(q), stream))
+        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, _code(dt), stream))
     if rc:
         _lib.check(rc, "ll_window_prefill_attention")
     return o
@@ -288,18 +297,20 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
 def window_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_batch, cache_k,
                             cache_v, out, window, sinks=0, sm_scale=None):
     """decode_attention over the last `window` tokens and the first `sinks` ones."""
-    (B, H, D), KVH, qs, ks, vs, os_, ts = _window_checks(q, cache_k, cache_v, out, req_to_tokens,
-                                                         window, sinks)
+    (B, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, cache_k, cache_v, out,
+                                                             req_to_tokens, window, sinks)
     assert b_req_idx.shape == (B,) and b_seq_len.shape == (B,)
     assert b_req_idx.is_contiguous() and b_seq_len.is_contiguous()
-    stream = _here(q, req_to_tokens, b_req_idx, b_seq_len, cache_k, cache_v, out)
+    stream = _here(q.get_device(), req_to_tokens.get_device(), b_req_idx.get_device(),
+                   b_seq_len.get_device(), cache_k.get_device(), cache_v.get_device(),
+                   out.get_device())
     window, sinks = min(window, _I62), min(sinks, _I62)
     # Under capture a buffer of the call's own, from the graph's memory, so that
     # graphs replayed at the same time share nothing; else the stream's.
     need = _window_decode_bytes(B, H, KVH, D, max_len_in_batch, window, sinks)
     ws = None
     if need > 0:
-        if torch._C._cuda_isCurrentStreamCapturing():
+        if _capturing():
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         else:
             ws = workspace(q.device, "window_decode", need)
@@ -308,7 +319,7 @@ def window_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_b
         vs[1], req_to_tokens.data_ptr(), ts, b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"),
         b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), out.data_ptr(), os_[0], os_[1],
         B, H, KVH, D, max_len_in_batch, window, sinks,
-        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, dtype_code(q),
+        1.0 / (D ** 0.5) if sm_scale is None else sm_scale, _code(dt),
         0 if ws is None else ws.data_ptr(), need, stream))
     if rc:
         _lib.check(rc, "ll_window_decode_attention")
@@ -457,17 +468,18 @@ def rope_positions(q, k, positions, inv_freq, interleaved=False, factor=1.0, q_o
     T, Hq, D = shape
     assert qs[2] == 1 and qos[2] == 1 and q_out.shape == shape and q_out.dtype == dt
     R = _rope_checks(positions, inv_freq, T, D)
-    kargs = (0, 0, 0, 0, 0, 0, 0)
+    dev, kargs = q.get_device(), (0, 0, 0, 0, 0, 0, 0)
     if k is not None:
         kshape, ks, kos = k.shape, k.stride(), k_out.stride()
         assert kshape[0] == T and kshape[2] == D and k.dtype == dt and k_out.dtype == dt
         assert ks[2] == 1 and kos[2] == 1 and k_out.shape == kshape
+        assert k.get_device() == dev and k_out.get_device() == dev
         kargs = (k.data_ptr(), ks[0], ks[1], k_out.data_ptr(), kos[0], kos[1], kshape[1])
-    stream = _here(q, k, positions, inv_freq, q_out, k_out)
+    stream = _here(dev, positions.get_device(), inv_freq.get_device(), q_out.get_device())
     rc = _L.ll_call_rope_positions(_lib.ROPE_POSITIONS_CALL.pack(
         q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], Hq, *kargs,
         positions.data_ptr(), _idx(positions, "positions"), inv_freq.data_ptr(), R,
-        bool(interleaved), factor, T, D, dtype_code(q), stream))
+        bool(interleaved), factor, T, D, _code(dt), stream))
     if rc:
         _lib.check(rc, "ll_rope_positions")
     return q_out, k_out
@@ -491,16 +503,22 @@ def qk_norm_rope_kv_scatter(qkv, q_heads, kv_heads, head_dim, q_gamma, k_gamma, 
     assert slots.dtype == torch.int32 and slots.shape == (T,) and slots.is_contiguous()
     assert pshape[1] == 2 * kv_heads and pshape[2] == D and ps[2] == 1 and pool_layer.dtype == dt
     R = _rope_checks(positions, inv_freq, T, D)
-    gammas = []
-    for g in (q_gamma, k_gamma):
-        assert g is None or (g.shape == (D,) and g.is_contiguous() and g.dtype == dt)
-        gammas.append(0 if g is None else g.data_ptr())
-    stream = _here(qkv, q_gamma, k_gamma, positions, inv_freq, slots, pool_layer, q_out)
+    dev, gq, gk = qkv.get_device(), 0, 0
+    if q_gamma is not None:
+        assert q_gamma.shape == (D,) and q_gamma.is_contiguous() and q_gamma.dtype == dt
+        assert q_gamma.get_device() == dev
+        gq = q_gamma.data_ptr()
+    if k_gamma is not None:
+        assert k_gamma.shape == (D,) and k_gamma.is_contiguous() and k_gamma.dtype == dt
+        assert k_gamma.get_device() == dev
+        gk = k_gamma.data_ptr()
+    stream = _here(dev, positions.get_device(), inv_freq.get_device(), slots.get_device(),
+                   pool_layer.get_device(), q_out.get_device())
     rc = _L.ll_call_qk_norm_rope_kv_scatter(_lib.QK_NORM_ROPE_KV_SCATTER_CALL.pack(
-        qkv.data_ptr(), xs[0], T, q_heads, kv_heads, D, q_out.data_ptr(), qos[0], qos[1], *gammas,
+        qkv.data_ptr(), xs[0], T, q_heads, kv_heads, D, q_out.data_ptr(), qos[0], qos[1], gq, gk,
         eps, positions.data_ptr(), _idx(positions, "positions"), inv_freq.data_ptr(), R,
         bool(interleaved), factor, slots.data_ptr(), pool_layer.data_ptr(), ps[0], ps[1],
-        pshape[0], dtype_code(qkv), stream))
+        pshape[0], _code(dt), stream))
     if rc:
         _lib.check(rc, "ll_qk_norm_rope_kv_scatter")
     return q_out
@@ -773,15 +791,18 @@ def build_slot_maps(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_token
     of range, 2: a bad or repeated row, 4: more tokens than `slots` holds, 8:
     too few free pages."""
     bs, i32 = b_req_idx.shape, torch.int32
-    assert len(bs) == 1
-    for t in (b_req_idx, b_seq_len, b_cached_len, b_start_loc, last_rows):
-        assert t.shape == bs and t.is_contiguous()
-    for t in (free_pages, req_to_tokens, slots, positions, b_start_loc, last_rows, counts):
-        assert t.dtype == i32
-    assert free_pages.ndim == 1 and slots.ndim == 1 and req_to_tokens.ndim == 2
-    n_free, n_tokens, (rows, cols) = free_pages.shape[0], slots.shape[0], req_to_tokens.shape
+    (B,) = bs
+    assert b_seq_len.shape == bs and b_cached_len.shape == bs
+    assert b_start_loc.shape == bs and last_rows.shape == bs
+    assert b_req_idx.is_contiguous() and b_seq_len.is_contiguous() and b_cached_len.is_contiguous()
+    assert b_start_loc.is_contiguous() and last_rows.is_contiguous()
+    assert b_start_loc.dtype == i32 and last_rows.dtype == i32 and counts.dtype == i32
+    assert slots.dtype == i32 and positions.dtype == i32
+    assert free_pages.dtype == i32 and req_to_tokens.dtype == i32
+    sshape, fshape, (rows, cols) = slots.shape, free_pages.shape, req_to_tokens.shape
+    assert len(sshape) == 1 and positions.shape == sshape and len(fshape) == 1
     assert free_pages.is_contiguous() and slots.is_contiguous() and positions.is_contiguous()
-    assert positions.shape == (n_tokens,) and counts.shape == (3,) and counts.is_contiguous()
+    assert counts.shape == (3,) and counts.is_contiguous()
     ts = req_to_tokens.stride()
     assert ts[1] == 1
     bt = (0, 0, 0)
@@ -793,14 +814,17 @@ def build_slot_maps(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_token
         bshape, bstride = block_table.shape, block_table.stride()
         assert block_table.dtype == i32 and len(bshape) == 2
         assert bstride[1] == 1 and bshape[0] == rows
+        assert block_table.get_device() == counts.get_device()
         bt = (block_table.data_ptr(), bstride[0], bshape[1])
-    stream = _here(counts, b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_tokens, slots,
-                   positions, b_start_loc, last_rows, block_table)
+    stream = _here(counts.get_device(), b_req_idx.get_device(), b_seq_len.get_device(),
+                   b_cached_len.get_device(), free_pages.get_device(), req_to_tokens.get_device(),
+                   slots.get_device(), positions.get_device(), b_start_loc.get_device(),
+                   last_rows.get_device())
     rc = _L.ll_call_build_slot_maps(_lib.BUILD_SLOT_MAPS_CALL.pack(
         b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(),
         _idx(b_seq_len, "b_seq_len"), b_cached_len.data_ptr(), _idx(b_cached_len, "b_cached_len"),
-        bs[0], free_pages.data_ptr(), n_free, page_size, *bt, req_to_tokens.data_ptr(), ts[0], rows,
-        cols, slots.data_ptr(), positions.data_ptr(), n_tokens, b_start_loc.data_ptr(),
+        B, free_pages.data_ptr(), fshape[0], page_size, *bt, req_to_tokens.data_ptr(), ts[0], rows,
+        cols, slots.data_ptr(), positions.data_ptr(), sshape[0], b_start_loc.data_ptr(),
         last_rows.data_ptr(), counts.data_ptr(), stream))
     if rc:
         _lib.check(rc, "ll_build_slot_maps")
