@@ -3,7 +3,8 @@
 // For request b with L = b_seq_len[b] keys (slot row req_to_tokens[b_req_idx[b]])
 // and S = shared[b] keys already cached from a previous request, the query
 // rows q[b_start_loc[b] + m], m in [0, L - S), attend to keys n <= m + S.
-// S = 0 is the plain NoPad prefill. Semantics:
+// S = 0 is the plain NoPad prefill. Windowed, the query at position p = m + S
+// attends to the keys n <= p with n > p - window or n < sinks. Semantics:
 //   litelang/kernel/develop_flash_attn/flash_attn_v2.py:392-566 (no prompt cache)
 //   litelang/kernel/develop_flash_attn/flash_attn_v2.py:569-762 (prompt cache)
 // including the rounding of the probabilities to the KV dtype before P.V.
@@ -13,12 +14,13 @@
 // waves). WPH waves take query rows row0 .. row0 + 32 WPH - 1 of one head and
 // the workgroup takes 8 / WPH heads of one KV head (WPH = 2 when the group
 // size is a multiple of 4, else 4), so every K/V tile staged in LDS serves 256
-// query rows. Per 64-key tile:
+// query rows. Two waves per SIMD half a tile apart (one's scores meet the
+// other's softmax). Per 64-key tile:
 //   * K and V rows are DMA'd through the slot table straight into a 4-stage
-//     LDS ring (global_load_lds_dwordx4), three tiles ahead of the one being
+//     LDS ring (global_load_lds_dwordx4), two tiles ahead of the one being
 //     computed, stored key-major with their 16-byte chunks XOR-swizzled by
 //     row so that the MFMA operand reads are bank-conflict free; the slot ids
-//     are DMA'd too, by every wave into a ring of its own, three tiles ahead
+//     are DMA'd too, by every wave into a ring of its own, two tiles ahead
 //     of their K/V copies. The P.V operand V^T is read from the key-major V
 //     tile with the gfx950 transposing LDS read (ds_read_b64_tr_b16), so no
 //     VALU work transposes V;
@@ -29,6 +31,14 @@
 //     rescaled about once per work item), and O^T += V^T . P^T with P
 //     rounded to the KV dtype;
 //   * one barrier per tile.
+// A tile that no mask touches takes 4,000 cycles of a SIMD (MFMA 2,048, VALU
+// about 2,300; the rest of the two is not overlapped), a masked one some 600
+// more, a change of item (Q in, output rows out, all workgroups at about the
+// same time) 5,000 to 7,000. us per call, bf16, 16/2 heads of 128, and
+// the share of the 1,230 TFLOP/s that a large library product reaches here:
+// 1 x 8192 causal 249 (1,100 TFLOP/s, 90%); 1 x 32,768 under a window of 4096
+// 967 (1,067, 87%); 40 x 600 under a window of 256 106 (380, 31%: six items of
+// one to six tiles per workgroup).
 #include <algorithm>
 #include <type_traits>
 
@@ -42,6 +52,7 @@ constexpr int kBK = 64;   // keys per tile
 constexpr int kVmcntZero = 0x0F70;
 
 constexpr int kStages = 4;  // LDS ring depth (K/V tiles)
+constexpr int kAhead = 2;   // tiles that K/V copies run ahead of the scores (slot ids twice that)
 // A row's running maximum (exp2 domain) moves only when a tile's maximum
 // passes it by more than this: the probabilities then stay at most 2^8
 // (exact range in fp32 and in the 16-bit P fed to P.V)
@@ -453,10 +464,10 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // The workgroup's items run as one stream of 64-key tiles. K and V tiles
   // go from the pool straight into an NST-stage LDS ring
   // (global_load_lds_dwordx4, no VGPR staging); the slot ids that address
-  // them are DMA'd likewise, by every wave into a ring of its own, NST - 1
+  // them are DMA'd likewise, by every wave into a ring of its own, kAhead
   // tiles before the tile's K/V copies. Per stream tile x every wave issues
-  // one group: its K/V copies of tile x + NST - 1 and its slot ids of tile
-  // x + 2 NST - 2, so that NST - 1 tiles are in flight while tile x is
+  // one group: its K/V copies of tile x + kAhead and its slot ids of tile
+  // x + 2 kAhead, so that kAhead tiles are in flight while tile x is
   // computed, across item boundaries too (the next item's first tiles load
   // under the current item's last ones). Past the stream's end the groups
   // repeat the last item's last key into stages nothing reads, so that
@@ -466,7 +477,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   constexpr int IPW = kBK * FG::ROWB / 1024 / SH::NW;  // K (and V) instructions per wave per tile
   constexpr int KVC = 2 * IPW;                         // K and V
   static_assert(IPW >= 1 && IPW * SH::NW * 1024 == kBK * FG::ROWB, "tile rows over the waves");
-  static_assert(NST == 4, "the waits below are written for 4 stages");
   char* wslots = smem + NST * FG::STAGE_B + wave * (NST * kBK * 4);
   const int dr = lane / FG::CH, dp = lane % FG::CH;
 
@@ -568,24 +578,24 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
 
   WaveItem cur = wave_item(k_first);
   load_q(cur);
-  // slot ids of stream tiles 0 .. NST-2, then (every load so far landed, Q
+  // slot ids of stream tiles 0 and 1, then (every load so far landed, Q
   // fragments included: a real s_waitcnt, which the compiler's own wait
-  // insertion accounts for) the groups of iterations -NST+1 .. -1
+  // insertion accounts for) the groups of iterations -2 and -1
   SlotCursor cs;
   slot_at(cs, k_first);
   KvCursor ck;
   kv_at(ck, k_first);
 #pragma unroll
-  for (int x = 0; x < NST - 1; ++x) {
+  for (int x = 0; x < kAhead; ++x) {
     slot_copy(x, cs);
     slot_next(cs);
   }
   __builtin_amdgcn_s_waitcnt(kVmcntZero);
 #pragma unroll
-  for (int x = 0; x < NST - 1; ++x) {
+  for (int x = 0; x < kAhead; ++x) {
     kv_copy(x, ck);
     kv_next(ck);
-    slot_copy(x + NST - 1, cs);
+    slot_copy(x + kAhead, cs);
     slot_next(cs);
   }
 
@@ -595,7 +605,8 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   f32x16 sacc[2][QB];
   float m_cand[QB];
   // (t0: the tile's first key; WIN: top is the last key of the tile's range)
-  auto scores = [&](int t0, int buf, int top) {
+  // (masked false_type: the caller knows that every row sees the whole tile)
+  auto scores = [&](auto masked, int t0, int buf, int top) {
     const char* kl = smem + buf * FG::STAGE_B;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -629,23 +640,34 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
                                : t0 + kBK - 1 > min(cur.row0 + cur.S, cur.Lm1);
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      if (need_mask) {
+      if (decltype(masked)::value && need_mask) {
         // last key this row sees, relative to the tile (rows past the
         // request see every key of it)
         const int p = cur.row0 + 32 * qb + l32 + cur.S;
         const int lim = min(p, WIN ? top : cur.Lm1) - t0;
-        const int below = p - a.window - t0, sink = a.sinks - t0;  // WIN
+        // The visible keys as bits, shifted out from the top in the order of
+        // the lane's elements: an add and a select per element where compares
+        // of each key with the row's limits take four and scalar logic (a
+        // masked tile took 1300 cycles more than another, 40 x 600 under a
+        // window of 256 112 us, now 108).
+        auto first = [](int n) -> uint32_t {  // bits 0 .. n - 1
+          const int m = min(max(n, 0), 32);
+          return m == 32 ? ~0u : (1u << m) - 1u;
+        };
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+          uint32_t see = first(lim + 1 - 32 * kb);
+          if constexpr (WIN)
+            see &= ~first(p - a.window + 1 - t0 - 32 * kb) | first(a.sinks - t0 - 32 * kb);
+          see = __builtin_bitreverse32(see) << (4 * hf);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = 32 * kb + 8 * (e >> 2) + 4 * hf + (e & 3);
-            // (bitwise: with && and || the compiler branches around every
-            // element, 130 -> 122 us at 40 x 600, window 256, 16/2 heads)
-            bool hide = key > lim;
-            if constexpr (WIN) hide |= (key <= below) & (key >= sink);
-            sacc[kb][qb][e] = hide ? -INFINITY : sacc[kb][qb][e];
+          for (int e = 0; e < 16; ++e) {  // key 32 kb + 8 (e / 4) + 4 hf + e % 4
+            uint32_t next;
+            const bool is = __builtin_uadd_overflow(see, see, &next);
+            sacc[kb][qb][e] = is ? sacc[kb][qb][e] : -INFINITY;
+            see = (e & 3) == 3 ? next << 4 : next;
           }
+        }
       }
       float tmax = -INFINITY;
 #pragma unroll
@@ -781,22 +803,80 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     dma4(qp, wsink);
   };
 
-  // iterations whose copies a full wait (at an item's first tile, before
-  // that iteration's copies) already covered: after it in iteration y the
-  // copies of tiles up to y + NST - 2 and the slot ids they read are in
+  // running maxima, moved only when a row of the wave meets a tile maximum
+  // more than kLazyMax above its own (the first tile always): until then the
+  // probabilities exp2(s - m_run) stay below 2^kLazyMax, and the output rows
+  // and sums are rescaled about once per item instead of at nearly every tile
+  auto rescale = [&]() {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      if (__builtin_amdgcn_ballot_w64(m_cand[qb] > m_run[qb] + kLazyMax)) {
+        // both halves of a row (its two lanes) take the row's maximum
+        const float m_new = fmaxf(m_run[qb], fmaxf(m_cand[qb], __shfl_xor(m_cand[qb], 32, 64)));
+        const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
+        m_run[qb] = m_new;
+        l_run[qb] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db][qb] *= alpha;
+      }
+    }
+  };
+
+  // One barrier per tile, the "event" of tile x: behind it every wave's copies
+  // of tile x are in, and stage (x + kAhead) % NST is free. The waves 0-3 meet
+  // it ahead of the tile's scores; the waves 4-7 ahead of the P.V of tile
+  // x - 1, whose scores they have: on each SIMD one wave's scores and P.V
+  // (MFMA) then meet the other's softmax (VALU) instead of its like (long
+  // windows, 5 x 4111 behind prefixes: 121 -> 117 us; 8 x 2000, 28/4: 184 ->
+  // 180). Every wave issues the copies of tile x + kAhead (and the slot ids of
+  // tile x + 2 kAhead) behind its scores of tile x, hence behind the event of
+  // tile x: all waves are then done with tile x - 2, which had that stage
+  // (waves 4-7 with its P.V before the event). So only the group of iteration
+  // x - 1 may be in flight at the event of tile x, besides older output stores
+  // and newer Q prefetches: vector memory operations complete in issue order,
+  // so both only make the wait longer.
+  static_assert(NST == kAhead + 2, "the stages the events free");
+  const bool lead = wave < SH::NW / 2;
+  // the next events whose copies a full wait (at an item's first tile) already
+  // covered: those of iteration x - 1 are in after it
   int covered = 0;
+  auto event = [&]() {
+    if (covered > 0) --covered; else vm_wait<1 + KVC>();
+    lds_barrier();
+  };
   int cc_k = k_first, cc_u = 0, cc_nt = rl(it_nt, k_first);  // item (pass) and tile computed
   WaveItem done = cur;  // at an item's first tile: the item whose rows acc holds
+  if (!lead) event();
   for (int x = 0; x < ntot; ++x) {
-    // Otherwise, at the top of iteration x only the groups of iterations
-    // x-NST+2 .. x-1 may be in flight (2 slot copies and 2 K/V groups; the
-    // groups are issued in every iteration), besides older output stores
-    // and newer Q prefetches: vector memory operations complete in issue
-    // order, so both only make the wait longer.
-    if (covered > 0) --covered; else vm_wait<(NST - 2) + 2 * KVC>();
-    // every wave's copies of tile x are in; every wave is done with tile
-    // x - 1, whose stage the copies of tile x + NST - 1 refill
-    lds_barrier();
+    // A run of tiles that every row of the wave sees whole, that are not their
+    // item's last and whose copies stay inside the cursors' items: the same
+    // steps without the decisions, whose scalar instructions and branches are
+    // on every wave's path (a fifth of a tile's time: 32,768 tokens under a
+    // window of 4096 1039 -> 985 us)
+    int run = cs.nt - 1 - cs.u;
+    if (run > 1 && cc_u > 0 && covered == 0 && cur.ok) {
+      const int u = WIN ? cc_u - cur.nst : cc_u, su = WIN ? cs.u - cs.nst : cs.u;
+      const int first = (WIN ? cur.low : 0) + u * kBK;  // key of tile x
+      const bool whole = !WIN || (u >= 0 && su >= 0 && first > cur.row0 + SH::RW - 1 + cur.S - a.window);
+      run = min(min(run, ck.left - 1), min(cc_nt - 1 - cc_u,
+                                           (min(cur.row0 + cur.S, cur.Lm1) + 1 - first) / kBK));
+      if (whole && run > 0) {
+        const int32_t* ids = cs.row + (WIN ? cs.low : 0) + su * kBK + lane;
+        cc_u += run;
+        ck.left -= run;
+        cs.u += run;
+        for (; run > 0; --run, ++x, ids += kBK) {
+          if (lead) event();
+          scores(std::false_type{}, 0, x % NST, 0);
+          kv_copy(x + kAhead, ck);
+          dma4(ids, wslots + ((x + 2 * kAhead) % NST) * (kBK * 4));
+          if (!lead) event();  // (of tile x + 1, which there is)
+          rescale();
+          accumulate(x % NST);
+        }
+      }
+    }
+    if (lead) event();
     if (cc_u == 0 && x > 0) {
       // An item's first tile (the first item's Q came with the prologue):
       // its Q fragments, from L2, and the wait for them, before this
@@ -807,7 +887,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       // would otherwise wait for every copy in flight before each scores).
       load_q(cur);
       q_wait_tie(qreg);
-      covered = NST - 2;
+      covered = 1;
       // the previous item's rows, then a fresh softmax state
       if (done.ok) store_rows(done);
       reset();
@@ -828,35 +908,19 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       }
     }
     const bool last = cc_u + 1 == cc_nt;
-    if (work) scores(t0, buf, top);
+    if (work) scores(std::true_type{}, t0, buf, top);
     // (behind the score MFMAs, which run on while the addresses are computed)
-    kv_copy(x + NST - 1, ck);
+    kv_copy(x + kAhead, ck);
     kv_next(ck);
-    slot_copy(x + 2 * NST - 2, cs);
+    slot_copy(x + 2 * kAhead, cs);
     slot_next(cs);
     if (last) {
       const int k2 = next_item(cc_k);
       if (k2 < 64) prefetch_q(wave_item(k2));
     }
+    if (!lead && x + 1 < ntot) event();
     if (work) {
-      // running maxima, moved only when a row of the wave meets a tile
-      // maximum more than kLazyMax above its own (the first tile always):
-      // until then the probabilities exp2(s - m_run) stay below 2^kLazyMax,
-      // and the output rows and sums are rescaled about once per item
-      // instead of at nearly every tile
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        if (__builtin_amdgcn_ballot_w64(m_cand[qb] > m_run[qb] + kLazyMax)) {
-          // both halves of a row (its two lanes) take the row's maximum
-          const float m_new =
-              fmaxf(m_run[qb], fmaxf(m_cand[qb], __shfl_xor(m_cand[qb], 32, 64)));
-          const float alpha = __builtin_amdgcn_exp2f(m_run[qb] - m_new);
-          m_run[qb] = m_new;
-          l_run[qb] *= alpha;
-#pragma unroll
-          for (int db = 0; db < DB; ++db) acc[db][qb] *= alpha;
-        }
-      }
+      rescale();
       accumulate(buf);
     }
     if (!last) {
