@@ -82,7 +82,7 @@ __global__ __launch_bounds__(64) void rotary_kernel(RotArgs a) {
     return g != nullptr ? v * r * ll_to_f32(g[d]) : v;
   };
   const int half = rot ? a.R / 2 : 0;
-  const int64_t p = rot ? ll_load_idx(a.pos, t, a.pos64) : 0;
+  const int64_t p = half > 0 ? ll_load_idx(a.pos, t, a.pos64) : 0;  // (null where R is 0)
   for (int i = lane; i < half; i += 64) {
     const int d0 = INTER ? 2 * i : i, d1 = INTER ? 2 * i + 1 : i + half;
     float c, s;

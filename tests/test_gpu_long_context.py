@@ -103,6 +103,21 @@ def test_rope_positions_strided_rows(cuda, pad):
             assert bool((row[:, -pad:] == 3.0).all()), "padding of the rows"
 
 
+@pytest.mark.parametrize("D", [64, 20])
+def test_rope_of_nothing_rotated_needs_no_positions(cuda, D):
+    """The C entry point takes null positions and frequencies with rotary_dim 0
+    (16-byte rows and others): a copy."""
+    import ctypes
+
+    from lite_lang_amd import _lib
+    x = torch.randn(5, 3, D, device=cuda).bfloat16()
+    y = torch.zeros_like(x)
+    rc = _lib.load().ll_rope_positions(x.data_ptr(), 3 * D, D, y.data_ptr(), 3 * D, D, 3, None, 0,
+                                       0, None, 0, 0, 0, None, 0, None, 0, 0, ctypes.c_float(1.0),
+                                       5, D, _ops().dtype_code(x), _ops()._stream(x))
+    assert rc == 0 and torch.equal(x, y)
+
+
 def test_calls_of_no_tokens(cuda):
     q, none, f = torch.zeros(0, 4, 64, device=cuda), _i32([], cuda), torch.ones(32, device=cuda)
     pool = torch.zeros(5, 4, 64, device=cuda)
