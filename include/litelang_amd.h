@@ -223,9 +223,10 @@ int ll_rope_kv_scatter(void* qkv, int64_t qkv_row_stride, int64_t ntok, int64_t 
  * is scaled by `factor` (1, or the attention factor of scaled frequencies).
  * The elements behind rotary_dim are copied. Angles are fp64, the rest fp32
  * with one rounding. positions [ntok] int32 or int64 (below 2^31), inv_freq
- * [rotary_dim/2] fp32; head_dim at most 1024, rotary_dim even. The outputs may
- * be the inputs (same strides), but not otherwise overlap them. No counterpart
- * in the reference, whose rotation is ll_rotary_emb's. */
+ * [rotary_dim/2] fp32; head_dim at most 1024, rotary_dim even, at most 2^24
+ * tokens. The outputs may be the inputs (same strides, none of them 0), but not
+ * otherwise overlap them. No counterpart in the reference, whose rotation is
+ * ll_rotary_emb's. */
 int ll_rope_positions(const void* q, int64_t q_stride_tok, int64_t q_stride_h, void* q_out,
                       int64_t q_out_stride_tok, int64_t q_out_stride_h, int64_t q_heads,
                       const void* k, int64_t k_stride_tok, int64_t k_stride_h, void* k_out,
@@ -240,8 +241,8 @@ int ll_rope_positions(const void* q, int64_t q_stride_tok, int64_t q_stride_h, v
  * no norm of those heads), and rotated as in ll_rope_positions; q goes to q_out
  * (which may be qkv itself), k and the plain v to pool_layer[slots[t]], K heads
  * first. A slot outside [0, pool_slots) is a padded token: its K and V are not
- * stored. slots of one call must differ. fp32 with one rounding. No
- * counterpart in the reference (ll_rope_kv_scatter without norms). */
+ * stored. slots of one call must differ. At most 2^24 tokens. fp32 with one
+ * rounding. No counterpart in the reference (ll_rope_kv_scatter without norms). */
 int ll_qk_norm_rope_kv_scatter(const void* qkv, int64_t qkv_row_stride, int64_t ntok,
                                int64_t q_heads, int64_t kv_heads, int64_t head_dim, void* q_out,
                                int64_t q_out_stride_tok, int64_t q_out_stride_h,

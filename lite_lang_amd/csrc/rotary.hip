@@ -321,8 +321,14 @@ int launch_rotary(const char* fn, const RotArgs& a, int interleaved, int dtype,
                "%s: head_dim %d, rotary_dim %d unsupported", fn, a.D, a.R);
   LL_CHECK_ARG(a.R == 0 || (a.pos && a.inv_freq), "%s: null pointer", fn);
   if (a.na + a.nb == 0) return LL_OK;
-  LL_CHECK_ARG(a.ntok < ((int64_t)1 << 31) && a.na + a.nb <= 65535,
+  // (a grid holds fewer than 2^32 threads, 256 for each token or two of them)
+  LL_CHECK_ARG(a.ntok <= (int64_t)1 << 24 && a.na + a.nb <= 65535,
                "%s: %lld tokens of %d heads unsupported", fn, (long long)a.ntok, a.na + a.nb);
+  // heads or tokens on one address would be rotated over one another
+  LL_CHECK_ARG((a.na == 0 || ((a.ao_st != 0 || a.ntok == 1) && (a.ao_sh != 0 || a.na == 1))) &&
+                   (a.nb == 0 || ((a.bo_st != 0 || (a.slots ? a.nslots <= 1 : a.ntok == 1)) &&
+                                  (a.bo_sh != 0 || a.nb == 1))),
+               "%s: an output of stride 0", fn);
   const bool vec = rotary_vec_ok(a, dtype == LL_F32 ? 4 : 2);
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     if (vec) {

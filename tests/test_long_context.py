@@ -259,6 +259,22 @@ def test_c_entry_points_refuse_before_any_launch():
     assert rope(R=66) == -1 and rope(R=63) == -1 and rope(ntok=-1) == -1 and rope(D=2048) == -1
     assert rope(ntok=0) == 0  # nothing to do
 
+    assert rope(ntok=(1 << 24) + 1) == -1 and "tokens" in err()
+
+    def wide(st, sh, heads=4, ntok=2):  # into rows or heads that share an address
+        return L.ll_rope_positions(p, 256, 64, p, st, sh, heads, None, 0, 0, None, 0, 0, 0, p, 0, p,
+                                   64, 0, f(1.0), ntok, 64, 2, None)
+
+    assert wide(0, 64) == -1 and "stride 0" in err()
+    assert wide(256, 0) == -1 and "stride 0" in err()
+
+    def norm(q_st=512, q_sh=64, pool_st=256, pool_sh=64):
+        return L.ll_qk_norm_rope_kv_scatter(p, 512, 2, 4, 2, 64, p, q_st, q_sh, p, p, f(1e-6), p, 0,
+                                            p, 64, 0, f(1.0), p, p, pool_st, pool_sh, 9, 2, None)
+
+    for kw in ({"q_st": 0}, {"q_sh": 0}, {"pool_st": 0}, {"pool_sh": 0}):
+        assert norm(**kw) == -1 and "stride 0" in err()
+
     def maps(page=1, blocks=None, batch=2, rows=4, counts=p, free=p, nfree=3):
         return L.ll_build_slot_maps(p, 0, p, 0, p, 0, batch, free, nfree, page, blocks, 8, 8, p, 8,
                                     rows, 8, p, p, 6, p, p, counts, None)
