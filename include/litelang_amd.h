@@ -145,8 +145,9 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * The two calls above for contexts of which only the last `window` tokens and
  * the first `sinks` ones are kept: a query at position p sees the keys n <= p
  * with n > p - window (its own included) or n < sinks. window >= 1, sinks >= 0
- * (both may exceed the length); sm_scale > 0. No counterpart in the reference (whose configs'
- * use_sliding_window it does not read).
+ * (both may exceed the length); lengths at most 2^30; sm_scale > 0. No
+ * counterpart in the reference (whose configs' use_sliding_window it does not
+ * read).
  * No entry of the slot table is read but those of keys that some query of the
  * request's call sees, so the tokens between the sinks and the window may have
  * left the cache and their entries may hold anything. Keys and values that one
@@ -171,7 +172,9 @@ int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_s
 /* ll_decode_attention under a window: the query is the token at b_seq_len - 1,
  * so its keys are one list, the sinks and the last `window` tokens. Sequences
  * of length 0 give zero rows. The workspace (0 bytes where the list is not
- * split) needs no initialisation and nothing in it lasts beyond the call. */
+ * split) needs no initialisation and nothing in it lasts beyond the call; it
+ * must not be one of ll_decode_attention, which has to find its own as it left
+ * it. */
 int64_t ll_window_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                   int64_t head_dim, int64_t max_len_in_batch,
                                                   int64_t window, int64_t sinks);
@@ -334,8 +337,8 @@ int ll_assign_slots(int32_t* req_to_tokens, int64_t req_to_tokens_stride, const 
  * counts written the sum of: 1 a length outside 0 <= cached <= len <= max_len
  * (or the block table), 2 a row outside the table or two requests with new
  * tokens on one row, 4 more new tokens than max_tokens, 8 than free pages.
- * Entries past the new tokens are left as they were. At most 8192 requests and
- * 2^18 table rows; pages and slots are int32. Replaces, for lengths that live
+ * Entries past the new tokens are left as they were. No output may overlap an
+ * input. At most 8192 requests and 2^18 table rows; pages and slots are int32. Replaces, for lengths that live
  * on the device, the host construction of PageCache.alloc_token_idxs
  *   (litelang/models/cache.py:225-249) and of RunnerBatch's start offsets and
  * positions (litelang/models/runner_batch.py:88-265). */

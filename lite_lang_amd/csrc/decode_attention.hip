@@ -1502,7 +1502,7 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
                "%s: q_heads %lld not a multiple of kv_heads %lld", fn, (long long)q_heads, (long long)kv_heads);
   LL_CHECK_ARG(head_dim > 0 && head_dim <= 256, "%s: head_dim %lld unsupported", fn,
                (long long)head_dim);
-  LL_CHECK_ARG(max_len_in_batch >= 0 && max_len_in_batch <= INT32_MAX,
+  LL_CHECK_ARG(max_len_in_batch >= 0 && max_len_in_batch <= (win ? 1 << 30 : INT32_MAX),
                "%s: max_len_in_batch %lld out of range", fn,
                (long long)max_len_in_batch);
   LL_CHECK_ARG(!win || (window >= 1 && sinks >= 0), "%s: window %lld (min 1), sinks %lld (min 0)", fn,
@@ -1524,7 +1524,7 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
   a.slots_cap = 0;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.part_acc = nullptr; a.part_ml = nullptr;
-  // (token indices are below 2^31, so a larger window or count sees as much)
+  // (lengths are at most 2^30, so a larger window or count sees as much)
   a.window = (int)std::min<int64_t>(window, 1 << 30);
   a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
 

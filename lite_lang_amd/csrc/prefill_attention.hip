@@ -1037,6 +1037,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                (long long)window, (long long)sinks);
   LL_CHECK_ARG(!win || (sm_scale > 0.f && sm_scale < INFINITY), "%s: sm_scale %g must be positive",
                fn, (double)sm_scale);
+  LL_CHECK_ARG(!win || max_input_len <= 1 << 30, "%s: max_input_len %lld out of range", fn,
+               (long long)max_input_len);
   if (batch == 0 || max_input_len <= 0) return LL_OK;
   PrefillArgs a;
   a.q = q; a.q_st = q_stride_tok; a.q_sh = q_stride_h;
@@ -1050,7 +1052,7 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   a.shared = b_shared_seq_len; a.shared64 = shared_i64;
   a.H = (int)q_heads; a.G = (int)(q_heads / kv_heads);
   a.sm_scale = sm_scale;
-  // (token indices are below 2^31, so a larger window or count sees as much)
+  // (lengths are at most 2^30, so a larger window or count sees as much)
   a.window = (int)std::min<int64_t>(window, 1 << 30);
   a.sinks = (int)std::min<int64_t>(sinks, 1 << 30);
   a.scale_log2 = sm_scale * 1.4426950408889634f;
