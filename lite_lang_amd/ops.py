@@ -397,7 +397,8 @@ def rope_frequencies(rotary_dim, theta=1e6, scaling=None, max_position=None, len
       `length`, the longest context served (none below max_position);
     * yarn: pairs that turn more than beta_fast times within max_position keep
       their frequency, those below beta_slow are divided by `factor`, a linear
-      ramp between; the factor 0.1 ln(factor) + 1 (or attention_factor);
+      ramp between; the factor m(1), m(k) = 0.1 k ln(factor) + 1, or
+      m(mscale) / m(mscale_all_dim), or attention_factor;
     * longrope: frequencies divided pair by pair by `long_factor`, or by
       `short_factor` where `length` is given and within max_position."""
     if rotary_dim <= 0 or rotary_dim % 2 != 0:
@@ -431,7 +432,9 @@ def rope_frequencies(rotary_dim, theta=1e6, scaling=None, max_position=None, len
         f = f * (1 - stretch) + f / s * stretch
         factor = sc.get("attention_factor")
         if factor is None:
-            factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+            grow = 0.1 * math.log(s) if s > 1 else 0.0
+            m, all_dim = sc.get("mscale"), sc.get("mscale_all_dim")
+            factor = (1 + m * grow) / (1 + all_dim * grow) if m and all_dim else 1.0 + grow
     elif kind == "longrope":
         ext = sc["short_factor"] if length is not None and length <= orig else sc["long_factor"]
         if len(ext) != rotary_dim // 2:

@@ -75,6 +75,26 @@ def test_scaled_frequencies_match_transformers(scaling, length):
     assert torch.allclose(got.double(), want.double(), rtol=2.0 ** -18, atol=0)
 
 
+@pytest.mark.parametrize("extra", [{"mscale": 1.0, "mscale_all_dim": 0.8}, {"mscale": 0.7},
+                                   {"mscale": 1.0, "mscale_all_dim": 1.0}])
+@pytest.mark.parametrize("s", [1.0, 40.0])
+def test_yarn_factor_from_two_magnitudes(extra, s):
+    """m(mscale) / m(mscale_all_dim) where both are given, m(1) else."""
+    sc = {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": 4096, **extra}
+    f, factor = _ops().rope_frequencies(64, theta=10000.0, scaling=sc)
+    m = lambda k: 0.1 * k * math.log(s) + 1.0  # noqa: E731
+    want = m(extra["mscale"]) / m(extra["mscale_all_dim"]) if len(extra) == 2 else m(1.0)
+    assert factor == pytest.approx(want, rel=1e-12)
+    mod = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import Qwen2Config
+    cfg = Qwen2Config(hidden_size=256, num_attention_heads=4, num_key_value_heads=2,
+                      max_position_embeddings=int(4096 * s), rope_theta=10000.0,
+                      rope_scaling=dict(sc, rope_theta=10000.0))
+    theirs, theirs_factor = mod.ROPE_INIT_FUNCTIONS["yarn"](cfg, "cpu")
+    assert factor == pytest.approx(theirs_factor, rel=1e-6)
+    assert torch.allclose(f.double(), theirs.double(), rtol=2.0 ** -18, atol=0)
+
+
 def test_bad_frequencies_are_refused():
     ops = _ops()
     for bad in (0, -2, 7):
