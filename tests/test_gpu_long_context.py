@@ -692,3 +692,133 @@ def test_other_streams_and_threads(cuda):
         t.join()
     for o in outs:
         assert bool((o == want).all())
+
+
+# ---------------------------------------------------------------- the less usual calls
+@pytest.mark.parametrize("H,KVH,D,dtype", [(32, 1, 64, BF16), (20, 1, 128, F16), (10, 2, 128, BF16),
+                                           (6, 1, 64, F16)])
+def test_window_attention_of_other_head_groups(cuda, H, KVH, D, dtype):
+    """More query heads per KV head than a matrix tile's columns, groups that
+    leave a workgroup's head slots empty."""
+    _prefill_case(cuda, H, KVH, D, dtype, [70, 1, 140], [0, 0, 75], 50, 3, seed=H)
+    _decode_case(cuda, H, KVH, D, dtype, [70, 1, 900], 600, 3, seed=H)
+
+
+def test_window_prefill_attention_of_far_apart_prefixes(cuda):
+    """Requests hundreds of row blocks apart in their contexts, under a window
+    that is whole for none of them, and for some."""
+    for window, sinks in ((20000, 0), (3000, 5)):
+        _prefill_case(cuda, 4, 1, 64, BF16, [130, 9000, 1, 4500], [0, 8900, 0, 4444], window, sinks,
+                      seed=window)
+
+
+def test_window_prefill_attention_of_more_than_64_passes(cuda):
+    """More items than 64 for each of the card's workgroups."""
+    lens = [1 + i % 7 for i in range(300)]
+    _prefill_case(cuda, 64, 64, 64, BF16, lens, [0] * 300, 3, 1, seed=64)
+
+
+def test_window_prefill_attention_of_many_mixed_requests(cuda):
+    """More requests than a wave has lanes, with whole windows and without."""
+    g = np.random.RandomState(15)
+    lens = g.randint(1, 400, size=140).tolist()
+    before = [int(n * g.rand()) if i % 3 else 0 for i, n in enumerate(lens)]
+    _prefill_case(cuda, 2, 1, 64, BF16, lens, before, 150, 2, seed=15)
+
+
+def test_prefill_attention_into_rows_of_8_byte_alignment(cuda):
+    """The causal form takes output rows that start anywhere: the same bits as
+    into aligned ones."""
+    g = torch.Generator().manual_seed(17)
+    H, KVH, D, n = 8, 2, 64, 150
+    pool = torch.randn(n, 2 * KVH, D, generator=g).to(BF16).to(cuda)
+    table = torch.arange(n, dtype=torch.int32, device=cuda).view(1, n)
+    q = torch.randn(n, H, D, generator=g).to(BF16).to(cuda)
+    a = torch.empty_like(q)
+    wide = torch.full((n, H, D + 4), 7.0, dtype=BF16, device=cuda)
+    b = wide[..., 4:]
+    for o in (a, b):
+        _ops().prefill_attention(q, pool[:, :KVH], pool[:, KVH:], o, _i32([0], cuda),
+                                 _i32([0], cuda), _i32([n], cuda), n, table)
+    assert torch.equal(a, b) and bool((wide[..., :4] == 7.0).all())
+
+
+def test_captured_split_decodes_share_no_workspace(cuda):
+    """Two captured decodes whose lists are split, replayed on two streams at
+    once with eager ones of the same shape in between."""
+    g = torch.Generator().manual_seed(18)
+    H, KVH, D, n, window = 8, 2, 128, 3000, 2500
+    pool = torch.randn(2 * n, 2 * KVH, D, generator=g).to(BF16).to(cuda)
+    table = torch.randperm(2 * n, generator=g).to(torch.int32).view(2, n).to(cuda)
+    need = _ops()._window_decode_bytes(1, H, KVH, D, n, window, 0)
+    assert need > 0
+    k, v, lens = pool[:, :KVH], pool[:, KVH:], _i32([n], cuda)
+    qs = [torch.randn(1, H, D, generator=g).to(BF16).to(cuda) for _ in range(3)]
+    rows = [_i32([r], cuda) for r in (0, 1, 0)]
+    outs = [torch.empty_like(q) for q in qs]
+
+    def call(i):
+        _ops().window_decode_attention(qs[i], table, rows[i], lens, n, k, v, outs[i], window)
+
+    for i in range(3):
+        call(i)
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                call(i)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            for _ in range(20):
+                call(2)
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+
+
+def test_captured_window_prefill_follows_its_lengths(cuda):
+    """A captured prefill replayed after its lengths, offsets and prefixes
+    changed in place: the items follow the lengths on the device."""
+    g = torch.Generator().manual_seed(19)
+    H, KVH, D, window, sinks, most = 8, 2, 64, 70, 3, 300
+    pool = torch.randn(600, 2 * KVH, D, generator=g).to(BF16)
+    table = torch.randperm(600, generator=g).to(torch.int32).view(2, 300)
+    q = torch.randn(most, H, D, generator=g).to(BF16)
+    pd, td, qd = pool.to(cuda), table.to(cuda), q.to(cuda)
+    out = torch.empty_like(qd)
+    rows, start, lens, before = (_i32(x, cuda) for x in ([0, 1], [0, 100], [100, 200], [0, 0]))
+
+    def call():
+        _ops().window_prefill_attention(qd, pd[:, :KVH], pd[:, KVH:], out, rows, start, lens, most,
+                                        td, window, sinks=sinks, b_shared_seq_len=before)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for ls, bs in (([100, 200], [0, 0]), ([300, 1], [170, 0]), ([130, 130], [130, 0]),
+                   ([299, 300], [298, 100])):
+        new = [n - c for n, c in zip(ls, bs)]
+        for dst, val in ((start, [0, new[0]]), (lens, ls), (before, bs)):
+            dst.copy_(_i32(val, cuda))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, wgt, keys, mags = O.window_prefill(q, pool[:, :KVH], pool[:, KVH:], table, [0, 1],
+                                                 [0, new[0]], ls, bs, window, sinks)
+        b = O.bound_attention(want, wgt, keys, mags, BF16, D, O.p_rounding(BF16, False),
+                              float(pool[:, KVH:].float().abs().max()))
+        _inside(out, want, b, f"replay {ls}")
+        assert bool((out[sum(new):] == 7.0).all())
