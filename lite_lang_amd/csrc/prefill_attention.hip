@@ -13,8 +13,9 @@
 // wave's softmax overlaps the other's MFMAs, with the register budget of two
 // waves). WPH waves take query rows row0 .. row0 + 32 WPH - 1 of one head and
 // the workgroup takes 8 / WPH heads of one KV head (WPH = 2 when the group
-// size is a multiple of 4, else 4), so every K/V tile staged in LDS serves 256
-// query rows. Two waves per SIMD half a tile apart (one's scores meet the
+// size is a multiple of 4, else 4; windowed calls also take WPH = 1 and 8, by
+// the rule at the launch), so every K/V tile staged in LDS serves 256 query
+// rows. The two waves of a SIMD run half a tile apart (one's scores meet the
 // other's softmax). Per 64-key tile:
 //   * K and V rows are DMA'd through the slot table straight into a 4-stage
 //     LDS ring (global_load_lds_dwordx4), two tiles ahead of the one being
@@ -1080,9 +1081,23 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
       LL_RETURN_LAUNCH();
     });
   }
+  int cus = 0;
+  const int rc = ll_device_cus(&cus);
+  if (rc != LL_OK) return rc;
   // four heads of 64 rows per workgroup when the group size allows, else two
-  // heads of 128 rows (fewer idle head slots for G = 6 or 7)
-  const int wph = (a.G % 4 == 0) ? 2 : 4;
+  // heads of 128 rows (fewer idle head slots for G = 6 or 7). Windowed, also
+  // * eight heads of 32 rows for a group one short of eight: as few idle slots
+  //   as two heads, a shorter stretch of keys per item (28/4 heads, 40 x 600
+  //   under a window of 256 181 -> 159 us, under 64 146 -> 122, 64 x 150 74 ->
+  //   54; the worst of 14 shapes, 4 x 300, 19.8 -> 21.3);
+  // * one head of 256 rows for single-head groups (16/16 heads, 40 x 600 under
+  //   256 158 -> 136 us; 4 x 300 17.1 -> 18.7);
+  // * one head for short calls that fit one pass: the up to four waves with
+  //   rows then have a SIMD each, and rows and heads spread over more CUs
+  //   (16/2 heads, 1 x 20 tokens 9.6 -> 8.6 us, 8 x 128 17.1 -> 12.0; where
+  //   they do not fit one pass 40 x 100 20.7 -> 26.3).
+  const bool single = a.G == 1 || (max_input_len <= 128 && batch * q_heads <= cus);
+  const int wph = win && single ? 8 : win && a.G % 8 == 7 ? 1 : a.G % 4 == 0 ? 2 : 4;
   a.nblk = (int)ll_cdiv(max_input_len, 32 * wph);
   a.B = (int)batch;
   a.KVH = (int)kv_heads;
@@ -1093,9 +1108,6 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   // a multiple of 16 so that the head groups of a (row block, request, KV
   // head) share an XCD on the reversed passes too; more when the items
   // would need more than 64 passes
-  int cus = 0;
-  const int rc = ll_device_cus(&cus);
-  if (rc != LL_OK) return rc;
   int64_t P = std::max<int64_t>(16, cus / 16 * 16);
   if (ll_cdiv(nv, P) > 64) P = (int64_t)ll_cdiv(ll_cdiv(nv, 64), 16) * 16;
   P = std::min(P, nv);
@@ -1111,7 +1123,11 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
       hipLaunchKernelGGL(kernel, grid, block, lds, stream, a.seq_len, a.shared, a.start_loc,
                          a.req_idx, idx64, a.nblk, a.B, a.KVH, a.G, (int)nv, a);
     };
-    if (wph == 2) {
+    if (wph == 8) {
+      go(prefill_attn_fa_kernel<T, D, 8, true>);
+    } else if (wph == 1) {
+      go(prefill_attn_fa_kernel<T, D, 1, true>);
+    } else if (wph == 2) {
       if (win) go(prefill_attn_fa_kernel<T, D, 2, true>);
       else go(prefill_attn_fa_kernel<T, D, 2, false>);
     } else {

@@ -712,6 +712,30 @@ def test_window_prefill_attention_of_far_apart_prefixes(cuda):
                       seed=window)
 
 
+@pytest.mark.parametrize("H,KVH,D,dtype", HEADS[:4])
+def test_window_prefill_attention_of_short_prompts(cuda, H, KVH, D, dtype):
+    """Prompts of up to 128 tokens, few and many, alone and behind prefixes."""
+    for window, sinks in ((9, 2), (200, 0)):
+        _prefill_case(cuda, H, KVH, D, dtype, [1], [0], window, sinks, seed=1)
+        _prefill_case(cuda, H, KVH, D, dtype, [128, 1, 33], [0, 0, 0], window, sinks, seed=2)
+        _prefill_case(cuda, H, KVH, D, dtype, [128, 64, 70], [100, 64, 1], window, sinks, seed=3)
+        _prefill_case(cuda, H, KVH, D, dtype, [100 - 2 * i for i in range(40)], [0] * 40, window,
+                      sinks, seed=4)
+
+
+@pytest.mark.parametrize("H,KVH", [(7, 1), (14, 2), (2, 2)])
+def test_window_prefill_attention_of_one_head_or_all_per_item(cuda, H, KVH):
+    """Row blocks of 32 and of 256 rows: ragged ends, prefixes, whole windows
+    and not, several blocks and requests per workgroup."""
+    for window, sinks in ((31, 0), (32, 3), (257, 70)):
+        _prefill_case(cuda, H, KVH, 64, BF16, [600, 33, 257, 32], [0, 1, 256, 0], window, sinks,
+                      seed=window)
+    _prefill_case(cuda, H, KVH, 128, F16, [1500, 300], [1100, 0], 500, 1, seed=7)
+    lens = [1 + 13 * i % 190 for i in range(90)]
+    _prefill_case(cuda, H, KVH, 64, F16, lens, [n // 2 if i % 2 else 0 for i, n in enumerate(lens)],
+                  60, 4, seed=8)
+
+
 def test_window_prefill_attention_of_more_than_64_passes(cuda):
     """More items than 64 for each of the card's workgroups."""
     lens = [1 + i % 7 for i in range(300)]
