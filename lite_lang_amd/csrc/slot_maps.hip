@@ -14,12 +14,13 @@
 // more than having every workgroup sum the batch's lengths for itself. It
 // checks everything before it writes anything: what is wrong is reported in
 // counts[2] and the tables stay as they were.
+#include <algorithm>
+
 #include "ll_common.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 1024;      // new tokens per workgroup
 constexpr int kMaxBatch = 8192;    // requests (two int32 sums each in LDS: 64 KB)
 constexpr int kMaxRows = 1 << 18;  // slot-table rows (a bit each in LDS: 32 KB)
 
@@ -32,7 +33,7 @@ struct SlotMapArgs {
   int32_t* blocks; int64_t blocks_stride, blocks_cols;  // P > 1
   int32_t* slots; int32_t* positions; int64_t cap;
   int32_t* start; int32_t* last; int32_t* counts;
-  int B, page;
+  int B, page, per;  // per: new tokens per workgroup
 };
 
 enum { kBadLength = 1, kBadRow = 2, kNoRoom = 4, kNoPages = 8 };
@@ -127,8 +128,8 @@ __global__ __launch_bounds__(kThreads) void slot_maps_kernel(SlotMapArgs a) {
     bp += np;
   }
   __syncthreads();
-  const int64_t end = min(total_t, ((int64_t)blockIdx.x + 1) * kTokens);
-  for (int64_t i = (int64_t)blockIdx.x * kTokens + tid; i < end; i += kThreads) {
+  const int64_t end = min(total_t, ((int64_t)blockIdx.x + 1) * a.per);
+  for (int64_t i = (int64_t)blockIdx.x * a.per + tid; i < end; i += kThreads) {
     // the last request whose first new token is at or before i (requests
     // without new tokens share the start of the one behind them)
     int lo = 0, hi = a.B - 1;
@@ -192,8 +193,17 @@ extern "C" int ll_build_slot_maps(const void* b_req_idx, int req_idx_i64, const 
   a.slots = slots; a.positions = positions; a.cap = max_tokens;
   a.start = b_start_loc; a.last = last_rows; a.counts = counts;
   a.B = (int)batch; a.page = (int)page_size;
-  // the new tokens are known on the device only: workgroups for all that fit
-  const unsigned grid = (unsigned)(max_tokens > kTokens ? ll_cdiv(max_tokens, kTokens) : 1);
+  // The new tokens are known on the device only: workgroups for all that fit.
+  // A token's loads are a chain (its request's values, its page, the store), so
+  // a thread has one token while that gives up to 2048 workgroups, and the
+  // fewest tokens that does beyond, since each of those sums the batch for
+  // itself (in a graph, 1 / 2 / 4 per thread: 1 x 4096 tokens 4.4 / 4.9 / 6.1
+  // us, 128 x up to 4096 in pages of 16 6.6 / 7.0 / 8.2, 1000 x 600 11.5 / 11.1
+  // / 12.7, 256 x 8000 21.0 / 16.5 / 14.6).
+  int64_t per = kThreads;
+  while (max_tokens > 2048 * per) per *= 2;
+  a.per = (int)per;
+  const unsigned grid = (unsigned)std::max<int64_t>(1, ll_cdiv(max_tokens, per));
   const size_t lds = (size_t)batch * 8 + (size_t)((req_rows + 31) / 32) * 4;
   hipLaunchKernelGGL(slot_maps_kernel, dim3(grid), dim3(kThreads), lds, stream, a);
   LL_RETURN_LAUNCH();

@@ -503,6 +503,14 @@ def test_slot_maps_of_large_batches(cuda, B):
     _maps_case(cuda, lens, before, 4, seed=B)
 
 
+@pytest.mark.parametrize("page", [1, 16])
+def test_slot_maps_of_many_tokens(cuda, page):
+    """Room for more tokens than a thread each: none, few and all of it used."""
+    _maps_case(cuda, [3, 3], [3, 3], page, cap_extra=1300001)
+    _maps_case(cuda, [700, 30, 1], [11, 0, 0], page, seed=1, cap_extra=400000)
+    _maps_case(cuda, [70001, 0, 130000, 150003, 17], [33, 0, 1000, 0, 16], page, seed=2)
+
+
 def test_slot_maps_report_what_does_not_fit(cuda):
     """Nothing but counts is written where something is wrong."""
     _maps_case(cuda, [5, 9], [2, 0], 1, spare=-1, expect=8)
