@@ -268,6 +268,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // is valid when its row block starts inside its request's query rows.
   int it_L = 0, it_S = 0, it_blk0 = 0, it_kvend = 1, it_nt = 0, it_kvh = 0, it_hp = 0;
   int it_low = 0, it_sk = 0;  // WIN: first key of the window's tiles, sinks apart from them
+  int it_half = -1;           // WIN: the four waves (0-3, 4-7) that have the item, -1: all
   int64_t it_start = 0, it_rid = 0;
   bool it_ok = false;
   if constexpr (WIN) {
@@ -279,13 +280,37 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     // window is whole, all alike in cost, request after request; then those
     // nearer their context's start by level, the multiple of BQ that their
     // first position is at or above, the highest level first.
-    const int64_t vb = fa_item_of_pass(lane, P, w);
+    struct Requests { int64_t L, S, start, rid; };
+    auto requests = [&](int c0) {
+      const int b = min(c0 + lane, B - 1);
+      return Requests{ll_load_idx(p_len, b, idx64 & 1),
+                      p_shared ? ll_load_idx(p_shared, b, (idx64 >> 1) & 1) : 0,
+                      ll_load_idx(p_start, b, (idx64 >> 2) & 1),
+                      ll_load_idx(p_rid, b, (idx64 >> 3) & 1)};
+    };
+    auto scan = [&](int v) { return lane_scan(v, 0, [](int x, int y) { return x + y; }); };
+    auto blocks = [&](const Requests& q, int nreq) {
+      return lane < nreq && q.L > q.S ? ((int)q.L - (int)q.S + SH::BQ - 1) / SH::BQ : 0;
+    };
+    const Requests head = requests(0);
+    int total = rl(scan(blocks(head, min(B, 64))), 63);
+    for (int c0 = 64; c0 < B; c0 += 64) total += rl(scan(blocks(requests(c0), min(B - c0, 64))), 63);
+    // Items for at most half of the workgroups are dealt out by halves: two
+    // workgroups of an XCD take an item, one its waves 0-3, one its waves 4-7,
+    // which have a SIMD each (16/2 heads, 1 x 256 tokens 16.9 -> 14.5 us, 1 x 700
+    // under a window of 256 21.2 -> 18.5; the last pass of a longer call so: 16 x
+    // 300 under 100 24.3 -> 28.0).
+    const int nitems = (total * KVH + 7) / 8 * 8 * HP;
+    int64_t vb = fa_item_of_pass(lane, P, w);
+    if (SH::WPH < SH::NW && 2 * nitems <= P) {
+      it_half = (w >> 3) & 1;
+      vb = lane == 0 && w < 2 * nitems ? 8 * (w >> 4) + (w & 7) : nv;
+    }
     const int ui = vb < nv ? ((int)(vb >> 3) / HP) * 8 + (int)(vb & 7) : 0;
     const int want = vb < nv ? ui / KVH : INT32_MAX;  // the lane's (request, block) in that order
     it_kvh = ui % KVH;
     it_hp = vb < nv ? (int)(vb >> 3) % HP : 0;
     const int lam = (a.window + SH::BQ - 1) / SH::BQ;  // level from which the window is whole
-    auto scan = [&](int v) { return lane_scan(v, 0, [](int x, int y) { return x + y; }); };
     auto highest = [&](int v) {
       return rl(lane_scan(v, INT32_MIN, [](int x, int y) { return max(x, y); }), 63);
     };
@@ -299,14 +324,11 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     };
     int base = 0;  // (request, block)s listed so far
     for (int c0 = 0; c0 < B; c0 += 64) {
-      const int b = min(c0 + lane, B - 1), nreq = min(B - c0, 64);
-      const int64_t Lb = ll_load_idx(p_len, b, idx64 & 1);
-      const int64_t Sb = p_shared ? ll_load_idx(p_shared, b, (idx64 >> 1) & 1) : 0;
-      const int64_t start_b = ll_load_idx(p_start, b, (idx64 >> 2) & 1);
-      const int64_t rid_b = ll_load_idx(p_rid, b, (idx64 >> 3) & 1);
-      const int L = (int)Lb, S = (int)Sb;
+      const int nreq = min(B - c0, 64);
+      const Requests q = c0 == 0 ? head : requests(c0);
+      const int L = (int)q.L, S = (int)q.S;
       // its blocks, the levels of the first `ramp` of them, the number of whole ones
-      const int nb = lane < nreq && Lb > Sb ? (L - S + SH::BQ - 1) / SH::BQ : 0;
+      const int nb = blocks(q, nreq);
       const int l0 = S / SH::BQ;
       const int ramp = min(nb, max(0, lam - l0)), full = nb - ramp;
       int src = -1, blk = 0;  // lane's request (as a lane number) and row block
@@ -369,7 +391,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       }
       const int from = max(src, 0);
       const int Lx = __shfl(L, from, 64), Sx = __shfl(S, from, 64);
-      const int64_t startx = shfl64(start_b, from), ridx = shfl64(rid_b, from);
+      const int64_t startx = shfl64(q.start, from), ridx = shfl64(q.rid, from);
       if (src >= 0) {
         it_ok = true;
         it_L = Lx;
@@ -442,6 +464,10 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     r.row0 = blk0 + SH::RW * (wave % SH::WPH);
     r.qlast = L - S - 1;
     r.ok = gh < G && r.row0 <= r.qlast;
+    if constexpr (WIN) {
+      const int half = rl(it_half, k);
+      r.ok = r.ok && (half < 0 || half == wave / 4);
+    }
     r.S = S;
     r.Lm1 = L - 1;
     r.kv_end = (int)min((int64_t)L, (int64_t)r.row0 + SH::RW + S);
@@ -1093,9 +1119,10 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   // * one head of 256 rows for single-head groups (16/16 heads, 40 x 600 under
   //   256 158 -> 136 us; 4 x 300 17.1 -> 18.7);
   // * one head for short calls that fit one pass: the up to four waves with
-  //   rows then have a SIMD each, and rows and heads spread over more CUs
-  //   (16/2 heads, 1 x 20 tokens 9.6 -> 8.6 us, 8 x 128 17.1 -> 12.0; where
-  //   they do not fit one pass 40 x 100 20.7 -> 26.3).
+  //   rows then have a SIMD each, without a second workgroup for the other
+  //   half (16/2 heads, 1 x 20 tokens 9.6 -> 8.6 us, 8 x 128 17.1 -> 12.0, by
+  //   halves of two heads 9.1 and 14.9; where they do not fit one pass 40 x 100
+  //   20.7 -> 26.3).
   const bool single = a.G == 1 || (max_input_len <= 128 && batch * q_heads <= cus);
   const int wph = win && single ? 8 : win && a.G % 8 == 7 ? 1 : a.G % 4 == 0 ? 2 : 4;
   a.nblk = (int)ll_cdiv(max_input_len, 32 * wph);
@@ -1110,7 +1137,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   // would need more than 64 passes
   int64_t P = std::max<int64_t>(16, cus / 16 * 16);
   if (ll_cdiv(nv, P) > 64) P = (int64_t)ll_cdiv(ll_cdiv(nv, 64), 16) * 16;
-  P = std::min(P, nv);
+  // (windowed: room for the halves of a call with few items)
+  P = std::min(P, win && wph < 8 ? 2 * nv : nv);
   const dim3 grid((unsigned)P);
   const dim3 block(512);
   auto launch = [&](auto tag, auto dtag) {
