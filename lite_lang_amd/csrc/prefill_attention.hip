@@ -290,7 +290,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     };
     auto scan = [&](int v) { return lane_scan(v, 0, [](int x, int y) { return x + y; }); };
     auto blocks = [&](const Requests& q, int nreq) {
-      return lane < nreq && q.L > q.S ? ((int)q.L - (int)q.S + SH::BQ - 1) / SH::BQ : 0;
+      return lane < nreq && q.L > q.S ? min(((int)q.L - (int)q.S + SH::BQ - 1) / SH::BQ, nblk) : 0;
     };
     const Requests head = requests(0);
     int total = rl(scan(blocks(head, min(B, 64))), 63);

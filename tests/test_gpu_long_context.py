@@ -240,7 +240,7 @@ def _cache(g, lens, before, window, sinks, KVH, D, dtype):
 
 
 def _prefill_case(cuda, H, KVH, D, dtype, lens, before, window, sinks, seed=0, idx=torch.int32,
-                  pad=0, scale=None, mag=1.0):
+                  pad=0, scale=None, mag=1.0, most=None):
     print(f"case: window prefill H={H}/{KVH} D={D} {dtype} lens={lens} before={before} "
           f"window={window} sinks={sinks} pad={pad}", flush=True)
     g = torch.Generator().manual_seed(seed)
@@ -255,14 +255,17 @@ def _prefill_case(cuda, H, KVH, D, dtype, lens, before, window, sinks, seed=0, i
     pd = pool.to(cuda)
     shared = None if not any(before) else _i32(before, cuda, idx)
     _ops().window_prefill_attention(qd, pd[:, :KVH], pd[:, KVH:], out, _i32(rids, cuda, idx),
-                                    _i32(starts, cuda, idx), _i32(lens, cuda, idx), max(lens),
-                                    table.to(cuda), window, sinks=sinks, b_shared_seq_len=shared,
+                                    _i32(starts, cuda, idx), _i32(lens, cuda, idx),
+                                    max(lens) if most is None else most, table.to(cuda), window, sinks=sinks, b_shared_seq_len=shared,
                                     sm_scale=scale)
     torch.cuda.synchronize()
     want, wgt, keys, mags = O.window_prefill(q, pool[:, :KVH], pool[:, KVH:], table, rids, starts,
                                              lens, before, window, sinks, scale)
     b = O.bound_attention(want, wgt, keys, mags, dtype, D, O.p_rounding(dtype, False),
                           float(pool[:, KVH:].float().nan_to_num().abs().max()))
+    if most is not None:  # rows behind the bound may hold anything
+        for at, n in zip(starts, new):
+            want[at + most:at + max(n, most)] = float("nan")
     _inside(out, want, b, "out")
     nobody = torch.ones(T, dtype=torch.bool)
     nobody[2:2 + sum(new)] = False
@@ -718,6 +721,14 @@ def test_window_prefill_attention_of_far_apart_prefixes(cuda):
     for window, sinks in ((20000, 0), (3000, 5)):
         _prefill_case(cuda, 4, 1, 64, BF16, [130, 9000, 1, 4500], [0, 8900, 0, 4444], window, sinks,
                       seed=window)
+
+
+@pytest.mark.parametrize("H,KVH,D,dtype", HEADS[:5])
+def test_window_prefill_attention_takes_the_bound(cuda, H, KVH, D, dtype):
+    """A bound of the query rows alone, and requests with more rows than it."""
+    for lens, before, most in (([500, 40, 333], [430, 0, 333], 70), ([130, 900], [0, 890], 130),
+                               ([700, 5, 64], [0, 0, 0], 200), ([90] * 70, [0, 80] * 35, 32)):
+        _prefill_case(cuda, H, KVH, D, dtype, lens, before, 50, 3, seed=most, most=most)
 
 
 @pytest.mark.parametrize("H,KVH,D,dtype", HEADS[:4])
