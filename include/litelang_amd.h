@@ -145,9 +145,9 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * The two calls above for contexts of which only the last `window` tokens and
  * the first `sinks` ones are kept: a query at position p sees the keys n <= p
  * with n > p - window (its own included) or n < sinks. window >= 1, sinks >= 0
- * (both may exceed the length); lengths at most 2^30; sm_scale > 0. No
- * counterpart in the reference (whose configs' use_sliding_window it does not
- * read).
+ * (both may exceed the length); lengths at most 2^30, at most 2^24 requests and
+ * 65535 query heads; sm_scale > 0. No counterpart in the
+ * reference (whose configs' use_sliding_window it does not read).
  * No entry of the slot table is read but those of keys that some query of the
  * request's call sees, so the tokens between the sinks and the window may have
  * left the cache and their entries may hold anything. Keys and values that one

@@ -1500,6 +1500,8 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
                "%s: null pointer", fn);
   LL_CHECK_ARG(kv_heads > 0 && q_heads % kv_heads == 0,
                "%s: q_heads %lld not a multiple of kv_heads %lld", fn, (long long)q_heads, (long long)kv_heads);
+  LL_CHECK_ARG(!win || (batch >= 0 && batch <= 1 << 24 && q_heads > 0 && q_heads <= 65535),
+               "%s: %lld requests of %lld heads", fn, (long long)batch, (long long)q_heads);
   LL_CHECK_ARG(head_dim > 0 && head_dim <= 256, "%s: head_dim %lld unsupported", fn,
                (long long)head_dim);
   LL_CHECK_ARG(max_len_in_batch >= 0 && max_len_in_batch <= (win ? 1 << 30 : INT32_MAX),

@@ -1057,6 +1057,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                "%s: null pointer", fn);
   LL_CHECK_ARG(kv_heads > 0 && q_heads % kv_heads == 0,
                "%s: q_heads %lld not a multiple of kv_heads %lld", fn, (long long)q_heads, (long long)kv_heads);
+  LL_CHECK_ARG(!win || (batch >= 0 && batch <= 1 << 24 && q_heads > 0 && q_heads <= 65535),
+               "%s: %lld requests of %lld heads", fn, (long long)batch, (long long)q_heads);
   LL_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0,
                "%s: head_dim %lld unsupported", fn, (long long)head_dim);
   // window 1 sees the query's own token alone: no row is left without a key

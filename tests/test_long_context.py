@@ -251,14 +251,14 @@ def test_c_entry_points_refuse_before_any_launch():
     def err():
         return L.ll_last_error().decode()
 
-    def prefill(H=4, KVH=2, D=64, window=8, sinks=0, q=p, scale=1.0, most=8):
+    def prefill(H=4, KVH=2, D=64, window=8, sinks=0, q=p, scale=1.0, most=8, B=2):
         return L.ll_window_prefill_attention(q, H * D, D, p, 2 * KVH * D, D, p, 2 * KVH * D, D, p,
-                                             H * D, D, p, 8, p, 0, p, 0, p, 0, None, 0, 2, H, KVH,
+                                             H * D, D, p, 8, p, 0, p, 0, p, 0, None, 0, B, H, KVH,
                                              D, most, window, sinks, f(scale), 2, None)
 
-    def decode(H=4, KVH=2, D=64, window=8, sinks=0, q=p, scale=1.0, most=8):
+    def decode(H=4, KVH=2, D=64, window=8, sinks=0, q=p, scale=1.0, most=8, B=2):
         return L.ll_window_decode_attention(q, H * D, D, p, 2 * KVH * D, D, p, 2 * KVH * D, D, p, 8,
-                                            p, 0, p, 0, p, H * D, D, 2, H, KVH, D, most, window,
+                                            p, 0, p, 0, p, H * D, D, B, H, KVH, D, most, window,
                                             sinks, f(scale), 2, None, 0, None)
 
     for call in (prefill, decode):
@@ -269,6 +269,9 @@ def test_c_entry_points_refuse_before_any_launch():
         for scale in (0.0, -1.0, float("nan"), float("inf")):
             assert call(scale=scale) == -1 and "sm_scale" in err()
         assert call(D=512) == -1 and "head_dim" in err()
+        assert call(B=-1) == -1 and "requests" in err()
+        assert call(B=1 << 25) == -1 and "requests" in err()
+        assert call(H=0) == -1 and "heads" in err()
         assert call(most=(1 << 30) + 1) == -1 and "out of range" in err()
 
     def rope(R=64, D=64, ntok=2, out=p, pos=p):
