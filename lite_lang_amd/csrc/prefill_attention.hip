@@ -232,11 +232,13 @@ __device__ __forceinline__ int64_t fa_item_of_pass(int j, int P, int w) {
 // SGPRs at dispatch, so those loads do not wait for the argument block's
 // load. idx64: bit 0 lengths, 1 shared, 2 starts, 3 request rows are int64.
 // nv: virtual blocks (items, valid or not) of the launch.
-// WIN: windowed. An item's tiles are its sinks' (none where they meet its
-// window, whose range then starts at key 0) and then those of its window,
-// which starts at the first key that the item's first row sees, so that no
-// table entry below it is read. A wave leaves out the tiles in which none of
-// its rows sees a key, and masks those that some of its rows see in part.
+// WIN: windowed. An item's keys are its sinks and, from the first key that its
+// first row sees, its window, taken as one list (a tile of their own for the
+// sinks cost 16/2 heads, 40 x 600 under 256 with 4 sinks one tile in six), so
+// that no table entry in between is read. In the list's positions the masks
+// are those of a window with sinks from key 0 on. A wave leaves out the tiles in
+// which none of its rows sees a key, and masks those that some of its rows see
+// in part.
 template <typename T, int D, int WPH, bool WIN>
 __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     const void* __restrict__ p_len, const void* __restrict__ p_shared,
@@ -267,7 +269,9 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // and head group, its first query row, key count and tile count). An item
   // is valid when its row block starts inside its request's query rows.
   int it_L = 0, it_S = 0, it_blk0 = 0, it_kvend = 1, it_nt = 0, it_kvh = 0, it_hp = 0;
-  int it_low = 0, it_sk = 0;  // WIN: first key of the window's tiles, sinks apart from them
+  // WIN: the item's keys are one list, key j below it_sk (sinks apart from its
+  // window), else j + it_skip; its lengths and positions are counted in it
+  int it_sk = 0, it_skip = 0;
   int it_half = -1;           // WIN: the four waves (0-3, 4-7) that have the item, -1: all
   int64_t it_start = 0, it_rid = 0;
   bool it_ok = false;
@@ -394,16 +398,16 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       const int64_t startx = shfl64(q.start, from), ridx = shfl64(q.rid, from);
       if (src >= 0) {
         it_ok = true;
-        it_L = Lx;
-        it_S = Sx;
         it_start = startx;
         it_rid = ridx;
         it_blk0 = blk * SH::BQ;
-        it_kvend = (int)min((int64_t)Lx, (int64_t)it_blk0 + SH::BQ + Sx);
         const WindowRange r = window_range((int64_t)it_blk0 + Sx, a.window, a.sinks);
-        it_low = r.low;
         it_sk = r.sinks;
-        it_nt = (it_sk + kBK - 1) / kBK + (it_kvend - it_low + kBK - 1) / kBK;
+        it_skip = r.low - r.sinks;
+        it_L = Lx - it_skip;
+        it_S = Sx - it_skip;  // (below 0 from a row block past the window on)
+        it_kvend = min(it_L, it_blk0 + SH::BQ + it_S);
+        it_nt = (it_kvend + kBK - 1) / kBK;
       }
     }
   } else {
@@ -452,7 +456,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   struct WaveItem {
     int64_t start;
     int h, row0, qlast, S, Lm1, kv_end;
-    int low, sk, nst;  // WIN: the item's window start, sinks apart from it, their tiles
     bool ok;
   };
   auto wave_item = [&](int k) -> WaveItem {
@@ -471,11 +474,6 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     r.S = S;
     r.Lm1 = L - 1;
     r.kv_end = (int)min((int64_t)L, (int64_t)r.row0 + SH::RW + S);
-    if constexpr (WIN) {
-      r.low = rl(it_low, k);
-      r.sk = rl(it_sk, k);
-      r.nst = (r.sk + kBK - 1) / kBK;
-    }
     return r;
   };
   // Q^T fragments (B operand: column = query row row0 + l32, clamped into the
@@ -514,7 +512,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // stays on the last item's last tile.
   struct SlotCursor {
     int k, u, nt, last_key;
-    int low, last_sink, nst;  // WIN
+    int sk, skip;  // WIN
     const int32_t* row;
   };
   struct KvCursor {
@@ -528,9 +526,8 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     c.nt = rl(it_nt, k);
     c.last_key = rl(it_kvend, k) - 1;
     if constexpr (WIN) {
-      c.low = rl(it_low, k);
-      c.last_sink = rl(it_sk, k) - 1;
-      c.nst = (c.last_sink + kBK) / kBK;
+      c.sk = rl(it_sk, k);
+      c.skip = rl(it_skip, k);
     }
     c.row = a.r2t + rl64(it_rid, k) * a.r2t_s;
   };
@@ -555,12 +552,9 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   };
   const int k_first = (int)__builtin_ctzll(items);
   // slot ids of cursor c's tile (keys 64 u + lane, clamped) -> ring entry x % NST
-  // (WIN: the window's tiles start at its first key, clamped likewise)
   auto slot_copy = [&](int x, const SlotCursor& c) {
     int key = min(c.u * kBK + lane, c.last_key);
-    if constexpr (WIN)
-      key = c.u < c.nst ? min(c.u * kBK + lane, c.last_sink)
-                        : min(c.low + (c.u - c.nst) * kBK + lane, c.last_key);
+    if (WIN && key >= c.sk) key += c.skip;
     dma4(c.row + key, wslots + (x % NST) * (kBK * 4));
   };
   // this wave's K and V rows of cursor c's tile (slot ids in ring entry
@@ -631,9 +625,9 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // half-wave's keys in m_cand
   f32x16 sacc[2][QB];
   float m_cand[QB];
-  // (t0: the tile's first key; WIN: top is the last key of the tile's range)
+  // (t0: the tile's first key)
   // (masked false_type: the caller knows that every row sees the whole tile)
-  auto scores = [&](auto masked, int t0, int buf, int top) {
+  auto scores = [&](auto masked, int t0, int buf) {
     const char* kl = smem + buf * FG::STAGE_B;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -662,16 +656,15 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     // row's limit (masked keys -> -inf), then the tile's row maxima in the
     // exp2 domain (finite: key 0 is visible to every row, scale_log2 > 0)
     const int last_row_low = cur.row0 + SH::RW - 1 + cur.S - a.window;  // below its window
-    const bool need_mask = WIN ? t0 + kBK - 1 > min(cur.row0 + cur.S, top) ||
-                                     (t0 <= last_row_low && t0 + kBK > a.sinks)
-                               : t0 + kBK - 1 > min(cur.row0 + cur.S, cur.Lm1);
+    const bool need_mask = t0 + kBK - 1 > min(cur.row0 + cur.S, cur.Lm1) ||
+                           (WIN && t0 <= last_row_low && t0 + kBK > a.sinks);
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       if (decltype(masked)::value && need_mask) {
         // last key this row sees, relative to the tile (rows past the
         // request see every key of it)
         const int p = cur.row0 + 32 * qb + l32 + cur.S;
-        const int lim = min(p, WIN ? top : cur.Lm1) - t0;
+        const int lim = min(p, cur.Lm1) - t0;
         // The visible keys as bits, shifted out from the top in the order of
         // the lane's elements: an add and a select per element where compares
         // of each key with the row's limits take four and scalar logic (a
@@ -882,19 +875,19 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
     // window of 4096 1039 -> 985 us)
     int run = cs.nt - 1 - cs.u;
     if (run > 1 && cc_u > 0 && covered == 0 && cur.ok) {
-      const int u = WIN ? cc_u - cur.nst : cc_u, su = WIN ? cs.u - cs.nst : cs.u;
-      const int first = (WIN ? cur.low : 0) + u * kBK;  // key of tile x
-      const bool whole = !WIN || (u >= 0 && su >= 0 && first > cur.row0 + SH::RW - 1 + cur.S - a.window);
+      const int first = cc_u * kBK;  // key of tile x
+      const bool whole = !WIN || (cs.u * kBK >= cs.sk &&
+                                  first > cur.row0 + SH::RW - 1 + cur.S - a.window);
       run = min(min(run, ck.left - 1), min(cc_nt - 1 - cc_u,
                                            (min(cur.row0 + cur.S, cur.Lm1) + 1 - first) / kBK));
       if (whole && run > 0) {
-        const int32_t* ids = cs.row + (WIN ? cs.low : 0) + su * kBK + lane;
+        const int32_t* ids = cs.row + (WIN ? cs.skip : 0) + cs.u * kBK + lane;
         cc_u += run;
         ck.left -= run;
         cs.u += run;
         for (; run > 0; --run, ++x, ids += kBK) {
           if (lead) event();
-          scores(std::false_type{}, 0, x % NST, 0);
+          scores(std::false_type{}, 0, x % NST);
           kv_copy(x + kAhead, ck);
           dma4(ids, wslots + ((x + 2 * kAhead) % NST) * (kBK * 4));
           if (!lead) event();  // (of tile x + 1, which there is)
@@ -920,22 +913,13 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
       reset();
     }
     const int buf = x % NST;
-    int t0 = cc_u * kBK, top = cur.Lm1;
-    bool work = cur.ok && t0 < cur.kv_end;
-    if constexpr (WIN) {
-      if (cc_u < cur.nst) {
-        top = cur.sk - 1;  // a sink tile: every row sees all of its keys
-        work = cur.ok;
-      } else {
-        // not where the causal limit or the wave's first row's window leaves
-        // the tile out, but where it holds sinks
-        t0 = cur.low + (cc_u - cur.nst) * kBK;
-        work = cur.ok && t0 < cur.kv_end &&
-               (t0 + kBK - 1 > cur.row0 + cur.S - a.window || t0 < a.sinks);
-      }
-    }
+    const int t0 = cc_u * kBK;
+    // not where the causal limit or the wave's first row's window leaves the
+    // tile out, but where it holds sinks
+    const bool work = cur.ok && t0 < cur.kv_end &&
+                      (!WIN || t0 + kBK - 1 > cur.row0 + cur.S - a.window || t0 < a.sinks);
     const bool last = cc_u + 1 == cc_nt;
-    if (work) scores(std::true_type{}, t0, buf, top);
+    if (work) scores(std::true_type{}, t0, buf);
     // (behind the score MFMAs, which run on while the addresses are computed)
     kv_copy(x + kAhead, ck);
     kv_next(ck);
@@ -1118,6 +1102,9 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   //   as two heads, a shorter stretch of keys per item (28/4 heads, 40 x 600
   //   under a window of 256 181 -> 159 us, under 64 146 -> 122, 64 x 150 74 ->
   //   54; the worst of 14 shapes, 4 x 300, 19.8 -> 21.3);
+  //   the same for a multiple of eight where the shorter stretch is a tile less
+  //   (16/2 heads with 4 sinks, 40 x 600 under 128 91 -> 80 us, under 256 101 ->
+  //   94; where it is not, 1 x 8192 under 64 without sinks 29.3 -> 34.7);
   // * one head of 256 rows for single-head groups (16/16 heads, 40 x 600 under
   //   256 158 -> 136 us; 4 x 300 17.1 -> 18.7);
   // * one head for short calls that fit one pass: the up to four waves with
@@ -1126,7 +1113,11 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   //   halves of two heads 9.1 and 14.9; where they do not fit one pass 40 x 100
   //   20.7 -> 26.3).
   const bool single = a.G == 1 || (max_input_len <= 128 && batch * q_heads <= cus);
-  const int wph = win && single ? 8 : win && a.G % 8 == 7 ? 1 : a.G % 4 == 0 ? 2 : 4;
+  auto tiles = [&](int w) {  // of an item whose window is whole
+    return ((int64_t)a.window + a.sinks + 32 * w - 1 + kBK - 1) / kBK;
+  };
+  const bool eight = a.G % 8 == 7 || (a.G % 8 == 0 && tiles(1) < tiles(2));
+  const int wph = win && single ? 8 : win && eight ? 1 : a.G % 4 == 0 ? 2 : 4;
   a.nblk = (int)ll_cdiv(max_input_len, 32 * wph);
   a.B = (int)batch;
   a.KVH = (int)kv_heads;
