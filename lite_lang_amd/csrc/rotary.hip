@@ -47,8 +47,7 @@ __device__ __forceinline__ void rot_angle(int64_t pos, float inv_freq, float fac
 
 // Any head_dim, rotary_dim and alignment, for the shapes and strides that the
 // 16-byte form below does not take (24,000 tokens of 28/4 heads of 128: 247 us
-// against its 68): one wave per (token, head), a lane
-// per pair.
+// against its 68): one wave per (token, head), a lane per pair.
 template <typename T, bool INTER>
 __global__ __launch_bounds__(64) void rotary_kernel(RotArgs a) {
   const int64_t t = blockIdx.x;
@@ -102,7 +101,9 @@ __global__ __launch_bounds__(64) void rotary_kernel(RotArgs a) {
 // sincospif, are computed once per token and pair into LDS and shared by its
 // heads, while the first heads' loads are in flight; a workgroup takes TB
 // tokens so that there are enough heads to cover that. The norm's sum stays in
-// the LPH lanes of its head.
+// the LPH lanes of its head; the gammas are read for every head again (from the
+// L1; in registers they cost a fifth of the waves: 4000 tokens of 16/2 heads of
+// 128 10.4 -> 13.0 us).
 template <typename T> struct alignas(16) Chunk { T v[8]; };
 
 // Stores go out non-temporally: nothing of this call reads them, and the lines
@@ -120,28 +121,46 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* p, const Ch
 
 constexpr int kRotThreads = 256;
 
+// What the 16-byte form's addresses are made of. A workgroup's tokens and their
+// heads are small numbers and strides are below 2^24 units of 16 bytes, so that
+// an address is two 24-bit multiplies and a shifted add to a scalar base: the
+// same in 64 bits, at a quarter of the vector unit's rate, cost as much as the
+// rotation (16/2 heads of 128 with norms, 2000 tokens 7.4 -> 5.6 us, 24,000 55.6
+// -> 51.7; those now 47.1, 5.2 TB/s).
+struct RotVec {
+  uint32_t a_st, a_sh, ao_st, ao_sh, b_st, b_sh, bo_st, bo_sh;
+  uint32_t row_st;  // of a cache slot, to 2^32
+  uint32_t nslots;
+  int tb;                                         // tokens per workgroup
+  int heads_mul, heads_shift, half_mul, half_shift;  // division by heads and pairs
+  float inv_d;
+};
+
 template <typename T, int LPH, bool INTER, bool NORM>
-__global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int TB, int heads_mul,
-                                                                 int heads_shift) {
+__global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, RotVec v) {
   extern __shared__ __attribute__((aligned(16))) float sh[];  // [TB][R/2] cos, then sin
   typedef Chunk<T> C;
   constexpr int kGroups = kRotThreads / LPH;
   const int half = a.R / 2, heads = a.na + a.nb;
-  const int64_t t0 = (int64_t)blockIdx.x * TB;
-  const int nt = (int)min((int64_t)TB, a.ntok - t0);
+  const int64_t t0 = (int64_t)blockIdx.x * v.tb;
+  const int nt = (int)min((int64_t)v.tb, a.ntok - t0);
   const int items = nt * heads;
   const int u = threadIdx.x % LPH;
   const int units = a.D / 16, runits = a.R / 16;
-  const bool live = u < units;
+  const bool live = u < units;  // (the others read the head's first chunk and store nothing)
   // The chunks of unit u, such that neighbouring lanes read neighbouring
   // chunks. Half layout: u and u + R / 16 hold pairs 8u .. 8u + 7, and the
   // units behind R share its chunks out likewise; interleaved: u and u + D / 16,
   // chunk c with pairs 4c .. 4c + 3.
   const bool rot0 = INTER ? u < 2 * runits : u < runits;
   const bool rot1 = INTER ? u + units < 2 * runits : rot0;
-  const int c0 = INTER || rot0 ? u : runits + u;
-  const int c1 = INTER ? u + units : rot0 ? u + runits : units + u;
+  const int c0 = !live ? 0 : INTER || rot0 ? u : runits + u;
+  const int c1 = !live ? 0 : INTER ? u + units : rot0 ? u + runits : units + u;
   const int p0 = INTER ? 4 * u : 8 * u, p1 = INTER ? 4 * (u + units) : 8 * u + 4;
+  const char* const xa = (const char*)a.a + (uint64_t)t0 * v.a_st * 16;
+  const char* const xb = (const char*)a.b + (uint64_t)t0 * v.b_st * 16;
+  char* const ya = (char*)a.ao + (uint64_t)t0 * v.ao_st * 16;
+  char* const yb = (char*)a.bo + (uint64_t)t0 * v.bo_st * 16;
 
   struct Item {
     C x0, x1;
@@ -151,35 +170,35 @@ __global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int 
   auto load = [&](int i) {
     Item it;
     // i / heads by multiplication (exact for the items of a workgroup)
-    it.tok = (int)(((uint32_t)i * (uint32_t)heads_mul) >> heads_shift);
-    const int h = i - it.tok * heads;
-    const int64_t t = t0 + it.tok;
+    it.tok = (int)(__umul24(i, v.heads_mul) >> v.heads_shift);
+    const int h = i - __umul24(it.tok, heads);
     const bool isa = h < a.na;
-    const int hb = h - a.na;
-    const T* x = isa ? (const T*)a.a + t * a.a_st + (int64_t)h * a.a_sh
-                     : (const T*)a.b + t * a.b_st + (int64_t)hb * a.b_sh;
-    it.y = isa ? (T*)a.ao + t * a.ao_st + (int64_t)h * a.ao_sh
-               : (T*)a.bo + t * a.bo_st + (int64_t)hb * a.bo_sh;
+    const int hb = isa ? h : h - a.na;
+    const uint32_t x_at = __umul24(it.tok, isa ? v.a_st : v.b_st) + __umul24(hb, isa ? v.a_sh : v.b_sh);
+    const uint32_t y_at =
+        __umul24(it.tok, isa ? v.ao_st : v.bo_st) + __umul24(hb, isa ? v.ao_sh : v.bo_sh);
+    const T* x = (const T*)((isa ? xa : xb) + 16 * (uint64_t)x_at);
+    char* y = (isa ? ya : yb) + 16 * (uint64_t)y_at;
     if (!isa && a.slots != nullptr) {
-      const int64_t row = a.slots[t];
-      it.y = row >= 0 && row < a.nslots ? (T*)a.bo + row * a.bo_st + (int64_t)hb * a.bo_sh : nullptr;
+      const uint32_t row = (uint32_t)a.slots[t0 + it.tok];
+      y = row < v.nslots ? y + 16 * ((uint64_t)row * v.row_st) : nullptr;
     }
+    it.y = live ? (T*)y : nullptr;
     it.kind = h < a.nrot ? (isa ? 1 : 2) : 0;
-    if (live) {
-      it.x0 = *(const C*)(x + 8 * c0);
-      it.x1 = *(const C*)(x + 8 * c1);
-    }
+    it.x0 = *(const C*)(x + 8 * c0);
+    it.x1 = *(const C*)(x + 8 * c1);
     return it;
   };
   int i = threadIdx.x / LPH;
   Item cur;
   if (i < items) cur = load(i);
   float* s_cos = sh;
-  float* s_sin = sh + TB * half;
+  float* s_sin = sh + v.tb * half;
   for (int j = threadIdx.x; j < nt * half; j += kRotThreads) {
-    const int tok = j / half;
+    const int tok = (int)(__umul24(j, v.half_mul) >> v.half_shift);
     float c, s;
-    rot_angle(ll_load_idx(a.pos, t0 + tok, a.pos64), a.inv_freq[j - tok * half], a.factor, c, s);
+    rot_angle(ll_load_idx(a.pos, t0 + tok, a.pos64), a.inv_freq[j - __umul24(tok, half)], a.factor,
+              c, s);
     s_cos[j] = c;
     s_sin[j] = s;
   }
@@ -191,7 +210,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int 
     const bool more = i + kGroups < items;
     if (more) next = load(i + kGroups);
     if (cur.kind == 0) {
-      if (live && cur.y != nullptr) {
+      if (cur.y != nullptr) {
         store_chunk(cur.y + 8 * c0, cur.x0);
         store_chunk(cur.y + 8 * c1, cur.x1);
       }
@@ -199,23 +218,23 @@ __global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int 
       float x[16];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = live ? ll_to_f32(cur.x0.v[e]) : 0.f;
-        x[8 + e] = live ? ll_to_f32(cur.x1.v[e]) : 0.f;
+        x[e] = ll_to_f32(cur.x0.v[e]);
+        x[8 + e] = ll_to_f32(cur.x1.v[e]);
       }
       if constexpr (NORM) {
-        const T* g = (const T*)(cur.kind == 1 ? a.ga : a.gb);
-        if (g != nullptr) {
-          C g0, g1;
-          if (live) {
-            g0 = *(const C*)(g + 8 * c0);
-            g1 = *(const C*)(g + 8 * c1);
-          }
+        const bool of_a = cur.kind == 1;
+        if ((of_a ? a.ga : a.gb) != nullptr) {
+          const T* g = (const T*)(of_a ? a.ga : a.gb);
+          const C g0 = *(const C*)(g + 8 * c0), g1 = *(const C*)(g + 8 * c1);
           float ss = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
+          if (!live) ss = 0.f;
 #pragma unroll
           for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-          const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+          const float var = ss * v.inv_d + a.eps;
+          // (v_rsq_f32, 1 ulp, takes normal numbers)
+          const float r = var >= 1e-37f ? __builtin_amdgcn_rsqf(var) : 1.0f / sqrtf(var);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             x[e] = x[e] * r * ll_to_f32(g0.v[e]);
@@ -223,7 +242,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_vec_kernel(RotArgs a, int 
           }
         }
       }
-      if (live && cur.y != nullptr) {
+      if (cur.y != nullptr) {
         float y[16];
         const int at = cur.tok * half;
         if constexpr (INTER) {
@@ -273,22 +292,42 @@ template <typename T, int LPH>
 void launch_rotary_vec(const RotArgs& a, int interleaved, hipStream_t stream) {
   const int heads = a.na + a.nb;
   // tokens per workgroup: one until the grid fills the CUs eight times over,
-  // then up to 2 where a token's heads fill the workgroup's lanes, else 8
-  // (24,000 tokens, 28/4 heads of 128: 1 69.9 us, 2 68.0, 4 74.2, 8 80.1; 16/2
-  // heads with norms: 71.5, 57.3, 57.3, 55.5); LDS 32 KB at most
-  int tb = (int)std::min<int64_t>(heads * LPH >= kRotThreads ? 2 : 8,
-                                  std::max<int64_t>(1, a.ntok / 2048));
+  // then as many as fill its lanes twice, at most 8 (1, 2, 4, 8 of them at 24,000
+  // tokens: 16/2 heads of 128 46.8, 41.0, 41.2, 42.7 us, with norms 52.9, 47.2,
+  // 47.7, 51.8; 12/2 35.9, 32.3, 29.2, 33.2; 8/2 heads of 64 22.1, 15.6, 14.2,
+  // 12.8); where one token's heads do, two while what the call moves stays in the
+  // memory side's 256 MB (28/4 heads of 128, 8000 tokens: 1 23.3, 2 21.3), else
+  // one (24,000: 67.8, 70.5; 64/8, 8000: 53.8, 57.0). LDS 32 KB at most
+  const int lanes = heads * LPH;
+  int tb = lanes >= kRotThreads
+               ? (2 * a.ntok * heads * a.D * (int64_t)sizeof(T) > (int64_t)256 << 20 ? 1 : 2)
+               : 2 * kRotThreads / lanes >= 8 ? 8 : 2 * kRotThreads / lanes >= 4 ? 4 : 2;
+  tb = (int)std::min<int64_t>(tb, std::max<int64_t>(1, a.ntok / 2048));
   while (tb > 1 && tb * a.R * 4 > 32768) tb /= 2;
-  // i / heads = (i * mul) >> shift for i < tb * heads <= 2^19 / 8 * 8: with
-  // mul = ceil(2^shift / heads), exact while i * heads < 2^shift
-  int shift = 0;
-  while (((int64_t)1 << shift) < (int64_t)tb * heads * heads) ++shift;
-  const int mul = (int)((((int64_t)1 << shift) + heads - 1) / heads);
+  // i / n = (i * mul) >> shift for i < tb * n: with mul = ceil(2^shift / n), exact
+  // while i * n < 2^shift; i and mul have 24 bits and their product 32
+  auto divide = [tb](int n, int& mul, int& shift) {
+    shift = 0;
+    while (((int64_t)1 << shift) < (int64_t)tb * n * n) ++shift;
+    mul = n ? (int)((((int64_t)1 << shift) + n - 1) / n) : 0;
+  };
+  const int64_t es = sizeof(T);
+  auto units = [es](int64_t stride) { return (uint32_t)(stride * es / 16); };
+  RotVec v = {};
+  v.a_st = units(a.a_st); v.a_sh = units(a.a_sh); v.ao_st = units(a.ao_st); v.ao_sh = units(a.ao_sh);
+  v.b_st = units(a.b_st); v.b_sh = units(a.b_sh); v.bo_sh = units(a.bo_sh);
+  if (a.slots != nullptr) v.row_st = units(a.bo_st);
+  else v.bo_st = units(a.bo_st);
+  v.nslots = (uint32_t)std::min<int64_t>(a.nslots, (int64_t)1 << 31);  // (a negative slot is above it)
+  v.tb = tb;
+  divide(heads, v.heads_mul, v.heads_shift);
+  divide(a.R / 2, v.half_mul, v.half_shift);
+  v.inv_d = 1.0f / (float)a.D;
   const unsigned grid = (unsigned)((a.ntok + tb - 1) / tb);
   const size_t lds = (size_t)tb * a.R * 4;
   const bool norm = a.ga != nullptr || a.gb != nullptr;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kRotThreads), lds, stream, a, tb, mul, shift);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kRotThreads), lds, stream, a, v);
   };
   if (norm) {
     if (interleaved) go(rotary_vec_kernel<T, LPH, true, true>);
@@ -299,20 +338,29 @@ void launch_rotary_vec(const RotArgs& a, int interleaved, hipStream_t stream) {
   }
 }
 
-// Whether every head of the call can be read and written in 16-byte chunks.
+// Whether every head of the call can be read and written in 16-byte chunks, at
+// addresses of the 24-bit kind.
 bool rotary_vec_ok(const RotArgs& a, int64_t es) {
   if (a.D % 16 != 0 || a.D > 256 || a.R % 16 != 0) return false;
-  // (the division by multiplication holds for i * mul < 2^32)
   const int64_t heads = a.na + a.nb;
   if (8 * heads * heads >= (int64_t)1 << 24) return false;
-  int64_t strides = a.na ? a.a_st | a.a_sh | a.ao_st | a.ao_sh : 0;
-  uintptr_t at = a.na ? (uintptr_t)a.a | (uintptr_t)a.ao : 0;
+  // (the heads that there are none of have no strides)
+  int64_t st[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  uintptr_t at = (uintptr_t)a.ga | (uintptr_t)a.gb;
+  if (a.na) {
+    st[0] = a.a_st; st[1] = a.a_sh; st[2] = a.ao_st; st[3] = a.ao_sh;
+    at |= (uintptr_t)a.a | (uintptr_t)a.ao;
+  }
   if (a.nb) {
-    strides |= a.b_st | a.b_sh | a.bo_st | a.bo_sh;
+    st[4] = a.b_st; st[5] = a.b_sh; st[6] = a.bo_st; st[7] = a.bo_sh;
     at |= (uintptr_t)a.b | (uintptr_t)a.bo;
   }
-  at |= (uintptr_t)a.ga | (uintptr_t)a.gb;
-  return (strides * es) % 16 == 0 && at % 16 == 0;
+  for (int i = 0; i < 8; ++i) {
+    const int64_t most = i == 6 && a.slots != nullptr ? (int64_t)1 << 32 : (int64_t)1 << 24;
+    if (st[i] * es % 16 != 0 || st[i] < 0 || st[i] * es / 16 >= most) return false;
+    if (i % 2 == 1 && st[i] * es / 16 * heads >= (int64_t)1 << 31) return false;
+  }
+  return at % 16 == 0;
 }
 
 int launch_rotary(const char* fn, const RotArgs& a, int interleaved, int dtype,

@@ -103,6 +103,53 @@ def test_rope_positions_strided_rows(cuda, pad):
             assert bool((row[:, -pad:] == 3.0).all()), "padding of the rows"
 
 
+@pytest.mark.parametrize("row", [(1 << 27) - 8, 1 << 27])
+def test_rope_of_rows_far_apart(cuda, row):
+    """Rows 2^24 units of 16 bytes apart, and one less."""
+    H, D = 2, 64
+    q, _, pos, f = _rot_inputs(cuda, 3, H, 1, D, D, BF16, 7, far=9000)
+    wide = torch.empty(3, row, dtype=BF16, device=cuda)
+    qd = wide[:, 64:64 + H * D].unflatten(1, (H, D))
+    qd.copy_(q)
+    wide[:, :64], wide[:, 64 + H * D:64 + 2 * H * D] = 5.0, 6.0
+    print(f"case: rope rows of {row}", flush=True)
+    _ops().rope_positions(qd, None, pos.to(cuda), f.to(cuda))
+    want, mag = O.rotate(q, pos, f)
+    _inside(qd, want, O.bound_rotary(want, mag, BF16, pos, f), "q")
+    assert bool((wide[:, :64] == 5.0).all())
+    assert bool((wide[:, 64 + H * D:64 + 2 * H * D] == 6.0).all())
+
+
+def test_qk_norm_to_far_slots(cuda):
+    """Cache rows behind 2^32 bytes of the pool; padded tokens among them."""
+    H, K, D, T = 4, 8, 128, 40
+    P = (1 << 31) // (2 * K * D) + 5000
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(T, (H + 2 * K) * D, generator=g).to(BF16)
+    gk = (1 + 0.2 * torch.randn(D, generator=g)).to(BF16)
+    pos = torch.randint(0, 9000, (T,), generator=g).to(torch.int32)
+    f, _ = _ops().rope_frequencies(D)
+    slots = (P - 1 - torch.randperm(4000, generator=g)[:T]).to(torch.int32)
+    slots[3], slots[7], slots[11] = -1, P, -(1 << 31)
+    pool = torch.empty(P, 2 * K, D, dtype=BF16, device=cuda)
+    pool[-5000:] = 7.0
+    print("case: qk norm far slots", flush=True)
+    _ops().qk_norm_rope_kv_scatter(x.to(cuda), H, K, D, None, gk.to(cuda), 1e-6, pos.to(cuda),
+                                   f.to(cuda), slots.to(cuda), pool)
+    tail = pool[-5000:].cpu()
+    rows = x.view(T, H + 2 * K, D)
+    normed = O.head_norm(rows[:, H:H + K], gk, 1e-6)
+    want, mag = O.rotate(normed, pos, f)
+    stored = [t for t in range(T) if t not in (3, 7, 11)]
+    at = [int(slots[t]) - (P - 5000) for t in stored]
+    b = O.bound_rotary(want, mag, BF16, pos, f, D)
+    _inside(tail[at, :K], want[stored], b[stored], "k")
+    assert torch.equal(tail[at, K:], rows[stored, H + K:])
+    rest = torch.ones(5000, dtype=torch.bool)
+    rest[at] = False
+    assert bool((tail[rest] == 7.0).all())
+
+
 @pytest.mark.parametrize("D", [64, 20])
 def test_rope_of_nothing_rotated_needs_no_positions(cuda, D):
     """The C entry point takes null positions and frequencies with rotary_dim 0
@@ -214,6 +261,10 @@ def test_qk_norm_of_a_long_prefill(cuda):
     """More tokens than one pass of the grid, and the head group of 7."""
     _qk_case(cuda, 3001, 7, 1, 128, 128, False, BF16, 4)
     _qk_case(cuda, 2050, 8, 2, 64, 64, True, F16, 5, scale=30.0)
+    # two to eight tokens per workgroup
+    _qk_case(cuda, 4099, 28, 4, 64, 64, False, BF16, 6)
+    _qk_case(cuda, 8197, 6, 1, 80, 48, True, F16, 7, inplace=True)
+    _qk_case(cuda, 16391, 1, 1, 64, 32, False, F32, 8)
 
 
 # ---------------------------------------------------------------- attention
