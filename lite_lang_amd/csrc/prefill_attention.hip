@@ -38,8 +38,8 @@
 // same time) 5,000 to 7,000. us per call, bf16, 16/2 heads of 128, and
 // the share of the 1,230 TFLOP/s that a large library product reaches here:
 // 1 x 8192 causal 249 (1,100 TFLOP/s, 90%); 1 x 32,768 under a window of 4096
-// 967 (1,067, 87%); 40 x 600 under a window of 256 97 to 106 by card (380-420,
-// 31-34%: six items of one to six tiles per workgroup).
+// 967-980 (1,053-1,067, 86-87%); 40 x 600 under a window of 256 90 to 101 by
+// card (400-450, 32-36%: six items of one to five tiles per workgroup).
 #include <algorithm>
 #include <type_traits>
 
