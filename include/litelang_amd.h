@@ -172,7 +172,7 @@ int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_s
 
 /* ll_decode_attention under a window: the query is the token at b_seq_len - 1,
  * so its keys are one list, the sinks and the last `window` tokens. Sequences
- * of length 0 give zero rows. The workspace (0 bytes where the list is not
+ * of length 0 give zero rows and may have any b_req_idx. The workspace (0 bytes where the list is not
  * split) needs no initialisation and nothing in it lasts beyond the call; it
  * must not be one of ll_decode_attention, which has to find its own as it left
  * it. */

@@ -506,11 +506,14 @@ __device__ __forceinline__ void decode_attn_split_stage(
   int64_t len = len32 > a.max_len ? a.max_len : len32;
   WindowList wl = {0, 0, 0};
   if constexpr (WIN) {
-    wl = window_list(len, window, sinks);
+    wl = window_list(max(len, (int64_t)0), window, sinks);
     len = wl.n;
   }
   const int64_t rid = rid32;
   const int32_t* slot_row = a.r2t + rid * a.r2t_s;
+  // A sequence without tokens may sit on any row (a padded entry of a batch):
+  // the first round's reads, of entry 0 alone, go to the lengths instead.
+  if (WIN && len == 0) slot_row = p_len;
   const int ntiles = (int)((len + kTT - 1) / kTT);
   const int per = (ntiles + nsplit - 1) / nsplit;
   const int tb = min(ntiles, split * per);
@@ -1535,8 +1538,7 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
                        (k_stride_tok % 8 == 0) && (k_stride_head % 8 == 0) &&
                        (v_stride_tok % 8 == 0) && (v_stride_head % 8 == 0) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  // (without a token the split stage would still read a table entry per sequence)
-  if (!mfma_ok || (win && max_len_in_batch == 0)) {
+  if (!mfma_ok) {
     LL_CHECK_ARG(!win || batch <= 65535, "%s: more than 65535 requests", fn);
     a.nsplit = 1;
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 8;

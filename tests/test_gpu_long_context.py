@@ -916,3 +916,46 @@ def test_captured_window_prefill_follows_its_lengths(cuda):
                               float(pool[:, KVH:].float().abs().max()))
         _inside(out, want, b, f"replay {ls}")
         assert bool((out[sum(new):] == 7.0).all())
+
+
+@pytest.mark.parametrize("H,KVH,D,dtype", HEADS)
+@pytest.mark.parametrize("n,window", [(90, 40), (3000, 2500)])
+def test_window_attention_padded_entries_may_sit_on_any_row(cuda, H, KVH, D, dtype, n, window):
+    """Entries of length 0 beside live ones, of one split and several, on rows
+    before and behind the table: they give zero rows, and the live ones what
+    they give alone. A prefill's requests without query rows may sit there too.
+    (The table is the middle of a larger buffer, whose other entries lead to NaN:
+    a use of such a row would show, and read no other memory.)"""
+    g = torch.Generator().manual_seed(n)
+    pool = torch.randn(n + 5, 2 * KVH, D, generator=g).to(dtype).to(cuda)
+    pool[n:] = float("nan")
+    wide = torch.full((5, n), n, dtype=torch.int32, device=cuda)
+    wide[2] = torch.randperm(n, generator=g).to(torch.int32)
+    table = wide[2:3]
+    q = torch.randn(4, H, D, generator=g).to(dtype).to(cuda)
+    k, v = pool[:, :KVH], pool[:, KVH:]
+    for idx in (torch.int32, torch.int64):
+        print(f"case: padded decode H={H}/{KVH} D={D} {dtype} n={n} {idx}", flush=True)
+        rows, lens = _i32([-1, 0, 1, -2], cuda, idx), _i32([0, n, 0, 0], cuda, idx)
+        out = torch.full_like(q, 7.0)
+        _ops().window_decode_attention(q, table, rows, lens, n, k, v, out, window, sinks=3)
+        alone = torch.empty_like(q)
+        _ops().window_decode_attention(q, table, _i32([0] * 4, cuda), _i32([n] * 4, cuda), n, k, v,
+                                       alone, window, sinks=3)
+        assert torch.equal(out[1], alone[1])
+        assert not out[[0, 2, 3]].any()
+        # all of them empty, under a bound of no tokens and of some
+        for most in (0, 5):
+            out.fill_(7.0)
+            _ops().window_decode_attention(q, table, rows, _i32([0] * 4, cuda, idx), most, k, v,
+                                           out, window, sinks=3)
+            assert not out.any()
+        print(f"case: padded prefill H={H}/{KVH} D={D} {dtype} n={n} {idx}", flush=True)
+        start, before = _i32([0, 0, 9, 4], cuda, idx), _i32([0, n - 4, 9, 8], cuda, idx)
+        out.fill_(7.0)
+        _ops().window_prefill_attention(q, k, v, out, rows, start, _i32([0, n, 9, 5], cuda, idx), 4,
+                                        table, window, sinks=3, b_shared_seq_len=before)
+        _ops().window_prefill_attention(q, k, v, alone, _i32([0], cuda), _i32([0], cuda),
+                                        _i32([n], cuda), 4, table, window, sinks=3,
+                                        b_shared_seq_len=_i32([n - 4], cuda))
+        assert torch.equal(out, alone)
