@@ -146,8 +146,10 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * the first `sinks` ones are kept: a query at position p sees the keys n <= p
  * with n > p - window (its own included) or n < sinks. window >= 1, sinks >= 0
  * (both may exceed the length); lengths at most 2^30, at most 2^24 requests and
- * 65535 query heads; sm_scale > 0. No counterpart in the
- * reference (whose configs' use_sliding_window it does not read).
+ * 65535 query heads, and no more of both than one launch holds (a decode's
+ * requests x KV heads x splits below 2^23; 65535 requests off the 16-bit paths
+ * of heads of 64 and 128); sm_scale > 0. No counterpart in the reference (whose
+ * configs' use_sliding_window it does not read).
  * No entry of the slot table is read but those of keys that some query of the
  * request's call sees, so the tokens between the sinks and the window may have
  * left the cache and their entries may hold anything. Keys and values that one
@@ -172,8 +174,8 @@ int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_s
 
 /* ll_decode_attention under a window: the query is the token at b_seq_len - 1,
  * so its keys are one list, the sinks and the last `window` tokens. Sequences
- * of length 0 give zero rows and may have any b_req_idx. The workspace (0 bytes where the list is not
- * split) needs no initialisation and nothing in it lasts beyond the call; it
+ * of length 0 give zero rows and may have any b_req_idx. The workspace (0 bytes
+ * where the list is not split, and for shapes that the call refuses) needs no initialisation and nothing in it lasts beyond the call; it
  * must not be one of ll_decode_attention, which has to find its own as it left
  * it. */
 int64_t ll_window_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,

@@ -1077,6 +1077,15 @@ __global__ __launch_bounds__(64) void decode_attn_generic_kernel(DecodeArgs a, i
   }
 }
 
+// Workgroups of a launch: the grid of a dispatch has fewer than 2^32 threads.
+constexpr int64_t kMaxGrid = ((int64_t)1 << 32) / (kWaves * 64) - 1;
+
+// Whether a (sequence, KV head) each can have a workgroup, so that their number
+// and what the split rules make of it fit 32 bits.
+bool units_fit(int64_t batch, int64_t kv_heads) {
+  return batch > 0 && kv_heads > 0 && batch <= kMaxGrid / kv_heads;
+}
+
 constexpr int kMaxSplitTokens = 4096;  // LDS slot table bound per split (16 KB)
 constexpr int kSplitCostTiles2 = 13;    // twice the cost of one more split, in 16-token tiles
 constexpr int kMaxSplitsFill = 16;      // split bound from 8 units up (head_dim 128)
@@ -1170,7 +1179,11 @@ struct SplitPlan {
 //   the bound, and stays spread).
 // No shape takes more splits than one XCD would give it (the workspace does
 // not grow).
-SplitPlan choose_splits(int B, int KVH, int64_t max_len, int64_t head_dim) {
+// (shapes that no launch takes: one split, for the size queries; the entry points
+// refuse them)
+SplitPlan choose_splits(int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim) {
+  if (!units_fit(batch, kv_heads) || max_len < 0 || max_len > INT32_MAX) return {1, false};
+  const int B = (int)batch, KVH = (int)kv_heads;
   int ns = choose_nsplit_xcd(B, KVH, max_len, head_dim);
   const int units = B * KVH, seqs = (B + 7) / 8;  // sequences of the busiest XCD
   const int64_t tiles = (max_len + kTT - 1) / kTT;
@@ -1199,8 +1212,20 @@ SplitPlan choose_splits(int B, int KVH, int64_t max_len, int64_t head_dim) {
 }
 
 // workgroups of the split stage
-unsigned split_grid(int B, int KVH, const SplitPlan& p) {
-  return (unsigned)((p.spread ? B : (B + 7) / 8 * 8) * KVH * p.ns);
+int64_t split_grid(int64_t B, int64_t KVH, const SplitPlan& p) {
+  return (p.spread ? B : (B + 7) / 8 * 8) * KVH * p.ns;
+}
+
+// (fn: an entry point; before the counts are taken as 32 bits)
+int check_units(const char* fn, int64_t batch, int64_t kv_heads) {
+  LL_CHECK_ARG(units_fit(batch, kv_heads), "%s: %lld sequences of %lld KV heads (max %lld workgroups)",
+               fn, (long long)batch, (long long)kv_heads, (long long)kMaxGrid);
+  return LL_OK;
+}
+int check_grid(int64_t grid) {
+  LL_CHECK_ARG(grid <= kMaxGrid, "decode attention: %lld workgroups (max %lld)", (long long)grid,
+               (long long)kMaxGrid);
+  return LL_OK;
 }
 
 int64_t align256(int64_t x) { return ((x + 255) / 256) * 256; }
@@ -1280,8 +1305,9 @@ std::atomic<int> g_same_launch_merge{1};
 
 int64_t workspace_bytes_for(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                             int64_t max_len) {
-  const int ns = choose_splits((int)batch, (int)kv_heads, max_len, head_dim).ns;
-  if (ns <= 1) return 0;
+  const SplitPlan plan = choose_splits(batch, kv_heads, max_len, head_dim);
+  const int ns = plan.ns;
+  if (ns <= 1 || split_grid(batch, kv_heads, plan) > kMaxGrid) return 0;
   const int64_t parts = batch * q_heads * ns;
   return kTicketBytes                      // split tickets
          + align256(parts * head_dim * 4)  // partial acc
@@ -1294,6 +1320,9 @@ int64_t workspace_bytes_for(int64_t batch, int64_t q_heads, int64_t kv_heads, in
 int launch_mfma(DecodeArgs& a, int64_t head_dim, int dtype, bool rope, int64_t max_len,
                 void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const SplitPlan plan = choose_splits(a.B, a.KVH, max_len, head_dim);
+  const int64_t wgs = split_grid(a.B, a.KVH, plan);
+  if (const int rc = check_grid(wgs)) return rc;
+  const unsigned grid = (unsigned)wgs;
   a.nsplit = plan.ns;
   a.spread = plan.spread ? 1 : 0;
   if (a.unit_spin <= 0) a.unit_spin = kUnitMergeSpin;
@@ -1321,7 +1350,6 @@ int launch_mfma(DecodeArgs& a, int64_t head_dim, int dtype, bool rope, int64_t m
   }
   const int64_t tiles = (max_len + kTT - 1) / kTT;
   a.slots_cap = (int)((tiles + a.nsplit - 1) / a.nsplit) * kTT;
-  const unsigned grid = split_grid(a.B, a.KVH, plan);
   // No other thread's call may come between the split stage and its merge
   // kernel on this workspace, one that merges in its own launch neither: it
   // would take the partial words there for its own.
@@ -1383,7 +1411,7 @@ int choose_window_splits(int64_t B, int64_t KVH, int64_t bound, int64_t head_dim
   const int64_t tiles = (bound + kTT - 1) / kTT;
   if (tiles <= 3 * kWaves) return 1;
   const int min_ns = (int)((tiles * kTT + kMaxSplitTokens - 1) / kMaxSplitTokens);
-  const int ns = choose_splits((int)B, (int)KVH, bound, head_dim).ns;
+  const int ns = choose_splits(B, KVH, bound, head_dim).ns;
   if (head_dim == 64 && ns <= 3) return min_ns;
   if (ns == 4 && tiles >= 48 && B * KVH * 8 <= 256 * split_wg_per_cu(head_dim)) return 8;
   return ns;
@@ -1396,9 +1424,9 @@ int64_t window_workspace_bytes(int64_t parts, int64_t head_dim) {
 int launch_window_mfma(DecodeArgs& a, int64_t head_dim, int dtype, int64_t bound, void* workspace,
                        int64_t workspace_bytes, hipStream_t stream) {
   a.nsplit = choose_window_splits(a.B, a.KVH, bound, head_dim);
-  LL_CHECK_ARG((int64_t)a.B * a.H * a.nsplit <= INT32_MAX,
-               "window decode attention: %d sequences of %d heads in %d splits (max 2^31 - 1 rows)",
-               a.B, a.H, a.nsplit);
+  // (with at most 16 heads a unit, the rows of the splits then have 32 bits too)
+  const int64_t wgs = (int64_t)a.units * a.nsplit;
+  if (const int rc = check_grid(wgs)) return rc;
   a.spread = 1;
   a.merge_cnt = nullptr;
   const int64_t parts = (int64_t)a.B * a.H * a.nsplit;
@@ -1415,7 +1443,7 @@ int launch_window_mfma(DecodeArgs& a, int64_t head_dim, int dtype, int64_t bound
   }
   const int64_t tiles = (bound + kTT - 1) / kTT;
   a.slots_cap = (int)((tiles + a.nsplit - 1) / a.nsplit) * kTT;
-  const unsigned grid = (unsigned)(a.units * a.nsplit);
+  const unsigned grid = (unsigned)wgs;
   const size_t extra = (size_t)a.slots_cap * 4;
   if (head_dim == 128) {
     if (dtype == LL_BF16) launch_window<__bf16, 128>(a, grid, TileGeom<128>::MAIN_B + extra, stream);
@@ -1444,9 +1472,11 @@ extern "C" int ll_decode_attention_xcc_probe(int64_t batch, int64_t q_heads, int
   LL_CHECK_ARG(out != nullptr && batch > 0 && kv_heads > 0 && q_heads % kv_heads == 0 &&
                    (head_dim == 64 || head_dim == 128) && max_len_in_batch > 0,
                "ll_decode_attention_xcc_probe: bad arguments");
-  const SplitPlan plan = choose_splits((int)batch, (int)kv_heads, max_len_in_batch, head_dim);
+  if (const int rc = check_units("ll_decode_attention_xcc_probe", batch, kv_heads)) return rc;
+  const SplitPlan plan = choose_splits(batch, kv_heads, max_len_in_batch, head_dim);
   const int nsplit = plan.ns;
-  const int64_t grid = split_grid((int)batch, (int)kv_heads, plan);
+  const int64_t grid = split_grid(batch, kv_heads, plan);
+  if (const int rc = check_grid(grid)) return rc;
   LL_CHECK_ARG(out_len >= grid, "ll_decode_attention_xcc_probe: out holds %lld of %lld entries",
                (long long)out_len, (long long)grid);
   const int64_t tiles = (max_len_in_batch + kTT - 1) / kTT;
@@ -1470,12 +1500,12 @@ extern "C" int ll_decode_attention_set_same_launch_merge(int enable) {
 
 extern "C" int ll_decode_attention_split_count(int64_t batch, int64_t kv_heads, int64_t head_dim,
                                                int64_t max_len_in_batch) {
-  return choose_splits((int)batch, (int)kv_heads, max_len_in_batch, head_dim).ns;
+  return choose_splits(batch, kv_heads, max_len_in_batch, head_dim).ns;
 }
 
 extern "C" int ll_decode_attention_splits_spread(int64_t batch, int64_t kv_heads, int64_t head_dim,
                                                  int64_t max_len_in_batch) {
-  return choose_splits((int)batch, (int)kv_heads, max_len_in_batch, head_dim).spread ? 1 : 0;
+  return choose_splits(batch, kv_heads, max_len_in_batch, head_dim).spread ? 1 : 0;
 }
 
 extern "C" int64_t ll_decode_attention_workspace_size(int64_t batch, int64_t q_heads,
@@ -1524,7 +1554,7 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
   a.seq_len = b_seq_len; a.len64 = seq_len_i64;
   a.out = out; a.o_sb = out_stride_b; a.o_sh = out_stride_h;
   a.B = (int)batch; a.H = (int)q_heads; a.KVH = (int)kv_heads; a.G = (int)(q_heads / kv_heads);
-  a.units = a.B * a.KVH;
+  a.units = (int)(batch * kv_heads);  // (of use where it fits, check_units)
   a.max_len = (int)max_len_in_batch;
   a.slots_cap = 0;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
@@ -1554,6 +1584,7 @@ int decode_attention(const char* fn, const void* q, int64_t q_stride_b, int64_t 
     });
   }
 
+  if (const int rc = check_units(fn, batch, kv_heads)) return rc;
   if (win)
     return launch_window_mfma(a, head_dim, dtype, window_bound(max_len_in_batch, window, sinks),
                               workspace, workspace_bytes, stream);
@@ -1601,12 +1632,13 @@ extern "C" int64_t ll_window_decode_attention_workspace_size(int64_t batch, int6
                                                              int64_t kv_heads, int64_t head_dim,
                                                              int64_t max_len_in_batch,
                                                              int64_t window, int64_t sinks) {
-  if (batch <= 0 || kv_heads <= 0 || max_len_in_batch <= 0 || window < 1 || sinks < 0 ||
-      (head_dim != 64 && head_dim != 128))
+  if (!units_fit(batch, kv_heads) || max_len_in_batch <= 0 || max_len_in_batch > 1 << 30 ||
+      window < 1 || sinks < 0 || q_heads > 65535 || (head_dim != 64 && head_dim != 128))
     return 0;
   const int ns = choose_window_splits(batch, kv_heads,
                                       window_bound(max_len_in_batch, window, sinks), head_dim);
-  return ns > 1 ? window_workspace_bytes(batch * q_heads * ns, head_dim) : 0;
+  if (ns <= 1 || batch * kv_heads * ns > kMaxGrid) return 0;
+  return window_workspace_bytes(batch * q_heads * ns, head_dim);
 }
 
 // ---------------------------------------------------------------- no-allocation variant
@@ -1729,6 +1761,7 @@ int rope_attention_impl(const LLPartials& qkv, const void* qkv_bias, const void*
                "ll_decode_attention_rope_splitk: max_len_in_batch %lld out of range",
                (long long)max_len_in_batch);
   if (batch == 0) return LL_OK;
+  if (const int rc = check_units("ll_decode_attention_rope_splitk", batch, kv_heads)) return rc;
   DecodeArgs a = {};
   a.k = k_cache; a.k_st = k_stride_tok; a.k_sh = k_stride_head;
   a.v = v_cache; a.v_st = v_stride_tok; a.v_sh = v_stride_head;

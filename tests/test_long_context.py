@@ -307,3 +307,71 @@ def test_c_entry_points_refuse_before_any_launch():
     assert maps(free=None) == -1 and "null" in err()
     assert maps(page=0) == -1 and maps(page=16) == -1 and "block table" in err()
     assert maps(batch=8193) == -1 and maps(rows=1 << 19) == -1 and maps(nfree=-1) == -1
+
+
+# ---------------------------------------------------------------- counts beyond 32 bits
+_QUERIES = """
+import ctypes, json, sys
+L = ctypes.CDLL(sys.argv[1])
+out = []
+for name, args in json.load(sys.stdin):
+    fn = getattr(L, name)
+    fn.restype = ctypes.c_int64
+    out.append(fn(*[ctypes.c_int64(a) for a in args]))
+print(json.dumps(out))
+"""
+
+
+def test_decode_size_queries_take_any_counts():
+    """Counts whose product wraps to 0 in 32 bits, and none at all: no bytes, for
+    the entry points refuse them. (In a process of its own: a division by such a
+    product ends it.)"""
+    import json
+    import subprocess
+    import sys
+
+    from lite_lang_amd import build
+    name = "ll_window_decode_attention_workspace_size"
+    calls = [(name, [1 << 24, 256, 256, 128, 4096, 1024, 0]),
+             (name, [1 << 32, 256, 256, 128, 4096, 1024, 0]),
+             (name, [1 << 22, 4, 2, 128, 4096, 1024, 0]),
+             (name, [1 << 40, 16, 2, 64, 1 << 30, 1 << 30, 0]),
+             (name, [4, 16, 1 << 40, 64, 1 << 20, 1 << 20, 0]),
+             (name, [4, 16, 2, 64, 1 << 40, 1 << 40, 0]),
+             (name, [1 << 16, 8, 1, 128, 1 << 30, 1 << 30, 0]),
+             (name, [0, 16, 2, 64, 1 << 20, 1 << 20, 0])]
+    plain = "ll_decode_attention_workspace_size"
+    calls += [(plain, [1 << 24, 256, 256, 128, 4096]), (plain, [1 << 32, 16, 2, 128, 4096]),
+              (plain, [1 << 16, 8, 1, 128, 1 << 30]), (plain, [0, 16, 2, 128, 4096]), (plain, [4, 16, 0, 128, 4096])]
+    live = [(name, [1, 16, 2, 128, 4096, 4096, 0]), (plain, [1, 16, 2, 128, 4096])]
+    r = subprocess.run([sys.executable, "-c", _QUERIES, build.LIB_PATH], capture_output=True,
+                       input=json.dumps(calls + live), text=True)
+    assert r.returncode == 0, f"ended with {r.returncode}: {r.stderr}"
+    sizes = json.loads(r.stdout)
+    assert sizes[:len(calls)] == [0] * len(calls) and min(sizes[len(calls):]) > 0
+
+
+def test_decode_refuses_more_workgroups_than_a_launch_holds():
+    from lite_lang_amd import _lib
+    L, p = _lib.load(), 256
+
+    def window(B, H, KVH, D=128, most=4096, win=1024):
+        return L.ll_window_decode_attention(p, H * D, D, p, 2 * KVH * D, D, p, 2 * KVH * D, D, p, 8,
+                                            p, 0, p, 0, p, H * D, D, B, H, KVH, D, most, win, 0,
+                                            ctypes.c_float(1.0), 2, None, 0, None)
+
+    def plain(B, H, KVH, D=128, most=4096):
+        return L.ll_decode_attention(p, H * D, D, p, 2 * KVH * D, D, p, 2 * KVH * D, D, p, 8, p, 0,
+                                     p, 0, p, H * D, D, B, H, KVH, D, most, ctypes.c_float(1.0), 2,
+                                     None, 0, None)
+
+    for B, H, KVH in ((1 << 24, 256, 256), (1 << 23, 1, 1), (1 << 22, 4, 2), (1 << 24, 16, 2)):
+        for call in (window, plain):
+            assert call(B, H, KVH) == -1 and "workgroups" in L.ll_last_error().decode()
+    # fewer units, each of many splits (4096 tokens at most in one)
+    assert window(1 << 16, 8, 1, most=1 << 30, win=1 << 30) == -1
+    assert "workgroups" in L.ll_last_error().decode()
+    assert plain(1 << 16, 8, 1, most=1 << 30) == -1
+    assert "workgroups" in L.ll_last_error().decode()
+    # a product that wraps to 0, off the 16-bit paths
+    assert window(1 << 24, 256, 256, D=96) == -1 and "65535" in L.ll_last_error().decode()
