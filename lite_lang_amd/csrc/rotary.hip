@@ -304,6 +304,8 @@ void launch_rotary_vec(const RotArgs& a, int interleaved, hipStream_t stream) {
                : 2 * kRotThreads / lanes >= 8 ? 8 : 2 * kRotThreads / lanes >= 4 ? 4 : 2;
   tb = (int)std::min<int64_t>(tb, std::max<int64_t>(1, a.ntok / 2048));
   while (tb > 1 && tb * a.R * 4 > 32768) tb /= 2;
+  // (a grid has fewer than 2^32 threads: 2^24 tokens, the most, go two by two)
+  if (a.ntok >= ((int64_t)1 << 32) / kRotThreads) tb = std::max(tb, 2);
   // i / n = (i * mul) >> shift for i < tb * n: with mul = ceil(2^shift / n), exact
   // while i * n < 2^shift; i and mul have 24 bits and their product 32
   auto divide = [tb](int n, int& mul, int& shift) {
@@ -369,7 +371,7 @@ int launch_rotary(const char* fn, const RotArgs& a, int interleaved, int dtype,
                "%s: head_dim %d, rotary_dim %d unsupported", fn, a.D, a.R);
   LL_CHECK_ARG(a.R == 0 || (a.pos && a.inv_freq), "%s: null pointer", fn);
   if (a.na + a.nb == 0) return LL_OK;
-  // (a grid holds fewer than 2^32 threads, 256 for each token or two of them)
+  // (a grid holds fewer than 2^32 threads, up to 256 for each token)
   LL_CHECK_ARG(a.ntok <= (int64_t)1 << 24 && a.na + a.nb <= 65535,
                "%s: %lld tokens of %d heads unsupported", fn, (long long)a.ntok, a.na + a.nb);
   // heads or tokens on one address would be rotated over one another

@@ -959,3 +959,22 @@ def test_window_attention_padded_entries_may_sit_on_any_row(cuda, H, KVH, D, dty
                                         _i32([n], cuda), 4, table, window, sinks=3,
                                         b_shared_seq_len=_i32([n - 4], cuda))
         assert torch.equal(out, alone)
+
+
+def test_rope_of_the_most_tokens(cuda):
+    """2^24 tokens whose heads fill a workgroup each (a grid of 2^32 threads has
+    no room for one token per workgroup): the bits of smaller calls."""
+    T, H, D, part = 1 << 24, 64, 16, 1 << 21
+    g = torch.Generator().manual_seed(24)
+    q = torch.randn(1, H, D, generator=g).to(BF16).to(cuda).expand(T, H, D)
+    pos = torch.arange(T, dtype=torch.int32, device=cuda)
+    f, _ = _ops().rope_frequencies(D)
+    f = f.to(cuda)
+    print("case: rope of 2^24 tokens", flush=True)
+    out, small = (torch.zeros(n, H, D, dtype=BF16, device=cuda) for n in (T, part))
+    _ops().rope_positions(q, None, pos, f, q_out=out)
+    for at in range(0, T, part):
+        _ops().rope_positions(q[:part], None, pos[at:at + part], f, q_out=small)
+        assert torch.equal(out[at:at + part], small), f"tokens from {at}"
+    del out, small
+    torch.cuda.empty_cache()
