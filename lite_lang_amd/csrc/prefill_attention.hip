@@ -181,6 +181,14 @@ template <typename Op> __device__ __forceinline__ int lane_scan(int v, int id, O
   return v;
 }
 
+// Between accesses of one wave's lanes to the LDS words of each other. The
+// hardware keeps their order; without it the compiler need not, as it may take
+// a lane's store for the value of the lane's next load of that word.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int D> struct FaGeom {
   static constexpr int ROWB = D * 2;            // bytes of a K or V row
   static constexpr int CH = ROWB / 16;          // 16 B chunks per row
@@ -364,10 +372,12 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
         for (int hi = top; hi >= bot; hi -= 64) {
           const int i0 = hi - (l0 + ramp - 1), i1 = hi - l0 + 1;
           edge[lane] = 0;
+          wave_lds_fence();
           if (ramp > 0 && i1 > 0 && i0 < 64) {
             atomicAdd(&edge[max(i0, 0)], 1);
             if (i1 < 64) atomicAdd(&edge[i1], -1);
           }
+          wave_lds_fence();
           const int cnt = scan(edge[lane]), lincl = scan(cnt);
           const int ltotal = rl(lincl, 63), lrel = want - base;
           base += ltotal;

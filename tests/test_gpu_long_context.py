@@ -978,3 +978,20 @@ def test_rope_of_the_most_tokens(cuda):
         assert torch.equal(out[at:at + part], small), f"tokens from {at}"
     del out, small
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("B", [2, 40, 64, 65, 130])
+def test_window_prefill_attention_of_levels_beside_none(cuda, B):
+    """Requests whose row blocks lie at many levels of their context's start
+    beside requests that have none of those (whole windows behind long prefixes,
+    no new tokens): the lanes of a wave that list the levels without adding any."""
+    g = np.random.RandomState(B)
+    lens, before = [], []
+    for i in range(B):
+        kind = i % 3
+        at = int(g.randint(300, 900)) if kind == 1 else 0
+        new = 0 if kind == 2 else int(g.randint(1, 260))
+        lens.append(max(1, at + new))
+        before.append(lens[-1] if kind == 2 else at)
+    for H, KVH, window in ((8, 2, 290), (7, 1, 200)):
+        _prefill_case(cuda, H, KVH, 64, BF16, lens, before, window, 2, seed=B)
