@@ -157,8 +157,9 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * statistics are fp32. */
 
 /* ll_prefill_attention under a window. Requests whose b_seq_len is not above
- * their b_shared_seq_len have no query rows; rows of `out` that no request
- * owns are left as they were. max_input_len: no request has more query rows
+ * their b_shared_seq_len have no query rows (q and out may both be NULL where
+ * none has any: nothing is done); rows of `out` that no request owns are left as
+ * they were. max_input_len: no request has more query rows
  * (of one that has, those behind it may be left out). */
 int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h,
                                 const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,

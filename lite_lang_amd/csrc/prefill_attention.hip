@@ -1045,7 +1045,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                       int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_input_len,
                       bool win, int64_t window, int64_t sinks, float sm_scale, int dtype,
                       hipStream_t stream) {
-  if (win && batch == 0) return LL_OK;  // (an empty tensor has no address)
+  // (an empty tensor has no address: no requests, or none with query rows)
+  if (win && (batch == 0 || (!q && !out))) return LL_OK;
   LL_CHECK_ARG(q && k_cache && v_cache && out && req_to_tokens && b_req_idx && b_start_loc &&
                    b_seq_len,
                "%s: null pointer", fn);

@@ -268,8 +268,9 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
                              req_to_tokens, window, sinks=0, b_shared_seq_len=None, sm_scale=None):
     """prefill_attention in which the query at position p sees the keys n <= p
     with n > p - window or n < sinks. Slot-table entries of keys that no query
-    of the call sees are not read, so those tokens may have left the cache."""
-    (_, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window,
+    of the call sees are not read, so those tokens may have left the cache.
+    Requests may have no new token, and q no row."""
+    (T, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window,
                                                              sinks)
     bs = b_seq_len.shape
     assert len(bs) == 1 and b_req_idx.shape == bs and b_start_loc.shape == bs
@@ -281,6 +282,8 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
         sh_ptr, sh64 = b_shared_seq_len.data_ptr(), _idx(b_shared_seq_len, "b_shared_seq_len")
     stream = _here(dev, k.get_device(), v.get_device(), o.get_device(), b_req_idx.get_device(),
                    b_start_loc.get_device(), b_seq_len.get_device(), req_to_tokens.get_device())
+    if T == 0:
+        return o
     rc = _L.ll_call_window_prefill_attention(_lib.WINDOW_PREFILL_ATTENTION_CALL.pack(
         q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
         o.data_ptr(), os_[0], os_[1], req_to_tokens.data_ptr(), ts,

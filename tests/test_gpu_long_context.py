@@ -995,3 +995,19 @@ def test_window_prefill_attention_of_levels_beside_none(cuda, B):
         before.append(lens[-1] if kind == 2 else at)
     for H, KVH, window in ((8, 2, 290), (7, 1, 200)):
         _prefill_case(cuda, H, KVH, 64, BF16, lens, before, window, 2, seed=B)
+
+
+def test_window_prefill_of_cached_requests_alone(cuda):
+    """A step whose requests are all in the cache has no query row."""
+    pool = torch.full((20, 4, 64), float("nan"), device=cuda)
+    table = torch.zeros(3, 8, dtype=torch.int32, device=cuda)
+    a = [_i32(x, cuda) for x in ([2, 0, 1], [0, 0, 0], [8, 3, 0])]
+    none, wide = torch.zeros(0, 4, 64, device=cuda), torch.full((4, 4, 64), 7.0, device=cuda)
+    for q, o in ((none, none.clone()), (none, wide[:0]), (wide[4:], none), (wide[:0], wide[1:1])):
+        r = _ops().window_prefill_attention(q, pool[:, :2], pool[:, 2:], o, *a, 8, table, 4,
+                                            b_shared_seq_len=a[2])
+        assert r is o
+    torch.cuda.synchronize()
+    assert bool((wide == 7.0).all())
+    with pytest.raises(ValueError, match="device"):  # still checked
+        _ops().window_prefill_attention(none.cpu(), pool[:, :2], pool[:, 2:], none, *a, 8, table, 4)

@@ -375,3 +375,19 @@ def test_decode_refuses_more_workgroups_than_a_launch_holds():
     assert "workgroups" in L.ll_last_error().decode()
     # a product that wraps to 0, off the 16-bit paths
     assert window(1 << 24, 256, 256, D=96) == -1 and "65535" in L.ll_last_error().decode()
+
+
+def test_window_prefill_without_query_rows_does_nothing():
+    """Requests that are all in the cache: the tensors of their 0 rows have no
+    address. One address without the other is still an error."""
+    from lite_lang_amd import _lib
+    L, p = _lib.load(), 256
+
+    def call(q, out):
+        return L.ll_window_prefill_attention(q, 256, 64, p, 256, 64, p, 256, 64, out, 256, 64, p, 8,
+                                             p, 0, p, 0, p, 0, p, 0, 2, 4, 2, 64, 8, 8, 0,
+                                             ctypes.c_float(1.0), 2, None)
+
+    assert call(None, None) == 0
+    for q, out in ((None, p), (p, None)):
+        assert call(q, out) == -1 and "null pointer" in L.ll_last_error().decode()
