@@ -128,8 +128,10 @@ int ll_decode_attention_set_same_launch_merge(int enable);
  * q / o [T, q_heads, head_dim] hold, for request b, the rows
  * b_start_loc[b] .. b_start_loc[b] + (b_seq_len[b] - shared[b]) - 1; the keys
  * are the first b_seq_len[b] slots of row b_req_idx[b] of req_to_tokens.
- * The bf16/fp16, head_dim 64/128 path rejects (LL_ERR_ARG) launches of 2^31
- * or more work items (query-row blocks x requests x KV heads x head groups). */
+ * The bf16/fp16, head_dim 64/128 path rejects (LL_ERR_ARG) launches of more
+ * than 2^29 - 1024 work items (query-row blocks x requests x KV heads x head
+ * groups, which 2^32 threads take), the other one more than 2^26 - 1 rows of a
+ * request, both more than 2^31 - 1. */
 int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h,
                          const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
                          const void* v_cache, int64_t v_stride_tok, int64_t v_stride_head,
@@ -147,8 +149,8 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * with n > p - window (its own included) or n < sinks. window >= 1, sinks >= 0
  * (both may exceed the length); lengths at most 2^30, at most 2^24 requests and
  * 65535 query heads, and no more of both than one launch holds (a decode's
- * requests x KV heads x splits below 2^23; 65535 requests off the 16-bit paths
- * of heads of 64 and 128); sm_scale > 0. No counterpart in the reference (whose
+ * requests x KV heads x splits below 2^23, a prefill's work items as above;
+ * 65535 requests off the 16-bit paths of heads of 64 and 128); sm_scale > 0. No counterpart in the reference (whose
  * configs' use_sliding_window it does not read).
  * No entry of the slot table is read but those of keys that some query of the
  * request's call sees, so the tokens between the sinks and the window may have

@@ -1034,6 +1034,12 @@ __global__ __launch_bounds__(64) void prefill_attn_generic_kernel(PrefillArgs a,
   }
 }
 
+// A grid has fewer than 2^32 threads: workgroups of the generic path (one wave)
+// in a row, and work items of the MFMA path (512 threads for up to 64 of them,
+// in a multiple of 16 workgroups).
+constexpr int64_t kMaxRows = (((int64_t)1 << 32) - 1) / 64;
+constexpr int64_t kMaxItems = 64 * (((int64_t)1 << 32) / 512 - 16);
+
 // Both entry points: win false is the whole context (window and sinks unused).
 int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64_t q_stride_h,
                       const void* k_cache, int64_t k_stride_tok, int64_t k_stride_head,
@@ -1061,8 +1067,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                (long long)window, (long long)sinks);
   LL_CHECK_ARG(!win || (sm_scale > 0.f && sm_scale < INFINITY), "%s: sm_scale %g must be positive",
                fn, (double)sm_scale);
-  LL_CHECK_ARG(!win || max_input_len <= 1 << 30, "%s: max_input_len %lld out of range", fn,
-               (long long)max_input_len);
+  LL_CHECK_ARG(max_input_len <= (win ? 1 << 30 : INT32_MAX), "%s: max_input_len %lld out of range",
+               fn, (long long)max_input_len);
   if (batch == 0 || max_input_len <= 0) return LL_OK;
   PrefillArgs a;
   a.q = q; a.q_st = q_stride_tok; a.q_sh = q_stride_h;
@@ -1091,7 +1097,8 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   // (its rows are stored 16 bytes at a time; a causal call's may be anywhere)
   const bool out_ok = out_stride_tok % 8 == 0 && out_stride_h % 8 == 0 && (uintptr_t)out % 16 == 0;
   if (!mfma_ok || (win && !out_ok)) {
-    LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535, "%s: more than 65535 heads or requests", fn);
+    LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535 && max_input_len <= kMaxRows,
+                 "%s: more than 65535 heads or requests, or %lld rows", fn, (long long)kMaxRows);
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 4;
     return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
       const dim3 grid((unsigned)max_input_len, (unsigned)q_heads, (unsigned)batch);
@@ -1104,9 +1111,6 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
       LL_RETURN_LAUNCH();
     });
   }
-  int cus = 0;
-  const int rc = ll_device_cus(&cus);
-  if (rc != LL_OK) return rc;
   // four heads of 64 rows per workgroup when the group size allows, else two
   // heads of 128 rows (fewer idle head slots for G = 6 or 7). Windowed, also
   // * eight heads of 32 rows for a group one short of eight: as few idle slots
@@ -1123,18 +1127,26 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
   //   half (16/2 heads, 1 x 20 tokens 9.6 -> 8.6 us, 8 x 128 17.1 -> 12.0, by
   //   halves of two heads 9.1 and 14.9; where they do not fit one pass 40 x 100
   //   20.7 -> 26.3).
-  const bool single = a.G == 1 || (max_input_len <= 128 && batch * q_heads <= cus);
   auto tiles = [&](int w) {  // of an item whose window is whole
     return ((int64_t)a.window + a.sinks + 32 * w - 1 + kBK - 1) / kBK;
   };
   const bool eight = a.G % 8 == 7 || (a.G % 8 == 0 && tiles(1) < tiles(2));
-  const int wph = win && single ? 8 : win && eight ? 1 : a.G % 4 == 0 ? 2 : 4;
-  a.nblk = (int)ll_cdiv(max_input_len, 32 * wph);
+  int wph = win && a.G == 1 ? 8 : win && eight ? 1 : a.G % 4 == 0 ? 2 : 4;
+  auto blocks = [&](int w) { return (max_input_len + 32 * w - 1) / (32 * w); };
+  auto items = [&](int w) {
+    return (blocks(w) * batch * kv_heads + 7) / 8 * 8 * ll_cdiv(a.G, 8 / w);
+  };
+  LL_CHECK_ARG(batch <= kMaxItems / kv_heads / blocks(wph) && items(wph) <= kMaxItems,
+               "%s: %lld blocks of %d rows, %lld requests, %lld KV heads: more than %lld work items",
+               fn, (long long)blocks(wph), 32 * wph, (long long)batch, (long long)kv_heads,
+               (long long)kMaxItems);
+  int cus = 0;
+  if (const int rc = ll_device_cus(&cus)) return rc;
+  if (win && max_input_len <= 128 && batch * q_heads <= cus) wph = 8;
+  a.nblk = (int)blocks(wph);
   a.B = (int)batch;
   a.KVH = (int)kv_heads;
-  const int64_t units = (int64_t)a.nblk * batch * kv_heads;
-  const int64_t nv = (int64_t)ll_cdiv(units, 8) * 8 * ll_cdiv(a.G, 8 / wph);  // work items
-  LL_CHECK_ARG(nv < ((int64_t)1 << 31), "%s: %lld work items (max 2^31 - 1)", fn, (long long)nv);
+  const int64_t nv = items(wph);
   // persistent grid: one workgroup per CU (the LDS ring takes the whole CU),
   // a multiple of 16 so that the head groups of a (row block, request, KV
   // head) share an XCD on the reversed passes too; more when the items

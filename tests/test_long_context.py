@@ -391,3 +391,39 @@ def test_window_prefill_without_query_rows_does_nothing():
     assert call(None, None) == 0
     for q, out in ((None, p), (p, None)):
         assert call(q, out) == -1 and "null pointer" in L.ll_last_error().decode()
+
+
+def test_prefill_refuses_more_work_items_than_a_launch_holds():
+    """Counts of row blocks, requests and heads whose product wraps in 32 bits
+    (to none, and to fewer items than there are) and ones just above what a grid
+    of 2^32 threads takes."""
+    from lite_lang_amd import _lib
+    L, p = _lib.load(), 256
+
+    def args(H, KVH, D, B, most):
+        return [p, H * D, D, p, 2 * KVH * D, D, p, 2 * KVH * D, D, p, H * D, D, p, 8, p, 0, p, 0, p,
+                0, None, 0, B, H, KVH, D, most]
+
+    def window(H, KVH, B, most, win=100, D=128, dtype=2):
+        return L.ll_window_prefill_attention(*args(H, KVH, D, B, most), win, 0, ctypes.c_float(1.0),
+                                             dtype, None)
+
+    def plain(H, KVH, B, most, D=128, dtype=2):
+        return L.ll_prefill_attention(*args(H, KVH, D, B, most), ctypes.c_float(1.0), dtype, None)
+
+    # 2^24 blocks of 64 rows x 2^11 (request, KV head)s: 2^35; the same and one block
+    for call in (window, plain):
+        for most in (1 << 30, (1 << 30) - 63, (1 << 30) - (1 << 20)):
+            for H, KVH, B in ((8, 2, 1 << 10), (16, 2, 1 << 10), (7, 1, 1 << 11), (2, 2, 1 << 20),
+                              (4, 4, 1 << 24)):
+                assert call(H, KVH, B, most) == -1 and "work items" in L.ll_last_error().decode()
+    # 2^22 blocks of 256 rows, 2^23 of 64 and of 128, one head group each: 2^29 items
+    for H, KVH, B, most in ((2, 2, 64, 1 << 30), (8, 2, 32, 1 << 29), (4, 2, 32, 1 << 30)):
+        assert window(H, KVH, B, most) == -1 and "work items" in L.ll_last_error().decode()
+    assert plain(4, 1, 1 << 24, 1 << 30) == -1 and "work items" in L.ll_last_error().decode()
+    # off the 16-bit paths: a grid of one wave per row
+    for call in (window, plain):
+        assert call(4, 2, 2, 1 << 26, D=96) == -1 and "rows" in L.ll_last_error().decode()
+        assert call(4, 2, 2, 1 << 26, dtype=0) == -1 and "rows" in L.ll_last_error().decode()
+    assert plain(4, 2, 2, 1 << 31) == -1 and "out of range" in L.ll_last_error().decode()
+    assert plain(4, 2, 2, (1 << 38) + 5) == -1 and "out of range" in L.ll_last_error().decode()
