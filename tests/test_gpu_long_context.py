@@ -1011,3 +1011,23 @@ def test_window_prefill_of_cached_requests_alone(cuda):
     assert bool((wide == 7.0).all())
     with pytest.raises(ValueError, match="device"):  # still checked
         _ops().window_prefill_attention(none.cpu(), pool[:, :2], pool[:, 2:], none, *a, 8, table, 4)
+
+
+@pytest.mark.parametrize("B,H,KVH,D,n,sinks,splits", [(3, 8, 2, 128, 131072, 4, 42),
+                                                      (3, 4, 2, 64, 70000, 4, 85),
+                                                      (2, 2, 1, 128, 131072, 0, 128),
+                                                      (1, 2, 1, 64, 131072, 0, 336)])
+def test_window_decode_attention_of_more_splits_than_a_chunk(cuda, B, H, KVH, D, n, sinks, splits):
+    """Windows so long that the merge takes its splits 16 at a time, a last chunk
+    that is not full, sequences too short for most of the splits, and a workspace
+    that held NaN before the call. (Sharp scores, so that a split's keys show: the
+    outputs are a few dozen keys' mean.)"""
+    window = n - 5
+    need = _ops()._window_decode_bytes(B, H, KVH, D, n, window, sinks)
+    rows = B * H * splits
+    assert need == (rows * D * 4 + 255) // 256 * 256 + rows * 8, "the split count of this case"
+    lens = [n, 100, 5000][:B]
+    for seed in (1, 2):
+        _ops().workspace(cuda, "window_decode", need).fill_(255)  # NaN as fp32
+        out = _decode_case(cuda, H, KVH, D, BF16, lens, window, sinks, seed=seed, mag=3.0)
+        assert float(out.float().abs().mean()) > 0.05
