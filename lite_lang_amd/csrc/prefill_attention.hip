@@ -790,6 +790,9 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
   // each stores 8 elements of it at a time: half the store instructions, whose
   // 32 rows each take the memory path about 50 cycles (40 x 600, window 256,
   // 16/2 heads: 122 -> 114 us; the same rows as whole lines through LDS: 118).
+  // The rows of `out` may start at any element (global memory takes 16 bytes
+  // from any address).
+  typedef u32x4 __attribute__((aligned(2))) u32x4_any;
   auto store_rows = [&](const WaveItem& it) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -817,7 +820,7 @@ __global__ __launch_bounds__(512) void prefill_attn_fa_kernel(
             w[i] = p[0];
             w[2 + i] = p[1];
           }
-          *(u32x4*)(op + 32 * db + 8 * g) = w;
+          *(u32x4_any*)(op + 32 * db + 8 * g) = w;
         }
     }
   };
@@ -1094,9 +1097,7 @@ int prefill_attention(const char* fn, const void* q, int64_t q_stride_tok, int64
                        k_stride_tok >= 0 && k_stride_tok < ((int64_t)1 << 31) &&
                        v_stride_tok >= 0 && v_stride_tok < ((int64_t)1 << 31) &&
                        (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0);
-  // (its rows are stored 16 bytes at a time; a causal call's may be anywhere)
-  const bool out_ok = out_stride_tok % 8 == 0 && out_stride_h % 8 == 0 && (uintptr_t)out % 16 == 0;
-  if (!mfma_ok || (win && !out_ok)) {
+  if (!mfma_ok) {
     LL_CHECK_ARG(q_heads <= 65535 && batch <= 65535 && max_input_len <= kMaxRows,
                  "%s: more than 65535 heads or requests, or %lld rows", fn, (long long)kMaxRows);
     const size_t shm = head_dim * 4 + 64 * 4 + 64 * 4;

@@ -1031,3 +1031,34 @@ def test_window_decode_attention_of_more_splits_than_a_chunk(cuda, B, H, KVH, D,
         _ops().workspace(cuda, "window_decode", need).fill_(255)  # NaN as fp32
         out = _decode_case(cuda, H, KVH, D, BF16, lens, window, sinks, seed=seed, mag=3.0)
         assert float(out.float().abs().mean()) > 0.05
+
+
+@pytest.mark.parametrize("H,KVH,D,dtype", HEADS[:4])
+def test_prefill_into_rows_that_start_anywhere(cuda, H, KVH, D, dtype):
+    """Outputs whose rows start at 8-byte, 4-byte and 2-byte addresses, windowed
+    and causal: the bits of aligned rows, and nothing beside them. (The kernel of
+    other shapes sums in another order: its bits would differ.)"""
+    g = torch.Generator().manual_seed(D + H)
+    lens, before = [150, 40, 33], [0, 7, 0]
+    new = [n - c for n, c in zip(lens, before)]
+    T, n = sum(new), max(lens)
+    pool = torch.randn(3 * n, 2 * KVH, D, generator=g).to(dtype).to(cuda)
+    table = torch.randperm(3 * n, generator=g).to(torch.int32).view(3, n).to(cuda)
+    q = torch.randn(T, H, D, generator=g).to(dtype).to(cuda)
+    k, v, start = pool[:, :KVH], pool[:, KVH:], [0, new[0], new[0] + new[1]]
+    a = [_i32(x, cuda) for x in ([0, 1, 2], start, lens)]
+    for window in (None, 60):
+        for pad, at in ((4, 4), (2, 2), (3, 1), (1, 1)):
+            print(f"case: rows of {D + pad} from {at}, window {window} {dtype}", flush=True)
+            wide = torch.full((T, H, D + pad), 7.0, dtype=dtype, device=cuda)
+            outs = [torch.empty_like(q), wide[..., at:at + D]]
+            for o in outs:
+                if window is None:
+                    _ops().prefill_attention(q, k, v, o, *a, n, table,
+                                             b_shared_seq_len=_i32(before, cuda))
+                else:
+                    _ops().window_prefill_attention(q, k, v, o, *a, n, table, window, sinks=2,
+                                                    b_shared_seq_len=_i32(before, cuda))
+            assert torch.equal(*outs)
+            wide[..., at:at + D] = 7.0
+            assert bool((wide == 7.0).all())
