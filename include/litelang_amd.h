@@ -156,7 +156,13 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * request's call sees, so the tokens between the sinks and the window may have
  * left the cache and their entries may hold anything. Keys and values that one
  * query of the call sees and another does not must be finite. Sums and softmax
- * statistics are fp32. */
+ * statistics are fp32; the probabilities are rounded to the KV type ahead of P.V
+ * in the prefill, as ll_prefill_attention does (half a step each), and held as
+ * two numbers of it in the decode (2^-17 of each in bf16, 2^-22 in fp16).
+ * bf16 and fp16 with heads of 64 or 128 whose q, K and V rows start at 16-byte
+ * addresses (a decode's groups at most 16 query heads) run on the matrix cores;
+ * everything else takes a wave per query row and head: 11 to 160 times the time
+ * of a prefill of 4 x 300 to 1 x 8192 tokens, 15 to 200 times a decode's. */
 
 /* ll_prefill_attention under a window. Requests whose b_seq_len is not above
  * their b_shared_seq_len have no query rows (q and out may both be NULL where
@@ -344,10 +350,12 @@ int ll_assign_slots(int32_t* req_to_tokens, int64_t req_to_tokens_stride, const 
  * (or the block table), 2 a row outside the table or two requests with new
  * tokens on one row, 4 more new tokens than max_tokens, 8 than free pages.
  * Entries past the new tokens are left as they were. No output may overlap an
- * input. At most 8192 requests and 2^18 table rows; pages and slots are int32. Replaces, for lengths that live
- * on the device, the host construction of PageCache.alloc_token_idxs
- *   (litelang/models/cache.py:225-249) and of RunnerBatch's start offsets and
- * positions (litelang/models/runner_batch.py:88-265). */
+ * input. At most 8192 requests and 2^18 table rows; pages and slots are int32:
+ * the page ids of free_pages and block_table are not checked, and have to be in
+ * [0, 2^31 / page_size). Replaces, for lengths that live on the device, the host
+ * construction of PageCache.alloc_token_idxs (litelang/models/cache.py:225-249)
+ * and of RunnerBatch's start offsets and positions
+ * (litelang/models/runner_batch.py:88-265). */
 int ll_build_slot_maps(const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
                        int seq_len_i64, const void* b_cached_len, int cached_len_i64,
                        int64_t batch, const int32_t* free_pages, int64_t n_free, int64_t page_size,

@@ -1013,7 +1013,9 @@ __global__ __launch_bounds__(1024) void decode_attn_combine_quant_kernel(DecodeA
 // ---------------------------------------------------------------- generic path
 // One 64-lane workgroup per (sequence, query head); tokens are spread over the
 // lanes for q.k, the head dim over the lanes for p.v. Used for fp32 and for
-// shapes the MFMA path does not cover; exactness, not speed, is its purpose.
+// shapes the MFMA path does not cover; exactness, not speed, is its purpose
+// (windowed, 16/2 heads, 40 x 256 visible tokens: bf16 heads of 128 9.7 us on the
+// MFMA path, of 96 145 here, fp32 of 128 189; 40 x 4100: 35, 2660, 3730).
 template <typename T, bool WIN>
 __global__ __launch_bounds__(64) void decode_attn_generic_kernel(DecodeArgs a, int D, float sm_scale) {
   const int b = blockIdx.y;

@@ -12,8 +12,9 @@
 // step writes a few hundred bytes; 260,000 new tokens write 3 MB, half a
 // microsecond of HBM time), so a second launch for the prefix sums would cost
 // more than having every workgroup sum the batch's lengths for itself. It
-// checks everything before it writes anything: what is wrong is reported in
-// counts[2] and the tables stay as they were.
+// checks lengths, rows and room before it writes anything: what is wrong there
+// is reported in counts[2] and the tables stay as they were. Page ids are taken
+// as they are: every workgroup would have to read all that the call takes.
 #include <algorithm>
 
 #include "ll_common.h"

@@ -269,7 +269,10 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
     """prefill_attention in which the query at position p sees the keys n <= p
     with n > p - window or n < sinks. Slot-table entries of keys that no query
     of the call sees are not read, so those tokens may have left the cache.
-    Requests may have no new token, and q no row."""
+    Requests may have no new token, and q no row. Probabilities are rounded to
+    the cache's dtype ahead of P.V, as in prefill_attention. Heads of other than
+    64 and 128, fp32 and rows of q, k or v off 16-byte addresses are served one
+    row and head per wave, 10 to 160 times slower."""
     (T, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, k, v, o, req_to_tokens, window,
                                                              sinks)
     bs = b_seq_len.shape
@@ -299,7 +302,11 @@ def window_prefill_attention(q, k, v, o, b_req_idx, b_start_loc, b_seq_len, max_
 
 def window_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_batch, cache_k,
                             cache_v, out, window, sinks=0, sm_scale=None):
-    """decode_attention over the last `window` tokens and the first `sinks` ones."""
+    """decode_attention over the last `window` tokens and the first `sinks` ones.
+    Entries of length 0 give zero rows and may sit on any row. Heads of other than
+    64 and 128, more than 16 query heads to a KV head, fp32 and rows of q or the
+    cache off 16-byte addresses are served one head per wave, 15 to 200 times
+    slower."""
     (B, H, D), KVH, dt, qs, ks, vs, os_, ts = _window_checks(q, cache_k, cache_v, out,
                                                              req_to_tokens, window, sinks)
     assert b_req_idx.shape == (B,) and b_seq_len.shape == (B,)
@@ -392,7 +399,8 @@ def rope_frequencies(rotary_dim, theta=1e6, scaling=None, max_position=None, len
     qk_norm_rope_kv_scatter: theta^(-2i/rotary_dim), scaled for contexts beyond
     the max_position tokens a model was trained on as a Hugging Face config's
     `rope_scaling` dict says (rope_type or type; `original_max_position_embeddings`
-    in it takes max_position's place):
+    in it takes max_position's place) if it is of one of these types; others,
+    such as llama3, are refused:
 
     * default: none;
     * linear: every frequency divided by `factor`;
@@ -795,7 +803,7 @@ def build_slot_maps(b_req_idx, b_seq_len, b_cached_len, free_pages, req_to_token
     req_to_tokens; counts [3] = (new tokens, pages taken, error). The error
     word is 0, or, with nothing but counts written, the sum of 1: a length out
     of range, 2: a bad or repeated row, 4: more tokens than `slots` holds, 8:
-    too few free pages."""
+    too few free pages. Page ids are not checked (below 2^31 / page_size)."""
     bs, i32 = b_req_idx.shape, torch.int32
     (B,) = bs
     assert b_seq_len.shape == bs and b_cached_len.shape == bs
