@@ -150,8 +150,9 @@ int ll_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * (both may exceed the length); lengths at most 2^30, at most 2^24 requests and
  * 65535 query heads, and no more of both than one launch holds (a decode's
  * requests x KV heads x splits below 2^23, a prefill's work items as above;
- * 65535 requests off the 16-bit paths of heads of 64 and 128); sm_scale > 0. No counterpart in the reference (whose
- * configs' use_sliding_window it does not read).
+ * 65535 requests off the 16-bit paths of heads of 64 and 128); sm_scale > 0. No
+ * counterpart in the reference (whose configs' use_sliding_window it does not
+ * read).
  * No entry of the slot table is read but those of keys that some query of the
  * request's call sees, so the tokens between the sinks and the window may have
  * left the cache and their entries may hold anything. Keys and values that one
