@@ -185,9 +185,9 @@ int ll_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_s
 /* ll_decode_attention under a window: the query is the token at b_seq_len - 1,
  * so its keys are one list, the sinks and the last `window` tokens. Sequences
  * of length 0 give zero rows and may have any b_req_idx. The workspace (0 bytes
- * where the list is not split, and for shapes that the call refuses) needs no initialisation and nothing in it lasts beyond the call; it
- * must not be one of ll_decode_attention, which has to find its own as it left
- * it. */
+ * where the list is not split, and for shapes that the call refuses) needs no
+ * initialisation and nothing in it lasts beyond the call; it must not be one of
+ * ll_decode_attention, which has to find its own as it left it. */
 int64_t ll_window_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                   int64_t head_dim, int64_t max_len_in_batch,
                                                   int64_t window, int64_t sinks);
