@@ -716,6 +716,116 @@ int ll_quant_static(const void* X, int64_t ldx, int64_t M, int64_t K, int dtype,
 int ll_dequant_splitk(const int32_t* part, int splits, const float* s_tok, const void* s_ch,
                       int s_ch_dtype, float* out, int64_t M, int64_t N, hipStream_t stream);
 
+/* ------------------------------------------------- 8-bit KV cache (kv8.hip)
+ * No counterpart in the reference, whose cache is in the model's dtype.
+ *
+ * k_codes / v_codes [slots_n, kv_heads, head_dim] hold one byte per element,
+ * of `code` kind LL_KV8_INT8 or LL_KV8_E4M3; k_scale / v_scale hold an fp32
+ * scale per block of `block` consecutive slots (a power of two up to 128) and
+ * head: value = code * scale[slot / block, head]. Strides in elements, the last
+ * dimension contiguous. Slots are int32; one outside [0, slots_n) is no token:
+ * it is not stored, reads as zeros and is not attended to. A table row outside
+ * [0, req_rows) makes its request an empty one. */
+#define LL_KV8_INT8 0
+#define LL_KV8_E4M3 1
+
+/* k, v [ntok, kv_heads, head_dim] in `dtype`, quantised on their way to their
+ * slots. Tokens that follow each other in one block (padded ones among them
+ * aside) are a run; a run that starts at the block's first slot begins the block
+ * anew, any other continues it. The scale is max(fl32(max |x| / top), 2^-80) over the run, top 127 or 448,
+ * and where the run continues a block no less than the block's: where it grows,
+ * the codes of the slots in front of the run are rounded again. Codes are the
+ * nearest to x / scale, ties to even. An infinity or NaN among a head's elements
+ * of a run makes that block and head's scale NaN (until the block begins anew)
+ * and the run's codes 0. The slots of a call differ, and those of one block
+ * stand next to each other in ascending order (ll_build_slot_maps lists them
+ * so). No output may overlap an input. head_dim at most 1024, 2^24 tokens. */
+int ll_kv8_store(const void* k, int64_t k_stride_tok, int64_t k_stride_h, const void* v,
+                 int64_t v_stride_tok, int64_t v_stride_h, const int32_t* slots, int64_t ntok,
+                 int64_t kv_heads, int64_t head_dim, void* k_codes, int64_t kc_stride_tok,
+                 int64_t kc_stride_h, void* v_codes, int64_t vc_stride_tok, int64_t vc_stride_h,
+                 float* k_scale, int64_t ks_stride_block, int64_t ks_stride_h, float* v_scale,
+                 int64_t vs_stride_block, int64_t vs_stride_h, int64_t slots_n, int64_t block,
+                 int code, int dtype, hipStream_t stream);
+
+/* k_out / v_out[b_start_loc[b] + n] = dtype(code * scale) of the token
+ * req_to_tokens[b_req_idx[b], n], n < b_seq_len[b] (and max_len_in_batch): the
+ * contexts one after the other, as ll_prefill_attention reads them through a
+ * slot table of b_start_loc[b] + n. Rows outside [0, out_rows) are not written,
+ * rows of no request are left as they were. head_dim at most 1024, 65535
+ * requests. */
+int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t kc_stride_h,
+                const void* v_codes, int64_t vc_stride_tok, int64_t vc_stride_h,
+                const float* k_scale, int64_t ks_stride_block, int64_t ks_stride_h,
+                const float* v_scale, int64_t vs_stride_block, int64_t vs_stride_h,
+                int64_t slots_n, int64_t block, int code, const int32_t* req_to_tokens,
+                int64_t req_to_tokens_stride, int64_t req_rows, const void* b_req_idx,
+                int req_idx_i64, const void* b_start_loc, int start_loc_i64,
+                const void* b_seq_len, int seq_len_i64, int64_t batch, int64_t max_len_in_batch,
+                void* k_out, int64_t ko_stride_tok, int64_t ko_stride_h, void* v_out,
+                int64_t vo_stride_tok, int64_t vo_stride_h, int64_t out_rows, int64_t kv_heads,
+                int64_t head_dim, int dtype, hipStream_t stream);
+
+/* ll_decode_attention over this cache: q, out [batch, q_heads, head_dim] in
+ * `dtype`. Requests of length 0 give zero rows. head_dim at most 512. The
+ * workspace needs no initialisation. */
+int64_t ll_kv8_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t max_len_in_batch);
+int ll_kv8_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                            const void* k_codes, int64_t kc_stride_tok, int64_t kc_stride_h,
+                            const void* v_codes, int64_t vc_stride_tok, int64_t vc_stride_h,
+                            const float* k_scale, int64_t ks_stride_block, int64_t ks_stride_h,
+                            const float* v_scale, int64_t vs_stride_block, int64_t vs_stride_h,
+                            int64_t slots_n, int64_t block, int code,
+                            const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                            int64_t req_rows, const void* b_req_idx, int req_idx_i64,
+                            const void* b_seq_len, int seq_len_i64, void* out,
+                            int64_t out_stride_b, int64_t out_stride_h, int64_t batch,
+                            int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_len_in_batch, float sm_scale, int dtype, void* workspace,
+                            int64_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------- 4-bit weights (w4.hip)
+ * No counterpart in the reference's runtime. codes [N, K / 2] (strides in
+ * bytes) hold input 2 i of a row in the low and 2 i + 1 in the high half of byte
+ * i; scale [N, K / group] in the activations' 16-bit dtype, zero [N, K / group]
+ * one byte each (its low 4 bits count), or null: 8 throughout. group is 32, 64
+ * or 128 and divides K. ll_w4_pack lays a weight out as ll_linear_w4 reads it:
+ *   Y[m, n] = dtype(sum_k X[m, k] (c[n, k] - zero) scale + bias[n])
+ * with fp32 sums (bf16 / fp16; M at most 2^19). An infinity or NaN in X makes
+ * its row of Y NaN or infinite. */
+int64_t ll_w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zero);
+int ll_w4_pack(const uint8_t* codes, int64_t ldc, const void* scale, int64_t ld_scale,
+               const uint8_t* zero, int64_t ld_zero, int64_t N, int64_t K, int64_t group,
+               void* packed, int64_t packed_bytes, hipStream_t stream);
+int ll_linear_w4(const void* x, int64_t ldx, const void* packed, int has_zero, int64_t group,
+                 const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                 int dtype, hipStream_t stream);
+
+/* ------------------------------------------------ logit controls (logits.hip)
+ * out[b, v] from logits[b, v] (which out may be, with the same stride) and the
+ * request's tokens, row b_req_idx[b] of tokens [tokens_rows, tokens_cols]: its
+ * prompt [0, b_prompt_len[b]) and its answer up to b_seq_len[b] (at most
+ * tokens_cols). In this order, in fp32 with one rounding at the end:
+ *   x / repetition[b] (x > 0) or x * repetition[b], where v is in either;
+ *   x - frequency[b] * (count of v in the answer);
+ *   x - presence[b] where v is in the answer;
+ *   x + every bias_values[b, i] with bias_ids[b, i] == v, added up in order;
+ *   -inf where bit v % 32 of mask[b, v / 32] is 0.
+ * Any of repetition, frequency, presence, the biases (n_bias 0) and the mask may
+ * be null; without penalties tokens too. Ids outside [0, vocab) and rows outside
+ * the table count for nothing. 65535 requests, 2^20 biases. The reference takes
+ * its argmax of the plain logits (post_layer.py:75-77). */
+int ll_adjust_logits(const void* logits, int64_t ld_logits, void* out, int64_t ld_out,
+                     int64_t batch, int64_t vocab, const int32_t* tokens, int64_t tokens_stride,
+                     int64_t tokens_rows, int64_t tokens_cols, const void* b_req_idx,
+                     int req_idx_i64, const void* b_prompt_len, int prompt_len_i64,
+                     const void* b_seq_len, int seq_len_i64, const float* repetition,
+                     const float* frequency, const float* presence, const int32_t* bias_ids,
+                     int64_t bias_ids_stride, const float* bias_values,
+                     int64_t bias_values_stride, int64_t n_bias, const uint32_t* mask,
+                     int64_t mask_stride, int dtype, hipStream_t stream);
+
 /* ---- Measurement probes (no counterpart in the reference; bench.py
  * --attention-floor times the first two against the decode attention,
  * bench.py --launch-floor the third).
@@ -834,6 +944,47 @@ typedef struct {
       b_start_loc, last_rows, counts, stream;
 } LLBuildSlotMapsCall;
 int64_t ll_call_build_slot_maps(const LLBuildSlotMapsCall* c);
+
+typedef struct {
+  int64_t k, k_stride_tok, k_stride_h, v, v_stride_tok, v_stride_h, slots, ntok, kv_heads, head_dim,
+      k_codes, kc_stride_tok, kc_stride_h, v_codes, vc_stride_tok, vc_stride_h, k_scale,
+      ks_stride_block, ks_stride_h, v_scale, vs_stride_block, vs_stride_h, slots_n, block, code,
+      dtype, stream;
+} LLKv8StoreCall;
+int64_t ll_call_kv8_store(const LLKv8StoreCall* c);
+
+typedef struct {
+  int64_t k_codes, kc_stride_tok, kc_stride_h, v_codes, vc_stride_tok, vc_stride_h, k_scale,
+      ks_stride_block, ks_stride_h, v_scale, vs_stride_block, vs_stride_h, slots_n, block, code,
+      req_to_tokens, req_to_tokens_stride, req_rows, b_req_idx, req_idx_i64, b_start_loc,
+      start_loc_i64, b_seq_len, seq_len_i64, batch, max_len_in_batch, k_out, ko_stride_tok,
+      ko_stride_h, v_out, vo_stride_tok, vo_stride_h, out_rows, kv_heads, head_dim, dtype, stream;
+} LLKv8LoadCall;
+int64_t ll_call_kv8_load(const LLKv8LoadCall* c);
+
+typedef struct {
+  int64_t q, q_stride_b, q_stride_h, k_codes, kc_stride_tok, kc_stride_h, v_codes, vc_stride_tok,
+      vc_stride_h, k_scale, ks_stride_block, ks_stride_h, v_scale, vs_stride_block, vs_stride_h,
+      slots_n, block, code, req_to_tokens, req_to_tokens_stride, req_rows, b_req_idx, req_idx_i64,
+      b_seq_len, seq_len_i64, out, out_stride_b, out_stride_h, batch, q_heads, kv_heads, head_dim,
+      max_len_in_batch;
+  double sm_scale;
+  int64_t dtype, workspace, workspace_bytes, stream;
+} LLKv8DecodeAttentionCall;
+int64_t ll_call_kv8_decode_attention(const LLKv8DecodeAttentionCall* c);
+
+typedef struct {
+  int64_t x, ldx, packed, has_zero, group, bias, y, ldy, M, N, K, dtype, stream;
+} LLLinearW4Call;
+int64_t ll_call_linear_w4(const LLLinearW4Call* c);
+
+typedef struct {
+  int64_t logits, ld_logits, out, ld_out, batch, vocab, tokens, tokens_stride, tokens_rows,
+      tokens_cols, b_req_idx, req_idx_i64, b_prompt_len, prompt_len_i64, b_seq_len, seq_len_i64,
+      repetition, frequency, presence, bias_ids, bias_ids_stride, bias_values, bias_values_stride,
+      n_bias, mask, mask_stride, dtype, stream;
+} LLAdjustLogitsCall;
+int64_t ll_call_adjust_logits(const LLAdjustLogitsCall* c);
 
 #ifdef __cplusplus
 }

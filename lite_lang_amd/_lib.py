@@ -29,6 +29,11 @@ WINDOW_DECODE_ATTENTION_CALL = struct.Struct("=25qd4q")
 ROPE_POSITIONS_CALL = struct.Struct("=19qd4q")
 QK_NORM_ROPE_KV_SCATTER_CALL = struct.Struct("=11qd5qd7q")
 BUILD_SLOT_MAPS_CALL = struct.Struct("=24q")
+KV8_STORE_CALL = struct.Struct("=27q")
+KV8_LOAD_CALL = struct.Struct("=37q")
+KV8_DECODE_ATTENTION_CALL = struct.Struct("=33qd4q")
+LINEAR_W4_CALL = struct.Struct("=13q")
+ADJUST_LOGITS_CALL = struct.Struct("=28q")
 
 # name -> (restype, argtypes), mirroring include/litelang_amd.h
 SIGNATURES = {
@@ -138,6 +143,20 @@ SIGNATURES = {
     "ll_silu_and_mul_splitk_i32": (I32, [P, I32, P, P, I32, P, I64, I64, I64, I32, P]),
     "ll_rope_kv_scatter_splitk": (I32, [P, I32, P, P, I64, I64, I64, I64, I64, P, I32, P, P, I64,
                                         I32, P, P, I64, I64, I32, P]),
+    "ll_kv8_store": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, P,
+                           I64, I64, P, I64, I64, I64, I64, I32, I32, P]),
+    "ll_kv8_load": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I64, I64, I32, P, I64,
+                          I64, P, I32, P, I32, P, I32, I64, I64, P, I64, I64, P, I64, I64, I64, I64,
+                          I64, I32, P]),
+    "ll_kv8_decode_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64,
+                                      I64, I64, I64, I32, P, I64, I64, P, I32, P, I32, P, I64, I64,
+                                      I64, I64, I64, I64, I64, F32, I32, P, I64, P]),
+    "ll_linear_w4": (I32, [P, I64, P, I32, I64, P, P, I64, I64, I64, I64, I32, P]),
+    "ll_adjust_logits": (I32, [P, I64, P, I64, I64, I64, P, I64, I64, I64, P, I32, P, I32, P, I32,
+                               P, P, P, P, I64, P, I64, I64, P, I64, I32, P]),
+    "ll_kv8_decode_attention_workspace_size": (I64, [I64] * 5),
+    "ll_w4_packed_bytes": (I64, [I64, I64, I64, I32]),
+    "ll_w4_pack": (I32, [P, I64, P, I64, P, I64, I64, I64, I64, P, I64, P]),
     "ll_probe_stream_read": (I32, [P, I64, I64, P, P]),
     "ll_probe_kv_gather": (I32, [P, I64, I64, P, I64, I64, P, I64, P, I32, P, I32, I64, I64, I64,
                                  I64, I64, I64, I32, P, P]),
@@ -154,6 +173,11 @@ SIGNATURES = {
     "ll_call_rope_positions": (I64, [ctypes.c_char_p]),
     "ll_call_qk_norm_rope_kv_scatter": (I64, [ctypes.c_char_p]),
     "ll_call_build_slot_maps": (I64, [ctypes.c_char_p]),
+    "ll_call_kv8_store": (I64, [ctypes.c_char_p]),
+    "ll_call_kv8_load": (I64, [ctypes.c_char_p]),
+    "ll_call_kv8_decode_attention": (I64, [ctypes.c_char_p]),
+    "ll_call_linear_w4": (I64, [ctypes.c_char_p]),
+    "ll_call_adjust_logits": (I64, [ctypes.c_char_p]),
 }
 
 

@@ -1,0 +1,596 @@
+// A KV cache held in 8 bits (gfx950): K and V quantised as they are written,
+// read back, and attention of one query token per request over them.
+//
+// A code is an int8 number or an e4m3 float; a block is `block` consecutive
+// slots (a power of two, the page size or a part of it), and every block holds
+// an fp32 scale for each K head and each V head:
+//   value = code * scale[slot / block, head].
+// Tokens of a call that follow each other in one block (padded ones among them
+// aside) are a run. With top the
+// largest code (127, 448), a run alone asks for the scale
+//   s = max(fl32(max |x| / top), 2^-80)
+// (the floor keeps every quotient below and its residual normal numbers). A run
+// that starts at a block's first slot begins the block anew: whatever a former
+// owner of the page left there is forgotten. Any other run continues the block:
+// its scale is the larger one of the block's and the run's, and where it grew
+// the codes in front of the run are rounded again, to
+//   code' = round(code * s_old / s_new).
+// Codes are the nearest ones to the quotient itself, ties to even: no code
+// depends on how a division rounds.
+#include <algorithm>
+#include <mutex>
+
+#include "ll_common.h"
+
+namespace {
+
+enum { KV8_INT8 = LL_KV8_INT8, KV8_E4M3 = LL_KV8_E4M3 };
+
+constexpr float kScaleFloor = 0x1p-80f;
+
+template <int CODE> struct CodeOf;
+template <> struct CodeOf<KV8_INT8> {
+  static constexpr float top = 127.f;
+  static __device__ __forceinline__ uint32_t encode(float q) {
+    return (uint32_t)(uint8_t)(int8_t)(int)__builtin_rintf(q);
+  }
+  // byte i of w as a number
+  static __device__ __forceinline__ float decode(uint32_t w, int i) {
+    return (float)(int8_t)(uint8_t)(w >> (8 * i));
+  }
+};
+template <> struct CodeOf<KV8_E4M3> {
+  static constexpr float top = 448.f;
+  static __device__ __forceinline__ uint32_t encode(float q) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false) & 0xffu;
+  }
+  static __device__ __forceinline__ float decode(uint32_t w, int i) {
+    switch (i) {
+      case 0: return __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+      case 1: return __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+      case 2: return __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+      default: return __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+    }
+  }
+};
+
+// x / s rounded toward zero, its last bit set where that was inexact (rounding
+// to odd): rounding the result once more to 16 bits or fewer gives what rounding
+// the quotient itself gives. r is 1 / s. The first two lines are within an ulp
+// of the quotient; the residual x - q s then has the quotient's error's sign
+// (the scale's floor keeps it from underflowing where a code depends on it).
+__device__ __forceinline__ float quotient_to_odd(float x, float s, float r) {
+  float q = x * r;
+  q = __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q);
+  const float e = __builtin_fmaf(-q, s, x);
+  uint32_t b = __builtin_bit_cast(uint32_t, q);
+  const bool over = (__builtin_bit_cast(uint32_t, e) ^ b) >> 31;  // |q| is too large
+  const bool off = e != 0.f;
+  b -= (off && over) ? 1u : 0u;
+  b |= off ? 1u : 0u;
+  return __builtin_bit_cast(float, b);
+}
+
+// A code times s_old / s_new, rounded to a code again.
+template <int CODE>
+__device__ __forceinline__ uint32_t recode(float c, float s_old, float s_new) {
+  const double q = (double)c * (double)s_old / (double)s_new;
+  float f = (float)q;
+  uint32_t b = __builtin_bit_cast(uint32_t, f);
+  if ((double)f != q) {
+    if (fabs((double)f) > fabs(q)) b -= 1u;
+    b |= 1u;
+  }
+  return CodeOf<CODE>::encode(__builtin_bit_cast(float, b));
+}
+
+struct StoreArgs {
+  const void* x[2]; int64_t x_st[2], x_sh[2];  // K, V: [ntok, heads, D]
+  const int32_t* slots;
+  uint8_t* c[2]; int64_t c_st[2], c_sh[2];
+  float* s[2]; int64_t s_sb[2], s_sh[2];
+  int64_t T, nslots;
+  int KVH, D, shift, per;  // block = 1 << shift; tokens per wave
+};
+
+constexpr int kStoreWaves = 4;
+
+// 8 elements from d on as floats; those at D and behind are 0
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int d, int D, float (&v)[8]) {
+  if constexpr (VEC) {
+    constexpr int kW = sizeof(T) / 2;
+    u32x4 w[kW];
+#pragma unroll
+    for (int i = 0; i < kW; ++i) w[i] = ((const u32x4*)(p + d))[i];
+    const T* e = (const T*)w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ll_to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = d + i < D ? ll_to_f32(p[d + i]) : 0.f;
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* p, int d, int D, const uint32_t (&w)[2]) {
+  if constexpr (VEC) {
+    *(uint2*)(p + d) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d + i < D) p[d + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// One wave: the runs that start among `per` tokens, of one head's K or V.
+// A row takes as many lanes as it has groups of 8 elements, and the wave as many
+// rows at a time as fit; the run's rows are read twice, for its largest element
+// and for its codes (the second time from the cache).
+template <typename T, int CODE, bool VEC>
+__global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * kStoreWaves + (threadIdx.x >> 6);
+  const int units = 2 * a.KVH;
+  const int64_t t0 = wave / units * a.per;
+  const int unit = (int)(wave % units);
+  if (t0 >= a.T) return;
+  const int kv = unit / a.KVH, head = unit % a.KVH;
+  const T* x = (const T*)a.x[kv] + head * a.x_sh[kv];
+  uint8_t* c = a.c[kv] + head * a.c_sh[kv];
+  float* sc = a.s[kv] + head * a.s_sh[kv];
+  const int64_t xs = a.x_st[kv], cs = a.c_st[kv];
+  const int D = a.D, groups = (D + 7) / 8;
+  int lpr = 1;  // lanes per row
+  while (lpr < groups && lpr < 64) lpr *= 2;
+  const int rows = 64 / lpr, row = lane / lpr, d0 = lane % lpr * 8;
+
+  const auto valid = [&](int32_t s) { return s >= 0 && s < a.nslots; };
+  const int64_t t1 = min(t0 + (int64_t)a.per, a.T);
+  bool ours = false;  // whether the next token stored begins a run (known behind the first run)
+  for (int64_t t = t0; t < t1;) {
+    const int32_t first = a.slots[t];
+    if (!valid(first)) {
+      ++t;
+      continue;
+    }
+    const int32_t blk = first >> a.shift;
+    // the run's end (the first token of another block; padded ones among the
+    // run's belong to no block) and its last token, 256 tokens at a time
+    int64_t end = -1, last = t + 1;
+    for (int64_t i0 = t + 1; end < 0; i0 += 256) {
+      int32_t s[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] = a.slots[min(i0 + c * 64 + lane, a.T - 1)];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int64_t base = i0 + c * 64;
+        const bool in = base + lane < a.T, here = valid(s[c]) && s[c] >> a.shift == blk;
+        const uint64_t other = __ballot(!in || (valid(s[c]) && !here));
+        uint64_t same = __ballot(in && here);
+        if (end >= 0) continue;
+        const int cut = other ? __builtin_ctzll(other) : 64;
+        if (other) {
+          same &= ((uint64_t)1 << cut) - 1;
+          end = base + cut;
+        }
+        if (same) last = base + 64 - __builtin_clzll(same);
+      }
+    }
+    if (!ours) {  // a run that began before this wave's tokens is another wave's
+      bool theirs = false;
+      for (int64_t i0 = t - 1; i0 >= 0; i0 -= 64) {
+        const int64_t i = i0 - lane;
+        const int32_t s = a.slots[max(i, (int64_t)0)];
+        const bool is = i >= 0 && valid(s);
+        const uint64_t m = __ballot(is), same = __ballot(is && s >> a.shift == blk);
+        if (m) {
+          theirs = same >> __builtin_ctzll(m) & 1;
+          break;
+        }
+      }
+      ours = true;
+      if (theirs) {
+        t = end;
+        continue;
+      }
+    }
+    float top = 0.f;
+    bool bad = false;
+    for (int64_t i = t + row; i < last; i += rows)
+      for (int d = d0; d < D; d += lpr * 8) {
+        if (!valid(a.slots[i])) continue;
+        float v[8];
+        load8<T, VEC>(x + i * xs, d, D, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          bad |= !(fabsf(v[e]) < INFINITY);
+          top = fmaxf(top, fabsf(v[e]));
+        }
+      }
+    top = ll_wave_max(top);
+    float s = fmaxf(top / CodeOf<CODE>::top, kScaleFloor);
+    if (__ballot(bad)) s = __builtin_nanf("");
+    float* sp = sc + blk * a.s_sb[kv];
+    const int off = first & ((1 << a.shift) - 1);
+    if (off > 0) {
+      const float old = *sp;
+      if (!(s <= old)) {  // it grew, or either is NaN (which stays)
+        if (!(s > old)) s = __builtin_nanf("");
+        else
+          for (int j = row; j < off; j += rows)
+            for (int d = d0; d < D; d += lpr * 8) {
+              uint8_t* p = c + (((int64_t)blk << a.shift) + j) * cs + d;
+              for (int e = 0; e < min(8, D - d); ++e)
+                p[e] = (uint8_t)recode<CODE>(CodeOf<CODE>::decode(p[e], 0), old, s);
+            }
+      } else {
+        s = old;
+      }
+    }
+    const bool ok = s < INFINITY;
+    const float r = 1.f / s;
+    for (int64_t i = t + row; i < last; i += rows)
+      for (int d = d0; d < D; d += lpr * 8) {
+        const int32_t slot = a.slots[i];
+        if (!valid(slot)) continue;
+        float v[8];
+        load8<T, VEC>(x + i * xs, d, D, v);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (ok) w[e >> 2] |= CodeOf<CODE>::encode(quotient_to_odd(v[e], s, r)) << (8 * (e & 3));
+        store8<VEC>(c + slot * cs, d, D, w);
+      }
+    if (lane == 0) *sp = s;
+    t = end;
+  }
+}
+
+struct LoadArgs {
+  const uint8_t* c[2]; int64_t c_st[2], c_sh[2];
+  const float* s[2]; int64_t s_sb[2], s_sh[2];
+  const int32_t* r2t; int64_t r2t_s, r2t_rows;
+  const void* req; int req64;
+  const void* start; int start64;
+  const void* len; int len64;
+  void* o[2]; int64_t o_st[2], o_sh[2];
+  int64_t nslots, orows;
+  int KVH, D, shift, max_len, pieces;  // pieces: of a head's row
+};
+
+constexpr int kLoadThreads = 256;
+
+// A thread takes 16 codes of a row (VEC) or one; rows of a token first, then
+// the request's next tokens.
+template <typename T, int CODE, bool VEC>
+__global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
+  const int b = blockIdx.y;
+  const int64_t row = ll_load_idx(a.req, b, a.req64);
+  const int64_t n = std::min<int64_t>(ll_load_idx(a.len, b, a.len64), a.max_len);
+  if (row < 0 || row >= a.r2t_rows) return;
+  const int64_t base = ll_load_idx(a.start, b, a.start64);
+  const int32_t* table = a.r2t + row * a.r2t_s;
+  const int per = 2 * a.KVH * a.pieces;
+  const int64_t total = n * per;
+  for (int64_t i = (int64_t)blockIdx.x * kLoadThreads + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * kLoadThreads) {
+    const int64_t tok = i / per;
+    int k = (int)(i - tok * per);
+    const int64_t orow = base + tok;
+    if (orow < 0 || orow >= a.orows) continue;
+    const int piece = k % a.pieces;
+    k /= a.pieces;
+    const int head = k % a.KVH, kv = k / a.KVH;
+    const int32_t slot = table[tok];
+    const bool there = slot >= 0 && slot < a.nslots;
+    const float s = there ? a.s[kv][(slot >> a.shift) * a.s_sb[kv] + head * a.s_sh[kv]] : 0.f;
+    const uint8_t* c = a.c[kv] + (there ? slot : 0) * a.c_st[kv] + head * a.c_sh[kv];
+    T* o = (T*)a.o[kv] + orow * a.o_st[kv] + head * a.o_sh[kv];
+    if constexpr (VEC) {
+      u32x4 w = {0, 0, 0, 0};
+      if (there) w = *(const u32x4*)(c + piece * 16);
+      constexpr int kW = sizeof(T);
+      u32x4 y[kW];
+      T* e = (T*)y;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) e[j] = ll_from_f32<T>(CodeOf<CODE>::decode(w[j >> 2], j & 3) * s);
+#pragma unroll
+      for (int j = 0; j < kW; ++j) ((u32x4*)(o + piece * 16))[j] = y[j];
+    } else {
+      o[piece] = there ? ll_from_f32<T>(CodeOf<CODE>::decode(c[piece], 0) * s) : ll_from_f32<T>(0.f);
+    }
+  }
+}
+
+struct DecodeArgs8 {
+  const void* q; int64_t q_sb, q_sh;
+  const uint8_t* c[2]; int64_t c_st[2], c_sh[2];
+  const float* s[2]; int64_t s_sb[2], s_sh[2];
+  const int32_t* r2t; int64_t r2t_s, r2t_rows;
+  const void* req; int req64;
+  const void* len; int len64;
+  void* out; int64_t o_sb, o_sh;
+  int64_t nslots;
+  int B, H, KVH, G, D, shift, max_len;
+  float scale_log2;
+};
+
+__device__ __forceinline__ int decode_len(const DecodeArgs8& a, int b, int64_t* row) {
+  *row = ll_load_idx(a.req, b, a.req64);
+  const int64_t n = ll_load_idx(a.len, b, a.len64);
+  if (*row < 0 || *row >= a.r2t_rows || n <= 0) return 0;
+  return (int)std::min<int64_t>(n, a.max_len);
+}
+
+constexpr int kAnyMaxD = 512;
+
+// Any head dim and alignment: a wave per request and query head, 64 tokens at a
+// time: a lane's own token's score, then every lane's own elements of the sum.
+template <typename T, int CODE>
+__global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
+  __shared__ float sq[kAnyMaxD], sp[64];
+  __shared__ int32_t ss[64];
+  const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, lane = threadIdx.x, kvh = h / a.G;
+  int64_t row;
+  const int n = decode_len(a, b, &row);
+  const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
+  for (int d = lane; d < a.D; d += 64) sq[d] = ll_to_f32(q[d]);
+  __syncthreads();
+  const int32_t* table = a.r2t + (n > 0 ? row : 0) * a.r2t_s;
+  float m = -INFINITY, l = 0.f, acc[kAnyMaxD / 64] = {};
+  for (int t0 = 0; t0 < n; t0 += 64) {
+    const int t = t0 + lane;
+    const int32_t slot = t < n ? table[t] : -1;
+    const bool see = slot >= 0 && slot < a.nslots;
+    float x = -INFINITY;
+    if (see) {
+      const uint8_t* k = a.c[0] + slot * a.c_st[0] + kvh * a.c_sh[0];
+      float dot = 0.f;
+      for (int d = 0; d < a.D; ++d) dot = __builtin_fmaf(sq[d], CodeOf<CODE>::decode(k[d], 0), dot);
+      x = dot * a.s[0][(slot >> a.shift) * a.s_sb[0] + kvh * a.s_sh[0]] * a.scale_log2;
+    }
+    const float mt = fmaxf(m, ll_wave_max(x));
+    const float ms = mt == -INFINITY ? 0.f : mt;
+    const float alpha = exp2f(m - ms);
+    const float p = see ? exp2f(x - ms) : 0.f;
+    l = l * alpha + ll_wave_sum(p);
+    m = mt;
+    sp[lane] = see ? p * a.s[1][(slot >> a.shift) * a.s_sb[1] + kvh * a.s_sh[1]] : 0.f;
+    ss[lane] = see ? slot : -1;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kAnyMaxD / 64; ++j) {
+      const int d = lane + 64 * j;
+      if (d < a.D) {
+        float y = acc[j] * alpha;
+        for (int i = 0; i < min(64, n - t0); ++i)
+          if (ss[i] >= 0)
+            y = __builtin_fmaf(sp[i],
+                               CodeOf<CODE>::decode(a.c[1][ss[i] * a.c_st[1] + kvh * a.c_sh[1] + d], 0),
+                               y);
+        acc[j] = y;
+      }
+    }
+    __syncthreads();
+  }
+  T* o = (T*)a.out + b * a.o_sb + h * a.o_sh;
+#pragma unroll
+  for (int j = 0; j < kAnyMaxD / 64; ++j) {
+    const int d = lane + 64 * j;
+    if (d < a.D) o[d] = ll_from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
+  }
+}
+
+// log2 of a block size, -1 for others
+int block_shift(int64_t block) {
+  for (int s = 0; s <= 7; ++s)
+    if (block == (int64_t)1 << s) return s;
+  return -1;
+}
+
+// f with the code kind as a compile-time constant
+template <typename F> int dispatch_code(int code, F f) {
+  if (code == KV8_INT8) return f(std::integral_constant<int, KV8_INT8>());
+  return f(std::integral_constant<int, KV8_E4M3>());
+}
+
+#define KV8_CHECK_FORM(fn)                                                                     \
+  LL_CHECK_ARG(code == KV8_INT8 || code == KV8_E4M3, "%s: code kind %d", fn, code);           \
+  LL_CHECK_ARG(block_shift(block) >= 0, "%s: block %lld is no power of two up to 128", fn,    \
+               (long long)block);                                                             \
+  LL_CHECK_ARG(slots_n >= 0 && slots_n <= INT32_MAX, "%s: %lld slots", fn, (long long)slots_n); \
+  LL_CHECK_ARG(kv_heads > 0 && kv_heads <= 65535, "%s: %lld KV heads", fn, (long long)kv_heads)
+
+// whether n rows this far apart are rows of their own
+bool apart(int64_t stride, int64_t n) { return n < 2 || stride != 0; }
+
+bool aligned(int64_t bytes, std::initializer_list<int64_t> vs) {
+  for (int64_t v : vs)
+    if (v % bytes != 0) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" int ll_kv8_store(const void* k, int64_t k_stride_tok, int64_t k_stride_h, const void* v,
+                            int64_t v_stride_tok, int64_t v_stride_h, const int32_t* slots,
+                            int64_t ntok, int64_t kv_heads, int64_t head_dim, void* k_codes,
+                            int64_t kc_stride_tok, int64_t kc_stride_h, void* v_codes,
+                            int64_t vc_stride_tok, int64_t vc_stride_h, float* k_scale,
+                            int64_t ks_stride_block, int64_t ks_stride_h, float* v_scale,
+                            int64_t vs_stride_block, int64_t vs_stride_h, int64_t slots_n,
+                            int64_t block, int code, int dtype, hipStream_t stream) {
+  const char* fn = "ll_kv8_store";
+  if (ntok == 0) return LL_OK;
+  LL_CHECK_ARG(k && v && slots && k_codes && v_codes && k_scale && v_scale, "%s: null pointer", fn);
+  KV8_CHECK_FORM(fn);
+  LL_CHECK_ARG(ntok > 0 && ntok <= 1 << 24, "%s: %lld tokens (max 2^24)", fn, (long long)ntok);
+  LL_CHECK_ARG(head_dim > 0 && head_dim <= 1024, "%s: head_dim %lld unsupported", fn,
+               (long long)head_dim);
+  LL_CHECK_ARG(apart(kc_stride_tok, slots_n) && apart(kc_stride_h, kv_heads) &&
+                   apart(vc_stride_tok, slots_n) && apart(vc_stride_h, kv_heads) &&
+                   apart(ks_stride_block, (slots_n + block - 1) / block) &&
+                   apart(ks_stride_h, kv_heads) &&
+                   apart(vs_stride_block, (slots_n + block - 1) / block) &&
+                   apart(vs_stride_h, kv_heads),
+               "%s: rows or heads of the cache share an address (stride 0)", fn);
+  StoreArgs a;
+  a.x[0] = k; a.x_st[0] = k_stride_tok; a.x_sh[0] = k_stride_h;
+  a.x[1] = v; a.x_st[1] = v_stride_tok; a.x_sh[1] = v_stride_h;
+  a.slots = slots;
+  a.c[0] = (uint8_t*)k_codes; a.c_st[0] = kc_stride_tok; a.c_sh[0] = kc_stride_h;
+  a.c[1] = (uint8_t*)v_codes; a.c_st[1] = vc_stride_tok; a.c_sh[1] = vc_stride_h;
+  a.s[0] = k_scale; a.s_sb[0] = ks_stride_block; a.s_sh[0] = ks_stride_h;
+  a.s[1] = v_scale; a.s_sb[1] = vs_stride_block; a.s_sh[1] = vs_stride_h;
+  a.T = ntok; a.nslots = slots_n;
+  a.KVH = (int)kv_heads; a.D = (int)head_dim; a.shift = block_shift(block);
+  a.per = 1;
+  const int64_t waves = (ntok + a.per - 1) / a.per * 2 * kv_heads;
+  LL_CHECK_ARG(waves <= (int64_t)INT32_MAX / 64, "%s: %lld tokens of %lld heads", fn,
+               (long long)ntok, (long long)kv_heads);
+  const int es = dtype == LL_F32 ? 4 : 2;
+  const bool vec = head_dim % 8 == 0 &&
+                   aligned(16, {(int64_t)(uintptr_t)k, (int64_t)(uintptr_t)v, k_stride_tok * es,
+                                k_stride_h * es, v_stride_tok * es, v_stride_h * es}) &&
+                   aligned(8, {(int64_t)(uintptr_t)k_codes, (int64_t)(uintptr_t)v_codes,
+                               kc_stride_tok, kc_stride_h, vc_stride_tok, vc_stride_h});
+  const dim3 grid((unsigned)((waves + kStoreWaves - 1) / kStoreWaves));
+  return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    return dispatch_code(code, [&](auto C) -> int {
+      constexpr int CODE = decltype(C)::value;
+      if (vec)
+        hipLaunchKernelGGL((store_kernel<T, CODE, true>), grid, dim3(kStoreWaves * 64), 0, stream, a);
+      else
+        hipLaunchKernelGGL((store_kernel<T, CODE, false>), grid, dim3(kStoreWaves * 64), 0, stream, a);
+      LL_RETURN_LAUNCH();
+    });
+  });
+}
+
+extern "C" int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t kc_stride_h,
+                           const void* v_codes, int64_t vc_stride_tok, int64_t vc_stride_h,
+                           const float* k_scale, int64_t ks_stride_block, int64_t ks_stride_h,
+                           const float* v_scale, int64_t vs_stride_block, int64_t vs_stride_h,
+                           int64_t slots_n, int64_t block, int code, const int32_t* req_to_tokens,
+                           int64_t req_to_tokens_stride, int64_t req_rows, const void* b_req_idx,
+                           int req_idx_i64, const void* b_start_loc, int start_loc_i64,
+                           const void* b_seq_len, int seq_len_i64, int64_t batch,
+                           int64_t max_len_in_batch, void* k_out, int64_t ko_stride_tok,
+                           int64_t ko_stride_h, void* v_out, int64_t vo_stride_tok,
+                           int64_t vo_stride_h, int64_t out_rows, int64_t kv_heads,
+                           int64_t head_dim, int dtype, hipStream_t stream) {
+  const char* fn = "ll_kv8_load";
+  if (batch == 0 || max_len_in_batch == 0 || out_rows == 0) return LL_OK;
+  LL_CHECK_ARG(k_codes && v_codes && k_scale && v_scale && req_to_tokens && b_req_idx &&
+                   b_start_loc && b_seq_len && k_out && v_out,
+               "%s: null pointer", fn);
+  KV8_CHECK_FORM(fn);
+  LL_CHECK_ARG(batch > 0 && batch <= 65535, "%s: %lld requests (max 65535)", fn, (long long)batch);
+  LL_CHECK_ARG(max_len_in_batch > 0 && max_len_in_batch <= 1 << 30 && out_rows > 0,
+               "%s: max_len_in_batch %lld, %lld output rows", fn, (long long)max_len_in_batch,
+               (long long)out_rows);
+  LL_CHECK_ARG(head_dim > 0 && head_dim <= 1024, "%s: head_dim %lld unsupported", fn,
+               (long long)head_dim);
+  LL_CHECK_ARG(apart(ko_stride_tok, out_rows) && apart(ko_stride_h, kv_heads) &&
+                   apart(vo_stride_tok, out_rows) && apart(vo_stride_h, kv_heads),
+               "%s: rows or heads of the output share an address (stride 0)", fn);
+  LoadArgs a;
+  a.c[0] = (const uint8_t*)k_codes; a.c_st[0] = kc_stride_tok; a.c_sh[0] = kc_stride_h;
+  a.c[1] = (const uint8_t*)v_codes; a.c_st[1] = vc_stride_tok; a.c_sh[1] = vc_stride_h;
+  a.s[0] = k_scale; a.s_sb[0] = ks_stride_block; a.s_sh[0] = ks_stride_h;
+  a.s[1] = v_scale; a.s_sb[1] = vs_stride_block; a.s_sh[1] = vs_stride_h;
+  a.r2t = req_to_tokens; a.r2t_s = req_to_tokens_stride; a.r2t_rows = req_rows;
+  a.req = b_req_idx; a.req64 = req_idx_i64;
+  a.start = b_start_loc; a.start64 = start_loc_i64;
+  a.len = b_seq_len; a.len64 = seq_len_i64;
+  a.o[0] = k_out; a.o_st[0] = ko_stride_tok; a.o_sh[0] = ko_stride_h;
+  a.o[1] = v_out; a.o_st[1] = vo_stride_tok; a.o_sh[1] = vo_stride_h;
+  a.nslots = slots_n; a.orows = out_rows;
+  a.KVH = (int)kv_heads; a.D = (int)head_dim; a.shift = block_shift(block);
+  a.max_len = (int)max_len_in_batch;
+  const int es = dtype == LL_F32 ? 4 : 2;
+  const bool vec =
+      head_dim % 16 == 0 &&
+      aligned(16, {(int64_t)(uintptr_t)k_codes, (int64_t)(uintptr_t)v_codes, kc_stride_tok,
+                   kc_stride_h, vc_stride_tok, vc_stride_h, (int64_t)(uintptr_t)k_out,
+                   (int64_t)(uintptr_t)v_out, ko_stride_tok * es, ko_stride_h * es,
+                   vo_stride_tok * es, vo_stride_h * es});
+  a.pieces = vec ? a.D / 16 : a.D;
+  const int64_t items = max_len_in_batch * 2 * kv_heads * a.pieces;
+  const int64_t most = std::max<int64_t>(1, 8192 / batch);
+  const dim3 grid((unsigned)std::min<int64_t>((items + kLoadThreads - 1) / kLoadThreads, most),
+                  (unsigned)batch);
+  return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    return dispatch_code(code, [&](auto C) -> int {
+      constexpr int CODE = decltype(C)::value;
+      if (vec)
+        hipLaunchKernelGGL((load_kernel<T, CODE, true>), grid, dim3(kLoadThreads), 0, stream, a);
+      else
+        hipLaunchKernelGGL((load_kernel<T, CODE, false>), grid, dim3(kLoadThreads), 0, stream, a);
+      LL_RETURN_LAUNCH();
+    });
+  });
+}
+
+extern "C" int64_t ll_kv8_decode_attention_workspace_size(int64_t batch, int64_t q_heads,
+                                                          int64_t kv_heads, int64_t head_dim,
+                                                          int64_t max_len_in_batch) {
+  (void)batch; (void)q_heads; (void)kv_heads; (void)head_dim; (void)max_len_in_batch;
+  return 0;
+}
+
+extern "C" int ll_kv8_decode_attention(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_codes,
+    int64_t kc_stride_tok, int64_t kc_stride_h, const void* v_codes, int64_t vc_stride_tok,
+    int64_t vc_stride_h, const float* k_scale, int64_t ks_stride_block, int64_t ks_stride_h,
+    const float* v_scale, int64_t vs_stride_block, int64_t vs_stride_h, int64_t slots_n,
+    int64_t block, int code, const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+    int64_t req_rows, const void* b_req_idx, int req_idx_i64, const void* b_seq_len,
+    int seq_len_i64, void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t batch,
+    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_len_in_batch, float sm_scale,
+    int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const char* fn = "ll_kv8_decode_attention";
+  if (batch == 0) return LL_OK;
+  LL_CHECK_ARG(q && k_codes && v_codes && k_scale && v_scale && req_to_tokens && b_req_idx &&
+                   b_seq_len && out,
+               "%s: null pointer", fn);
+  KV8_CHECK_FORM(fn);
+  LL_CHECK_ARG(batch > 0 && batch <= 1 << 24 && q_heads > 0 && q_heads <= 65535 &&
+                   q_heads % kv_heads == 0,
+               "%s: %lld requests of %lld query and %lld KV heads", fn, (long long)batch,
+               (long long)q_heads, (long long)kv_heads);
+  LL_CHECK_ARG(head_dim > 0 && head_dim <= kAnyMaxD, "%s: head_dim %lld unsupported", fn,
+               (long long)head_dim);
+  LL_CHECK_ARG(max_len_in_batch >= 0 && max_len_in_batch <= 1 << 30,
+               "%s: max_len_in_batch %lld out of range", fn, (long long)max_len_in_batch);
+  LL_CHECK_ARG(sm_scale > 0.f && sm_scale < INFINITY, "%s: sm_scale %g must be positive", fn,
+               (double)sm_scale);
+  LL_CHECK_ARG(apart(out_stride_b, batch) && apart(out_stride_h, q_heads),
+               "%s: rows or heads of the output share an address (stride 0)", fn);
+  DecodeArgs8 a;
+  a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h;
+  a.c[0] = (const uint8_t*)k_codes; a.c_st[0] = kc_stride_tok; a.c_sh[0] = kc_stride_h;
+  a.c[1] = (const uint8_t*)v_codes; a.c_st[1] = vc_stride_tok; a.c_sh[1] = vc_stride_h;
+  a.s[0] = k_scale; a.s_sb[0] = ks_stride_block; a.s_sh[0] = ks_stride_h;
+  a.s[1] = v_scale; a.s_sb[1] = vs_stride_block; a.s_sh[1] = vs_stride_h;
+  a.r2t = req_to_tokens; a.r2t_s = req_to_tokens_stride; a.r2t_rows = req_rows;
+  a.req = b_req_idx; a.req64 = req_idx_i64;
+  a.len = b_seq_len; a.len64 = seq_len_i64;
+  a.out = out; a.o_sb = out_stride_b; a.o_sh = out_stride_h;
+  a.nslots = slots_n;
+  a.B = (int)batch; a.H = (int)q_heads; a.KVH = (int)kv_heads; a.G = (int)(q_heads / kv_heads);
+  a.D = (int)head_dim; a.shift = block_shift(block); a.max_len = (int)max_len_in_batch;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  (void)workspace; (void)workspace_bytes;
+  LL_CHECK_ARG(batch * q_heads <= INT32_MAX / 64, "%s: %lld requests of %lld heads", fn,
+               (long long)batch, (long long)q_heads);
+  return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+    return dispatch_code(code, [&](auto C) -> int {
+      constexpr int CODE = decltype(C)::value;
+      hipLaunchKernelGGL((decode_any_kernel<T, CODE>), dim3((unsigned)(batch * q_heads)), dim3(64),
+                         0, stream, a);
+      LL_RETURN_LAUNCH();
+    });
+  });
+}

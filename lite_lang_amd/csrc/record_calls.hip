@@ -124,3 +124,67 @@ extern "C" int64_t ll_call_build_slot_maps(const LLBuildSlotMapsCall* c) {
       ptr<int32_t>(c->positions), c->max_tokens, ptr<int32_t>(c->b_start_loc),
       ptr<int32_t>(c->last_rows), ptr<int32_t>(c->counts), ptr<ihipStream_t>(c->stream));
 }
+
+extern "C" int64_t ll_call_kv8_store(const LLKv8StoreCall* c) {
+  LL_CHECK_ARG(c, "ll_call_kv8_store: null record");
+  return ll_kv8_store(
+      ptr<const void>(c->k), c->k_stride_tok, c->k_stride_h, ptr<const void>(c->v),
+      c->v_stride_tok, c->v_stride_h, ptr<const int32_t>(c->slots), c->ntok, c->kv_heads,
+      c->head_dim, ptr<void>(c->k_codes), c->kc_stride_tok, c->kc_stride_h,
+      ptr<void>(c->v_codes), c->vc_stride_tok, c->vc_stride_h, ptr<float>(c->k_scale),
+      c->ks_stride_block, c->ks_stride_h, ptr<float>(c->v_scale), c->vs_stride_block,
+      c->vs_stride_h, c->slots_n, c->block, (int)c->code, (int)c->dtype,
+      ptr<ihipStream_t>(c->stream));
+}
+
+extern "C" int64_t ll_call_kv8_load(const LLKv8LoadCall* c) {
+  LL_CHECK_ARG(c, "ll_call_kv8_load: null record");
+  return ll_kv8_load(
+      ptr<const void>(c->k_codes), c->kc_stride_tok, c->kc_stride_h,
+      ptr<const void>(c->v_codes), c->vc_stride_tok, c->vc_stride_h, ptr<const float>(c->k_scale),
+      c->ks_stride_block, c->ks_stride_h, ptr<const float>(c->v_scale), c->vs_stride_block,
+      c->vs_stride_h, c->slots_n, c->block, (int)c->code, ptr<const int32_t>(c->req_to_tokens),
+      c->req_to_tokens_stride, c->req_rows, ptr<const void>(c->b_req_idx), (int)c->req_idx_i64,
+      ptr<const void>(c->b_start_loc), (int)c->start_loc_i64, ptr<const void>(c->b_seq_len),
+      (int)c->seq_len_i64, c->batch, c->max_len_in_batch, ptr<void>(c->k_out), c->ko_stride_tok,
+      c->ko_stride_h, ptr<void>(c->v_out), c->vo_stride_tok, c->vo_stride_h, c->out_rows,
+      c->kv_heads, c->head_dim, (int)c->dtype, ptr<ihipStream_t>(c->stream));
+}
+
+extern "C" int64_t ll_call_kv8_decode_attention(const LLKv8DecodeAttentionCall* c) {
+  LL_CHECK_ARG(c, "ll_call_kv8_decode_attention: null record");
+  const int64_t need = ll_kv8_decode_attention_workspace_size(c->batch, c->q_heads, c->kv_heads,
+                                                              c->head_dim, c->max_len_in_batch);
+  if (need > c->workspace_bytes) return need;
+  return ll_kv8_decode_attention(
+      ptr<const void>(c->q), c->q_stride_b, c->q_stride_h, ptr<const void>(c->k_codes),
+      c->kc_stride_tok, c->kc_stride_h, ptr<const void>(c->v_codes), c->vc_stride_tok,
+      c->vc_stride_h, ptr<const float>(c->k_scale), c->ks_stride_block, c->ks_stride_h,
+      ptr<const float>(c->v_scale), c->vs_stride_block, c->vs_stride_h, c->slots_n, c->block,
+      (int)c->code, ptr<const int32_t>(c->req_to_tokens), c->req_to_tokens_stride, c->req_rows,
+      ptr<const void>(c->b_req_idx), (int)c->req_idx_i64, ptr<const void>(c->b_seq_len),
+      (int)c->seq_len_i64, ptr<void>(c->out), c->out_stride_b, c->out_stride_h, c->batch,
+      c->q_heads, c->kv_heads, c->head_dim, c->max_len_in_batch, (float)c->sm_scale,
+      (int)c->dtype, ptr<void>(c->workspace), c->workspace_bytes, ptr<ihipStream_t>(c->stream));
+}
+
+extern "C" int64_t ll_call_linear_w4(const LLLinearW4Call* c) {
+  LL_CHECK_ARG(c, "ll_call_linear_w4: null record");
+  return ll_linear_w4(
+      ptr<const void>(c->x), c->ldx, ptr<const void>(c->packed), (int)c->has_zero, c->group,
+      ptr<const void>(c->bias), ptr<void>(c->y), c->ldy, c->M, c->N, c->K, (int)c->dtype,
+      ptr<ihipStream_t>(c->stream));
+}
+
+extern "C" int64_t ll_call_adjust_logits(const LLAdjustLogitsCall* c) {
+  LL_CHECK_ARG(c, "ll_call_adjust_logits: null record");
+  return ll_adjust_logits(
+      ptr<const void>(c->logits), c->ld_logits, ptr<void>(c->out), c->ld_out, c->batch,
+      c->vocab, ptr<const int32_t>(c->tokens), c->tokens_stride, c->tokens_rows, c->tokens_cols,
+      ptr<const void>(c->b_req_idx), (int)c->req_idx_i64, ptr<const void>(c->b_prompt_len),
+      (int)c->prompt_len_i64, ptr<const void>(c->b_seq_len), (int)c->seq_len_i64,
+      ptr<const float>(c->repetition), ptr<const float>(c->frequency), ptr<const float>(c->presence),
+      ptr<const int32_t>(c->bias_ids), c->bias_ids_stride, ptr<const float>(c->bias_values),
+      c->bias_values_stride, c->n_bias, ptr<const uint32_t>(c->mask), c->mask_stride,
+      (int)c->dtype, ptr<ihipStream_t>(c->stream));
+}

@@ -341,6 +341,133 @@ def _window_decode_bytes(*shape):
     return _L.ll_window_decode_attention_workspace_size(*shape)
 
 
+# ------------------------------------------------------------------ 8-bit KV cache
+_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _kv8_cache(cache_k, cache_v, k_scale, v_scale, block):
+    """Checks of an 8-bit cache; (record fields of its tensors, (slots, block,
+    code kind), its device, (KV heads, head dim))."""
+    kshape, sshape = cache_k.shape, k_scale.shape
+    P, KVH, D = kshape
+    assert cache_v.shape == kshape and v_scale.shape == sshape and sshape[1] == KVH
+    assert cache_v.dtype == cache_k.dtype
+    assert k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32
+    try:
+        code = _CODES[cache_k.dtype]
+    except KeyError:
+        raise TypeError("an 8-bit cache is int8 or float8_e4m3fn, "
+                        f"got {cache_k.dtype}") from None
+    ks, vs, ss, ws = cache_k.stride(), cache_v.stride(), k_scale.stride(), v_scale.stride()
+    assert ks[2] == 1 and vs[2] == 1
+    if block < 1 or sshape[0] * block < P:
+        raise ValueError(f"{sshape[0]} scales of {block} slots do not cover {P} slots")
+    dev = cache_k.get_device()
+    for t in (cache_v, k_scale, v_scale):
+        if t.get_device() != dev:
+            _here(dev, t.get_device())
+    return ((cache_k.data_ptr(), ks[0], ks[1], cache_v.data_ptr(), vs[0], vs[1],
+             k_scale.data_ptr(), ss[0], ss[1], v_scale.data_ptr(), ws[0], ws[1]),
+            (P, block, code), dev, (KVH, D))
+
+
+def kv8_store(k, v, slots, cache_k, cache_v, k_scale, v_scale, block):
+    """Quantise k, v [T, KVH, D] into cache_k, cache_v [slots, KVH, D] (int8 or
+    float8_e4m3fn) at slots [T] int32, with an fp32 scale per block of `block`
+    slots (a power of two up to 128) and head in k_scale, v_scale [blocks, KVH].
+
+    The tokens of one block stand next to each other, in ascending slots. Those
+    that start at a block's first slot begin it anew; others continue it: the
+    scale grows where they need it and the codes in front of them are rounded
+    again. A slot outside the cache (-1) is a padded token. An infinity or NaN
+    makes its block and head NaN."""
+    cache, (P, block, code), dev, (KVH, D) = _kv8_cache(cache_k, cache_v, k_scale, v_scale, block)
+    shape, dt = k.shape, k.dtype
+    T = shape[0]
+    assert shape == (T, KVH, D) and v.shape == shape and v.dtype == dt
+    xs, ys = k.stride(), v.stride()
+    assert xs[2] == 1 and ys[2] == 1
+    assert slots.dtype == torch.int32 and slots.shape == (T,) and slots.is_contiguous()
+    stream = _here(dev, k.get_device(), v.get_device(), slots.get_device())
+    rc = _L.ll_call_kv8_store(_lib.KV8_STORE_CALL.pack(
+        k.data_ptr(), xs[0], xs[1], v.data_ptr(), ys[0], ys[1], slots.data_ptr(), T, KVH, D,
+        *cache, P, block, code, _code(dt), stream))
+    if rc:
+        _lib.check(rc, "ll_kv8_store")
+
+
+def kv8_load(cache_k, cache_v, k_scale, v_scale, block, req_to_tokens, b_req_idx, b_start_loc,
+             b_seq_len, max_len_in_batch, k_out, v_out):
+    """The contexts of a batch out of an 8-bit cache: k_out, v_out[b_start_loc[b]
+    + n] = the value of the token req_to_tokens[b_req_idx[b], n], n < b_seq_len[b].
+    What prefill_attention attends over behind cached prefixes, with a slot table
+    of b_start_loc[b] + n. Rows of no request are left as they were."""
+    cache, (P, block, code), dev, (KVH, D) = _kv8_cache(cache_k, cache_v, k_scale, v_scale, block)
+    oshape, dt = k_out.shape, k_out.dtype
+    R = oshape[0]
+    assert oshape == (R, KVH, D) and v_out.shape == oshape and v_out.dtype == dt
+    xs, ys = k_out.stride(), v_out.stride()
+    assert xs[2] == 1 and ys[2] == 1
+    bs = b_seq_len.shape
+    assert len(bs) == 1 and b_req_idx.shape == bs and b_start_loc.shape == bs
+    assert b_req_idx.is_contiguous() and b_start_loc.is_contiguous() and b_seq_len.is_contiguous()
+    (rows, cols), ts = req_to_tokens.shape, req_to_tokens.stride()
+    assert req_to_tokens.dtype == torch.int32 and ts[1] == 1
+    assert 0 <= max_len_in_batch <= cols
+    stream = _here(dev, req_to_tokens.get_device(), b_req_idx.get_device(),
+                   b_start_loc.get_device(), b_seq_len.get_device(), k_out.get_device(),
+                   v_out.get_device())
+    rc = _L.ll_call_kv8_load(_lib.KV8_LOAD_CALL.pack(
+        *cache, P, block, code, req_to_tokens.data_ptr(), ts[0], rows, b_req_idx.data_ptr(),
+        _idx(b_req_idx, "b_req_idx"), b_start_loc.data_ptr(), _idx(b_start_loc, "b_start_loc"),
+        b_seq_len.data_ptr(), _idx(b_seq_len, "b_seq_len"), bs[0], max_len_in_batch,
+        k_out.data_ptr(), xs[0], xs[1], v_out.data_ptr(), ys[0], ys[1], R, KVH, D, _code(dt),
+        stream))
+    if rc:
+        _lib.check(rc, "ll_kv8_load")
+
+
+def kv8_decode_attention(q, req_to_tokens, b_req_idx, b_seq_len, max_len_in_batch, cache_k,
+                         cache_v, k_scale, v_scale, block, out, sm_scale=None):
+    """decode_attention over an 8-bit cache (kv8_store). Entries of length 0 give
+    zero rows."""
+    cache, (P, block, code), dev, (KVH, D) = _kv8_cache(cache_k, cache_v, k_scale, v_scale, block)
+    shape, dt = q.shape, q.dtype
+    B, H, _ = shape
+    assert shape[2] == D and H % KVH == 0 and out.shape == shape and out.dtype == dt
+    qs, os_ = q.stride(), out.stride()
+    assert qs[2] == 1 and os_[2] == 1
+    assert b_req_idx.shape == (B,) and b_seq_len.shape == (B,)
+    assert b_req_idx.is_contiguous() and b_seq_len.is_contiguous()
+    (rows, cols), ts = req_to_tokens.shape, req_to_tokens.stride()
+    assert req_to_tokens.dtype == torch.int32 and ts[1] == 1
+    assert 0 <= max_len_in_batch <= cols
+    stream = _here(dev, q.get_device(), req_to_tokens.get_device(), b_req_idx.get_device(),
+                   b_seq_len.get_device(), out.get_device())
+    # (under capture a buffer of the call's own, as in window_decode_attention)
+    need = _kv8_decode_bytes(B, H, KVH, D, max_len_in_batch)
+    ws = None
+    if need > 0:
+        if _capturing():
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        else:
+            ws = workspace(q.device, "kv8_decode", need)
+    rc = _L.ll_call_kv8_decode_attention(_lib.KV8_DECODE_ATTENTION_CALL.pack(
+        q.data_ptr(), qs[0], qs[1], *cache, P, block, code, req_to_tokens.data_ptr(), ts[0], rows,
+        b_req_idx.data_ptr(), _idx(b_req_idx, "b_req_idx"), b_seq_len.data_ptr(),
+        _idx(b_seq_len, "b_seq_len"), out.data_ptr(), os_[0], os_[1], B, H, KVH, D,
+        max_len_in_batch, 1.0 / (D ** 0.5) if sm_scale is None else sm_scale, _code(dt),
+        0 if ws is None else ws.data_ptr(), need, stream))
+    if rc:
+        _lib.check(rc, "ll_kv8_decode_attention")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv8_decode_bytes(*shape):
+    return _L.ll_kv8_decode_attention_workspace_size(*shape)
+
+
 # ------------------------------------------------------------------ elementwise
 def rmsnorm(x, gamma, eps, residual=None, out=None):
     """out = rmsnorm(x [+ residual]) * gamma; with residual, x is updated in place."""
@@ -774,6 +901,80 @@ def gemm_i8_gate_up_silu_tiled(xq, s_tok, wq_il, s_ch, out_dtype=torch.bfloat16,
                                           M, I, K, dtype_code(out), out.data_ptr(), out.stride(0),
                                           _stream(xq))
     _lib.check(rc, "ll_gemm_i8_gate_up_silu_tiled")
+    return out
+
+
+def adjust_logits(logits, tokens=None, b_req_idx=None, b_prompt_len=None, b_seq_len=None,
+                  repetition=None, frequency=None, presence=None, bias_ids=None, bias_values=None,
+                  mask=None, out=None):
+    """The logits [B, V] that the next tokens are taken from, into out (None: a
+    new tensor; logits: in place). Request b's tokens are row b_req_idx[b] of
+    `tokens` [rows, columns] int32: its prompt [0, b_prompt_len[b]) and its answer
+    up to b_seq_len[b]. In this order, in fp32:
+
+    * repetition [B]: a token of either is divided by it where its logit is
+      positive, multiplied else;
+    * frequency [B]: times the token's count in the answer, subtracted;
+    * presence [B]: subtracted from the answer's tokens;
+    * bias_values [B, n] fp32, added to the tokens bias_ids [B, n] int32 (a token
+      with several gets their sum; ids outside the vocabulary, such as -1, are
+      unused);
+    * mask [B, at least V / 32] int32: tokens whose bit v % 32 of word v / 32 is 0
+      become -inf (a row of zeros leaves none; argmax then gives token 0).
+
+    repetition, frequency and presence are fp32."""
+    shape, dt = logits.shape, logits.dtype
+    B, V = shape
+    xs = logits.stride()
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=logits.device)
+    os_ = out.stride()
+    assert xs[1] == 1 and out.shape == shape and out.dtype == dt and os_[1] == 1
+    dev = logits.get_device()
+    devs = [out.get_device()]
+    f32, i32 = torch.float32, torch.int32
+    tok, pen = [0] * 10, [0, 0, 0]
+    if tokens is not None:
+        (rows, cols), ts = tokens.shape, tokens.stride()
+        assert tokens.dtype == i32 and ts[1] == 1
+        tok = [tokens.data_ptr(), ts[0], rows, cols]
+        devs.append(tokens.get_device())
+        for t, name in ((b_req_idx, "b_req_idx"), (b_prompt_len, "b_prompt_len"),
+                        (b_seq_len, "b_seq_len")):
+            assert t is not None and t.shape == (B,) and t.is_contiguous()
+            tok += [t.data_ptr(), _idx(t, name)]
+            devs.append(t.get_device())
+        for i, t in enumerate((repetition, frequency, presence)):
+            if t is not None:
+                assert t.shape == (B,) and t.dtype == f32 and t.is_contiguous()
+                pen[i] = t.data_ptr()
+                devs.append(t.get_device())
+    elif not (repetition is None and frequency is None and presence is None):
+        raise ValueError("repetition, frequency and presence penalties need the tokens")
+    bias = [0] * 5
+    if bias_ids is not None:
+        bshape = bias_ids.shape
+        assert bshape[0] == B and len(bshape) == 2 and bias_values.shape == bshape
+        assert bias_ids.dtype == i32 and bias_values.dtype == f32
+        s0, s1 = bias_ids.stride(), bias_values.stride()
+        assert bshape[1] < 2 or (s0[1] == 1 and s1[1] == 1)
+        bias = [bias_ids.data_ptr(), s0[0], bias_values.data_ptr(), s1[0], bshape[1]]
+        devs += [bias_ids.get_device(), bias_values.get_device()]
+    elif bias_values is not None:
+        raise ValueError("bias_values need bias_ids")
+    mk = (0, 0)
+    if mask is not None:
+        mshape, ms = mask.shape, mask.stride()
+        assert mshape[0] == B and len(mshape) == 2 and mshape[1] * 32 >= V
+        assert mask.dtype == i32 and (mshape[1] < 2 or ms[1] == 1)
+        mk = (mask.data_ptr(), ms[0])
+        devs.append(mask.get_device())
+    stream = _here(dev, *devs)
+    rc = _L.ll_call_adjust_logits(_lib.ADJUST_LOGITS_CALL.pack(
+        logits.data_ptr(), xs[0], out.data_ptr(), os_[0], B, V, *tok, *pen, *bias, *mk, _code(dt),
+        stream))
+    if rc:
+        _lib.check(rc, "ll_adjust_logits")
     return out
 
 
@@ -1467,3 +1668,61 @@ def linear_w8a8(x, qw: QuantWeight, bias=None):
     if bias is not None:
         y = y + bias.float()
     return y.to(x.dtype)
+
+
+# ------------------------------------------------------------------ 4-bit weights
+class W4Weight:
+    """A [N, K] weight of 4 bits, laid out for linear_w4: codes [N, K / 2] uint8
+    (input 2 i in the low, 2 i + 1 in the high half of byte i), scale [N, K /
+    group] bf16 or fp16 and optionally zero [N, K / group] uint8 (0 .. 15; without,
+    8 throughout): w[n, k] = (c[n, k] - zero) scale. The group (32, 64 or 128)
+    follows from the shapes. The inputs are copied."""
+
+    def __init__(self, codes, scale, zero=None):
+        N, half = codes.shape
+        K = 2 * half
+        assert codes.dtype == torch.uint8 and scale.shape[0] == N and scale.dim() == 2
+        assert scale.dtype in (torch.bfloat16, torch.float16)
+        groups = scale.shape[1]
+        group = K // groups if groups and K % groups == 0 else 0
+        if group not in (32, 64, 128):
+            raise ValueError(f"{groups} scales for {K} inputs: groups are of 32, 64 or 128")
+        if zero is not None:
+            assert zero.shape == scale.shape and zero.dtype == torch.uint8
+            zero = zero.contiguous()
+        codes, scale = codes.contiguous(), scale.contiguous()
+        stream = _here(codes.get_device(), scale.get_device(),
+                       codes.get_device() if zero is None else zero.get_device())
+        nbytes = _L.ll_w4_packed_bytes(N, K, group, int(zero is not None))
+        if nbytes <= 0:
+            raise _lib.LiteLangError(f"ll_w4_pack: no layout for N={N} K={K} group={group}")
+        self.shape, self.group, self.has_zero = (N, K), group, int(zero is not None)
+        self.dtype, self.device = scale.dtype, codes.device
+        self.data = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        rc = _L.ll_w4_pack(codes.data_ptr(), half, scale.data_ptr(), groups,
+                           0 if zero is None else zero.data_ptr(), groups, N, K, group,
+                           self.data.data_ptr(), nbytes, stream)
+        _lib.check(rc, "ll_w4_pack")
+
+
+def linear_w4(x, w: W4Weight, bias=None, out=None):
+    """x [M, K] @ w^T (+ bias) with fp32 sums and one rounding, for any M."""
+    M, K = x.shape
+    N, wk = w.shape
+    dt, xs = x.dtype, x.stride()
+    assert wk == K and dt == w.dtype and xs[1] == 1
+    if out is None:
+        out = torch.empty((M, N), dtype=dt, device=x.device)
+    os_ = out.stride()
+    assert out.shape == (M, N) and out.dtype == dt and os_[1] == 1
+    dev, b_ptr, b_dev = x.get_device(), 0, x.get_device()
+    if bias is not None:
+        assert bias.shape == (N,) and bias.dtype == dt and bias.is_contiguous()
+        b_ptr, b_dev = bias.data_ptr(), bias.get_device()
+    stream = _here(dev, w.data.get_device(), b_dev, out.get_device())
+    rc = _L.ll_call_linear_w4(_lib.LINEAR_W4_CALL.pack(
+        x.data_ptr(), xs[0], w.data.data_ptr(), w.has_zero, w.group, b_ptr, out.data_ptr(), os_[0],
+        M, N, K, _code(dt), stream))
+    if rc:
+        _lib.check(rc, "ll_linear_w4")
+    return out

@@ -1,0 +1,707 @@
+"""GPU parity of the 8-bit cache, 4-bit products and logit controls against
+oracle/low_bits.py.
+
+Codes and scales are compared exactly, other floating outputs are held to the
+oracle's bounds. Memory that a call must not read holds NaN (scales, floating
+codes), memory that it must not write holds a pattern that is compared.
+"""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import low_bits as O
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+INT8, E4M3 = O.INT8, O.E4M3
+
+
+def _ops():
+    from lite_lang_amd import ops
+    return ops
+
+
+def _i32(v, dev="cuda", dtype=torch.int32):
+    return torch.tensor(v, dtype=dtype, device=dev)
+
+
+def _inside(got, want, bound, what=""):
+    """got within bound of want, element by element; NaN and infinities where want has them."""
+    got = got.detach().cpu().to(torch.float64)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN"
+    fin = torch.isfinite(want)
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]), f"{what}: infinities"
+    excess = (got - want).abs()[fin] - bound[fin]
+    if excess.numel():
+        worst = float(((got - want).abs()[fin] / bound[fin].clamp_min(1e-300)).max())
+        print(f"  {what}: worst {worst:.3f} of the bound", flush=True)
+        assert float(excess.max()) <= 0.0, f"{what}: {worst:.3f} of the bound"
+
+
+class Cache:
+    """An 8-bit cache on the device beside the oracle's: K and V heads of one
+    pool (or with rows of other strides), unused codes and scales NaN."""
+
+    def __init__(self, slots, kvh, d, code, block, pad=0, extra=3):
+        self.P, self.kvh, self.d, self.code, self.block = slots, kvh, d, code, block
+        blocks = -(-slots // block)
+        self.raw = torch.full((slots, 2 * kvh, d + pad), 0x7f, dtype=torch.uint8, device="cuda")
+        pool = self.raw.view(code)[..., :d]
+        self.k, self.v = pool[:, :kvh], pool[:, kvh:]
+        self.scale = torch.full((blocks, 2 * kvh + extra), float("nan"), device="cuda")
+        self.ks, self.vs = self.scale[:, :kvh], self.scale[:, kvh:2 * kvh]
+        self.codes = pool.cpu().float().to(torch.float64)
+        self.want = self.scale[:, :2 * kvh].cpu().to(torch.float64)
+
+    @property
+    def args(self):
+        return self.k, self.v, self.ks, self.vs, self.block
+
+    def store(self, k, v, slots):
+        _ops().kv8_store(k.cuda() if not k.is_cuda else k, v.cuda() if not v.is_cuda else v,
+                         _i32(slots), *self.args)
+        O.kv8_store(torch.cat([k.cpu(), v.cpu()], 1), slots, self.codes, self.want, self.block,
+                    self.code)
+
+    def check(self):
+        pool = self.raw.view(self.code)
+        got = pool[..., :self.d].cpu().float().to(torch.float64)
+        assert torch.equal(torch.nan_to_num(self.scale[:, :2 * self.kvh].cpu().double(), nan=-1.0),
+                           torch.nan_to_num(self.want, nan=-1.0)), "scales"
+        assert torch.equal(torch.nan_to_num(got, nan=999.0),
+                           torch.nan_to_num(self.codes, nan=999.0)), "codes"
+        assert bool((self.raw[..., self.d:] == 0x7f).all()), "beside the rows"
+        assert bool(torch.isnan(self.scale[:, 2 * self.kvh:]).all()), "beside the scales"
+
+    def values(self):
+        y = O.kv8_values(self.codes, self.want, self.block)
+        return y[:, :self.kvh], y[:, self.kvh:]
+
+
+FORMS = [(2, 128, BF16, INT8, 16), (4, 128, F16, E4M3, 64), (8, 64, BF16, E4M3, 1),
+         (1, 96, F32, INT8, 4), (3, 80, BF16, INT8, 32), (1, 10, F16, E4M3, 2),
+         (2, 256, F32, E4M3, 8), (1, 128, BF16, INT8, 1), (5, 64, F16, INT8, 128),
+         (2, 520, BF16, INT8, 16)]
+
+
+def _pages(g, lens, block, spare=2):
+    """(slot table rows, pages in no order) of requests with whole pages of a block."""
+    need = [-(-n // block) for n in lens]
+    perm = torch.randperm(sum(need) + spare, generator=g)
+    table = torch.full((len(lens) + 1, max(need + [1]) * block), -1, dtype=torch.int32)
+    at = 0
+    for i, m in enumerate(need):
+        ids = perm[at:at + m]
+        table[i, :m * block] = (ids[:, None] * block + torch.arange(block)).flatten().int()
+        at += m
+    return table, (sum(need) + spare) * block
+
+
+@pytest.mark.parametrize("kvh,d,dtype,code,block", FORMS)
+def test_kv8_store(cuda, kvh, d, dtype, code, block):
+    """Prompts, then single tokens and chunks that continue blocks, with ever
+    larger values (scales grow, codes are rounded again) and smaller ones."""
+    print(f"case: store {kvh}x{d} {dtype} {code} block {block}", flush=True)
+    g = torch.Generator().manual_seed(d + block)
+    final = [3 * block + 5, 40, block, 1, 70]
+    table, slots = _pages(g, final, block)
+    c = Cache(slots, kvh, d, code, block)
+    done = [0] * len(final)
+    for step in range(9):
+        new = [min(n - a, (n * 2 // 3 if step == 0 else 1 if step < 5 else 7) if i != 4 or step else 0)
+               for i, (n, a) in enumerate(zip(final, done))]
+        sl = [int(s) for i, m in enumerate(new) for s in table[i, done[i]:done[i] + m]]
+        sl = sl[:3] + [-1] + sl[3:] + [slots, -5, 2 ** 31 - 1]  # padded tokens among them
+        mag = (1.0, 0.5, 2.0, 2.1, 0.01, 8.0, 1.0, 30.0, 1.0)[step]
+        k = (torch.randn(len(sl), kvh, d, generator=g) * mag).to(dtype)
+        v = (torch.randn(len(sl), kvh, d, generator=g) * mag * 3).to(dtype)
+        c.store(k, v, sl)
+        c.check()
+        done = [a + m for a, m in zip(done, new)]
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_kv8_store_ties_and_borders(cuda, code, dtype):
+    """Quotients half-way between two codes, and fp32 values one step beside
+    those, for scales of 1 and of 24 bits."""
+    gr = O.grid(code)
+    mids = (gr[1:] + gr[:-1]) / 2
+    for scale in ((1.0, 0.25) if dtype == BF16 else (1.0, 1.7182818, 0.0333333, 3.1e-7, 5.5e20)):
+        s = float(np.float32(O.top(code) * np.float32(scale)) / np.float32(O.top(code)))
+        x = torch.cat([mids, gr[:-1]]) * s
+        x = torch.cat([x, torch.nextafter(x.float(), torch.tensor(3e38)).double(),
+                       torch.nextafter(x.float(), torch.tensor(0.0)).double(), -x])
+        x = x[x.abs() < O.top(code) * scale]
+        d = 128
+        x = torch.nn.functional.pad(x, (0, -len(x) % (d - 1))).view(-1, 1, d - 1)
+        x = torch.cat([x, torch.full((x.shape[0], 1, 1), O.top(code) * scale)], -1).to(dtype)
+        print(f"case: ties {code} {dtype} scale {scale} x {tuple(x.shape)}", flush=True)
+        c = Cache(x.shape[0], 1, d, code, 1)
+        c.store(x, -x, list(range(x.shape[0])))
+        c.check()
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_kv8_store_extremes(cuda, code):
+    """Zeros, the smallest and the largest numbers, infinities and NaN: the scale's
+    floor, a NaN scale for that head alone, and a block that begins anew."""
+    d, block = 64, 4
+    rows = {"zero": 0.0, "tiny": 1e-44, "small": 1e-30, "huge": 3.4e38, "inf": float("inf"),
+            "-inf": -float("inf"), "nan": float("nan")}
+    for name, val in rows.items():
+        print(f"case: extremes {code} {name}", flush=True)
+        c = Cache(8 * block, 2, d, code, block)
+        x = torch.randn(3, 2, d, generator=torch.Generator().manual_seed(1))
+        x[1, 1] = 0.0
+        x[1, 1, 3] = val
+        x[0, 1] = x[2, 1] = 0.0
+        c.store(x, torch.randn(3, 2, d), [4, 5, 6])
+        c.check()
+        c.store(torch.ones(1, 2, d), torch.ones(1, 2, d), [7])  # continues the block
+        c.check()
+        bad = not np.isfinite(val)
+        assert bool(torch.isnan(c.ks[1]).any()) == bad
+        c.store(torch.ones(2, 2, d), torch.ones(2, 2, d), [4, 5])  # begins it anew
+        c.check()
+        assert bool(torch.isfinite(c.ks[1]).all())
+
+
+def test_kv8_store_strides(cuda):
+    """Heads inside a projection's rows, rows of odd strides, pools whose rows are
+    not aligned, K and V in pools of their own."""
+    g = torch.Generator().manual_seed(3)
+    for d, pad, width in ((64, 3, 0), (128, 8, 5), (96, 1, 8), (64, 0, 3)):
+        print(f"case: strides {d} {pad} {width}", flush=True)
+        kvh, T, block = 2, 21, 8
+        c = Cache(48, kvh, d, INT8, block, pad=pad)
+        row = torch.randn(T, (4 + 2 * kvh) * d + width, generator=g).to(BF16).cuda()
+        k = row[:, 4 * d:(4 + kvh) * d].unflatten(1, (kvh, d))
+        v = row[:, (4 + kvh) * d:(4 + 2 * kvh) * d].unflatten(1, (kvh, d))
+        c.store(k, v, list(range(16, 16 + T)))
+        c.check()
+        one = k[:, :1].expand(T, kvh, d)  # one head for all
+        c.store(one, v, list(range(16, 16 + T)))
+        c.check()
+
+
+def test_kv8_store_of_a_long_prompt(cuda):
+    """More runs than a wave takes, runs across the waves' borders."""
+    g = torch.Generator().manual_seed(8)
+    for block in (1, 16, 64):
+        final = [1500, 777, 1024, 33]
+        table, slots = _pages(g, final, block)
+        c = Cache(slots, 2, 64, INT8, block)
+        for lo, hi in ((0.0, 0.37), (0.37, 1.0)):
+            sl = [int(s) for i, n in enumerate(final) for s in table[i, int(n * lo):int(n * hi)]]
+            x = torch.randn(len(sl), 2, 64, generator=g).to(BF16)
+            c.store(x, x.flip(0) * 2, sl)
+            c.check()
+
+
+def test_kv8_far_slots(cuda):
+    """Slots whose rows lie beyond 2^31 and 2^32 bytes."""
+    kvh, d, block = 8, 128, 16
+    P = ((1 << 32) // (2 * kvh * d) + 4096) // block * block
+    pool = torch.empty(P, 2 * kvh, d, dtype=INT8, device="cuda")
+    scale = torch.empty(P // block, 2 * kvh, device="cuda")
+    cache = (pool[:, :kvh], pool[:, kvh:], scale[:, :kvh], scale[:, kvh:], block)
+    g = torch.Generator().manual_seed(2)
+    n = 40
+    for first in ((1 << 31) // (2 * kvh * d) - 32, P - 48):
+        print(f"case: far slots from {first}", flush=True)
+        sl = torch.arange(first, first + n, dtype=torch.int32)
+        x = torch.randn(n, kvh, d, generator=g).to(BF16)
+        small = Cache(n, kvh, d, INT8, block)
+        small.store(x, x * 2, list(range(n)))
+        small.check()
+        _ops().kv8_store(x.cuda(), (x * 2).cuda(), sl.cuda(), *cache)
+        blocks = slice(first // block, first // block + 3)
+        assert torch.equal(pool[first:first + n], small.raw.view(INT8))
+        assert torch.equal(scale[blocks], small.scale[:, :2 * kvh])
+        q = torch.randn(1, 16, d, generator=g).to(BF16).cuda()
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        req, ln, st = _i32([0]), _i32([n]), _i32([0])
+        ko = [torch.empty(n, kvh, d, dtype=BF16, device="cuda") for _ in range(4)]
+        for cc, t, o, kk in ((cache, sl.view(1, n).cuda(), a, ko[:2]),
+                             (small.args, torch.arange(n, dtype=torch.int32).view(1, n).cuda(), b,
+                              ko[2:])):
+            _ops().kv8_decode_attention(q, t, req, ln, n, *cc, o)
+            _ops().kv8_load(*cc, t, req, st, ln, n, *kk)
+        assert torch.equal(a, b) and torch.equal(ko[0], ko[2]) and torch.equal(ko[1], ko[3])
+
+
+# ---------------------------------------------------------------- reading back
+def _filled(g, lens, kvh, d, code, block, dtype, pad=0, mag=1.0):
+    """A cache that holds contexts of these lengths, its table (garbage behind
+    them) and the request rows."""
+    table, slots = _pages(g, lens, block)
+    c = Cache(slots, kvh, d, code, block, pad=pad)
+    sl = [int(s) for i, n in enumerate(lens) for s in table[i, :n]]
+    if sl:
+        x = (torch.randn(len(sl), kvh, d, generator=g) * mag).to(dtype)
+        y = torch.randn(len(sl), kvh, d, generator=g).to(dtype)
+        c.store(x, y, sl)
+    order = torch.randperm(len(lens) + 1, generator=g)
+    rids = torch.argsort(order)[:len(lens)].tolist()
+    return c, table[order], rids
+
+
+@pytest.mark.parametrize("kvh,d,dtype,code,block", FORMS)
+def test_kv8_load(cuda, kvh, d, dtype, code, block):
+    g = torch.Generator().manual_seed(d)
+    lens = [37, 0, 1, 2 * block + 3, 90]
+    c, table, rids = _filled(g, lens, kvh, d, code, block, dtype)
+    table[rids[4], 5], table[rids[4], 7] = -1, c.P  # no tokens: zeros
+    start = [3, 40, 41, 45, 50 + 2 * block]
+    rows = start[4] + 90 - 4  # the last request's last rows do not fit
+    for idx in (torch.int32, torch.int64):
+        print(f"case: load {kvh}x{d} {dtype} {code} block {block} {idx}", flush=True)
+        out = [torch.full((rows, kvh, d), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+        _ops().kv8_load(*c.args, table.cuda(), _i32(rids, dtype=idx), _i32(start, dtype=idx),
+                        _i32(lens, dtype=idx), max(lens), *out)
+        for got, val in zip(out, c.values()):
+            want = torch.full((rows, kvh, d), 7.0, dtype=torch.float64)
+            for r, s, n in zip(rids, start, lens):
+                for i in range(min(n, rows - s)):
+                    slot = int(table[r, i])
+                    want[s + i] = val[slot] if 0 <= slot < c.P else 0.0
+            _inside(got, want, O.bound_value(want, dtype), "values")
+
+
+def test_kv8_load_bounds_and_strides(cuda):
+    """Lengths beyond the bound, requests outside the table, outputs of other
+    strides, rows of pools that are not aligned."""
+    g = torch.Generator().manual_seed(4)
+    for d, pad in ((64, 0), (64, 3), (96, 8)):
+        print(f"case: load strides {d} {pad}", flush=True)
+        c, table, rids = _filled(g, [30, 20, 9], 2, d, INT8, 8, BF16, pad=pad)
+        wide = torch.full((70, 5, d + pad), 7.0, dtype=BF16, device="cuda")
+        k, v = wide[:, 1:3, :d], wide[:, 3:5, :d]
+        req = rids[:1] + [-1] + rids[1:] + [table.shape[0]]
+        _ops().kv8_load(*c.args, table.cuda(), _i32(req), _i32([0, 12, 15, 40, 50]),
+                        _i32([30, 4, 20, -3, 9]), 12, k, v)
+        for got, val in zip((k, v), c.values()):
+            want = torch.full((70, 2, d), 7.0, dtype=torch.float64)
+            want[:12] = val[table[rids[0], :12].long()]
+            want[15:27] = val[table[rids[1], :12].long()]
+            _inside(got, want, O.bound_value(want, BF16), "values")
+        assert bool((wide[:, 0] == 7.0).all()) and bool((wide[..., d:] == 7.0).all())
+
+
+# ---------------------------------------------------------------- attention
+ATT = [(16, 2, 128, BF16, INT8, 16), (12, 2, 128, BF16, E4M3, 64), (28, 4, 128, F16, INT8, 1),
+       (32, 8, 64, F16, E4M3, 16), (8, 2, 64, BF16, INT8, 32), (4, 4, 128, F32, INT8, 16),
+       (40, 2, 64, BF16, INT8, 8), (17, 1, 128, F32, E4M3, 2), (4, 1, 256, BF16, INT8, 16),
+       (6, 3, 96, BF16, INT8, 4), (2, 1, 10, F16, E4M3, 16), (2, 2, 512, BF16, INT8, 128)]
+
+
+def _decode_case(H, kvh, d, dtype, code, block, lens, seed=0, idx=torch.int32, bound=None,
+                 scale=None, mag=1.0, pad=0, spoil=False):
+    print(f"case: kv8 decode H={H}/{kvh} D={d} {dtype} {code} block {block} lens={lens[:6]} "
+          f"x{len(lens)}", flush=True)
+    g = torch.Generator().manual_seed(seed)
+    c, table, rids = _filled(g, lens, kvh, d, code, block, BF16 if dtype == F32 else dtype, pad=pad)
+    if spoil:  # slots that are none, whole requests of them
+        for i, (r, n) in enumerate(zip(rids, lens)):
+            at = torch.randperm(max(n, 1), generator=g)[:n // 3 if i else n]
+            table[r, at] = torch.where(torch.rand(len(at), generator=g) < 0.5, -1, c.P).int()
+    cap = [min(max(n, 0), bound) if bound is not None else n for n in lens]
+    B = len(lens)
+    q = (torch.randn(B, H, d, generator=g) * mag).to(dtype)
+    wide = torch.full((B, H, d + pad), 7.0, dtype=dtype, device="cuda")
+    qd = wide.clone()
+    qd[..., :d] = q.cuda()
+    out = wide[..., :d]
+    _ops().kv8_decode_attention(qd[..., :d], table.cuda(), _i32(rids, dtype=idx),
+                                _i32(lens, dtype=idx), bound if bound is not None else max(lens),
+                                *c.args, out, sm_scale=scale)
+    torch.cuda.synchronize()
+    want = O.kv8_decode(q, *c.values(), table, rids, cap, c.P, scale)
+    _inside(out, want[0], O.bound_kv8_decode(*want, dtype, d), "out")
+    assert bool((wide[..., d:] == 7.0).all())
+    return out
+
+
+@pytest.mark.parametrize("H,kvh,d,dtype,code,block", ATT)
+def test_kv8_decode_attention(cuda, H, kvh, d, dtype, code, block):
+    _decode_case(H, kvh, d, dtype, code, block, [1, 2, 0, 333, 16, 17, 129], seed=d,
+                 idx=torch.int64 if block == 16 else torch.int32)
+
+
+@pytest.mark.parametrize("H,kvh,d,dtype,code,block", ATT)
+def test_kv8_decode_attention_of_slots_that_are_none(cuda, H, kvh, d, dtype, code, block):
+    """Table entries outside the cache are not attended to; a request of them
+    alone is an empty one."""
+    out = _decode_case(H, kvh, d, dtype, code, block, [40, 100, 33, 260], seed=d, spoil=True)
+    assert bool((out[0] == 0).all())
+
+
+@pytest.mark.parametrize("B,n", [(1, 9000), (3, 5000), (8, 3000), (40, 700), (130, 90)])
+def test_kv8_decode_attention_splits(cuda, B, n):
+    """Few long sequences and many short ones, a workspace that held NaN."""
+    lens = [max(1, n - 131 * i) if i % 5 else n for i in range(B)]
+    for H, kvh, d, dtype, code in ((4, 2, 128, BF16, INT8), (2, 1, 64, F16, E4M3)):
+        need = _ops()._kv8_decode_bytes(B, H, kvh, d, n)
+        if need:
+            _ops().workspace(cuda, "kv8_decode", need).fill_(255)
+        _decode_case(H, kvh, d, dtype, code, 16, lens, seed=B, mag=3.0)
+
+
+def test_kv8_decode_attention_bounds_and_scales(cuda):
+    _decode_case(8, 2, 128, BF16, INT8, 16, [500, 90, 3], bound=100)
+    _decode_case(4, 2, 64, BF16, INT8, 16, [0, 0], bound=16)
+    _decode_case(4, 2, 64, BF16, INT8, 16, [30, 2], bound=0)
+    _decode_case(4, 2, 128, BF16, INT8, 16, [200, 31], scale=0.5)
+    _decode_case(4, 2, 128, F16, INT8, 16, [200, 31], mag=6.0)
+    for pad in (3, 8):
+        _decode_case(4, 2, 128, BF16, INT8, 16, [200, 31], pad=pad)
+        _decode_case(4, 2, 64, F32, E4M3, 16, [200, 31], pad=pad)
+
+
+def test_kv8_decode_attention_rows_outside_the_table(cuda):
+    g = torch.Generator().manual_seed(1)
+    c, table, rids = _filled(g, [20, 30], 2, 64, INT8, 16, BF16)
+    q = torch.randn(4, 4, 64, generator=g).to(BF16).cuda()
+    out, ref = torch.full_like(q, 7.0), torch.full_like(q[1:3], 7.0)
+    req = [-1] + rids + [table.shape[0]]
+    _ops().kv8_decode_attention(q, table.cuda(), _i32(req), _i32([5, 20, 30, 9]), 30, *c.args, out)
+    _ops().kv8_decode_attention(q[1:3], table.cuda(), _i32(rids), _i32([20, 30]), 30, *c.args, ref)
+    assert torch.equal(out[1:3], ref)
+    assert bool((out[0] == 0).all()) and bool((out[3] == 0).all())
+
+
+def test_kv8_nan_scales_stay_in_their_head(cuda):
+    """A NaN among one head's tokens reaches that head's outputs and no others."""
+    g = torch.Generator().manual_seed(1)
+    for d, kind in ((128, 0), (64, 1)):
+        c, table, rids = _filled(g, [70, 40], 2, d, INT8, 16, BF16)
+        (c.ks, c.vs)[kind][int(table[rids[0], 50]) // 16, 1] = float("nan")
+        q = torch.randn(2, 8, d, generator=g).to(BF16).cuda()
+        out = torch.empty_like(q)
+        _ops().kv8_decode_attention(q, table.cuda(), _i32(rids), _i32([70, 40]), 70, *c.args, out)
+        nan = torch.isnan(out).cpu()
+        assert bool(nan[0, 4:].all()) and not bool(nan[0, :4].any()) and not bool(nan[1].any())
+
+
+# ---------------------------------------------------------------- 4-bit products
+def _weight(g, N, K, group, dtype, zero):
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    scale = ((torch.rand(N, K // group, generator=g) + 0.5) * 0.05).to(dtype)
+    z = torch.randint(0, 16, scale.shape, generator=g, dtype=torch.uint8) if zero else None
+    return codes, scale, z, _ops().W4Weight(codes.cuda(), scale.cuda(), None if z is None else z.cuda())
+
+
+@pytest.mark.parametrize("N,K,group", [(16, 32, 32), (1, 128, 128), (17, 64, 64), (100, 96, 32),
+                                       (100, 192, 64), (256, 128, 128), (333, 1536, 128),
+                                       (2053, 640, 128), (70, 8960, 64), (48, 11008, 128)])
+@pytest.mark.parametrize("dtype,zero", [(BF16, False), (BF16, True), (F16, False), (F16, True)])
+def test_linear_w4(cuda, N, K, group, dtype, zero):
+    g = torch.Generator().manual_seed(N + K)
+    codes, scale, z, w = _weight(g, N, K, group, dtype, zero)
+    assert w.shape == (N, K) and w.group == group
+    for M in (1, 2, 7, 16, 17, 33, 40, 64, 65, 150):
+        print(f"case: w4 {M}x{N}x{K} group {group} {dtype} zero={zero}", flush=True)
+        x = torch.randn(M, K, generator=g).to(dtype)
+        if M == 7:
+            x = x + 2  # sums that do not cancel
+        bias = torch.randn(N, generator=g).to(dtype) if M % 2 else None
+        out = torch.full((M + 1, N), 7.0, dtype=dtype, device="cuda")
+        r = _ops().linear_w4(x.cuda(), w, None if bias is None else bias.cuda(), out=out[:M])
+        assert r.data_ptr() == out.data_ptr() and bool((out[M] == 7.0).all())
+        y, mag = O.linear_w4(x, codes, scale, z, bias)
+        _inside(out[:M], y, O.bound_linear_w4(y, mag, dtype, K), "y")
+
+
+def test_linear_w4_strides(cuda):
+    """Rows of x and y inside wider ones, aligned and not; the row order; M = 0."""
+    g = torch.Generator().manual_seed(5)
+    N, K = 130, 256
+    codes, scale, z, w = _weight(g, N, K, 64, BF16, True)
+    for M in (3, 20, 70):
+        for pad, at in ((8, 8), (3, 1), (1, 0)):
+            print(f"case: w4 strides M={M} pad={pad} at={at}", flush=True)
+            wide = torch.randn(M, K + pad, generator=g).to(BF16).cuda()
+            x = wide[:, at:at + K]
+            out = torch.full((M, N + pad), 7.0, dtype=BF16, device="cuda")
+            _ops().linear_w4(x, w, out=out[:, at:at + N])
+            y, mag = O.linear_w4(x.cpu(), codes, scale, z)
+            _inside(out[:, at:at + N], y, O.bound_linear_w4(y, mag, BF16, K), "y")
+            out[:, at:at + N] = 7.0
+            assert bool((out == 7.0).all())
+    assert _ops().linear_w4(torch.empty(0, K, dtype=BF16, device="cuda"), w).shape == (0, N)
+    one = torch.randn(1, K, generator=g).to(BF16).cuda()
+    same = _ops().linear_w4(one.expand(5, K), w)
+    assert torch.equal(same, same[:1].expand(5, N))
+
+
+def test_linear_w4_zero_bytes_count_by_four_bits(cuda):
+    g = torch.Generator().manual_seed(6)
+    codes, scale, z, w = _weight(g, 32, 128, 32, BF16, True)
+    w2 = _ops().W4Weight(codes.cuda(), scale.cuda(), (z | 0xa0).cuda())
+    x = torch.randn(4, 128, generator=g).to(BF16).cuda()
+    assert torch.equal(_ops().linear_w4(x, w), _ops().linear_w4(x, w2))
+
+
+def test_linear_w4_rows_do_not_mix(cuda):
+    """Infinities and NaN in one row of x leave the other rows' bits."""
+    g = torch.Generator().manual_seed(6)
+    for dtype in (BF16, F16):
+        _, _, _, w = _weight(g, 80, 256, 128, dtype, False)
+        for M in (2, 20, 70):
+            x = torch.randn(M, 256, generator=g).to(dtype).cuda()
+            good = _ops().linear_w4(x, w)
+            x[M // 2, 9], x[M // 2, 200] = float("inf"), float("nan")
+            bad = _ops().linear_w4(x, w)
+            assert not bool(torch.isfinite(bad[M // 2]).any())
+            keep = torch.arange(M) != M // 2
+            assert torch.equal(bad[keep], good[keep])
+
+
+# ---------------------------------------------------------------- logits
+def _logit_case(B, V, n, nb, masked, dtype, seed=0, which=(1, 1, 1), idx=torch.int32, pad=0,
+                inplace=False):
+    print(f"case: logits {B}x{V} tokens {n} biases {nb} mask {masked} {dtype} {which}", flush=True)
+    g = torch.Generator().manual_seed(seed)
+    wide = (torch.randn(B, V + pad, generator=g) * 4).to(dtype).cuda()
+    x = wide[:, :V]
+    toks = rids = prompt = lens = None
+    pen = [None, None, None]
+    if n is not None:
+        toks = torch.randint(-2, V + 3, (B + 2, max(n, 1)), generator=g, dtype=torch.int32)
+        toks[:, ::3] = toks[:, :1].clone()  # one token over and over
+        rids = torch.randperm(B + 2, generator=g)[:B].tolist()
+        lens = [n, 0, n // 2, 1, n + 9][:B] + [n] * max(0, B - 5)
+        prompt = [n // 2, 0, n, 0, 1][:B] + [n // 3] * max(0, B - 5)
+        rep = 0.5 + torch.rand(B, generator=g)
+        pen = [t if on else None for t, on in
+               zip((rep, torch.randn(B, generator=g), torch.randn(B, generator=g)), which)]
+    ids = vals = mask = None
+    if nb is not None:
+        ids = torch.randint(-1, V + 2, (B, nb), generator=g, dtype=torch.int32)
+        vals = torch.randn(B, nb, generator=g) * 10
+    if masked:
+        mask = torch.randint(-2 ** 31, 2 ** 31, (B, -(-V // 32) + 1), generator=g).to(torch.int32)
+        mask[0] = 0  # nothing is left
+    dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    ii = lambda v: None if v is None else _i32(v, dtype=idx)  # noqa: E731
+    out = x if inplace else torch.full_like(wide, 7.0)[:, :V]
+    xc = x.cpu()
+    r = _ops().adjust_logits(x, dev(toks), ii(rids), ii(prompt), ii(lens), repetition=dev(pen[0]),
+                             frequency=dev(pen[1]), presence=dev(pen[2]), bias_ids=dev(ids),
+                             bias_values=dev(vals), mask=dev(mask), out=out)
+    assert r is out
+    want, mag = O.adjust_logits(xc, toks, rids, prompt, lens, *pen, ids, vals, mask)
+    _inside(out, want, O.bound_logits(want, mag, dtype, 6 + (nb or 0)), "logits")
+    if not inplace:
+        assert torch.equal(x.cpu(), xc)
+        if pad:
+            assert bool((out.as_strided((B, V + pad), (V + pad, 1))[:, V:] == 7.0).all())
+    return out
+
+
+@pytest.mark.parametrize("V", [1, 31, 33, 1000, 4096, 4097, 10001])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_adjust_logits(cuda, V, dtype):
+    """Ids outside the vocabulary, tokens over and over, empty and over-long
+    histories, several biases for one token, rows that the mask leaves empty."""
+    for seed, (n, nb, masked) in enumerate([(50, 7, True), (1, None, False), (300, 40, False),
+                                            (None, 3, True), (700, 0, True)]):
+        _logit_case(5, V, n, nb, masked, dtype, seed=seed, idx=torch.int64 if seed else torch.int32)
+
+
+def test_adjust_logits_parts(cuda):
+    """Each control alone; odd row strides; in place."""
+    for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 0, 0)):
+        _logit_case(3, 5000, 200, None, False, F32, which=which)
+    _logit_case(3, 5000, None, None, False, BF16)
+    _logit_case(3, 5000, None, None, True, BF16)
+    for pad in (1, 3, 8):
+        _logit_case(4, 4999, 60, 5, True, F32, pad=pad)
+        _logit_case(4, 4999, 60, 5, True, BF16, pad=pad, inplace=True)
+    _logit_case(2, 300, 9000, 1, False, F32)
+
+
+def test_adjust_logits_counts_many(cuda):
+    """One token 100,000 times; every token of a long prompt; argmax of a row that
+    nothing is left of."""
+    V, n = 5003, 100000
+    t = torch.full((1, n), 4097, dtype=torch.int32, device="cuda")
+    x = torch.ones(1, V, device="cuda")
+    args = (t, _i32([0]), _i32([0]), _i32([n]))
+    y = _ops().adjust_logits(x, *args, frequency=torch.ones(1, device="cuda"))
+    assert float(y[0, 4097]) == 1.0 - n and float(y.sum()) == V - n
+    y = _ops().adjust_logits(x, t, _i32([0]), _i32([n]), _i32([n]),
+                             repetition=torch.full((1,), 2.0, device="cuda"),
+                             frequency=torch.ones(1, device="cuda"))
+    assert float(y[0, 4097]) == 0.5  # of the prompt: no frequency
+    y = _ops().adjust_logits(x, mask=torch.zeros(1, 157, dtype=torch.int32, device="cuda"))
+    assert bool(torch.isneginf(y).all()) and int(_ops().argmax(y)[0]) == 0
+
+
+def test_adjust_logits_infinities(cuda):
+    """-inf stays -inf under a penalty and a bias, a mask rules NaN out."""
+    inf = float("inf")
+    x = torch.tensor([[-inf, inf, float("nan"), 1.0, float("nan")]], device="cuda")
+    t = torch.arange(5, dtype=torch.int32, device="cuda").view(1, 5)
+    y = _ops().adjust_logits(x, t, _i32([0]), _i32([0]), _i32([5]),
+                             repetition=torch.full((1,), 2.0, device="cuda"),
+                             presence=torch.ones(1, device="cuda"), bias_ids=t,
+                             bias_values=torch.ones(1, 5, device="cuda"), mask=_i32([[0b01111]]))
+    y = y.cpu()[0]
+    assert y[0] == -inf and y[1] == inf and torch.isnan(y[2]) and y[3] == 0.5 and y[4] == -inf
+
+
+# ---------------------------------------------------------------- a run of them
+class Server:
+    """A decode step of one layer and an lm head on 4-bit weights and an 8-bit
+    cache: the calls of one step, each on what the one before left."""
+
+    def __init__(self, B, seed, block=16, code=INT8):
+        ops, g = _ops(), torch.Generator().manual_seed(seed)
+        self.B, self.H, self.kvh, self.d, self.hid, self.V = B, 4, 2, 64, 256, 1000
+        self.cap = 128
+        H, kvh, d, hid = self.H, self.kvh, self.d, self.hid
+        mk = lambda n, k: _weight(g, n, k, 64, BF16, True)[3]  # noqa: E731
+        self.wqkv, self.wo, self.wl = mk((H + 2 * kvh) * d, hid), mk(hid, H * d), mk(self.V, hid)
+        self.emb = torch.randn(self.V, hid, generator=g).to(BF16).cuda()
+        self.f = ops.rope_frequencies(d)[0].cuda()
+        pages = B * self.cap // block
+        perm = torch.randperm(pages, generator=g)
+        self.table = (perm[:, None] * block + torch.arange(block)).view(B, self.cap).int().cuda()
+        pool = torch.zeros(pages * block, 2 * kvh, d, dtype=torch.uint8, device="cuda").view(code)
+        self.pool, self.block = pool, block
+        self.scale = torch.zeros(pages, 2 * kvh, device="cuda")
+        self.cache = (pool[:, :kvh], pool[:, kvh:], self.scale[:, :kvh], self.scale[:, kvh:], block)
+        self.rows = torch.arange(B, dtype=torch.int32, device="cuda")
+        self.lens = torch.tensor([3 + i for i in range(B)], dtype=torch.int32, device="cuda")
+        self.prompt = self.lens.clone()
+        self.history = torch.randint(0, self.V, (B, self.cap), generator=g, dtype=torch.int32).cuda()
+        self.rep = torch.full((B,), 1.3, device="cuda")
+        self.freq = torch.full((B,), 0.2, device="cuda")
+        self.mask = torch.randint(-2 ** 31, 2 ** 31, (B, 32), generator=g).to(torch.int32).cuda()
+        self.tok = torch.zeros(B, dtype=torch.int64, device="cuda")
+        self.out = torch.empty(B, H, d, dtype=BF16, device="cuda")
+        # the prompts' tokens
+        T = int(self.lens.sum())
+        x = torch.randn(T, (H + 2 * kvh) * d, generator=g).to(BF16).cuda()
+        k, v = (x[:, a * d:b * d].unflatten(1, (kvh, d)) for a, b in ((H, H + kvh), (H + kvh, H + 2 * kvh)))
+        slots = torch.cat([self.table[i, :n] for i, n in enumerate(self.lens.tolist())])
+        ops.kv8_store(k, v, slots, *self.cache)
+
+    def step(self):
+        ops, H, kvh, d = _ops(), self.H, self.kvh, self.d
+        pos = self.lens
+        slots = self.table.gather(1, pos[:, None].long())[:, 0].contiguous()
+        self.history.scatter_(1, pos[:, None].long(), self.tok[:, None].int())
+        self.lens.add_(1)
+        qkv = ops.linear_w4(self.emb[self.tok], self.wqkv)
+        q = qkv[:, :H * d].unflatten(1, (H, d))
+        k = qkv[:, H * d:(H + kvh) * d].unflatten(1, (kvh, d))
+        v = qkv[:, (H + kvh) * d:].unflatten(1, (kvh, d))
+        ops.rope_positions(q, k, self.lens - 1, self.f)
+        ops.kv8_store(k, v, slots, *self.cache)
+        ops.kv8_decode_attention(q, self.table, self.rows, self.lens, self.cap, *self.cache, self.out)
+        y = ops.linear_w4(ops.linear_w4(self.out.flatten(1), self.wo), self.wl)
+        y = ops.adjust_logits(y, self.history, self.rows, self.prompt, self.lens,
+                              repetition=self.rep, frequency=self.freq, mask=self.mask)
+        self.tok.copy_(ops.argmax(y))
+        return y
+
+
+def test_a_run_of_steps_stays_in_the_mask(cuda):
+    s = Server(5, 1)
+    for _ in range(30):
+        y = s.step()
+        assert bool(torch.isfinite(y[torch.arange(5), s.tok]).all())
+        bit = (s.mask[torch.arange(5), s.tok // 32] >> (s.tok % 32)) & 1
+        assert bool((bit == 1).all())
+    # the cache that the steps left gives what prefill attention gives of its values
+    n = s.lens.tolist()
+    start = [sum(n[:i]) for i in range(5)]
+    k, v = (torch.empty(sum(n), s.kvh, s.d, dtype=BF16, device="cuda") for _ in range(2))
+    _ops().kv8_load(*s.cache, s.table, s.rows, _i32(start), s.lens, s.cap, k, v)
+    q = torch.randn(5, s.H, s.d, device="cuda").to(BF16)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    _ops().kv8_decode_attention(q, s.table, s.rows, s.lens, s.cap, *s.cache, a)
+    table = torch.zeros(5, s.cap, dtype=torch.int32, device="cuda")
+    for i in range(5):
+        table[i, :n[i]] = torch.arange(start[i], start[i] + n[i], device="cuda")
+    _ops().prefill_attention(q, k, v, b, s.rows, s.rows, s.lens, 1, table, s.lens - 1)
+    # values rounded to bf16 and probabilities once more: a few of their roundings
+    assert float((a.float() - b.float()).abs().max()) <= 6 * O.u(BF16) * float(b.float().abs().max())
+
+
+def test_captured_steps_replay(cuda):
+    """Two servers' steps in two graphs, replayed in turn and at the same time on
+    two streams, equal to eager ones."""
+    servers = [Server(4, 7), Server(3, 8, code=E4M3)]
+    eager = [Server(4, 7), Server(3, 8, code=E4M3)]
+    graphs = []
+    for s, e in zip(servers, eager):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s.step()
+        torch.cuda.current_stream().wait_stream(side)
+        e.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s.y = s.step()
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in servers]
+    for it in range(8):
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+            if it % 2:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for s, e in zip(servers, eager):
+            want = e.step()
+            assert torch.equal(s.y, want) and torch.equal(s.tok, e.tok), f"replay {it}"
+            assert torch.equal(s.pool.view(torch.uint8), e.pool.view(torch.uint8))
+            assert torch.equal(s.scale, e.scale)
+
+
+def test_threads_with_streams_of_their_own(cuda):
+    """Four threads' servers, each on its stream, give what they give alone."""
+    alone = []
+    for i in range(4):
+        s = Server(3, 20 + i)
+        alone.append([s.step().clone() for _ in range(6)])
+    bad = []
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            s = Server(3, 20 + i)
+            for y in alone[i]:
+                if not torch.equal(s.step(), y):
+                    bad.append(i)
+            st.synchronize()
+
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
+def test_calls_of_nothing(cuda):
+    ops = _ops()
+    c = Cache(32, 2, 64, INT8, 16)
+    none = torch.empty(0, 2, 64, dtype=BF16, device="cuda")
+    ops.kv8_store(none, none, _i32([]), *c.args)
+    ops.kv8_load(*c.args, _i32([[0] * 8]), _i32([]), _i32([]), _i32([]), 8, none, none)
+    q = torch.empty(0, 4, 64, dtype=BF16, device="cuda")
+    assert ops.kv8_decode_attention(q, _i32([[0] * 8]), _i32([]), _i32([]), 8, *c.args, q) is q
+    ops.adjust_logits(torch.empty(0, 9, device="cuda"))
+    torch.cuda.synchronize()
+    c.check()
