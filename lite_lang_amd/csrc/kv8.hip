@@ -313,7 +313,10 @@ struct DecodeArgs8 {
   void* out; int64_t o_sb, o_sh;
   int64_t nslots;
   int B, H, KVH, G, D, shift, max_len;
+  int hb, nsplit, span;  // blocks of 16 query heads, splits of `span` tokens
+  int qvec, ovec;        // 16-byte loads of q, stores of out
   float scale_log2;
+  float* part; float2* part_ml;  // [B, H, nsplit, D], [B, H, nsplit]
 };
 
 __device__ __forceinline__ int decode_len(const DecodeArgs8& a, int b, int64_t* row) {
@@ -380,6 +383,347 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
     const int d = lane + 64 * j;
     if (d < a.D) o[d] = ll_from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
   }
+}
+
+// ------------------------------------------------------------------ matrix form
+// A workgroup takes a split of one request and a block of up to 16 query heads
+// that share a KV head; its waves take every fourth tile of 32 tokens.
+//   S [16 tokens x 16 heads] = K Q^T,  O^T [16 dims x 16 heads] += V^T P^T
+// by 16x16x32 MFMAs, whose k index may run in any order that both operands
+// agree on. So a lane's K operand is 16 bytes of its own token's row, and the
+// scores that a lane gets, tokens 4 g .. 4 g + 3 and 16 + 4 g .. (g = lane / 16)
+// of head lane % 16, are its P operand as they are; its V operand are those
+// tokens' bytes of the dims that it owns, each byte converted straight into its
+// place. No data passes through LDS but the slots and scales of the tile.
+//
+// Codes are exact in bf16. q is split into as many bf16 numbers as hold it (fp16
+// two, fp32 three), a probability times its V scale likewise into two (2^-16 of
+// itself; three for fp32), so that 8-bit codes are all that is lost. The maximum
+// moves only when a tile has a larger one.
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+
+template <typename T> constexpr int kQParts = __is_same(T, float) ? 3 : __is_same(T, __bf16) ? 1 : 2;
+template <typename T> constexpr int kPParts = __is_same(T, float) ? 3 : 2;
+
+// the upper halves of two floats: their bf16 values, where those are exact
+__device__ __forceinline__ uint32_t pack_exact(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo),
+                               0x07060302u);
+}
+
+// 8 codes (two dwords) as bf16
+template <int CODE> __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
+  u32x4 w;
+  if constexpr (CODE == KV8_INT8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = i < 2 ? a : b;
+      w[i] = pack_exact(CodeOf<CODE>::decode(v, 2 * (i & 1)), CodeOf<CODE>::decode(v, 2 * (i & 1) + 1));
+    }
+  } else {
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true));
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false));
+    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
+  }
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// parts[i]: what is left of x behind parts 0 .. i - 1, in bf16
+template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&parts)[N]) {
+  float left[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) left[e] = x[e];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      parts[i][e] = (__bf16)left[e];
+      left[e] -= (float)parts[i][e];
+    }
+  }
+}
+
+template <int N> struct BytesOf;
+template <> struct BytesOf<4> { typedef uint32_t V; };
+template <> struct BytesOf<8> { typedef uint2 V; };
+template <> struct BytesOf<16> { typedef uint4 V; };
+
+constexpr int kTile8 = 32, kWaves8 = 4;
+
+template <typename T, int CODE, int D>
+__global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a) {
+  constexpr int NQ = kQParts<T>, NP = kPParts<T>, NK = D / 64, NV = D / 16, VW = NV / 4;
+  typedef typename BytesOf<NV>::V VBytes;
+  __shared__ int32_t s_slot[kWaves8][kTile8];
+  __shared__ float s_scale[kWaves8][2][kTile8];
+  __shared__ float s_m[kWaves8][16], s_l[kWaves8][16];
+  __shared__ f32x4 s_acc[kWaves8 - 1][NV][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+  int unit = blockIdx.x;
+  const int split = unit % a.nsplit;
+  unit /= a.nsplit;
+  const int hb = unit % a.hb;
+  unit /= a.hb;
+  const int kvh = unit % a.KVH, b = unit / a.KVH;
+  const int head = hb * 16 + c16;  // of the KV head's
+  const bool live = head < a.G;
+  const int h = kvh * a.G + (live ? head : 0);
+  int64_t row;
+  const int n = decode_len(a, b, &row);
+  const int t0 = split * a.span, t1 = min(n, t0 + a.span);
+  if (t0 >= n && (split > 0 || n > 0)) return;  // (the merge reads no such split)
+
+  bf16x8 qf[NK * 2][NQ];
+  {
+    const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < NK * 2; ++i) {
+      const int d = (i >> 1) * 64 + g * 16 + (i & 1) * 8;
+      float v[8];
+      if (a.qvec) load8<T, true>(q, d, D, v);
+      else load8<T, false>(q, d, D, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = live ? v[e] : 0.f;
+      split8<NQ>(v, qf[i]);
+    }
+  }
+  const int32_t* table = a.r2t + (n > 0 ? row : 0) * a.r2t_s;
+  const uint8_t* kc = a.c[0] + kvh * a.c_sh[0];
+  const uint8_t* vc = a.c[1] + kvh * a.c_sh[1] + c16 * NV;
+  // a lane's own token of the tile, and which of its scales it fetches
+  const int tok = lane & 31, kv = lane >> 5;
+  const float* sc = a.s[kv] + kvh * a.s_sh[kv];
+  const int64_t ssb = a.s_sb[kv];
+
+  f32x4 acc[NV] = {};
+  float m = -INFINITY, l = 0.f;
+  const auto slot_of = [&](int t) {  // of the lane's token, -1: none
+    const int at = t + tok;
+    const int32_t s = table[min(at, n - 1)];
+    return at < t1 && s >= 0 && s < a.nslots ? s : -1;
+  };
+  int t = t0 + wave * kTile8;
+  int32_t slot = t < t1 ? slot_of(t) : -1;
+  for (; t < t1; t += kWaves8 * kTile8) {
+    const int32_t next = t + kWaves8 * kTile8 < t1 ? slot_of(t + kWaves8 * kTile8) : -1;
+    // (a wave's own LDS, in order: fences for the compiler)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (kv == 0) s_slot[wave][tok] = slot;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float myscale = sc[(max(slot, 0) >> a.shift) * ssb];
+    const i32x4 vs0 = *(const i32x4*)&s_slot[wave][g * 4];
+    const i32x4 vs1 = *(const i32x4*)&s_slot[wave][16 + g * 4];
+    u32x4 kw[2][NK];
+#pragma unroll
+    for (int grp = 0; grp < 2; ++grp) {
+      const int64_t s = max(s_slot[wave][grp * 16 + c16], 0);
+      const uint8_t* p = kc + s * a.c_st[0] + g * 16;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) kw[grp][i] = *(const u32x4*)(p + i * 64);
+    }
+    uint32_t vw[8][VW];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t s = max(j < 4 ? vs0[j & 3] : vs1[j & 3], 0);
+      const VBytes v = *(const VBytes*)(vc + s * a.c_st[1]);
+      __builtin_memcpy(vw[j], &v, NV);
+    }
+    s_scale[wave][kv][tok] = myscale;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float x[8];
+#pragma unroll
+    for (int grp = 0; grp < 2; ++grp) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NK * 2; ++i) {
+        const bf16x8 kf = codes8<CODE>(kw[grp][i >> 1][2 * (i & 1)], kw[grp][i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+        for (int p = 0; p < NQ; ++p)
+          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], s, 0, 0, 0);
+      }
+      const f32x4 ks = *(const f32x4*)&s_scale[wave][0][grp * 16 + g * 4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool see = (grp ? vs1[r] : vs0[r]) >= 0;
+        x[grp * 4 + r] = see ? s[r] * ks[r] * a.scale_log2 : -INFINITY;
+      }
+    }
+    float mt = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mt = fmaxf(mt, x[j]);
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    if (__ballot(mt > m)) {
+      const float mn = fmaxf(m, mt);
+      const float alpha = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) acc[i] *= alpha;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float pv[8];
+    bool none = false;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const f32x4 vs = *(const f32x4*)&s_scale[wave][1][half * 16 + g * 4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = half * 4 + r;
+        const bool see = (half ? vs1[r] : vs0[r]) >= 0;
+        const float p = exp2f(x[j] - ms);
+        l += p;
+        pv[j] = see ? p * vs[r] : 0.f;
+        none |= !see;
+      }
+    }
+    if (__ballot(none)) {  // the last tile: what is in no token's row may be NaN
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < VW; ++i) vw[j][i] = (j < 4 ? vs0[j & 3] : vs1[j & 3]) >= 0 ? vw[j][i] : 0u;
+    }
+    bf16x8 pf[NP];
+    split8<NP>(pv, pf);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = pack_exact(CodeOf<CODE>::decode(vw[2 * e][i >> 2], i & 3),
+                          CodeOf<CODE>::decode(vw[2 * e + 1][i >> 2], i & 3));
+      const bf16x8 vf = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p], acc[i], 0, 0, 0);
+    }
+    slot = next;
+  }
+  // the waves' sums, by their common maximum
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) {
+    s_m[wave][c16] = m;
+    s_l[wave][c16] = l;
+  }
+  __syncthreads();
+  float mm = s_m[0][c16], ll = 0.f;
+#pragma unroll
+  for (int w = 1; w < kWaves8; ++w) mm = fmaxf(mm, s_m[w][c16]);
+  const float mms = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+  for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * exp2f(s_m[w][c16] - mms);
+  const float mine = exp2f(m - mms);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] *= mine;
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s_acc[wave - 1][i][lane] = acc[i];
+  }
+  __syncthreads();
+  if (wave > 0 || !live) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int w = 0; w < kWaves8 - 1; ++w) acc[i] += s_acc[w][i][lane];
+  if (a.nsplit > 1) {
+    const int64_t at = ((int64_t)b * a.H + h) * a.nsplit + split;
+    if (g == 0) a.part_ml[at] = make_float2(mm, ll);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f32x4* o = (f32x4*)(a.part + at * D + (g * 4 + r) * NV);
+#pragma unroll
+      for (int i = 0; i < VW; ++i)
+        o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r], acc[4 * i + 3][r]};
+    }
+    return;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    T y[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] * inv);
+    T* o = out + (g * 4 + r) * NV;
+    if (a.ovec) {
+      __builtin_memcpy(__builtin_assume_aligned(o, sizeof(T) * NV < 16 ? sizeof(T) * NV : 16), y,
+                       sizeof(T) * NV);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) o[i] = y[i];
+    }
+  }
+}
+
+// The splits of one (request, query head): a thread has 4 dims of every
+// 1024 / D-th split.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void merge_kernel(DecodeArgs8 a) {
+  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+  __shared__ f32x4 s_acc[kRows][kLanes];
+  __shared__ float s_m[4], s_l[4];
+  const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
+  int64_t row;
+  const int n = decode_len(a, b, &row);
+  const int ns = (n + a.span - 1) / a.span;
+  const float2* ml = a.part_ml + (int64_t)blockIdx.x * a.nsplit;
+  const f32x4* part = (const f32x4*)(a.part + (int64_t)blockIdx.x * a.nsplit * D);
+  float m = -INFINITY;
+  for (int s = tid; s < ns; s += 256) m = fmaxf(m, ml[s].x);
+  m = ll_wave_max(m);
+  if ((tid & 63) == 0) s_m[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float ms = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int s = tid; s < ns; s += 256) l += ml[s].y * exp2f(ml[s].x - ms);
+  l = ll_wave_sum(l);
+  if ((tid & 63) == 0) s_l[tid >> 6] = l;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int r = tid / kLanes, c = tid % kLanes;
+  for (int s = r; s < ns; s += kRows) acc += part[s * kLanes + c] * exp2f(ml[s].x - ms);
+  s_acc[r][c] = acc;
+  __syncthreads();
+  if (r > 0) return;
+#pragma unroll
+  for (int i = 1; i < kRows; ++i) acc += s_acc[i][c];
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  T* o = (T*)a.out + b * a.o_sb + h * a.o_sh + c * 4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = ll_from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
+}
+
+constexpr int64_t kMaxGrid8 = (1 << 24) - 1;  // of 256 threads: fewer than 2^32
+
+// Splits of a call: enough workgroups for the card, none of fewer than kMinSpan tokens.
+struct Plan8 {
+  int64_t units, nsplit, span, bytes;
+};
+constexpr int kMinSpan = 256, kTargetWgs = 1024;
+
+bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
+           Plan8* p) {
+  if (batch <= 0 || batch > 1 << 24 || kv_heads <= 0 || kv_heads > 65535 || q_heads <= 0 ||
+      q_heads > 65535 || q_heads % kv_heads != 0 || max_len <= 0 || max_len > 1 << 30 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return false;
+  p->units = batch * kv_heads * ((q_heads / kv_heads + 15) / 16);
+  const int64_t most = (max_len + kMinSpan - 1) / kMinSpan;
+  const int64_t want = std::max<int64_t>(1, std::min(most, kTargetWgs / p->units));
+  constexpr int64_t kStep = kWaves8 * kTile8;
+  p->span = (max_len + want * kStep - 1) / (want * kStep) * kStep;
+  p->nsplit = (max_len + p->span - 1) / p->span;
+  p->bytes = p->nsplit > 1 ? batch * q_heads * p->nsplit * (head_dim * 4 + 8) : 0;
+  return p->units * p->nsplit <= kMaxGrid8 && batch * q_heads <= kMaxGrid8;
+}
+
+template <typename T, int CODE, int D> int launch_decode(const DecodeArgs8& a, unsigned grid, hipStream_t stream) {
+  hipLaunchKernelGGL((decode_mfma_kernel<T, CODE, D>), dim3(grid), dim3(kWaves8 * 64), 0, stream, a);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, stream, a);
+  LL_RETURN_LAUNCH();
 }
 
 // log2 of a block size, -1 for others
@@ -536,8 +880,8 @@ extern "C" int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t k
 extern "C" int64_t ll_kv8_decode_attention_workspace_size(int64_t batch, int64_t q_heads,
                                                           int64_t kv_heads, int64_t head_dim,
                                                           int64_t max_len_in_batch) {
-  (void)batch; (void)q_heads; (void)kv_heads; (void)head_dim; (void)max_len_in_batch;
-  return 0;
+  Plan8 p;
+  return plan8(batch, q_heads, kv_heads, head_dim, max_len_in_batch, &p) ? p.bytes : 0;
 }
 
 extern "C" int ll_kv8_decode_attention(
@@ -582,7 +926,39 @@ extern "C" int ll_kv8_decode_attention(
   a.B = (int)batch; a.H = (int)q_heads; a.KVH = (int)kv_heads; a.G = (int)(q_heads / kv_heads);
   a.D = (int)head_dim; a.shift = block_shift(block); a.max_len = (int)max_len_in_batch;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
-  (void)workspace; (void)workspace_bytes;
+  const int es = dtype == LL_F32 ? 4 : 2;
+  Plan8 p;
+  const bool planned = plan8(batch, q_heads, kv_heads, head_dim, max_len_in_batch, &p);
+  // (a cache without slots has no row that a masked token's lanes could read)
+  const bool mfma =
+      planned && slots_n > 0 &&
+      aligned(16, {(int64_t)(uintptr_t)k_codes, (int64_t)(uintptr_t)v_codes, kc_stride_tok,
+                   kc_stride_h, vc_stride_tok, vc_stride_h});
+  if (mfma) {
+    a.hb = (a.G + 15) / 16;
+    a.nsplit = (int)p.nsplit; a.span = (int)p.span;
+    a.qvec = aligned(16, {(int64_t)(uintptr_t)q, q_stride_b * es, q_stride_h * es});
+    a.ovec = aligned(16, {(int64_t)(uintptr_t)out, out_stride_b * es, out_stride_h * es});
+    std::unique_lock<std::mutex> lock;
+    if (p.bytes > 0) {
+      LL_CHECK_ARG(workspace && workspace_bytes >= p.bytes && (uintptr_t)workspace % 16 == 0,
+                   "%s: the workspace needs %lld bytes, 16 B aligned, got %lld", fn,
+                   (long long)p.bytes, (long long)workspace_bytes);
+      a.part = (float*)workspace;
+      a.part_ml = (float2*)((char*)workspace + batch * q_heads * p.nsplit * head_dim * 4);
+      // no other thread's call on this workspace between the two launches
+      lock = std::unique_lock<std::mutex>(ll_workspace_mutex(workspace));
+    }
+    const unsigned grid = (unsigned)(p.units * p.nsplit);
+    return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
+      return dispatch_code(code, [&](auto C) -> int {
+        constexpr int CODE = decltype(C)::value;
+        if (head_dim == 64) return launch_decode<T, CODE, 64>(a, grid, stream);
+        if (head_dim == 128) return launch_decode<T, CODE, 128>(a, grid, stream);
+        return launch_decode<T, CODE, 256>(a, grid, stream);
+      });
+    });
+  }
   LL_CHECK_ARG(batch * q_heads <= INT32_MAX / 64, "%s: %lld requests of %lld heads", fn,
                (long long)batch, (long long)q_heads);
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
