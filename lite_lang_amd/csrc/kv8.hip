@@ -313,10 +313,11 @@ struct DecodeArgs8 {
   void* out; int64_t o_sb, o_sh;
   int64_t nslots;
   int B, H, KVH, G, D, shift, max_len;
-  int hb, nsplit, span;  // blocks of 16 query heads, splits of `span` tokens
-  int qvec, ovec;        // 16-byte loads of q, stores of out
+  int hb, W, whole;  // blocks of 16 query heads, workgroups of each, a request for each
+  int qvec, ovec;    // 16-byte loads of q, stores of out
   float scale_log2;
-  float* part; float2* part_ml;  // [B, H, nsplit, D], [B, H, nsplit]
+  float* part; float2* part_ml;  // [W + B, H, D], [W + B, H]
+  int2* meta;                    // [B]: a request's first part, how many it has
 };
 
 __device__ __forceinline__ int decode_len(const DecodeArgs8& a, int b, int64_t* row) {
@@ -386,22 +387,28 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
 }
 
 // ------------------------------------------------------------------ matrix form
-// A workgroup takes a split of one request and a block of up to 16 query heads
-// that share a KV head; its waves take every fourth tile of 32 tokens.
+// A workgroup takes a block of up to 16 query heads that share a KV head, and
+// its share of the batch's tokens (below); its waves take every fourth tile of 32.
 //   S [16 tokens x 16 heads] = K Q^T,  O^T [16 dims x 16 heads] += V^T P^T
 // by 16x16x32 MFMAs, whose k index may run in any order that both operands
 // agree on. So a lane's K operand is 16 bytes of its own token's row, and the
 // scores that a lane gets, tokens 4 g .. 4 g + 3 and 16 + 4 g .. (g = lane / 16)
 // of head lane % 16, are its P operand as they are; its V operand are those
-// tokens' bytes of the dims that it owns, each byte converted straight into its
-// place. No data passes through LDS but the slots and scales of the tile.
+// tokens' bytes of the dims that it owns, each byte put straight into its place.
+// No data passes through LDS but the addresses and scales of the tile, and the
+// next tile's loads are in flight while one is computed.
 //
-// Codes are exact in bf16. q is split into as many bf16 numbers as hold it (fp16
-// two, fp32 three), a probability times its V scale likewise into two (2^-16 of
-// itself; three for fp32), so that 8-bit codes are all that is lost. The maximum
-// moves only when a tile has a larger one.
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-
+// q is split into as many bf16 numbers as hold it (fp16 two, fp32 three), a
+// probability times its V scale likewise into two (2^-16 of itself; three for
+// fp32), so that 8-bit codes are all that is lost. e4m3 codes are bf16 numbers.
+// An int8 code c becomes one without arithmetic: the byte u = c + 128 in the low
+// half of a bf16 number is u 2^-133 (a subnormal below 128, and the next
+// exponent goes on in the same steps), which the MFMA takes as it is. q and P
+// are scaled by powers of two to make up for it, and the 128 leaves as the same
+// sum of a constant operand: of q once per call, of P with every tile. Its cost
+// is a few more roundings of fp32 sums (2^-24 of 128 |sum q|); fp32 calls, where
+// that would show, convert the codes instead. The maximum moves only when a tile
+// has a larger one.
 template <typename T> constexpr int kQParts = __is_same(T, float) ? 3 : __is_same(T, __bf16) ? 1 : 2;
 template <typename T> constexpr int kPParts = __is_same(T, float) ? 3 : 2;
 
@@ -410,11 +417,15 @@ __device__ __forceinline__ uint32_t pack_exact(float lo, float hi) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo),
                                0x07060302u);
 }
-
-// 8 codes (two dwords) as bf16
-template <int CODE> __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
+// 8 codes of one row (two dwords; with BIAS their bytes are c + 128)
+template <int CODE, bool BIAS> __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
   u32x4 w;
-  if constexpr (CODE == KV8_INT8) {
+  if constexpr (BIAS) {
+    w[0] = __builtin_amdgcn_perm(0u, a, 0x0c010c00u);
+    w[1] = __builtin_amdgcn_perm(0u, a, 0x0c030c02u);
+    w[2] = __builtin_amdgcn_perm(0u, b, 0x0c010c00u);
+    w[3] = __builtin_amdgcn_perm(0u, b, 0x0c030c02u);
+  } else if constexpr (CODE == KV8_INT8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = i < 2 ? a : b;
@@ -427,6 +438,30 @@ template <int CODE> __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_
     w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
   }
   return __builtin_bit_cast(bf16x8, w);
+}
+
+// bytes 2 I and 2 I + 1 of 8 rows
+template <int CODE, bool BIAS, int I>
+__device__ __forceinline__ void codes_of_rows(const uint32_t (&v)[8], bf16x8& lo, bf16x8& hi) {
+  u32x4 w0, w1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = v[2 * e], b = v[2 * e + 1];
+    if constexpr (BIAS) {
+      w0[e] = __builtin_amdgcn_perm(b, a, 0x0c000c00u | (2u * I) | (4u + 2 * I) << 16);
+      w1[e] = __builtin_amdgcn_perm(b, a, 0x0c000c00u | (2u * I + 1) | (5u + 2 * I) << 16);
+    } else if constexpr (CODE == KV8_INT8) {
+      w0[e] = pack_exact(CodeOf<CODE>::decode(a, 2 * I), CodeOf<CODE>::decode(b, 2 * I));
+      w1[e] = pack_exact(CodeOf<CODE>::decode(a, 2 * I + 1), CodeOf<CODE>::decode(b, 2 * I + 1));
+    } else {  // the four bytes in their order, then two at a time
+      const uint32_t s = __builtin_amdgcn_perm(
+          b, a, (2u * I) | (4u + 2 * I) << 8 | (2u * I + 1) << 16 | (5u + 2 * I) << 24);
+      w0[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s, 1.f, false));
+      w1[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s, 1.f, true));
+    }
+  }
+  lo = __builtin_bit_cast(bf16x8, w0);
+  hi = __builtin_bit_cast(bf16x8, w1);
 }
 
 // parts[i]: what is left of x behind parts 0 .. i - 1, in bf16
@@ -444,109 +479,278 @@ template <int N> __device__ __forceinline__ void split8(const float (&x)[8], bf1
   }
 }
 
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
 template <int N> struct BytesOf;
 template <> struct BytesOf<4> { typedef uint32_t V; };
 template <> struct BytesOf<8> { typedef uint2 V; };
 template <> struct BytesOf<16> { typedef uint4 V; };
 
 constexpr int kTile8 = 32, kWaves8 = 4;
+// biased codes: a value of binary exponent e goes to about 2^kUp, and a sum of
+// its products, at 2^(kUp - 133), comes back by 2^(133 - kUp + e)
+constexpr int kUp = 60;
+
+// a tile's loads: K rows, V bytes, the scale of a lane's own token
+template <int D> struct Tile8 {
+  u32x4 kw[2][D / 64];
+  uint32_t vw[D / 64][8];
+  float scale;
+  uint32_t see;  // a bit per token that is one
+};
+
+// The batch's tokens are dealt out evenly whatever the lengths are: request after
+// request in steps of 128 tokens (a tile per wave), workgroup w of a head block
+// takes steps w * per .. of the list, per = ceil(steps / W). A request that lies
+// in one workgroup's share is finished there; of the others every workgroup
+// leaves its part (rows w + b of the workspace: along the list w or b grows from
+// part to part, so no two share one) to the merge.
+constexpr int kStep8 = kWaves8 * kTile8;
+
+__device__ __forceinline__ int steps_of(int n) { return (n + kStep8 - 1) / kStep8; }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 template <typename T, int CODE, int D>
-__global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a) {
-  constexpr int NQ = kQParts<T>, NP = kPParts<T>, NK = D / 64, NV = D / 16, VW = NV / 4;
+__global__ __launch_bounds__(kWaves8 * 64, D == 256 || __is_same(T, float) ? 1 : 2)
+void decode_mfma_kernel(DecodeArgs8 a) {
+  constexpr bool BIAS = CODE == KV8_INT8 && !__is_same(T, float);
+  constexpr int NQ = kQParts<T>, NP = kPParts<T>, NK = D / 64, NV = D / 16;
   typedef typename BytesOf<NV>::V VBytes;
-  __shared__ int32_t s_slot[kWaves8][kTile8];
+  __shared__ int64_t s_off[kWaves8][2][kTile8];
   __shared__ float s_scale[kWaves8][2][kTile8];
   __shared__ float s_m[kWaves8][16], s_l[kWaves8][16];
   __shared__ f32x4 s_acc[kWaves8 - 1][NV][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-  int unit = blockIdx.x;
-  const int split = unit % a.nsplit;
-  unit /= a.nsplit;
-  const int hb = unit % a.hb;
-  unit /= a.hb;
-  const int kvh = unit % a.KVH, b = unit / a.KVH;
+  __shared__ int s_sum[kWaves8], s_b, s_step, s_n;
+  __shared__ int64_t s_row;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+  // The heads of one share of tokens read its table, its scales' lines and, with
+  // narrow heads, its rows' lines: they sit on one XCD (workgroups go to the 8
+  // XCDs in turn).
+  const int heads = a.KVH * a.hb, i8 = blockIdx.x / 8, u = i8 % heads;
+  const int w = i8 / heads * 8 + blockIdx.x % 8;
+  if (w >= a.W) return;
+  const int hb = u % a.hb, kvh = u / a.hb;
   const int head = hb * 16 + c16;  // of the KV head's
   const bool live = head < a.G;
   const int h = kvh * a.G + (live ? head : 0);
-  int64_t row;
-  const int n = decode_len(a, b, &row);
-  const int t0 = split * a.span, t1 = min(n, t0 + a.span);
-  if (t0 >= n && (split > 0 || n > 0)) return;  // (the merge reads no such split)
 
-  bf16x8 qf[NK * 2][NQ];
+  int b = w, step = 0, left = INT32_MAX, per = 0;  // where in request b, steps to go
+  int64_t row;
+  int n;
+  if (a.whole) {
+    n = decode_len(a, b, &row);
+  } else {
+    const int each = (a.B + kWaves8 * 64 - 1) / (kWaves8 * 64);
+    const int b0 = min((int)threadIdx.x * each, a.B), b1 = min(b0 + each, a.B);
+    int mine = 0;
+    n = 0;
+    for (int i = b0; i < b1; ++i) mine += steps_of(n = decode_len(a, i, &row));
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 63) s_sum[wave] = upto;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves8; ++i) {
+      if (i < wave) upto += s_sum[i];
+      all += s_sum[i];
+    }
+    all = uniform(all);
+    per = max((int)(((int64_t)all + a.W - 1) / a.W), 1);
+    const int64_t from = (int64_t)w * per;
+    if (from >= all) return;
+    left = (int)min((int64_t)per, all - from);
+    if (from >= upto - mine && from < upto) {
+      int at = upto - mine, i = b0;
+      while (each > 1) {  // (of one, n and row are its own)
+        n = decode_len(a, i, &row);
+        if (from < at + steps_of(n)) break;
+        at += steps_of(n);
+        ++i;
+      }
+      s_b = i;
+      s_step = (int)from - at;
+      s_n = n;
+      s_row = row;
+    }
+    __syncthreads();
+    b = uniform(s_b);
+    step = uniform(s_step);
+    n = uniform(s_n);
+    row = s_row;
+  }
+  while (true) {
+  const int steps = steps_of(n);
+  const int take = min(steps - step, left);
+  const bool split = step > 0 || take < steps;
+  const int t0 = step * kStep8, t1 = (int)min((int64_t)n, ((int64_t)step + take) * kStep8);
+  if (!a.whole && step == 0 && u == 0 && threadIdx.x == 0 && n > 0) {
+    // what is left of the request lies in the following workgroups, `per` in each
+    a.meta[b] = make_int2(w + b, 1 + (steps - take + per - 1) / per);
+  }
+  left = a.whole ? 0 : left - take;
+  if (n == 0) {  // (in a list the merge writes its rows)
+    if (a.whole)
+      for (int i = threadIdx.x; i < min(16, a.G - hb * 16) * D; i += kWaves8 * 64)
+        ((T*)a.out)[b * a.o_sb + (kvh * a.G + hb * 16 + i / D) * a.o_sh + i % D] = ll_from_f32<T>(0.f);
+  } else {
+  const int32_t* table = a.r2t + row * a.r2t_s;
+  // a lane's own token of the tile, and whether it looks after its K or its V
+  const int tok = lane & 31, kv = lane >> 5;
+  const float* sc = a.s[kv] + kvh * a.s_sh[kv];
+  const int64_t ssb = a.s_sb[kv], cst = a.c_st[kv];
+  const uint8_t* kc = a.c[0] + kvh * a.c_sh[0] + g * 16;
+  const uint8_t* vc = a.c[1] + kvh * a.c_sh[1] + c16 * NV;
+  constexpr int kStep = kStep8;
+  // No load below stands under a condition, so that the waits count how many
+  // came after the one they are for: a tile behind the last one fetches row 0.
+  const auto entry_of = [&](int t) -> int32_t { return table[min(t + tok, n - 1)]; };
+  // (a wave's own LDS, in order: the fences are for the compiler)
+  const auto fetch = [&](Tile8<D>& f, int t, int32_t entry) {
+    const bool is = t + tok < t1 && entry >= 0 && entry < a.nslots;
+    const int64_t s = is ? entry : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    s_off[wave][kv][tok] = s * cst;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    f.scale = sc[(s >> a.shift) * ssb];
+    f.see = (uint32_t)__ballot(is);
+#pragma unroll
+    for (int grp = 0; grp < 2; ++grp) {
+      const uint8_t* p = kc + s_off[wave][0][grp * 16 + c16];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) f.kw[grp][i] = *(const u32x4*)(p + i * 64);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const VBytes v = *(const VBytes*)(vc + s_off[wave][1][(j >> 2) * 16 + g * 4 + (j & 3)]);
+      uint32_t w[NK];
+      __builtin_memcpy(w, &v, NV);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) f.vw[i][j] = w[i];
+    }
+  };
+
+  int t = t0 + wave * kTile8;
+  constexpr int kStages = D <= 128 ? 2 : 1;  // tiles held
+  Tile8<D> f[kStages];
+  int32_t entry[kStages];
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) entry[s] = entry_of(t + s * kStep);
+  u32x4 raw[NK * 2][sizeof(T) / 2];
   {
     const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
 #pragma unroll
     for (int i = 0; i < NK * 2; ++i) {
       const int d = (i >> 1) * 64 + g * 16 + (i & 1) * 8;
-      float v[8];
-      if (a.qvec) load8<T, true>(q, d, D, v);
-      else load8<T, false>(q, d, D, v);
+      if (a.qvec) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = live ? v[e] : 0.f;
-      split8<NQ>(v, qf[i]);
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e) raw[i][e] = ((const u32x4*)(q + d))[e];
+      } else {
+        __builtin_memcpy(raw[i], __builtin_assume_aligned(q + d, sizeof(T)), sizeof(raw[i]));
+      }
     }
   }
-  const int32_t* table = a.r2t + (n > 0 ? row : 0) * a.r2t_s;
-  const uint8_t* kc = a.c[0] + kvh * a.c_sh[0];
-  const uint8_t* vc = a.c[1] + kvh * a.c_sh[1] + c16 * NV;
-  // a lane's own token of the tile, and which of its scales it fetches
-  const int tok = lane & 31, kv = lane >> 5;
-  const float* sc = a.s[kv] + kvh * a.s_sh[kv];
-  const int64_t ssb = a.s_sb[kv];
+#pragma unroll
+  for (int s = 0; s < (kStages > 1 ? kStages - 1 : 1); ++s) fetch(f[s], t + s * kStep, entry[s]);
+  int32_t next = kStages > 1 ? entry[kStages - 1] : entry_of(t + kStep);
+  bf16x8 qf[NK * 2][NQ];
+  float cq = a.scale_log2;  // of a score's sum
+  f32x4 qoff = {0.f, 0.f, 0.f, 0.f};
+  {
+    float v[NK * 2][8];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK * 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = live ? ll_to_f32(((const T*)raw[i])[e]) : 0.f;
+        top = fmaxf(top, fabsf(v[i][e]));
+      }
+    float up = 1.f;
+    if constexpr (BIAS) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const int e = min(max(__builtin_amdgcn_frexp_expf(top), -50), 50);
+      up = __builtin_ldexpf(1.f, kUp - e);
+      cq *= __builtin_ldexpf(1.f, 133 - kUp + e);
+    }
+#pragma unroll
+    for (int i = 0; i < NK * 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= up;
+      split8<NQ>(v[i], qf[i]);
+    }
+  }
+  bf16x8 c128;  // 128 2^-133
+  {
+    const u32x4 w = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
+    c128 = __builtin_bit_cast(bf16x8, w);
+  }
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int i = 0; i < NK * 2; ++i)
+#pragma unroll
+      for (int p = 0; p < NQ; ++p) qoff = mfma16(c128, qf[i][p], qoff);
+    qoff = -qoff;
+  }
 
-  f32x4 acc[NV] = {};
+  f32x4 acc[NV] = {}, off = {0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  const auto slot_of = [&](int t) {  // of the lane's token, -1: none
-    const int at = t + tok;
-    const int32_t s = table[min(at, n - 1)];
-    return at < t1 && s >= 0 && s < a.nslots ? s : -1;
-  };
-  int t = t0 + wave * kTile8;
-  int32_t slot = t < t1 ? slot_of(t) : -1;
-  for (; t < t1; t += kWaves8 * kTile8) {
-    const int32_t next = t + kWaves8 * kTile8 < t1 ? slot_of(t + kWaves8 * kTile8) : -1;
-    // (a wave's own LDS, in order: fences for the compiler)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (kv == 0) s_slot[wave][tok] = slot;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const float myscale = sc[(max(slot, 0) >> a.shift) * ssb];
-    const i32x4 vs0 = *(const i32x4*)&s_slot[wave][g * 4];
-    const i32x4 vs1 = *(const i32x4*)&s_slot[wave][16 + g * 4];
-    u32x4 kw[2][NK];
+  float up = 1.f, limit = BIAS ? -1.f : INFINITY;  // of V scales; up: their power of two
+  int down = 0;                                    // and what takes it back, 2^(73 + down)
+  const auto compute = [&](Tile8<D>& f) {
+    const float scale = f.see >> tok & 1u ? f.scale : 0.f;
+    if constexpr (BIAS) {
+      if (__ballot(kv == 1 && scale > limit)) {  // the first tile, or scales 2^40 times larger
+        const float top = ll_wave_max(kv == 1 ? scale : 0.f);
+        const int e = min(max(__builtin_amdgcn_frexp_expf(top), -60), 100);
+        const float nu = __builtin_ldexpf(1.f, kUp - e), r = nu / up;
 #pragma unroll
-    for (int grp = 0; grp < 2; ++grp) {
-      const int64_t s = max(s_slot[wave][grp * 16 + c16], 0);
-      const uint8_t* p = kc + s * a.c_st[0] + g * 16;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) kw[grp][i] = *(const u32x4*)(p + i * 64);
+        for (int i = 0; i < NV; ++i) acc[i] *= r;
+        off *= r;
+        up = nu;
+        down = e;
+        limit = __builtin_ldexpf(1.f, min(e + 40, 127));
+      }
     }
-    uint32_t vw[8][VW];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t s = max(j < 4 ? vs0[j & 3] : vs1[j & 3], 0);
-      const VBytes v = *(const VBytes*)(vc + s * a.c_st[1]);
-      __builtin_memcpy(vw[j], &v, NV);
-    }
-    s_scale[wave][kv][tok] = myscale;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    s_scale[wave][kv][tok] = kv ? scale * up : scale;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float x[8];
 #pragma unroll
     for (int grp = 0; grp < 2; ++grp) {
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      f32x4 s = qoff;
 #pragma unroll
       for (int i = 0; i < NK * 2; ++i) {
-        const bf16x8 kf = codes8<CODE>(kw[grp][i >> 1][2 * (i & 1)], kw[grp][i >> 1][2 * (i & 1) + 1]);
+        uint32_t w0 = f.kw[grp][i >> 1][2 * (i & 1)], w1 = f.kw[grp][i >> 1][2 * (i & 1) + 1];
+        if constexpr (BIAS) {
+          w0 ^= 0x80808080u;
+          w1 ^= 0x80808080u;
+        }
+        const bf16x8 kf = codes8<CODE, BIAS>(w0, w1);
 #pragma unroll
-        for (int p = 0; p < NQ; ++p)
-          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], s, 0, 0, 0);
+        for (int p = 0; p < NQ; ++p) s = mfma16(kf, qf[i][p], s);
       }
       const f32x4 ks = *(const f32x4*)&s_scale[wave][0][grp * 16 + g * 4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool see = (grp ? vs1[r] : vs0[r]) >= 0;
-        x[grp * 4 + r] = see ? s[r] * ks[r] * a.scale_log2 : -INFINITY;
+      for (int r = 0; r < 4; ++r) x[grp * 4 + r] = s[r] * cq * ks[r];
+    }
+    const bool part = f.see != 0xffffffffu;  // the last tile, or slots that are none
+    if (part) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool is = f.see >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1u;
+        x[j] = is ? x[j] : -INFINITY;
+        if constexpr (CODE == KV8_E4M3) {  // (what is in no token's row may be NaN)
+#pragma unroll
+          for (int i = 0; i < NK; ++i) f.vw[i][j] = is ? f.vw[i][j] : 0u;
+        }
       }
     }
     float mt = x[0];
@@ -556,49 +760,71 @@ __global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
     if (__ballot(mt > m)) {
       const float mn = fmaxf(m, mt);
-      const float alpha = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < NV; ++i) acc[i] *= alpha;
+      off *= alpha;
     }
     const float ms = m == -INFINITY ? 0.f : m;
     float pv[8];
-    bool none = false;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const f32x4 vs = *(const f32x4*)&s_scale[wave][1][half * 16 + g * 4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int j = half * 4 + r;
-        const bool see = (half ? vs1[r] : vs0[r]) >= 0;
-        const float p = exp2f(x[j] - ms);
+        const float p = __builtin_amdgcn_exp2f(x[half * 4 + r] - ms);
         l += p;
-        pv[j] = see ? p * vs[r] : 0.f;
-        none |= !see;
+        pv[half * 4 + r] = p * vs[r];
       }
-    }
-    if (__ballot(none)) {  // the last tile: what is in no token's row may be NaN
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < VW; ++i) vw[j][i] = (j < 4 ? vs0[j & 3] : vs1[j & 3]) >= 0 ? vw[j][i] : 0u;
     }
     bf16x8 pf[NP];
     split8<NP>(pv, pf);
+    if constexpr (BIAS) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      u32x4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = pack_exact(CodeOf<CODE>::decode(vw[2 * e][i >> 2], i & 3),
-                          CodeOf<CODE>::decode(vw[2 * e + 1][i >> 2], i & 3));
-      const bf16x8 vf = __builtin_bit_cast(bf16x8, w);
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[p], acc[i], 0, 0, 0);
+      for (int p = 0; p < NP; ++p) off = mfma16(c128, pf[p], off);
     }
-    slot = next;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.vw[i][j] ^= 0x80808080u;
+      }
+      bf16x8 v0, v1, v2, v3;
+      codes_of_rows<CODE, BIAS, 0>(f.vw[i], v0, v1);
+      codes_of_rows<CODE, BIAS, 1>(f.vw[i], v2, v3);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        acc[4 * i + 0] = mfma16(v0, pf[p], acc[4 * i + 0]);
+        acc[4 * i + 1] = mfma16(v1, pf[p], acc[4 * i + 1]);
+        acc[4 * i + 2] = mfma16(v2, pf[p], acc[4 * i + 2]);
+        acc[4 * i + 3] = mfma16(v3, pf[p], acc[4 * i + 3]);
+      }
+    }
+  };
+
+  while (t < t1) {
+    if constexpr (kStages > 1) {
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) {
+        fetch(f[(s + kStages - 1) % kStages], t + (kStages - 1) * kStep, next);
+        next = entry_of(t + kStages * kStep);
+        compute(f[s]);
+        t += kStep;
+        if (t >= t1) break;
+      }
+    } else {
+      compute(f[0]);
+      t += kStep;
+      fetch(f[0], t, next);
+      next = entry_of(t + kStep);
+    }
+  }
+  if constexpr (BIAS) {
+    const float back = __builtin_ldexpf(1.f, 133 - kUp), back2 = __builtin_ldexpf(1.f, down);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = (acc[i] - off) * back * back2;
   }
   // the waves' sums, by their common maximum
   l += __shfl_xor(l, 16, 64);
@@ -613,8 +839,8 @@ __global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a
   for (int w = 1; w < kWaves8; ++w) mm = fmaxf(mm, s_m[w][c16]);
   const float mms = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-  for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * exp2f(s_m[w][c16] - mms);
-  const float mine = exp2f(m - mms);
+  for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - mms);
+  const float mine = __builtin_amdgcn_exp2f(m - mms);
 #pragma unroll
   for (int i = 0; i < NV; ++i) acc[i] *= mine;
   if (wave > 0) {
@@ -622,30 +848,28 @@ __global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a
     for (int i = 0; i < NV; ++i) s_acc[wave - 1][i][lane] = acc[i];
   }
   __syncthreads();
-  if (wave > 0 || !live) return;
+  if (wave == 0 && live) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int w = 0; w < kWaves8 - 1; ++w) acc[i] += s_acc[w][i][lane];
-  if (a.nsplit > 1) {
-    const int64_t at = ((int64_t)b * a.H + h) * a.nsplit + split;
+    for (int j = 0; j < kWaves8 - 1; ++j) acc[i] += s_acc[j][i][lane];
+  if (split) {
+    const int64_t at = (int64_t)(w + b) * a.H + h;
     if (g == 0) a.part_ml[at] = make_float2(mm, ll);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       f32x4* o = (f32x4*)(a.part + at * D + (g * 4 + r) * NV);
 #pragma unroll
-      for (int i = 0; i < VW; ++i)
+      for (int i = 0; i < NK; ++i)
         o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r], acc[4 * i + 3][r]};
     }
-    return;
-  }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  } else {
   T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     T y[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] * inv);
+    for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] / ll);
     T* o = out + (g * 4 + r) * NV;
     if (a.ovec) {
       __builtin_memcpy(__builtin_assume_aligned(o, sizeof(T) * NV < 16 ? sizeof(T) * NV : 16), y,
@@ -655,53 +879,96 @@ __global__ __launch_bounds__(kWaves8 * 64) void decode_mfma_kernel(DecodeArgs8 a
       for (int i = 0; i < NV; ++i) o[i] = y[i];
     }
   }
+  }
+  }
+  }
+  if (left <= 0 || ++b >= a.B) return;
+  step = 0;
+  n = decode_len(a, b, &row);
+  }
 }
 
-// The splits of one (request, query head): a thread has 4 dims of every
-// 1024 / D-th split.
-template <typename T, int D>
+// The parts of a request, and the zero rows of an empty one. A workgroup has 4 L
+// elements of its heads, L threads every (256 / L)-th part.
+template <typename T, int D, int L>
 __global__ __launch_bounds__(256) void merge_kernel(DecodeArgs8 a) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
-  __shared__ f32x4 s_acc[kRows][kLanes];
-  __shared__ float s_m[4], s_l[4];
-  const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, tid = threadIdx.x;
+  constexpr int kRows = 256 / L;
+  __shared__ f32x4 s_acc[kRows][L];
+  __shared__ float s_m[kRows][L], s_l[kRows][L];
+  const int tid = threadIdx.x, lane = tid % L, wave = tid / L;
+  const int cols = (a.H * D + 4 * L - 1) / (4 * L);
+  const int b = blockIdx.x / cols, at = blockIdx.x % cols * (4 * L) + lane * 4;
+  const bool in = at < a.H * D;
+  const int h = in ? at / D : 0, d = at % D;
   int64_t row;
   const int n = decode_len(a, b, &row);
-  const int ns = (n + a.span - 1) / a.span;
-  const float2* ml = a.part_ml + (int64_t)blockIdx.x * a.nsplit;
-  const f32x4* part = (const f32x4*)(a.part + (int64_t)blockIdx.x * a.nsplit * D);
-  float m = -INFINITY;
-  for (int s = tid; s < ns; s += 256) m = fmaxf(m, ml[s].x);
-  m = ll_wave_max(m);
-  if ((tid & 63) == 0) s_m[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const float ms = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = tid; s < ns; s += 256) l += ml[s].y * exp2f(ml[s].x - ms);
-  l = ll_wave_sum(l);
-  if ((tid & 63) == 0) s_l[tid >> 6] = l;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int r = tid / kLanes, c = tid % kLanes;
-  for (int s = r; s < ns; s += kRows) acc += part[s * kLanes + c] * exp2f(ml[s].x - ms);
-  s_acc[r][c] = acc;
-  __syncthreads();
-  if (r > 0) return;
+  T* o = (T*)a.out + b * a.o_sb + h * a.o_sh + d;
+  if (n == 0) {
+    if (wave == 0 && in)
 #pragma unroll
-  for (int i = 1; i < kRows; ++i) acc += s_acc[i][c];
-  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  T* o = (T*)a.out + b * a.o_sb + h * a.o_sh + c * 4;
+      for (int e = 0; e < 4; ++e) o[e] = ll_from_f32<T>(0.f);
+    return;
+  }
+  const int2 parts = a.meta[b];
+  const int first = uniform(parts.x), ns = uniform(parts.y);
+  if (ns == 1) return;
+  const float2* ml = a.part_ml + (int64_t)first * a.H + h;
+  const float* part = a.part + ((int64_t)first * a.H + h) * D + d;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = wave; s < ns; s += 8 * kRows) {  // 8 parts at a time
+    float2 v[8];
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t p = min(s + kRows * i, ns - 1);
+      v[i] = ml[p * a.H];
+      x[i] = *(const f32x4*)(part + p * a.H * D);
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mn = fmaxf(mn, v[i].x);
+    const float ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    l *= alpha;
+    acc *= alpha;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = s + kRows * i < ns ? __builtin_amdgcn_exp2f(v[i].x - ms) : 0.f;
+      l += s + kRows * i < ns ? v[i].y * f : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += s + kRows * i < ns ? x[i][e] * f : 0.f;
+    }
+  }
+  s_m[wave][lane] = m;
+  s_l[wave][lane] = l;
+  s_acc[wave][lane] = acc;
+  __syncthreads();
+  if (wave > 0 || !in) return;
+  float mm = m;
+#pragma unroll
+  for (int i = 1; i < kRows; ++i) mm = fmaxf(mm, s_m[i][lane]);
+  const float ms = mm == -INFINITY ? 0.f : mm, f0 = __builtin_amdgcn_exp2f(m - ms);
+  l *= f0;
+  acc *= f0;
+#pragma unroll
+  for (int i = 1; i < kRows; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_m[i][lane] - ms);
+    l += s_l[i][lane] * f;
+    acc += s_acc[i][lane] * f;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = ll_from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
 }
 
 constexpr int64_t kMaxGrid8 = (1 << 24) - 1;  // of 256 threads: fewer than 2^32
+constexpr int kPlaces = 512;                  // workgroups that run at a time: two per CU
 
-// Splits of a call: enough workgroups for the card, none of fewer than kMinSpan tokens.
+// Workgroups of a call per head block; bytes: of the parts (0: no request is split)
 struct Plan8 {
-  int64_t units, nsplit, span, bytes;
+  int64_t W, heads, bytes;
+  bool whole;
 };
-constexpr int kMinSpan = 256, kTargetWgs = 1024;
 
 bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
            Plan8* p) {
@@ -709,20 +976,29 @@ bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, i
       q_heads > 65535 || q_heads % kv_heads != 0 || max_len <= 0 || max_len > 1 << 30 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return false;
-  p->units = batch * kv_heads * ((q_heads / kv_heads + 15) / 16);
-  const int64_t most = (max_len + kMinSpan - 1) / kMinSpan;
-  const int64_t want = std::max<int64_t>(1, std::min(most, kTargetWgs / p->units));
-  constexpr int64_t kStep = kWaves8 * kTile8;
-  p->span = (max_len + want * kStep - 1) / (want * kStep) * kStep;
-  p->nsplit = (max_len + p->span - 1) / p->span;
-  p->bytes = p->nsplit > 1 ? batch * q_heads * p->nsplit * (head_dim * 4 + 8) : 0;
-  return p->units * p->nsplit <= kMaxGrid8 && batch * q_heads <= kMaxGrid8;
+  p->heads = kv_heads * ((q_heads / kv_heads + 15) / 16);
+  const int64_t steps = (max_len + kStep8 - 1) / kStep8;  // of a request at most
+  p->whole = steps == 1;
+  p->W = batch;
+  if (!p->whole)
+    p->W = std::min(std::max(kPlaces / p->heads, batch / 4), batch * steps);
+  p->bytes = p->whole ? 0 : (p->W + batch) * q_heads * (head_dim * 4 + 8) + batch * 8;
+  return (p->W + 7) / 8 * 8 * p->heads <= kMaxGrid8 && batch * steps <= INT32_MAX &&
+         batch * ((q_heads * head_dim + 255) / 256) <= kMaxGrid8;
 }
 
-template <typename T, int CODE, int D> int launch_decode(const DecodeArgs8& a, unsigned grid, hipStream_t stream) {
+template <typename T, int CODE, int D>
+int launch_decode(const DecodeArgs8& a, unsigned grid, hipStream_t stream) {
   hipLaunchKernelGGL((decode_mfma_kernel<T, CODE, D>), dim3(grid), dim3(kWaves8 * 64), 0, stream, a);
-  if (a.nsplit > 1)
-    hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, stream, a);
+  if (!a.whole) {
+    // few requests have many parts each: more threads along those
+    if (a.B <= 8)
+      hipLaunchKernelGGL((merge_kernel<T, D, 8>), dim3((unsigned)(a.B * ((a.H * D + 31) / 32))),
+                         dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((merge_kernel<T, D, 64>), dim3((unsigned)(a.B * ((a.H * D + 255) / 256))),
+                         dim3(256), 0, stream, a);
+  }
   LL_RETURN_LAUNCH();
 }
 
@@ -936,7 +1212,7 @@ extern "C" int ll_kv8_decode_attention(
                    kc_stride_h, vc_stride_tok, vc_stride_h});
   if (mfma) {
     a.hb = (a.G + 15) / 16;
-    a.nsplit = (int)p.nsplit; a.span = (int)p.span;
+    a.W = (int)p.W; a.whole = p.whole;
     a.qvec = aligned(16, {(int64_t)(uintptr_t)q, q_stride_b * es, q_stride_h * es});
     a.ovec = aligned(16, {(int64_t)(uintptr_t)out, out_stride_b * es, out_stride_h * es});
     std::unique_lock<std::mutex> lock;
@@ -945,11 +1221,12 @@ extern "C" int ll_kv8_decode_attention(
                    "%s: the workspace needs %lld bytes, 16 B aligned, got %lld", fn,
                    (long long)p.bytes, (long long)workspace_bytes);
       a.part = (float*)workspace;
-      a.part_ml = (float2*)((char*)workspace + batch * q_heads * p.nsplit * head_dim * 4);
+      a.part_ml = (float2*)((char*)workspace + (p.W + batch) * q_heads * head_dim * 4);
+      a.meta = (int2*)(a.part_ml + (p.W + batch) * q_heads);
       // no other thread's call on this workspace between the two launches
       lock = std::unique_lock<std::mutex>(ll_workspace_mutex(workspace));
     }
-    const unsigned grid = (unsigned)(p.units * p.nsplit);
+    const unsigned grid = (unsigned)((p.W + 7) / 8 * 8 * p.heads);
     return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
       return dispatch_code(code, [&](auto C) -> int {
         constexpr int CODE = decltype(C)::value;
