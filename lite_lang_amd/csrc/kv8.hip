@@ -31,8 +31,17 @@ constexpr float kScaleFloor = 0x1p-80f;
 template <int CODE> struct CodeOf;
 template <> struct CodeOf<KV8_INT8> {
   static constexpr float top = 127.f;
+  // the code of q, rounded: adding 1.5 2^23 leaves it in the lowest byte
   static __device__ __forceinline__ uint32_t encode(float q) {
-    return (uint32_t)(uint8_t)(int8_t)(int)__builtin_rintf(q);
+    return __builtin_bit_cast(uint32_t, q + 0x1.8p23f) & 0xffu;
+  }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    const uint32_t w0 = __builtin_bit_cast(uint32_t, a + 0x1.8p23f);
+    const uint32_t w1 = __builtin_bit_cast(uint32_t, b + 0x1.8p23f);
+    const uint32_t w2 = __builtin_bit_cast(uint32_t, c + 0x1.8p23f);
+    const uint32_t w3 = __builtin_bit_cast(uint32_t, d + 0x1.8p23f);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w3, w2, 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(w1, w0, 0x0c0c0400u), 0x05040100u);
   }
   // byte i of w as a number
   static __device__ __forceinline__ float decode(uint32_t w, int i) {
@@ -43,6 +52,10 @@ template <> struct CodeOf<KV8_E4M3> {
   static constexpr float top = 448.f;
   static __device__ __forceinline__ uint32_t encode(float q) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false) & 0xffu;
+  }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(
+        c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
   }
   static __device__ __forceinline__ float decode(uint32_t w, int i) {
     switch (i) {
@@ -94,100 +107,236 @@ struct StoreArgs {
 };
 
 constexpr int kStoreWaves = 4;
+constexpr int kStoreFill = 8192;  // waves that the card holds
+constexpr int kTeamBlock = 32;
 
-// 8 elements from d on as floats; those at D and behind are 0
+// 8 elements of a row as they lie in memory; those at D and behind are 0
+template <typename T> struct Raw8 { u32x4 w[sizeof(T) / 2]; };
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int d, int D, float (&v)[8]) {
+__device__ __forceinline__ Raw8<T> load8(const T* p, int d, int D) {
+  Raw8<T> r = {};
   if constexpr (VEC) {
-    constexpr int kW = sizeof(T) / 2;
-    u32x4 w[kW];
+    if (d < D)
 #pragma unroll
-    for (int i = 0; i < kW; ++i) w[i] = ((const u32x4*)(p + d))[i];
-    const T* e = (const T*)w;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __builtin_nontemporal_load((const u32x4*)(p + d) + i);
+  } else {
+    T* e = (T*)r.w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ll_to_f32(e[i]);
+    for (int i = 0; i < 8; ++i)
+      if (d + i < D) e[i] = p[d + i];
+  }
+  return r;
+}
+template <typename T> __device__ __forceinline__ float get(const Raw8<T>& r, int i) {
+  return ll_to_f32(((const T*)r.w)[i]);
+}
+
+// Magnitudes as integers: ordered like the numbers, infinities and NaN on top.
+// 16-bit types two at a time.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <typename T> __device__ __forceinline__ uint32_t widen(uint32_t m, const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = __builtin_bit_cast(uint32_t,
+                             __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                       __builtin_bit_cast(u16x2, r.w[0][i] & 0x7fff7fffu)));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = d + i < D ? ll_to_f32(p[d + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) m = max(m, r.w[i >> 2][i & 3] & 0x7fffffffu);
+  }
+  return m;
+}
+// the number of the larger magnitude held in m; infinite for NaN too
+template <typename T> __device__ __forceinline__ float widest(uint32_t m) {
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t b = (uint16_t)max(m & 0xffffu, m >> 16);
+    const float v = ll_to_f32(__builtin_bit_cast(T, b));
+    return v < INFINITY ? v : INFINITY;
+  } else {
+    const float v = __builtin_bit_cast(float, m);
+    return v < INFINITY ? v : INFINITY;
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t* p, int d, int D, const uint32_t (&w)[2]) {
+// The codes of 8 elements. Rounding x * (1 / s) gives the right one but where the
+// quotient is next to a border between two codes. For int8 the residual x - c s,
+// which is exact, tells: no more than s / 2 beside the border, s / 2 on it. For
+// e4m3 the product's bits below the code's last: within 4 steps of half of it
+// (the product is off by 1.5); 2^-6 added gives subnormal quotients the steps of
+// their codes. A wave with such an element takes the exact quotients.
+template <typename T, int CODE>
+__device__ __forceinline__ void codes_of(const Raw8<T>& r, float s, float inv, uint32_t& w0, uint32_t& w1) {
+  float v[8], q[8];
+  bool near;
+  if constexpr (CODE == KV8_INT8) {
+    float off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = get(r, e);
+      q[e] = __builtin_fmaf(v[e], inv, 0x1.8p23f);
+      off = fmaxf(off, fabsf(__builtin_fmaf(0x1.8p23f - q[e], s, v[e])));
+    }
+    near = !(off < 0.5f * s);
+    const auto pack = [](float a, float b, float c, float d) {
+      return __builtin_amdgcn_perm(
+          __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, d), __builtin_bit_cast(uint32_t, c), 0x0c0c0400u),
+          __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x0c0c0400u),
+          0x05040100u);
+    };
+    w0 = pack(q[0], q[1], q[2], q[3]);
+    w1 = pack(q[4], q[5], q[6], q[7]);
+  } else {
+    uint32_t gap = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = get(r, e);
+      q[e] = v[e] * inv;
+      const float z = fabsf(q[e]) < 0x1p-6f ? fabsf(q[e]) + 0x1p-6f : q[e];
+      gap = min(gap, (__builtin_bit_cast(uint32_t, z) + 0x80004u) & 0xfffffu);
+    }
+    near = gap <= 8u;
+    w0 = CodeOf<CODE>::encode4(q[0], q[1], q[2], q[3]);
+    w1 = CodeOf<CODE>::encode4(q[4], q[5], q[6], q[7]);
+  }
+  if (__ballot(near)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = quotient_to_odd(v[e], s, inv);
+    w0 = CodeOf<CODE>::encode4(q[0], q[1], q[2], q[3]);
+    w1 = CodeOf<CODE>::encode4(q[4], q[5], q[6], q[7]);
+  }
+  if (!(s < INFINITY)) w0 = w1 = 0;
+}
+
+template <typename T, int CODE, bool VEC>
+__device__ __forceinline__ void store8(uint8_t* p, int d, int D, const Raw8<T>& r, float s, float inv) {
+  uint32_t w0, w1;
+  codes_of<T, CODE>(r, s, inv, w0, w1);
   if constexpr (VEC) {
-    *(uint2*)(p + d) = make_uint2(w[0], w[1]);
+    if (d < D) *(uint2*)(p + d) = make_uint2(w0, w1);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (d + i < D) p[d + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      if (d + i < D) p[d + i] = (uint8_t)((i < 4 ? w0 : w1) >> (8 * (i & 3)));
   }
 }
 
-// One wave: the runs that start among `per` tokens, of one head's K or V.
-// A row takes as many lanes as it has groups of 8 elements, and the wave as many
-// rows at a time as fit; the run's rows are read twice, for its largest element
-// and for its codes (the second time from the cache).
+// The scale that elements of largest magnitude `top` ask for (infinite: NaN).
+template <int CODE> __device__ __forceinline__ float scale_of(float top) {
+  return top < INFINITY ? fmaxf(top / CodeOf<CODE>::top, kScaleFloor) : __builtin_nanf("");
+}
+
+// Lanes that hold a row of D elements, 8 each (a power of two).
+__device__ __forceinline__ int lanes_of(int D) {
+  int n = 1;
+  while (n * 8 < D && n < 64) n *= 2;
+  return n;
+}
+
+// Blocks of one slot: every row has a scale of its own. A row's elements stay in
+// the registers of its lanes between the maximum and the codes.
 template <typename T, int CODE, bool VEC>
+__global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs a) {
+  constexpr int kHold = 2;  // D up to 1024
+  const int lane = threadIdx.x & 63, lpr = lanes_of(a.D), units = 2 * a.KVH;
+  const int i = (blockIdx.x * kStoreWaves + (threadIdx.x >> 6)) * (64 / lpr) + lane / lpr;
+  const int t = min(i / units, (int)a.T - 1);
+  const int unit = i % units, d0 = lane % lpr * 8;
+  const int kv = unit >= a.KVH, head = unit - kv * a.KVH;
+  const int32_t slot = a.slots[t];
+  const T* x = (const T*)(kv ? a.x[1] : a.x[0]) + t * (kv ? a.x_st[1] : a.x_st[0]) +
+               head * (kv ? a.x_sh[1] : a.x_sh[0]);
+  Raw8<T> r[kHold];
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < kHold; ++k) {
+    r[k] = load8<T, VEC>(x, d0 + k * 512, a.D);
+    m = widen(m, r[k]);
+  }
+  float top = widest<T>(m);
+  for (int o = 1; o < lpr; o *= 2) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (i >= (int)a.T * units || slot < 0 || slot >= a.nslots) return;
+  const float s = scale_of<CODE>(top), inv = 1.f / s;
+  uint8_t* c = (kv ? a.c[1] : a.c[0]) + slot * (kv ? a.c_st[1] : a.c_st[0]) +
+               head * (kv ? a.c_sh[1] : a.c_sh[0]);
+#pragma unroll
+  for (int k = 0; k < kHold; ++k) store8<T, CODE, VEC>(c, d0 + k * 512, a.D, r[k], s, inv);
+  if (d0 == 0)
+    (kv ? a.s[1] : a.s[0])[slot * (kv ? a.s_sb[1] : a.s_sb[0]) + head * (kv ? a.s_sh[1] : a.s_sh[0])] = s;
+}
+
+// A team of waves: the runs that start among `per` tokens, of one head's K or V.
+// A row takes as many lanes as it has groups of 8 elements, and the team as many
+// rows at a time as fit. The first kHold such groups of rows stay in registers
+// between the run's largest element and its codes; the others are read again.
+// (Every wave of a team sees the same runs, so the barriers are for all.)
+template <typename T, int CODE, bool VEC, int TEAM>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t wave = (int64_t)blockIdx.x * kStoreWaves + (threadIdx.x >> 6);
-  const int units = 2 * a.KVH;
-  const int64_t t0 = wave / units * a.per;
-  const int unit = (int)(wave % units);
+  constexpr int kHold = 4, kWindow = 1;
+  __shared__ float s_top[2][TEAM];
+  const int lane = threadIdx.x & 63, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = (blockIdx.x * kStoreWaves + me) / TEAM, units = 2 * a.KVH, unit = team % units;
+  const int64_t t0 = (int64_t)(team / units) * a.per;
+  int turn = 0;
   if (t0 >= a.T) return;
-  const int kv = unit / a.KVH, head = unit % a.KVH;
+  const int kv = unit >= a.KVH, head = unit - kv * a.KVH;
   const T* x = (const T*)a.x[kv] + head * a.x_sh[kv];
   uint8_t* c = a.c[kv] + head * a.c_sh[kv];
   float* sc = a.s[kv] + head * a.s_sh[kv];
   const int64_t xs = a.x_st[kv], cs = a.c_st[kv];
-  const int D = a.D, groups = (D + 7) / 8;
-  int lpr = 1;  // lanes per row
-  while (lpr < groups && lpr < 64) lpr *= 2;
-  const int rows = 64 / lpr, row = lane / lpr, d0 = lane % lpr * 8;
-
+  const int D = a.D, lpr = lanes_of(D), rows = 64 / lpr * TEAM, d0 = lane % lpr * 8;
+  const int row = me % TEAM * (64 / lpr) + lane / lpr;
   const auto valid = [&](int32_t s) { return s >= 0 && s < a.nslots; };
+
   const int64_t t1 = min(t0 + (int64_t)a.per, a.T);
+  // the slots from t0 on, and of the 64 tokens before (no run starts beyond the
+  // first 64 of them)
+  int32_t sl[kWindow];
+#pragma unroll
+  for (int k = 0; k < kWindow; ++k) sl[k] = a.slots[min(t0 + k * 64 + lane, a.T - 1)];
+  const int32_t back = a.slots[max(t0 - 1 - lane, (int64_t)0)];
   bool ours = false;  // whether the next token stored begins a run (known behind the first run)
   for (int64_t t = t0; t < t1;) {
-    const int32_t first = a.slots[t];
+    const int32_t first = __builtin_amdgcn_readlane(sl[0], (int)(t - t0));
     if (!valid(first)) {
       ++t;
       continue;
     }
     const int32_t blk = first >> a.shift;
     // the run's end (the first token of another block; padded ones among the
-    // run's belong to no block) and its last token, 256 tokens at a time
+    // run's belong to no block) and its last token
     int64_t end = -1, last = t + 1;
-    for (int64_t i0 = t + 1; end < 0; i0 += 256) {
-      int32_t s[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[c] = a.slots[min(i0 + c * 64 + lane, a.T - 1)];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int64_t base = i0 + c * 64;
-        const bool in = base + lane < a.T, here = valid(s[c]) && s[c] >> a.shift == blk;
-        const uint64_t other = __ballot(!in || (valid(s[c]) && !here));
-        uint64_t same = __ballot(in && here);
-        if (end >= 0) continue;
-        const int cut = other ? __builtin_ctzll(other) : 64;
-        if (other) {
-          same &= ((uint64_t)1 << cut) - 1;
-          end = base + cut;
-        }
-        if (same) last = base + 64 - __builtin_clzll(same);
+    const auto look = [&](int32_t s, int64_t base) {
+      const bool in = base + lane < a.T, here = valid(s) && s >> a.shift == blk;
+      uint64_t other = __ballot(!in || (valid(s) && !here)), same = __ballot(in && here);
+      if (end >= 0) return;
+      if (base <= t) {  // (the tokens up to t are behind)
+        const uint64_t ahead = t - base == 63 ? 0 : ~(uint64_t)0 << (t - base + 1);
+        other &= ahead;
+        same &= ahead;
       }
-    }
+      if (other) {
+        const int cut = __builtin_ctzll(other);
+        same &= ((uint64_t)1 << cut) - 1;
+        end = base + cut;
+      }
+      if (same) last = base + 64 - __builtin_clzll(same);
+    };
+#pragma unroll
+    for (int k = 0; k < kWindow; ++k) look(sl[k], t0 + k * 64);
+    for (int64_t base = t0 + kWindow * 64; end < 0; base += 64)
+      look(a.slots[min(base + lane, a.T - 1)], base);
     if (!ours) {  // a run that began before this wave's tokens is another wave's
       bool theirs = false;
-      for (int64_t i0 = t - 1; i0 >= 0; i0 -= 64) {
-        const int64_t i = i0 - lane;
-        const int32_t s = a.slots[max(i, (int64_t)0)];
-        const bool is = i >= 0 && valid(s);
+      int32_t s = back;
+      for (int64_t base = t0 - 1; base >= 0; base -= 64) {
+        const bool is = base - lane >= 0 && valid(s);
         const uint64_t m = __ballot(is), same = __ballot(is && s >> a.shift == blk);
         if (m) {
           theirs = same >> __builtin_ctzll(m) & 1;
           break;
         }
+        if (base >= 64) s = a.slots[max(base - 64 - lane, (int64_t)0)];
       }
       ours = true;
       if (theirs) {
@@ -195,31 +344,51 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
         continue;
       }
     }
-    float top = 0.f;
-    bool bad = false;
-    for (int64_t i = t + row; i < last; i += rows)
-      for (int d = d0; d < D; d += lpr * 8) {
-        if (!valid(a.slots[i])) continue;
-        float v[8];
-        load8<T, VEC>(x + i * xs, d, D, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          bad |= !(fabsf(v[e]) < INFINITY);
-          top = fmaxf(top, fabsf(v[e]));
-        }
-      }
-    top = ll_wave_max(top);
-    float s = fmaxf(top / CodeOf<CODE>::top, kScaleFloor);
-    if (__ballot(bad)) s = __builtin_nanf("");
-    float* sp = sc + blk * a.s_sb[kv];
     const int off = first & ((1 << a.shift) - 1);
+    float* sp = sc + blk * a.s_sb[kv];
+    const float old = *sp;
+    Raw8<T> r[kHold];
+    int32_t slot[kHold];
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int64_t i = t + row + k * rows;
+      slot[k] = -1;
+      r[k] = {};
+      if (i < last) {
+        slot[k] = a.slots[i];
+        r[k] = load8<T, VEC>(x + i * xs, d0, D);
+      }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (valid(slot[k])) m = widen(m, r[k]);
+    // what is not held: more rows, and elements from 512 on
+    const auto others = [&](auto f) {
+      for (int64_t i = t + row; i < last; i += rows) {
+        const bool held = i < t + row + kHold * rows;
+        const int32_t s = a.slots[i];
+        if (!valid(s)) continue;
+        for (int d = held ? d0 + 512 : d0; d < D; d += 512) f(load8<T, VEC>(x + i * xs, d, D), s, d);
+      }
+    };
+    const bool more = last - t > kHold * rows || D > 512;
+    if (more) others([&](const Raw8<T>& v, int32_t, int) { m = widen(m, v); });
+    float top = ll_wave_max(widest<T>(m));
+    if constexpr (TEAM > 1) {
+      if (lane == 0) s_top[turn][me] = top;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < TEAM; ++k) top = fmaxf(top, s_top[turn][k]);
+      turn ^= 1;  // (the other half is read no more)
+    }
+    float s = scale_of<CODE>(top);
     if (off > 0) {
-      const float old = *sp;
       if (!(s <= old)) {  // it grew, or either is NaN (which stays)
         if (!(s > old)) s = __builtin_nanf("");
         else
           for (int j = row; j < off; j += rows)
-            for (int d = d0; d < D; d += lpr * 8) {
+            for (int d = d0; d < D; d += 512) {
               uint8_t* p = c + (((int64_t)blk << a.shift) + j) * cs + d;
               for (int e = 0; e < min(8, D - d); ++e)
                 p[e] = (uint8_t)recode<CODE>(CodeOf<CODE>::decode(p[e], 0), old, s);
@@ -228,21 +397,15 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
         s = old;
       }
     }
-    const bool ok = s < INFINITY;
-    const float r = 1.f / s;
-    for (int64_t i = t + row; i < last; i += rows)
-      for (int d = d0; d < D; d += lpr * 8) {
-        const int32_t slot = a.slots[i];
-        if (!valid(slot)) continue;
-        float v[8];
-        load8<T, VEC>(x + i * xs, d, D, v);
-        uint32_t w[2] = {0, 0};
+    const float inv = 1.f / s;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (ok) w[e >> 2] |= CodeOf<CODE>::encode(quotient_to_odd(v[e], s, r)) << (8 * (e & 3));
-        store8<VEC>(c + slot * cs, d, D, w);
-      }
-    if (lane == 0) *sp = s;
+    for (int k = 0; k < kHold; ++k)
+      if (valid(slot[k])) store8<T, CODE, VEC>(c + slot[k] * cs, d0, D, r[k], s, inv);
+    if (more)
+      others([&](const Raw8<T>& v, int32_t to, int d) {
+        store8<T, CODE, VEC>(c + to * cs, d, D, v, s, inv);
+      });
+    if (lane == 0 && me % TEAM == 0) *sp = s;
     t = end;
   }
 }
@@ -259,46 +422,68 @@ struct LoadArgs {
   int KVH, D, shift, max_len, pieces;  // pieces: of a head's row
 };
 
-constexpr int kLoadThreads = 256;
+constexpr int kLoadThreads = 256, kLoadTokens = 2;
+constexpr int kLoadFill = 4096;  // workgroups at most, the batch's requests aside
 
-// A thread takes 16 codes of a row (VEC) or one; rows of a token first, then
-// the request's next tokens.
+// A thread has one place in a token's rows, 16 codes (VEC) or one, and takes it
+// of every token that is its own, two at a time.
 template <typename T, int CODE, bool VEC>
 __global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
   const int b = blockIdx.y;
-  const int64_t row = ll_load_idx(a.req, b, a.req64);
-  const int64_t n = std::min<int64_t>(ll_load_idx(a.len, b, a.len64), a.max_len);
-  if (row < 0 || row >= a.r2t_rows) return;
+  const int64_t row = ll_load_idx(a.req, b, a.req64), len = ll_load_idx(a.len, b, a.len64);
   const int64_t base = ll_load_idx(a.start, b, a.start64);
+  if (row < 0 || row >= a.r2t_rows) return;
+  const int n = (int)min(len, (int64_t)a.max_len);
   const int32_t* table = a.r2t + row * a.r2t_s;
-  const int per = 2 * a.KVH * a.pieces;
-  const int64_t total = n * per;
-  for (int64_t i = (int64_t)blockIdx.x * kLoadThreads + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * kLoadThreads) {
-    const int64_t tok = i / per;
-    int k = (int)(i - tok * per);
-    const int64_t orow = base + tok;
-    if (orow < 0 || orow >= a.orows) continue;
-    const int piece = k % a.pieces;
-    k /= a.pieces;
-    const int head = k % a.KVH, kv = k / a.KVH;
-    const int32_t slot = table[tok];
-    const bool there = slot >= 0 && slot < a.nslots;
-    const float s = there ? a.s[kv][(slot >> a.shift) * a.s_sb[kv] + head * a.s_sh[kv]] : 0.f;
-    const uint8_t* c = a.c[kv] + (there ? slot : 0) * a.c_st[kv] + head * a.c_sh[kv];
-    T* o = (T*)a.o[kv] + orow * a.o_st[kv] + head * a.o_sh[kv];
-    if constexpr (VEC) {
-      u32x4 w = {0, 0, 0, 0};
-      if (there) w = *(const u32x4*)(c + piece * 16);
-      constexpr int kW = sizeof(T);
-      u32x4 y[kW];
-      T* e = (T*)y;
+  const int places = 2 * a.KVH * a.pieces;
+  const int here = min(places, kLoadThreads), tokens = kLoadThreads / here;  // of the workgroup
+  const int mine = threadIdx.x / here;
+  if (mine >= tokens) return;
+  const int step = gridDim.x * tokens;
+  for (int place = threadIdx.x % here; place < places; place += kLoadThreads) {
+    const int piece = place % a.pieces, kh = place / a.pieces;
+    const int kv = kh >= a.KVH, head = kh - kv * a.KVH;
+    const float* sc = (kv ? a.s[1] : a.s[0]) + head * (kv ? a.s_sh[1] : a.s_sh[0]);
+    const uint8_t* c = (kv ? a.c[1] : a.c[0]) + head * (kv ? a.c_sh[1] : a.c_sh[0]);
+    T* o = (T*)(kv ? a.o[1] : a.o[0]) + head * (kv ? a.o_sh[1] : a.o_sh[0]);
+    const int64_t ssb = kv ? a.s_sb[1] : a.s_sb[0], cst = kv ? a.c_st[1] : a.c_st[0],
+                  ost = kv ? a.o_st[1] : a.o_st[0];
+    for (int64_t t0 = blockIdx.x * tokens + mine; t0 < n; t0 += (int64_t)step * kLoadTokens) {
+      int32_t slot[kLoadTokens];
+      float s[kLoadTokens];
+      u32x4 w[kLoadTokens];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) e[j] = ll_from_f32<T>(CodeOf<CODE>::decode(w[j >> 2], j & 3) * s);
+      for (int k = 0; k < kLoadTokens; ++k) {
+        const int64_t t = t0 + (int64_t)k * step;
+        slot[k] = t < n ? table[t] : -1;
+      }
 #pragma unroll
-      for (int j = 0; j < kW; ++j) ((u32x4*)(o + piece * 16))[j] = y[j];
-    } else {
-      o[piece] = there ? ll_from_f32<T>(CodeOf<CODE>::decode(c[piece], 0) * s) : ll_from_f32<T>(0.f);
+      for (int k = 0; k < kLoadTokens; ++k) {
+        const bool is = slot[k] >= 0 && slot[k] < a.nslots;
+        s[k] = 0.f;
+        w[k] = (u32x4){0, 0, 0, 0};
+        if (is) {
+          s[k] = sc[(slot[k] >> a.shift) * ssb];
+          if constexpr (VEC) w[k] = *(const u32x4*)(c + slot[k] * cst + piece * 16);
+          else w[k][0] = c[slot[k] * cst + piece];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kLoadTokens; ++k) {
+        const int64_t t = t0 + (int64_t)k * step, to = base + t;
+        if (t >= n || to < 0 || to >= a.orows) continue;
+        if constexpr (VEC) {
+          u32x4 y[sizeof(T)];
+          T* e = (T*)y;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            e[j] = ll_from_f32<T>(CodeOf<CODE>::decode(w[k][j >> 2], j & 3) * s[k]);
+#pragma unroll
+          for (int j = 0; j < (int)sizeof(T); ++j) __builtin_nontemporal_store(y[j], (u32x4*)(o + to * ost + piece * 16) + j);
+        } else {
+          o[to * ost + piece] = ll_from_f32<T>(CodeOf<CODE>::decode(w[k][0], 0) * s[k]);
+        }
+      }
     }
   }
 }
@@ -1065,10 +1250,20 @@ extern "C" int ll_kv8_store(const void* k, int64_t k_stride_tok, int64_t k_strid
   a.s[1] = v_scale; a.s_sb[1] = vs_stride_block; a.s_sh[1] = vs_stride_h;
   a.T = ntok; a.nslots = slots_n;
   a.KVH = (int)kv_heads; a.D = (int)head_dim; a.shift = block_shift(block);
+  const int64_t units = 2 * kv_heads;
+  // Few tokens (a decode step, a run each): a wave for each, so that no run waits
+  // for another. Many: up to a block's tokens per wave, since a wave whose tokens
+  // start no run still reads their slots.
   a.per = 1;
-  const int64_t waves = (ntok + a.per - 1) / a.per * 2 * kv_heads;
-  LL_CHECK_ARG(waves <= (int64_t)INT32_MAX / 64, "%s: %lld tokens of %lld heads", fn,
-               (long long)ntok, (long long)kv_heads);
+  while (a.per < block && a.per < 64 && ntok * units / a.per >= kStoreFill) a.per *= 2;
+  int lpr = 1;
+  while (lpr * 8 < head_dim && lpr < 64) lpr *= 2;
+  // (a run of 32 rows and more takes four waves)
+  const int team = block >= kTeamBlock ? 4 : 1;
+  const int64_t waves = block == 1 ? (ntok * units + 64 / lpr - 1) / (64 / lpr)
+                                   : (ntok + a.per - 1) / a.per * units * team;
+  LL_CHECK_ARG(waves <= (int64_t)INT32_MAX / 64 && ntok * units <= INT32_MAX - 64,
+               "%s: %lld tokens of %lld heads", fn, (long long)ntok, (long long)kv_heads);
   const int es = dtype == LL_F32 ? 4 : 2;
   const bool vec = head_dim % 8 == 0 &&
                    aligned(16, {(int64_t)(uintptr_t)k, (int64_t)(uintptr_t)v, k_stride_tok * es,
@@ -1079,10 +1274,19 @@ extern "C" int ll_kv8_store(const void* k, int64_t k_stride_tok, int64_t k_strid
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return dispatch_code(code, [&](auto C) -> int {
       constexpr int CODE = decltype(C)::value;
-      if (vec)
-        hipLaunchKernelGGL((store_kernel<T, CODE, true>), grid, dim3(kStoreWaves * 64), 0, stream, a);
+      const dim3 threads(kStoreWaves * 64);
+      if (block == 1 && vec)
+        hipLaunchKernelGGL((store_rows_kernel<T, CODE, true>), grid, threads, 0, stream, a);
+      else if (block == 1)
+        hipLaunchKernelGGL((store_rows_kernel<T, CODE, false>), grid, threads, 0, stream, a);
+      else if (team == 1 && vec)
+        hipLaunchKernelGGL((store_kernel<T, CODE, true, 1>), grid, threads, 0, stream, a);
+      else if (team == 1)
+        hipLaunchKernelGGL((store_kernel<T, CODE, false, 1>), grid, threads, 0, stream, a);
+      else if (vec)
+        hipLaunchKernelGGL((store_kernel<T, CODE, true, 4>), grid, threads, 0, stream, a);
       else
-        hipLaunchKernelGGL((store_kernel<T, CODE, false>), grid, dim3(kStoreWaves * 64), 0, stream, a);
+        hipLaunchKernelGGL((store_kernel<T, CODE, false, 4>), grid, threads, 0, stream, a);
       LL_RETURN_LAUNCH();
     });
   });
@@ -1137,10 +1341,12 @@ extern "C" int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t k
                    (int64_t)(uintptr_t)v_out, ko_stride_tok * es, ko_stride_h * es,
                    vo_stride_tok * es, vo_stride_h * es});
   a.pieces = vec ? a.D / 16 : a.D;
-  const int64_t items = max_len_in_batch * 2 * kv_heads * a.pieces;
-  const int64_t most = std::max<int64_t>(1, 8192 / batch);
-  const dim3 grid((unsigned)std::min<int64_t>((items + kLoadThreads - 1) / kLoadThreads, most),
-                  (unsigned)batch);
+  const int64_t places = 2 * kv_heads * a.pieces;
+  LL_CHECK_ARG(places <= INT32_MAX, "%s: %lld heads of %lld", fn, (long long)kv_heads,
+               (long long)head_dim);
+  const int64_t tokens = std::max<int64_t>(1, kLoadThreads / places) * kLoadTokens;  // per workgroup
+  const int64_t most = std::max<int64_t>(1, kLoadFill / batch);
+  const dim3 grid((unsigned)std::min((max_len_in_batch + tokens - 1) / tokens, most), (unsigned)batch);
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return dispatch_code(code, [&](auto C) -> int {
       constexpr int CODE = decltype(C)::value;
