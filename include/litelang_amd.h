@@ -800,7 +800,8 @@ int ll_w4_pack(const uint8_t* codes, int64_t ldc, const void* scale, int64_t ld_
                void* packed, int64_t packed_bytes, hipStream_t stream);
 int ll_linear_w4(const void* x, int64_t ldx, const void* packed, int has_zero, int64_t group,
                  const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
-                 int dtype, hipStream_t stream);
+                 int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int64_t ll_linear_w4_workspace_size(int64_t M, int64_t N, int64_t K);
 
 /* ------------------------------------------------ logit controls (logits.hip)
  * out[b, v] from logits[b, v] (which out may be, with the same stride) and the
@@ -974,7 +975,8 @@ typedef struct {
 int64_t ll_call_kv8_decode_attention(const LLKv8DecodeAttentionCall* c);
 
 typedef struct {
-  int64_t x, ldx, packed, has_zero, group, bias, y, ldy, M, N, K, dtype, stream;
+  int64_t x, ldx, packed, has_zero, group, bias, y, ldy, M, N, K, dtype, workspace, workspace_bytes,
+      stream;
 } LLLinearW4Call;
 int64_t ll_call_linear_w4(const LLLinearW4Call* c);
 

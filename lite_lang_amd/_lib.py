@@ -32,7 +32,7 @@ BUILD_SLOT_MAPS_CALL = struct.Struct("=24q")
 KV8_STORE_CALL = struct.Struct("=27q")
 KV8_LOAD_CALL = struct.Struct("=37q")
 KV8_DECODE_ATTENTION_CALL = struct.Struct("=33qd4q")
-LINEAR_W4_CALL = struct.Struct("=13q")
+LINEAR_W4_CALL = struct.Struct("=15q")
 ADJUST_LOGITS_CALL = struct.Struct("=28q")
 
 # name -> (restype, argtypes), mirroring include/litelang_amd.h
@@ -151,7 +151,8 @@ SIGNATURES = {
     "ll_kv8_decode_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I64,
                                       I64, I64, I64, I32, P, I64, I64, P, I32, P, I32, P, I64, I64,
                                       I64, I64, I64, I64, I64, F32, I32, P, I64, P]),
-    "ll_linear_w4": (I32, [P, I64, P, I32, I64, P, P, I64, I64, I64, I64, I32, P]),
+    "ll_linear_w4": (I32, [P, I64, P, I32, I64, P, P, I64, I64, I64, I64, I32, P, I64, P]),
+    "ll_linear_w4_workspace_size": (I64, [I64, I64, I64]),
     "ll_adjust_logits": (I32, [P, I64, P, I64, I64, I64, P, I64, I64, I64, P, I32, P, I32, P, I32,
                                P, P, P, P, I64, P, I64, I64, P, I64, I32, P]),
     "ll_kv8_decode_attention_workspace_size": (I64, [I64] * 5),

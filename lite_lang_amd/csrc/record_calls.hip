@@ -170,10 +170,12 @@ extern "C" int64_t ll_call_kv8_decode_attention(const LLKv8DecodeAttentionCall* 
 
 extern "C" int64_t ll_call_linear_w4(const LLLinearW4Call* c) {
   LL_CHECK_ARG(c, "ll_call_linear_w4: null record");
-  return ll_linear_w4(
-      ptr<const void>(c->x), c->ldx, ptr<const void>(c->packed), (int)c->has_zero, c->group,
-      ptr<const void>(c->bias), ptr<void>(c->y), c->ldy, c->M, c->N, c->K, (int)c->dtype,
-      ptr<ihipStream_t>(c->stream));
+  const int64_t need = ll_linear_w4_workspace_size(c->M, c->N, c->K);
+  if (need > c->workspace_bytes) return need;
+  return ll_linear_w4(ptr<const void>(c->x), c->ldx, ptr<const void>(c->packed), (int)c->has_zero,
+                      c->group, ptr<const void>(c->bias), ptr<void>(c->y), c->ldy, c->M, c->N, c->K,
+                      (int)c->dtype, ptr<void>(c->workspace), c->workspace_bytes,
+                      ptr<ihipStream_t>(c->stream));
 }
 
 extern "C" int64_t ll_call_adjust_logits(const LLAdjustLogitsCall* c) {

@@ -1720,9 +1720,22 @@ def linear_w4(x, w: W4Weight, bias=None, out=None):
         assert bias.shape == (N,) and bias.dtype == dt and bias.is_contiguous()
         b_ptr, b_dev = bias.data_ptr(), bias.get_device()
     stream = _here(dev, w.data.get_device(), b_dev, out.get_device())
+    # (under capture a buffer of the call's own, as in window_decode_attention)
+    need = _linear_w4_bytes(M, N, K) if M > 16 else 0
+    ws = None
+    if need > 0:
+        if _capturing():
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        else:
+            ws = workspace(x.device, "linear_w4", need)
     rc = _L.ll_call_linear_w4(_lib.LINEAR_W4_CALL.pack(
         x.data_ptr(), xs[0], w.data.data_ptr(), w.has_zero, w.group, b_ptr, out.data_ptr(), os_[0],
-        M, N, K, _code(dt), stream))
+        M, N, K, _code(dt), 0 if ws is None else ws.data_ptr(), need, stream))
     if rc:
         _lib.check(rc, "ll_linear_w4")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_w4_bytes(M, N, K):
+    return _L.ll_linear_w4_workspace_size(M, N, K)

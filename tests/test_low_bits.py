@@ -181,7 +181,7 @@ def test_w4_entry_points_refuse_bad_arguments():
         return L.ll_w4_pack(codes, K // 2, p, 2, zero, 2, N, K, group, out, n, None)
 
     def lin(x=p, N=16, K=128, group=64, M=2, dtype=2, ldy=16, ldx=128):
-        return L.ll_linear_w4(x, ldx, p, 1, group, None, p, ldy, M, N, K, dtype, None)
+        return L.ll_linear_w4(x, ldx, p, 1, group, None, p, ldy, M, N, K, dtype, None, 0, None)
 
     assert pack(codes=None) == -1 and "null" in _err(L)
     assert lin(x=None) == -1 and "null" in _err(L)
