@@ -771,305 +771,306 @@ void decode_mfma_kernel(DecodeArgs8 a) {
     row = s_row;
   }
   while (true) {
-  const int steps = steps_of(n);
-  const int take = min(steps - step, left);
-  const bool split = step > 0 || take < steps;
-  const int t0 = step * kStep8, t1 = (int)min((int64_t)n, ((int64_t)step + take) * kStep8);
-  if (!a.whole && step == 0 && u == 0 && threadIdx.x == 0 && n > 0) {
-    // what is left of the request lies in the following workgroups, `per` in each
-    a.meta[b] = make_int2(w + b, 1 + (steps - take + per - 1) / per);
-  }
-  left = a.whole ? 0 : left - take;
-  if (n == 0) {  // (in a list the merge writes its rows)
-    if (a.whole)
-      for (int i = threadIdx.x; i < min(16, a.G - hb * 16) * D; i += kWaves8 * 64)
-        ((T*)a.out)[b * a.o_sb + (kvh * a.G + hb * 16 + i / D) * a.o_sh + i % D] = ll_from_f32<T>(0.f);
-  } else {
-  const int32_t* table = a.r2t + row * a.r2t_s;
-  // a lane's own token of the tile, and whether it looks after its K or its V
-  const int tok = lane & 31, kv = lane >> 5;
-  const float* sc = a.s[kv] + kvh * a.s_sh[kv];
-  const int64_t ssb = a.s_sb[kv], cst = a.c_st[kv];
-  const uint8_t* kc = a.c[0] + kvh * a.c_sh[0] + g * 16;
-  const uint8_t* vc = a.c[1] + kvh * a.c_sh[1] + c16 * NV;
-  constexpr int kStep = kStep8;
-  // No load below stands under a condition, so that the waits count how many
-  // came after the one they are for: a tile behind the last one fetches row 0.
-  const auto entry_of = [&](int t) -> int32_t { return table[min(t + tok, n - 1)]; };
-  // (a wave's own LDS, in order: the fences are for the compiler)
-  const auto fetch = [&](Tile8<D>& f, int t, int32_t entry) {
-    const bool is = t + tok < t1 && entry >= 0 && entry < a.nslots;
-    const int64_t s = is ? entry : 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    s_off[wave][kv][tok] = s * cst;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    f.scale = sc[(s >> a.shift) * ssb];
-    f.see = (uint32_t)__ballot(is);
-#pragma unroll
-    for (int grp = 0; grp < 2; ++grp) {
-      const uint8_t* p = kc + s_off[wave][0][grp * 16 + c16];
-#pragma unroll
-      for (int i = 0; i < NK; ++i) f.kw[grp][i] = *(const u32x4*)(p + i * 64);
+    const int steps = steps_of(n);
+    const int take = min(steps - step, left);
+    const bool split = step > 0 || take < steps;
+    const int t0 = step * kStep8, t1 = (int)min((int64_t)n, ((int64_t)step + take) * kStep8);
+    if (!a.whole && step == 0 && u == 0 && threadIdx.x == 0 && n > 0) {
+      // what is left of the request lies in the following workgroups, `per` in each
+      a.meta[b] = make_int2(w + b, 1 + (steps - take + per - 1) / per);
     }
+    left = a.whole ? 0 : left - take;
+    if (n == 0) {  // (in a list the merge writes its rows)
+      if (a.whole)
+        for (int i = threadIdx.x; i < min(16, a.G - hb * 16) * D; i += kWaves8 * 64)
+          ((T*)a.out)[b * a.o_sb + (kvh * a.G + hb * 16 + i / D) * a.o_sh + i % D] =
+              ll_from_f32<T>(0.f);
+    } else {
+      const int32_t* table = a.r2t + row * a.r2t_s;
+      // a lane's own token of the tile, and whether it looks after its K or its V
+      const int tok = lane & 31, kv = lane >> 5;
+      const float* sc = a.s[kv] + kvh * a.s_sh[kv];
+      const int64_t ssb = a.s_sb[kv], cst = a.c_st[kv];
+      const uint8_t* kc = a.c[0] + kvh * a.c_sh[0] + g * 16;
+      const uint8_t* vc = a.c[1] + kvh * a.c_sh[1] + c16 * NV;
+      constexpr int kStep = kStep8;
+      // No load below stands under a condition, so that the waits count how many
+      // came after the one they are for: a tile behind the last one fetches row 0.
+      const auto entry_of = [&](int t) -> int32_t { return table[min(t + tok, n - 1)]; };
+      // (a wave's own LDS, in order: the fences are for the compiler)
+      const auto fetch = [&](Tile8<D>& f, int t, int32_t entry) {
+        const bool is = t + tok < t1 && entry >= 0 && entry < a.nslots;
+        const int64_t s = is ? entry : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        s_off[wave][kv][tok] = s * cst;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        f.scale = sc[(s >> a.shift) * ssb];
+        f.see = (uint32_t)__ballot(is);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const VBytes v = *(const VBytes*)(vc + s_off[wave][1][(j >> 2) * 16 + g * 4 + (j & 3)]);
-      uint32_t w[NK];
-      __builtin_memcpy(w, &v, NV);
+        for (int grp = 0; grp < 2; ++grp) {
+          const uint8_t* p = kc + s_off[wave][0][grp * 16 + c16];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) f.vw[i][j] = w[i];
-    }
-  };
+          for (int i = 0; i < NK; ++i) f.kw[grp][i] = *(const u32x4*)(p + i * 64);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const VBytes v = *(const VBytes*)(vc + s_off[wave][1][(j >> 2) * 16 + g * 4 + (j & 3)]);
+          uint32_t w[NK];
+          __builtin_memcpy(w, &v, NV);
+#pragma unroll
+          for (int i = 0; i < NK; ++i) f.vw[i][j] = w[i];
+        }
+      };
 
-  int t = t0 + wave * kTile8;
-  constexpr int kStages = D <= 128 ? 2 : 1;  // tiles held
-  Tile8<D> f[kStages];
-  int32_t entry[kStages];
+      int t = t0 + wave * kTile8;
+      constexpr int kStages = D <= 128 ? 2 : 1;  // tiles held
+      Tile8<D> f[kStages];
+      int32_t entry[kStages];
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) entry[s] = entry_of(t + s * kStep);
-  u32x4 raw[NK * 2][sizeof(T) / 2];
-  {
-    const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
+      for (int s = 0; s < kStages; ++s) entry[s] = entry_of(t + s * kStep);
+      u32x4 raw[NK * 2][sizeof(T) / 2];
+      {
+        const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
 #pragma unroll
-    for (int i = 0; i < NK * 2; ++i) {
-      const int d = (i >> 1) * 64 + g * 16 + (i & 1) * 8;
-      if (a.qvec) {
+        for (int i = 0; i < NK * 2; ++i) {
+          const int d = (i >> 1) * 64 + g * 16 + (i & 1) * 8;
+          if (a.qvec) {
 #pragma unroll
-        for (int e = 0; e < (int)sizeof(T) / 2; ++e) raw[i][e] = ((const u32x4*)(q + d))[e];
-      } else {
-        __builtin_memcpy(raw[i], __builtin_assume_aligned(q + d, sizeof(T)), sizeof(raw[i]));
+            for (int e = 0; e < (int)sizeof(T) / 2; ++e) raw[i][e] = ((const u32x4*)(q + d))[e];
+          } else {
+            __builtin_memcpy(raw[i], __builtin_assume_aligned(q + d, sizeof(T)), sizeof(raw[i]));
+          }
+        }
       }
-    }
-  }
 #pragma unroll
-  for (int s = 0; s < (kStages > 1 ? kStages - 1 : 1); ++s) fetch(f[s], t + s * kStep, entry[s]);
-  int32_t next = kStages > 1 ? entry[kStages - 1] : entry_of(t + kStep);
-  bf16x8 qf[NK * 2][NQ];
-  float cq = a.scale_log2;  // of a score's sum
-  f32x4 qoff = {0.f, 0.f, 0.f, 0.f};
-  {
-    float v[NK * 2][8];
-    float top = 0.f;
+      for (int s = 0; s < (kStages > 1 ? kStages - 1 : 1); ++s) fetch(f[s], t + s * kStep, entry[s]);
+      int32_t next = kStages > 1 ? entry[kStages - 1] : entry_of(t + kStep);
+      bf16x8 qf[NK * 2][NQ];
+      float cq = a.scale_log2;  // of a score's sum
+      f32x4 qoff = {0.f, 0.f, 0.f, 0.f};
+      {
+        float v[NK * 2][8];
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < NK * 2; ++i)
+        for (int i = 0; i < NK * 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[i][e] = live ? ll_to_f32(((const T*)raw[i])[e]) : 0.f;
-        top = fmaxf(top, fabsf(v[i][e]));
-      }
-    float up = 1.f;
-    if constexpr (BIAS) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const int e = min(max(__builtin_amdgcn_frexp_expf(top), -50), 50);
-      up = __builtin_ldexpf(1.f, kUp - e);
-      cq *= __builtin_ldexpf(1.f, 133 - kUp + e);
-    }
-#pragma unroll
-    for (int i = 0; i < NK * 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] *= up;
-      split8<NQ>(v[i], qf[i]);
-    }
-  }
-  bf16x8 c128;  // 128 2^-133
-  {
-    const u32x4 w = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
-    c128 = __builtin_bit_cast(bf16x8, w);
-  }
-  if constexpr (BIAS) {
-#pragma unroll
-    for (int i = 0; i < NK * 2; ++i)
-#pragma unroll
-      for (int p = 0; p < NQ; ++p) qoff = mfma16(c128, qf[i][p], qoff);
-    qoff = -qoff;
-  }
-
-  f32x4 acc[NV] = {}, off = {0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  float up = 1.f, limit = BIAS ? -1.f : INFINITY;  // of V scales; up: their power of two
-  int down = 0;                                    // and what takes it back, 2^(73 + down)
-  const auto compute = [&](Tile8<D>& f) {
-    const float scale = f.see >> tok & 1u ? f.scale : 0.f;
-    if constexpr (BIAS) {
-      if (__ballot(kv == 1 && scale > limit)) {  // the first tile, or scales 2^40 times larger
-        const float top = ll_wave_max(kv == 1 ? scale : 0.f);
-        const int e = min(max(__builtin_amdgcn_frexp_expf(top), -60), 100);
-        const float nu = __builtin_ldexpf(1.f, kUp - e), r = nu / up;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] *= r;
-        off *= r;
-        up = nu;
-        down = e;
-        limit = __builtin_ldexpf(1.f, min(e + 40, 127));
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    s_scale[wave][kv][tok] = kv ? scale * up : scale;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    float x[8];
-#pragma unroll
-    for (int grp = 0; grp < 2; ++grp) {
-      f32x4 s = qoff;
-#pragma unroll
-      for (int i = 0; i < NK * 2; ++i) {
-        uint32_t w0 = f.kw[grp][i >> 1][2 * (i & 1)], w1 = f.kw[grp][i >> 1][2 * (i & 1) + 1];
+          for (int e = 0; e < 8; ++e) {
+          v[i][e] = live ? ll_to_f32(((const T*)raw[i])[e]) : 0.f;
+          top = fmaxf(top, fabsf(v[i][e]));
+        }
+        float up = 1.f;
         if constexpr (BIAS) {
-          w0 ^= 0x80808080u;
-          w1 ^= 0x80808080u;
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const int e = min(max(__builtin_amdgcn_frexp_expf(top), -50), 50);
+          up = __builtin_ldexpf(1.f, kUp - e);
+          cq *= __builtin_ldexpf(1.f, 133 - kUp + e);
         }
-        const bf16x8 kf = codes8<CODE, BIAS>(w0, w1);
 #pragma unroll
-        for (int p = 0; p < NQ; ++p) s = mfma16(kf, qf[i][p], s);
-      }
-      const f32x4 ks = *(const f32x4*)&s_scale[wave][0][grp * 16 + g * 4];
+        for (int i = 0; i < NK * 2; ++i) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[grp * 4 + r] = s[r] * cq * ks[r];
-    }
-    const bool part = f.see != 0xffffffffu;  // the last tile, or slots that are none
-    if (part) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool is = f.see >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1u;
-        x[j] = is ? x[j] : -INFINITY;
-        if constexpr (CODE == KV8_E4M3) {  // (what is in no token's row may be NaN)
-#pragma unroll
-          for (int i = 0; i < NK; ++i) f.vw[i][j] = is ? f.vw[i][j] : 0u;
+          for (int e = 0; e < 8; ++e) v[i][e] *= up;
+          split8<NQ>(v[i], qf[i]);
         }
       }
-    }
-    float mt = x[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) mt = fmaxf(mt, x[j]);
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    if (__ballot(mt > m)) {
-      const float mn = fmaxf(m, mt);
-      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) acc[i] *= alpha;
-      off *= alpha;
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-    float pv[8];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const f32x4 vs = *(const f32x4*)&s_scale[wave][1][half * 16 + g * 4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(x[half * 4 + r] - ms);
-        l += p;
-        pv[half * 4 + r] = p * vs[r];
+      bf16x8 c128;  // 128 2^-133
+      {
+        const u32x4 w = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
+        c128 = __builtin_bit_cast(bf16x8, w);
       }
-    }
-    bf16x8 pf[NP];
-    split8<NP>(pv, pf);
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int p = 0; p < NP; ++p) off = mfma16(c128, pf[p], off);
-    }
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
       if constexpr (BIAS) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f.vw[i][j] ^= 0x80808080u;
-      }
-      bf16x8 v0, v1, v2, v3;
-      codes_of_rows<CODE, BIAS, 0>(f.vw[i], v0, v1);
-      codes_of_rows<CODE, BIAS, 1>(f.vw[i], v2, v3);
+        for (int i = 0; i < NK * 2; ++i)
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        acc[4 * i + 0] = mfma16(v0, pf[p], acc[4 * i + 0]);
-        acc[4 * i + 1] = mfma16(v1, pf[p], acc[4 * i + 1]);
-        acc[4 * i + 2] = mfma16(v2, pf[p], acc[4 * i + 2]);
-        acc[4 * i + 3] = mfma16(v3, pf[p], acc[4 * i + 3]);
+          for (int p = 0; p < NQ; ++p) qoff = mfma16(c128, qf[i][p], qoff);
+        qoff = -qoff;
       }
-    }
-  };
 
-  while (t < t1) {
-    if constexpr (kStages > 1) {
+      f32x4 acc[NV] = {}, off = {0.f, 0.f, 0.f, 0.f};
+      float m = -INFINITY, l = 0.f;
+      float up = 1.f, limit = BIAS ? -1.f : INFINITY;  // of V scales; up: their power of two
+      int down = 0;                                    // and what takes it back, 2^(73 + down)
+      const auto compute = [&](Tile8<D>& f) {
+        const float scale = f.see >> tok & 1u ? f.scale : 0.f;
+        if constexpr (BIAS) {
+          if (__ballot(kv == 1 && scale > limit)) {  // the first tile, or scales 2^40 times larger
+            const float top = ll_wave_max(kv == 1 ? scale : 0.f);
+            const int e = min(max(__builtin_amdgcn_frexp_expf(top), -60), 100);
+            const float nu = __builtin_ldexpf(1.f, kUp - e), r = nu / up;
 #pragma unroll
-      for (int s = 0; s < kStages; ++s) {
-        fetch(f[(s + kStages - 1) % kStages], t + (kStages - 1) * kStep, next);
-        next = entry_of(t + kStages * kStep);
-        compute(f[s]);
-        t += kStep;
-        if (t >= t1) break;
+            for (int i = 0; i < NV; ++i) acc[i] *= r;
+            off *= r;
+            up = nu;
+            down = e;
+            limit = __builtin_ldexpf(1.f, min(e + 40, 127));
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        s_scale[wave][kv][tok] = kv ? scale * up : scale;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float x[8];
+#pragma unroll
+        for (int grp = 0; grp < 2; ++grp) {
+          f32x4 s = qoff;
+#pragma unroll
+          for (int i = 0; i < NK * 2; ++i) {
+            uint32_t w0 = f.kw[grp][i >> 1][2 * (i & 1)], w1 = f.kw[grp][i >> 1][2 * (i & 1) + 1];
+            if constexpr (BIAS) {
+              w0 ^= 0x80808080u;
+              w1 ^= 0x80808080u;
+            }
+            const bf16x8 kf = codes8<CODE, BIAS>(w0, w1);
+#pragma unroll
+            for (int p = 0; p < NQ; ++p) s = mfma16(kf, qf[i][p], s);
+          }
+          const f32x4 ks = *(const f32x4*)&s_scale[wave][0][grp * 16 + g * 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[grp * 4 + r] = s[r] * cq * ks[r];
+        }
+        const bool part = f.see != 0xffffffffu;  // the last tile, or slots that are none
+        if (part) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool is = f.see >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1u;
+            x[j] = is ? x[j] : -INFINITY;
+            if constexpr (CODE == KV8_E4M3) {  // (what is in no token's row may be NaN)
+#pragma unroll
+              for (int i = 0; i < NK; ++i) f.vw[i][j] = is ? f.vw[i][j] : 0u;
+            }
+          }
+        }
+        float mt = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) mt = fmaxf(mt, x[j]);
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if (__ballot(mt > m)) {
+          const float mn = fmaxf(m, mt);
+          const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+          m = mn;
+          l *= alpha;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) acc[i] *= alpha;
+          off *= alpha;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        float pv[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const f32x4 vs = *(const f32x4*)&s_scale[wave][1][half * 16 + g * 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(x[half * 4 + r] - ms);
+            l += p;
+            pv[half * 4 + r] = p * vs[r];
+          }
+        }
+        bf16x8 pf[NP];
+        split8<NP>(pv, pf);
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p) off = mfma16(c128, pf[p], off);
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          if constexpr (BIAS) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f.vw[i][j] ^= 0x80808080u;
+          }
+          bf16x8 v0, v1, v2, v3;
+          codes_of_rows<CODE, BIAS, 0>(f.vw[i], v0, v1);
+          codes_of_rows<CODE, BIAS, 1>(f.vw[i], v2, v3);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            acc[4 * i + 0] = mfma16(v0, pf[p], acc[4 * i + 0]);
+            acc[4 * i + 1] = mfma16(v1, pf[p], acc[4 * i + 1]);
+            acc[4 * i + 2] = mfma16(v2, pf[p], acc[4 * i + 2]);
+            acc[4 * i + 3] = mfma16(v3, pf[p], acc[4 * i + 3]);
+          }
+        }
+      };
+
+      while (t < t1) {
+        if constexpr (kStages > 1) {
+#pragma unroll
+          for (int s = 0; s < kStages; ++s) {
+            fetch(f[(s + kStages - 1) % kStages], t + (kStages - 1) * kStep, next);
+            next = entry_of(t + kStages * kStep);
+            compute(f[s]);
+            t += kStep;
+            if (t >= t1) break;
+          }
+        } else {
+          compute(f[0]);
+          t += kStep;
+          fetch(f[0], t, next);
+          next = entry_of(t + kStep);
+        }
       }
-    } else {
-      compute(f[0]);
-      t += kStep;
-      fetch(f[0], t, next);
-      next = entry_of(t + kStep);
+      if constexpr (BIAS) {
+        const float back = __builtin_ldexpf(1.f, 133 - kUp), back2 = __builtin_ldexpf(1.f, down);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] = (acc[i] - off) * back * back2;
+      }
+      // the waves' sums, by their common maximum
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      if (g == 0) {
+        s_m[wave][c16] = m;
+        s_l[wave][c16] = l;
+      }
+      __syncthreads();
+      float mm = s_m[0][c16], ll = 0.f;
+#pragma unroll
+      for (int w = 1; w < kWaves8; ++w) mm = fmaxf(mm, s_m[w][c16]);
+      const float mms = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+      for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - mms);
+      const float mine = __builtin_amdgcn_exp2f(m - mms);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) acc[i] *= mine;
+      if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s_acc[wave - 1][i][lane] = acc[i];
+      }
+      __syncthreads();
+      if (wave == 0 && live) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < kWaves8 - 1; ++j) acc[i] += s_acc[j][i][lane];
+        if (split) {
+          const int64_t at = (int64_t)(w + b) * a.H + h;
+          if (g == 0) a.part_ml[at] = make_float2(mm, ll);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f32x4* o = (f32x4*)(a.part + at * D + (g * 4 + r) * NV);
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+              o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r], acc[4 * i + 3][r]};
+          }
+        } else {
+          T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            T y[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] / ll);
+            T* o = out + (g * 4 + r) * NV;
+            if (a.ovec) {
+              __builtin_memcpy(__builtin_assume_aligned(o, sizeof(T) * NV < 16 ? sizeof(T) * NV : 16), y,
+                               sizeof(T) * NV);
+            } else {
+#pragma unroll
+              for (int i = 0; i < NV; ++i) o[i] = y[i];
+            }
+          }
+        }
+      }
     }
-  }
-  if constexpr (BIAS) {
-    const float back = __builtin_ldexpf(1.f, 133 - kUp), back2 = __builtin_ldexpf(1.f, down);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = (acc[i] - off) * back * back2;
-  }
-  // the waves' sums, by their common maximum
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (g == 0) {
-    s_m[wave][c16] = m;
-    s_l[wave][c16] = l;
-  }
-  __syncthreads();
-  float mm = s_m[0][c16], ll = 0.f;
-#pragma unroll
-  for (int w = 1; w < kWaves8; ++w) mm = fmaxf(mm, s_m[w][c16]);
-  const float mms = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-  for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - mms);
-  const float mine = __builtin_amdgcn_exp2f(m - mms);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) acc[i] *= mine;
-  if (wave > 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) s_acc[wave - 1][i][lane] = acc[i];
-  }
-  __syncthreads();
-  if (wave == 0 && live) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < kWaves8 - 1; ++j) acc[i] += s_acc[j][i][lane];
-  if (split) {
-    const int64_t at = (int64_t)(w + b) * a.H + h;
-    if (g == 0) a.part_ml[at] = make_float2(mm, ll);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f32x4* o = (f32x4*)(a.part + at * D + (g * 4 + r) * NV);
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-        o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r], acc[4 * i + 3][r]};
-    }
-  } else {
-  T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    T y[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] / ll);
-    T* o = out + (g * 4 + r) * NV;
-    if (a.ovec) {
-      __builtin_memcpy(__builtin_assume_aligned(o, sizeof(T) * NV < 16 ? sizeof(T) * NV : 16), y,
-                       sizeof(T) * NV);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) o[i] = y[i];
-    }
-  }
-  }
-  }
-  }
-  if (left <= 0 || ++b >= a.B) return;
-  step = 0;
-  n = decode_len(a, b, &row);
+    if (left <= 0 || ++b >= a.B) return;
+    step = 0;
+    n = decode_len(a, b, &row);
   }
 }
 

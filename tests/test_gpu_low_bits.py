@@ -387,6 +387,40 @@ def test_kv8_nan_scales_stay_in_their_head(cuda):
         assert bool(nan[0, 4:].all()) and not bool(nan[0, :4].any()) and not bool(nan[1].any())
 
 
+@pytest.mark.parametrize("B,most", [(300, 700), (700, 260), (257, 1300)])
+def test_kv8_decode_attention_of_many_requests(cuda, B, most):
+    """More requests than a workgroup has threads, empty ones among them, shares
+    that begin and end inside requests."""
+    g = np.random.RandomState(B)
+    lens = [0 if i % 7 == 3 else int(n) for i, n in enumerate(g.randint(1, most, size=B))]
+    lens[0], lens[-1], lens[5] = 0, 0, most
+    _decode_case(2, 1, 64, BF16, INT8, 16, lens, seed=B)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_kv8_decode_attention_of_scales_far_apart(cuda, code, dtype):
+    """V (and K) whose scales grow by 2^50 and fall by 2^80 along the context, and
+    queries of any size: no sum leaves fp32's range where the outputs do not."""
+    g = torch.Generator().manual_seed(9)
+    for mags in ((1e-12, 1.0, 1e4), (1e4, 1e-20, 1.0), (1e-22, 1e-22, 1e-22), (1e20, 1e20, 1e18)):
+        for qmag in (1e-6, 1.0):
+            print(f"case: scales {code} {dtype} {mags} {qmag}", flush=True)
+            n, d = 3 * 160, 64
+            c = Cache(n, 1, d, code, 16)
+            for i, m in enumerate(mags):
+                sl = list(range(160 * i, 160 * i + 160))
+                k = torch.randn(160, 1, d, generator=g) * min(m, 1.0)
+                c.store(k.to(BF16), (torch.randn(160, 1, d, generator=g) * m).to(BF16), sl)
+            q = (torch.randn(2, 4, d, generator=g) * qmag).to(dtype)
+            table = torch.arange(n, dtype=torch.int32).view(1, n)
+            out = torch.empty(2, 4, d, dtype=dtype, device="cuda")
+            _ops().kv8_decode_attention(q.cuda(), table.cuda(), _i32([0, 0]), _i32([n, 200]), n,
+                                        *c.args, out)
+            want = O.kv8_decode(q, *c.values(), table, [0, 0], [n, 200], n)
+            _inside(out, want[0], O.bound_kv8_decode(*want, dtype, d), "out")
+
+
 # ---------------------------------------------------------------- 4-bit products
 def _weight(g, N, K, group, dtype, zero):
     codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
@@ -414,6 +448,44 @@ def test_linear_w4(cuda, N, K, group, dtype, zero):
         assert r.data_ptr() == out.data_ptr() and bool((out[M] == 7.0).all())
         y, mag = O.linear_w4(x, codes, scale, z, bias)
         _inside(out[:M], y, O.bound_linear_w4(y, mag, dtype, K), "y")
+
+
+@pytest.mark.parametrize("N,K,group,dtype,zero", [(32800, 256, 128, BF16, False),
+                                                  (65553, 128, 64, F16, True),
+                                                  (65600, 160, 32, BF16, True),
+                                                  (9000, 384, 128, F16, False)])
+def test_linear_w4_of_many_outputs(cuda, N, K, group, dtype, zero):
+    """Weights wide enough for several tiles to a wave, and the plans between."""
+    g = torch.Generator().manual_seed(N)
+    codes, scale, z, w = _weight(g, N, K, group, dtype, zero)
+    for M in (1, 5, 20, 40, 64, 130):
+        print(f"case: w4 {M}x{N}x{K} group {group} {dtype} zero={zero}", flush=True)
+        x = torch.randn(M, K, generator=g).to(dtype)
+        y, mag = O.linear_w4(x, codes, scale, z)
+        _inside(_ops().linear_w4(x.cuda(), w), y, O.bound_linear_w4(y, mag, dtype, K), "y")
+
+
+def test_linear_w4_splits_are_added_in_order(cuda):
+    """Few outputs and long sums: the same bits from a workspace that held NaN and
+    from one of a captured graph, replayed beside other work."""
+    g = torch.Generator().manual_seed(11)
+    codes, scale, z, w = _weight(g, 130, 11008, 128, BF16, True)
+    for M in (17, 40, 100):
+        x = torch.randn(M, 11008, generator=g).to(BF16).cuda()
+        need = _ops()._linear_w4_bytes(M, 130, 11008)
+        assert need > M * 130 * 4
+        first = _ops().linear_w4(x, w).clone()
+        _ops().workspace(cuda, "linear_w4", need).fill_(255)
+        assert torch.equal(_ops().linear_w4(x, w), first)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = _ops().linear_w4(x, w)
+        for _ in range(3):
+            y.zero_()
+            graph.replay()
+            other = _ops().linear_w4(x * 2, w)
+            torch.cuda.synchronize()
+            assert torch.equal(y, first) and not torch.equal(other, first)
 
 
 def test_linear_w4_strides(cuda):
