@@ -35,13 +35,14 @@ template <> struct CodeOf<KV8_INT8> {
   static __device__ __forceinline__ uint32_t encode(float q) {
     return __builtin_bit_cast(uint32_t, q + 0x1.8p23f) & 0xffu;
   }
-  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-    const uint32_t w0 = __builtin_bit_cast(uint32_t, a + 0x1.8p23f);
-    const uint32_t w1 = __builtin_bit_cast(uint32_t, b + 0x1.8p23f);
-    const uint32_t w2 = __builtin_bit_cast(uint32_t, c + 0x1.8p23f);
-    const uint32_t w3 = __builtin_bit_cast(uint32_t, d + 0x1.8p23f);
+  static __device__ __forceinline__ uint32_t low4(float a, float b, float c, float d) {
+    const uint32_t w0 = __builtin_bit_cast(uint32_t, a), w1 = __builtin_bit_cast(uint32_t, b);
+    const uint32_t w2 = __builtin_bit_cast(uint32_t, c), w3 = __builtin_bit_cast(uint32_t, d);
     return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w3, w2, 0x0c0c0400u),
                                  __builtin_amdgcn_perm(w1, w0, 0x0c0c0400u), 0x05040100u);
+  }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    return low4(a + 0x1.8p23f, b + 0x1.8p23f, c + 0x1.8p23f, d + 0x1.8p23f);
   }
   // byte i of w as a number
   static __device__ __forceinline__ float decode(uint32_t w, int i) {
@@ -118,7 +119,8 @@ __device__ __forceinline__ Raw8<T> load8(const T* p, int d, int D) {
   if constexpr (VEC) {
     if (d < D)
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __builtin_nontemporal_load((const u32x4*)(p + d) + i);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        r.w[i] = __builtin_nontemporal_load((const u32x4*)(p + d) + i);
   } else {
     T* e = (T*)r.w;
 #pragma unroll
@@ -138,9 +140,9 @@ template <typename T> __device__ __forceinline__ uint32_t widen(uint32_t m, cons
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      m = __builtin_bit_cast(uint32_t,
-                             __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
-                                                       __builtin_bit_cast(u16x2, r.w[0][i] & 0x7fff7fffu)));
+      m = __builtin_bit_cast(
+          uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                              __builtin_bit_cast(u16x2, r.w[0][i] & 0x7fff7fffu)));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, r.w[i >> 2][i & 3] & 0x7fffffffu);
@@ -166,7 +168,8 @@ template <typename T> __device__ __forceinline__ float widest(uint32_t m) {
 // (the product is off by 1.5); 2^-6 added gives subnormal quotients the steps of
 // their codes. A wave with such an element takes the exact quotients.
 template <typename T, int CODE>
-__device__ __forceinline__ void codes_of(const Raw8<T>& r, float s, float inv, uint32_t& w0, uint32_t& w1) {
+__device__ __forceinline__ void codes_of(const Raw8<T>& r, float s, float inv, uint32_t& w0,
+                                         uint32_t& w1) {
   float v[8], q[8];
   bool near;
   if constexpr (CODE == KV8_INT8) {
@@ -178,14 +181,8 @@ __device__ __forceinline__ void codes_of(const Raw8<T>& r, float s, float inv, u
       off = fmaxf(off, fabsf(__builtin_fmaf(0x1.8p23f - q[e], s, v[e])));
     }
     near = !(off < 0.5f * s);
-    const auto pack = [](float a, float b, float c, float d) {
-      return __builtin_amdgcn_perm(
-          __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, d), __builtin_bit_cast(uint32_t, c), 0x0c0c0400u),
-          __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x0c0c0400u),
-          0x05040100u);
-    };
-    w0 = pack(q[0], q[1], q[2], q[3]);
-    w1 = pack(q[4], q[5], q[6], q[7]);
+    w0 = CodeOf<CODE>::low4(q[0], q[1], q[2], q[3]);
+    w1 = CodeOf<CODE>::low4(q[4], q[5], q[6], q[7]);
   } else {
     uint32_t gap = 0xffffffffu;
 #pragma unroll
@@ -209,7 +206,8 @@ __device__ __forceinline__ void codes_of(const Raw8<T>& r, float s, float inv, u
 }
 
 template <typename T, int CODE, bool VEC>
-__device__ __forceinline__ void store8(uint8_t* p, int d, int D, const Raw8<T>& r, float s, float inv) {
+__device__ __forceinline__ void store8(uint8_t* p, int d, int D, const Raw8<T>& r, float s,
+                                       float inv) {
   uint32_t w0, w1;
   codes_of<T, CODE>(r, s, inv, w0, w1);
   if constexpr (VEC) {
@@ -262,7 +260,8 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs 
 #pragma unroll
   for (int k = 0; k < kHold; ++k) store8<T, CODE, VEC>(c, d0 + k * 512, a.D, r[k], s, inv);
   if (d0 == 0)
-    (kv ? a.s[1] : a.s[0])[slot * (kv ? a.s_sb[1] : a.s_sb[0]) + head * (kv ? a.s_sh[1] : a.s_sh[0])] = s;
+    (kv ? a.s[1] : a.s[0])[slot * (kv ? a.s_sb[1] : a.s_sb[0]) +
+                           head * (kv ? a.s_sh[1] : a.s_sh[0])] = s;
 }
 
 // A team of waves: the runs that start among `per` tokens, of one head's K or V.
@@ -369,7 +368,8 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
         const bool held = i < t + row + kHold * rows;
         const int32_t s = a.slots[i];
         if (!valid(s)) continue;
-        for (int d = held ? d0 + 512 : d0; d < D; d += 512) f(load8<T, VEC>(x + i * xs, d, D), s, d);
+        for (int d = held ? d0 + 512 : d0; d < D; d += 512)
+          f(load8<T, VEC>(x + i * xs, d, D), s, d);
       }
     };
     const bool more = last - t > kHold * rows || D > 512;
@@ -479,7 +479,8 @@ __global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
           for (int j = 0; j < 16; ++j)
             e[j] = ll_from_f32<T>(CodeOf<CODE>::decode(w[k][j >> 2], j & 3) * s[k]);
 #pragma unroll
-          for (int j = 0; j < (int)sizeof(T); ++j) __builtin_nontemporal_store(y[j], (u32x4*)(o + to * ost + piece * 16) + j);
+          for (int j = 0; j < (int)sizeof(T); ++j)
+            __builtin_nontemporal_store(y[j], (u32x4*)(o + to * ost + piece * 16) + j);
         } else {
           o[to * ost + piece] = ll_from_f32<T>(CodeOf<CODE>::decode(w[k][0], 0) * s[k]);
         }
@@ -555,9 +556,8 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
         float y = acc[j] * alpha;
         for (int i = 0; i < min(64, n - t0); ++i)
           if (ss[i] >= 0)
-            y = __builtin_fmaf(sp[i],
-                               CodeOf<CODE>::decode(a.c[1][ss[i] * a.c_st[1] + kvh * a.c_sh[1] + d], 0),
-                               y);
+            y = __builtin_fmaf(
+                sp[i], CodeOf<CODE>::decode(a.c[1][ss[i] * a.c_st[1] + kvh * a.c_sh[1] + d], 0), y);
         acc[j] = y;
       }
     }
@@ -594,7 +594,8 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
 // is a few more roundings of fp32 sums (2^-24 of 128 |sum q|); fp32 calls, where
 // that would show, convert the codes instead. The maximum moves only when a tile
 // has a larger one.
-template <typename T> constexpr int kQParts = __is_same(T, float) ? 3 : __is_same(T, __bf16) ? 1 : 2;
+template <typename T>
+constexpr int kQParts = __is_same(T, float) ? 3 : __is_same(T, __bf16) ? 1 : 2;
 template <typename T> constexpr int kPParts = __is_same(T, float) ? 3 : 2;
 
 // the upper halves of two floats: their bf16 values, where those are exact
@@ -602,6 +603,11 @@ __device__ __forceinline__ uint32_t pack_exact(float lo, float hi) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo),
                                0x07060302u);
 }
+// the lower or upper two e4m3 codes of w as bf16
+template <bool HIGH> __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HIGH));
+}
+
 // 8 codes of one row (two dwords; with BIAS their bytes are c + 128)
 template <int CODE, bool BIAS> __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
   u32x4 w;
@@ -614,13 +620,14 @@ template <int CODE, bool BIAS> __device__ __forceinline__ bf16x8 codes8(uint32_t
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = i < 2 ? a : b;
-      w[i] = pack_exact(CodeOf<CODE>::decode(v, 2 * (i & 1)), CodeOf<CODE>::decode(v, 2 * (i & 1) + 1));
+      w[i] = pack_exact(CodeOf<CODE>::decode(v, 2 * (i & 1)),
+                        CodeOf<CODE>::decode(v, 2 * (i & 1) + 1));
     }
   } else {
-    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
-    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true));
-    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false));
-    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true));
+    w[0] = fp8_pair<false>(a);
+    w[1] = fp8_pair<true>(a);
+    w[2] = fp8_pair<false>(b);
+    w[3] = fp8_pair<true>(b);
   }
   return __builtin_bit_cast(bf16x8, w);
 }
@@ -641,8 +648,8 @@ __device__ __forceinline__ void codes_of_rows(const uint32_t (&v)[8], bf16x8& lo
     } else {  // the four bytes in their order, then two at a time
       const uint32_t s = __builtin_amdgcn_perm(
           b, a, (2u * I) | (4u + 2 * I) << 8 | (2u * I + 1) << 16 | (5u + 2 * I) << 24);
-      w0[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s, 1.f, false));
-      w1[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(s, 1.f, true));
+      w0[e] = fp8_pair<false>(s);
+      w1[e] = fp8_pair<true>(s);
     }
   }
   lo = __builtin_bit_cast(bf16x8, w0);
@@ -709,7 +716,8 @@ void decode_mfma_kernel(DecodeArgs8 a) {
   __shared__ f32x4 s_acc[kWaves8 - 1][NV][64];
   __shared__ int s_sum[kWaves8], s_b, s_step, s_n;
   __shared__ int64_t s_row;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
   // The heads of one share of tokens read its table, its scales' lines and, with
   // narrow heads, its rows' lines: they sit on one XCD (workgroups go to the 8
   // XCDs in turn).
@@ -843,7 +851,8 @@ void decode_mfma_kernel(DecodeArgs8 a) {
         }
       }
 #pragma unroll
-      for (int s = 0; s < (kStages > 1 ? kStages - 1 : 1); ++s) fetch(f[s], t + s * kStep, entry[s]);
+      for (int s = 0; s < (kStages > 1 ? kStages - 1 : 1); ++s)
+        fetch(f[s], t + s * kStep, entry[s]);
       int32_t next = kStages > 1 ? entry[kStages - 1] : entry_of(t + kStep);
       bf16x8 qf[NK * 2][NQ];
       float cq = a.scale_log2;  // of a score's sum
@@ -1025,7 +1034,8 @@ void decode_mfma_kernel(DecodeArgs8 a) {
       for (int w = 1; w < kWaves8; ++w) mm = fmaxf(mm, s_m[w][c16]);
       const float mms = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-      for (int w = 0; w < kWaves8; ++w) ll += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - mms);
+      for (int w = 0; w < kWaves8; ++w)
+        ll += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - mms);
       const float mine = __builtin_amdgcn_exp2f(m - mms);
 #pragma unroll
       for (int i = 0; i < NV; ++i) acc[i] *= mine;
@@ -1047,7 +1057,8 @@ void decode_mfma_kernel(DecodeArgs8 a) {
             f32x4* o = (f32x4*)(a.part + at * D + (g * 4 + r) * NV);
 #pragma unroll
             for (int i = 0; i < NK; ++i)
-              o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r], acc[4 * i + 3][r]};
+              o[i] = (f32x4){acc[4 * i][r], acc[4 * i + 1][r], acc[4 * i + 2][r],
+                             acc[4 * i + 3][r]};
           }
         } else {
           T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
@@ -1058,8 +1069,8 @@ void decode_mfma_kernel(DecodeArgs8 a) {
             for (int i = 0; i < NV; ++i) y[i] = ll_from_f32<T>(ll == 0.f ? 0.f : acc[i][r] / ll);
             T* o = out + (g * 4 + r) * NV;
             if (a.ovec) {
-              __builtin_memcpy(__builtin_assume_aligned(o, sizeof(T) * NV < 16 ? sizeof(T) * NV : 16), y,
-                               sizeof(T) * NV);
+              constexpr int kBytes = sizeof(T) * NV;
+              __builtin_memcpy(__builtin_assume_aligned(o, kBytes < 16 ? kBytes : 16), y, kBytes);
             } else {
 #pragma unroll
               for (int i = 0; i < NV; ++i) o[i] = y[i];
@@ -1175,7 +1186,8 @@ bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, i
 
 template <typename T, int CODE, int D>
 int launch_decode(const DecodeArgs8& a, unsigned grid, hipStream_t stream) {
-  hipLaunchKernelGGL((decode_mfma_kernel<T, CODE, D>), dim3(grid), dim3(kWaves8 * 64), 0, stream, a);
+  hipLaunchKernelGGL((decode_mfma_kernel<T, CODE, D>), dim3(grid), dim3(kWaves8 * 64), 0, stream,
+                     a);
   if (!a.whole) {
     // few requests have many parts each: more threads along those
     if (a.B <= 8)
@@ -1345,9 +1357,11 @@ extern "C" int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t k
   const int64_t places = 2 * kv_heads * a.pieces;
   LL_CHECK_ARG(places <= INT32_MAX, "%s: %lld heads of %lld", fn, (long long)kv_heads,
                (long long)head_dim);
-  const int64_t tokens = std::max<int64_t>(1, kLoadThreads / places) * kLoadTokens;  // per workgroup
+  // (tokens of a workgroup's turn)
+  const int64_t tokens = std::max<int64_t>(1, kLoadThreads / places) * kLoadTokens;
   const int64_t most = std::max<int64_t>(1, kLoadFill / batch);
-  const dim3 grid((unsigned)std::min((max_len_in_batch + tokens - 1) / tokens, most), (unsigned)batch);
+  const dim3 grid((unsigned)std::min((max_len_in_batch + tokens - 1) / tokens, most),
+                  (unsigned)batch);
   return LL_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return dispatch_code(code, [&](auto C) -> int {
       constexpr int CODE = decltype(C)::value;

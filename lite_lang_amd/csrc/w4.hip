@@ -42,11 +42,10 @@ PackedW4 layout_w4(int64_t N, int64_t K, int64_t group, bool zero) {
 }
 
 // One thread per dword of codes; the first ones also lay out scales and zeros.
-__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* __restrict__ codes, int64_t ldc,
-                                                      const uint16_t* __restrict__ scale, int64_t lds,
-                                                      const uint8_t* __restrict__ zero, int64_t ldz,
-                                                      int64_t N, int64_t K, int group, uint8_t* out,
-                                                      PackedW4 p) {
+__global__ __launch_bounds__(256) void w4_pack_kernel(
+    const uint8_t* __restrict__ codes, int64_t ldc, const uint16_t* __restrict__ scale, int64_t lds,
+    const uint8_t* __restrict__ zero, int64_t ldz, int64_t N, int64_t K, int group, uint8_t* out,
+    PackedW4 p) {
   const int64_t nt = (N + 15) / 16, kt = (K + kTileK - 1) / kTileK;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < nt * kt * 256) {
@@ -103,7 +102,8 @@ template <> struct W4Type<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ float add2(uint32_t x, float c) {
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, one), c, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, x), __builtin_bit_cast(V2, one),
+                                           c, false);
   }
 };
 template <> struct W4Type<_Float16> {
@@ -111,7 +111,7 @@ template <> struct W4Type<_Float16> {
   typedef _Float16 V2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t base = 0x64006400u, one = 0x3c003c00u;
   static constexpr float off(bool) { return 0.f; }
-  static constexpr bool summed(bool zero) { return zero; }  // (without zero points 8 is taken off here)
+  static constexpr bool summed(bool zero) { return zero; }  // (without, 8 is taken off in pair())
   static __device__ __forceinline__ uint32_t pair(uint32_t w, W4Bits b, bool zero) {
     const _Float16 o = zero ? (_Float16)1024.f : (_Float16)1032.f;
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(V2, (w & b.mask) | b.base) - (V2){o, o});
@@ -139,8 +139,8 @@ template <int GROUP, bool ZERO, int R> struct Stretch {
 };
 
 template <int GROUP, bool ZERO, int R>
-__device__ __forceinline__ void fetch_w(Stretch<GROUP, ZERO, R>& f, const W4Args& a, int nt0, int last, int kt,
-                                        int lane) {
+__device__ __forceinline__ void fetch_w(Stretch<GROUP, ZERO, R>& f, const W4Args& a, int nt0,
+                                        int last, int kt, int lane) {
   constexpr int kGpt = kTileK / GROUP;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -194,7 +194,8 @@ __device__ __forceinline__ void multiply(const Stretch<GROUP, ZERO, R>& f, W4Bit
         const float z = W::off(ZERO) + (ZERO ? (float)((f.z[r][gi] >> (8 * e)) & 255u) : 8.f);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const float v = W::summed(ZERO) ? __builtin_fmaf(-z, xsum[mb], part[r][mb][e]) : part[r][mb][e];
+          float v = part[r][mb][e];
+          if constexpr (W::summed(ZERO)) v = __builtin_fmaf(-z, xsum[mb], v);
           acc[r][mb][e] = __builtin_fmaf(s, v, acc[r][mb][e]);
         }
       }
@@ -209,7 +210,8 @@ template <typename T, int GROUP, typename X> __device__ __forceinline__ float su
   const u32x4 o = {W::one, W::one, W::one, W::one};
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int jj = 0; jj < GROUP / 32; ++jj) s = W::mfma(__builtin_bit_cast(V, o), x(gi * (GROUP / 32) + jj), s);
+  for (int jj = 0; jj < GROUP / 32; ++jj)
+    s = W::mfma(__builtin_bit_cast(V, o), x(gi * (GROUP / 32) + jj), s);
   return s[0];
 }
 
@@ -252,8 +254,10 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args a) {
     for (int i = 0; i < AHEAD; ++i) {
       fetch((i + AHEAD - 1) % AHEAD, kt + (AHEAD - 1) * WAVES);
       const auto x = [&](int j, int mb) { return __builtin_bit_cast(V, xv[i][j][mb]); };
-      multiply<T, GROUP, ZERO, R, MB>(
-          f[i], bits, x, [&](int gi, int mb) { return sum_of<T, GROUP>(gi, [&](int j) { return x(j, mb); }); }, acc);
+      const auto sum = [&](int gi, int mb) {
+        return sum_of<T, GROUP>(gi, [&](int j) { return x(j, mb); });
+      };
+      multiply<T, GROUP, ZERO, R, MB>(f[i], bits, x, sum, acc);
       kt += WAVES;
       if (kt >= kts) break;
     }
@@ -300,8 +304,10 @@ __global__ __launch_bounds__(kWavesW4 * 64) void w4_any_kernel(W4Args a) {
       for (int i = 0; i < 8; ++i) e[i] = xrow[k + i];
     }
     const auto x = [&](int j, int) { return __builtin_bit_cast(V, xv[j]); };
-    multiply<T, GROUP, ZERO, 1, 1>(
-        f, w4_bits<T>(), x, [&](int gi, int) { return sum_of<T, GROUP>(gi, [&](int j) { return x(j, 0); }); }, acc);
+    const auto sum = [&](int gi, int) {
+      return sum_of<T, GROUP>(gi, [&](int j) { return x(j, 0); });
+    };
+    multiply<T, GROUP, ZERO, 1, 1>(f, w4_bits<T>(), x, sum, acc);
   }
   red[wave][lane] = acc[0][0];
   __syncthreads();
@@ -324,8 +330,9 @@ __global__ __launch_bounds__(kWavesW4 * 64) void w4_any_kernel(W4Args a) {
 // row (16 lanes of 8 inputs each)
 template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {
   const auto add = [&](auto ctrl) {
-    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value,
-                                                            0xf, 0xf, true));
+    const int i = __builtin_bit_cast(int, v);
+    v += __builtin_bit_cast(
+        float, __builtin_amdgcn_mov_dpp(i, decltype(ctrl)::value, 0xf, 0xf, true));
   };
   add(std::integral_constant<int, 0xb1>());                          // lane ^ 1
   add(std::integral_constant<int, 0x4e>());                          // lane ^ 2
@@ -402,7 +409,8 @@ __global__ __launch_bounds__(kWavesW4 * 64 * KG, KG == 4 ? 4 : 2) void w4_tile_k
   Stretch<GROUP, ZERO, R> f[kDeep];
   fetch_x(k0);
 #pragma unroll
-  for (int i = 0; i < kDeep - 1; ++i) fetch_w<GROUP, ZERO, R>(f[i], a, nt0, last, within(k0 + i), lane);
+  for (int i = 0; i < kDeep - 1; ++i)
+    fetch_w<GROUP, ZERO, R>(f[i], a, nt0, last, within(k0 + i), lane);
   put_x(0);
   fetch_x(k0 + 1);
   wait();
@@ -410,14 +418,16 @@ __global__ __launch_bounds__(kWavesW4 * 64 * KG, KG == 4 ? 4 : 2) void w4_tile_k
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
       const int cur = i & 1, nxt = cur ^ 1;
-      fetch_w<GROUP, ZERO, R>(f[(i + kDeep - 1) % kDeep], a, nt0, last, within(kt + kDeep - 1), lane);
+      fetch_w<GROUP, ZERO, R>(f[(i + kDeep - 1) % kDeep], a, nt0, last, within(kt + kDeep - 1),
+                              lane);
       put_x(nxt);
       fetch_x(kt + 2);
       if (kt < k1)
         multiply<T, GROUP, ZERO, R, MB>(
             f[i], bits,
             [&](int j, int mb) {
-              return __builtin_bit_cast(V, xs[cur * kRows + (mb * 16 + c16) * 16 + ((j * 4 + g) ^ c16)]);
+              return __builtin_bit_cast(
+                  V, xs[cur * kRows + (mb * 16 + c16) * 16 + ((j * 4 + g) ^ c16)]);
             },
             [&](int gi, int mb) { return xsum[cur][gi][mb * 16 + c16]; }, acc);
       wait();
@@ -514,7 +524,7 @@ struct PlanW4 {
   int64_t bytes;     // workspace
 };
 
-constexpr int kTwoTiles = 4096;  // pairs of a weight tile and a block of x from which on a wave takes two
+constexpr int kTwoTiles = 4096;  // weight tiles times blocks of x from which on a wave takes two
 
 PlanW4 plan_w4(int64_t M, int64_t N, int64_t K) {
   PlanW4 p;
@@ -532,8 +542,10 @@ PlanW4 plan_w4(int64_t M, int64_t N, int64_t K) {
 
 template <typename T, int GROUP, bool ZERO, int R, int MB, int WAVES, int AHEAD>
 int launch_stream(const W4Args& a, hipStream_t stream) {
-  const dim3 grid((unsigned)(((a.N + 15) / 16 + R - 1) / R), (unsigned)((a.M + MB * 16 - 1) / (MB * 16)));
-  hipLaunchKernelGGL((w4_stream_kernel<T, GROUP, ZERO, R, MB, WAVES, AHEAD>), grid, dim3(WAVES * 64), 0, stream, a);
+  const dim3 grid((unsigned)(((a.N + 15) / 16 + R - 1) / R),
+                  (unsigned)((a.M + MB * 16 - 1) / (MB * 16)));
+  hipLaunchKernelGGL((w4_stream_kernel<T, GROUP, ZERO, R, MB, WAVES, AHEAD>), grid,
+                     dim3(WAVES * 64), 0, stream, a);
   LL_RETURN_LAUNCH();
 }
 
@@ -544,10 +556,12 @@ int launch_tiles(W4Args a, const PlanW4& p, hipStream_t stream) {
                   (unsigned)((a.M + MB * 16 - 1) / (MB * 16)), (unsigned)p.splits);
   a.span = p.span;
   a.splits = p.splits;
-  hipLaunchKernelGGL((w4_tile_kernel<T, GROUP, ZERO, R, MB, KG>), grid, dim3(kWavesW4 * 64 * KG), 0, stream, a);
+  hipLaunchKernelGGL((w4_tile_kernel<T, GROUP, ZERO, R, MB, KG>), grid, dim3(kWavesW4 * 64 * KG), 0,
+                     stream, a);
   if (p.splits > 1) {
     const int64_t items = a.M * ((a.N + 3) / 4);
-    hipLaunchKernelGGL((w4_finish_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((w4_finish_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0,
+                       stream, a);
   }
   LL_RETURN_LAUNCH();
 }
@@ -613,7 +627,8 @@ extern "C" int ll_w4_pack(const uint8_t* codes, int64_t ldc, const void* scale, 
 }
 
 extern "C" int64_t ll_linear_w4_workspace_size(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || M > 1 << 19 || N <= 0 || N > INT32_MAX / 16 || K <= 0 || K > INT32_MAX / 16) return 0;
+  if (M <= 0 || M > 1 << 19 || N <= 0 || N > INT32_MAX / 16 || K <= 0 || K > INT32_MAX / 16)
+    return 0;
   return plan_w4(M, N, K).bytes;
 }
 
@@ -634,7 +649,8 @@ extern "C" int ll_linear_w4(const void* x, int64_t ldx, const void* packed, int 
   const PlanW4 p = plan_w4(M, N, K);
   LL_CHECK_ARG((M + 15) / 16 <= 65535 && (N + 15) / 16 <= (1 << 22) &&
                    (p.bytes == 0 || M * ((N + 3) / 4) < (int64_t)1 << 31),
-               "%s: %lld rows of %lld outputs are more than a launch holds", fn, (long long)M, (long long)N);
+               "%s: %lld rows of %lld outputs are more than a launch holds", fn, (long long)M,
+               (long long)N);
   W4Args a = {};
   a.x = x; a.ldx = ldx;
   a.codes = (const uint8_t*)packed + l.codes;

@@ -614,6 +614,15 @@ def test_adjust_logits_counts_many(cuda):
     assert bool(torch.isneginf(y).all()) and int(_ops().argmax(y)[0]) == 0
 
 
+def test_adjust_logits_of_no_history(cuda):
+    """A table without columns counts nothing."""
+    x = torch.randn(2, 50, device="cuda")
+    none = torch.empty(3, 0, dtype=torch.int32, device="cuda")
+    y = _ops().adjust_logits(x, none, _i32([0, 1]), _i32([0, 0]), _i32([0, 0]),
+                             repetition=torch.full((2,), 2.0, device="cuda"))
+    assert torch.equal(x, y)
+
+
 def test_adjust_logits_infinities(cuda):
     """-inf stays -inf under a penalty and a bias, a mask rules NaN out."""
     inf = float("inf")
