@@ -232,7 +232,8 @@ __device__ __forceinline__ int lanes_of(int D) {
 }
 
 // Blocks of one slot: every row has a scale of its own. A row's elements stay in
-// the registers of its lanes between the maximum and the codes.
+// the registers of its lanes between the maximum and the codes. Bound by memory
+// and its one chain (row, maximum, codes): 24,000 tokens of 2 x 128 in about 15 us.
 template <typename T, int CODE, bool VEC>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs a) {
   constexpr int kHold = 2;  // D up to 1024
@@ -269,6 +270,11 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs 
 // rows at a time as fit. The first kHold such groups of rows stay in registers
 // between the run's largest element and its codes; the others are read again.
 // (Every wave of a team sees the same runs, so the barriers are for all.)
+// A run is a chain of round trips (slots, rows, codes), so what counts is how many
+// run at a time: registers for 4 groups of rows leave 28 waves per CU (8 groups: 20
+// waves, 24,000 tokens of 2 x 128 in blocks of 16 16.6 us, now 12.6: 2.9 TB/s),
+// and a run of 64 rows is quicker in four waves (blocks of 64, 8,600 new tokens of
+// 4 x 128 behind prefixes: 26 us in one wave, 18.8). Rows are read past the L2 (-2).
 template <typename T, int CODE, bool VEC, int TEAM>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
   constexpr int kHold = 4, kWindow = 1;
@@ -426,7 +432,9 @@ constexpr int kLoadThreads = 256, kLoadTokens = 2;
 constexpr int kLoadFill = 4096;  // workgroups at most, the batch's requests aside
 
 // A thread has one place in a token's rows, 16 codes (VEC) or one, and takes it
-// of every token that is its own, two at a time.
+// of every token that is its own, two at a time (four: 10.8 us for 24,000 tokens
+// of 2 x 128, two: 10.4, 3.6 TB/s). Bound by memory; the outputs are stored past
+// the L2, 2 us quicker.
 template <typename T, int CODE, bool VEC>
 __global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
   const int b = blockIdx.y;
@@ -516,7 +524,8 @@ __device__ __forceinline__ int decode_len(const DecodeArgs8& a, int b, int64_t* 
 constexpr int kAnyMaxD = 512;
 
 // Any head dim and alignment: a wave per request and query head, 64 tokens at a
-// time: a lane's own token's score, then every lane's own elements of the sum.
+// time: a lane's own token's score, then every lane's own elements of the sum. Its
+// bytes come one by one: 57 ms for 131,072 tokens of 12/2 x 128.
 template <typename T, int CODE>
 __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
   __shared__ float sq[kAnyMaxD], sp[64];
@@ -699,6 +708,12 @@ template <int D> struct Tile8 {
 // in one workgroup's share is finished there; of the others every workgroup
 // leaves its part (rows w + b of the workspace: along the list w or b grows from
 // part to part, so no two share one) to the merge.
+//
+// Bound by memory: 40 requests of up to 16,384 tokens, 16/2 x 128, 229 MB in 50 us
+// (4.6 TB/s; 70 with a fixed number of splits per request and loads under
+// conditions). Two workgroups per CU: a third spills registers (62 us). Short
+// shares are bound by their chain (length, slots, rows): one context of 131,072
+// tokens, 4 steps to a workgroup, takes 20 us for 68 MB.
 constexpr int kStep8 = kWaves8 * kTile8;
 
 __device__ __forceinline__ int steps_of(int n) { return (n + kStep8 - 1) / kStep8; }
@@ -1086,7 +1101,9 @@ void decode_mfma_kernel(DecodeArgs8 a) {
 }
 
 // The parts of a request, and the zero rows of an empty one. A workgroup has 4 L
-// elements of its heads, L threads every (256 / L)-th part.
+// elements of its heads, L threads every (256 / L)-th part, 8 parts' loads at a
+// time: a chain of round trips, 5 us (one request of 256 parts: 5.7 with L = 8, 11
+// with 64).
 template <typename T, int D, int L>
 __global__ __launch_bounds__(256) void merge_kernel(DecodeArgs8 a) {
   constexpr int kRows = 256 / L;
@@ -1175,7 +1192,12 @@ bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, i
     return false;
   p->heads = kv_heads * ((q_heads / kv_heads + 15) / 16);
   const int64_t steps = (max_len + kStep8 - 1) / kStep8;  // of a request at most
-  p->whole = steps == 1;
+  // Short contexts take a workgroup per request and head block, which needs no list,
+  // no parts and no second launch (us, so and dealt out: 40 x 600 tokens of 2 KV
+  // heads 13.1, 15.8; 1 x 300 9.3, 11.7; 100 x up to 1000 of 4 27.3, 33.1; 128 x up
+  // to 2000 of 2 18.6, 21.1), unless longer ones would leave CUs idle (8 x up to
+  // 1000 of 2: 14.1, 12.9).
+  p->whole = steps <= 6 || (steps <= 16 && batch * p->heads >= 64);
   p->W = batch;
   if (!p->whole)
     p->W = std::min(std::max(kPlaces / p->heads, batch / 4), batch * steps);

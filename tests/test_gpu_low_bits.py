@@ -351,6 +351,47 @@ def test_kv8_decode_attention_splits(cuda, B, n):
         _decode_case(H, kvh, d, dtype, code, 16, lens, seed=B, mag=3.0)
 
 
+def test_captured_kv8_decodes_share_no_workspace(cuda):
+    """Two captured decodes in parts, replayed on two streams at the same time after
+    their lengths changed, equal to eager calls."""
+    servers, graphs, streams = [], [], []
+    for seed, (H, kvh, d, dtype, code) in enumerate([(8, 2, 128, BF16, INT8), (4, 1, 64, F16, E4M3)]):
+        g = torch.Generator().manual_seed(seed)
+        c, table, rids = _filled(g, [2500, 900, 1800], kvh, d, code, 16, BF16)
+        q = torch.randn(3, H, d, generator=g).to(dtype).cuda()
+        lens, out = _i32([2500, 900, 1800]), torch.empty(3, H, d, dtype=dtype, device="cuda")
+        assert _ops()._kv8_decode_bytes(3, H, kvh, d, 2500) > 0, "a case in parts"
+        args = (q, table.cuda(), _i32(rids), lens, 2500, *c.args)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _ops().kv8_decode_attention(*args, out)
+        servers.append((args, lens, out))
+        graphs.append(graph)
+        streams.append(torch.cuda.Stream())
+    for new in ([2500, 900, 1800], [1, 0, 1700], [2049, 2, 128], [2500, 900, 1800]):
+        for _, lens, out in servers:
+            lens.copy_(_i32(new))
+            out.fill_(7.0)
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for args, _, out in servers:
+            ref = torch.empty_like(out)
+            _ops().kv8_decode_attention(*args, ref)
+            assert torch.equal(out, ref), f"lengths {new}"
+
+
+@pytest.mark.parametrize("B,most", [(1, 768), (1, 769), (70, 2000), (33, 2049)])
+def test_kv8_decode_attention_around_the_plans_border(cuda, B, most):
+    """Contexts in one workgroup and in parts, lengths below the call's bound."""
+    g = np.random.RandomState(most)
+    lens = [most] + [0 if i % 9 == 4 else int(n) for i, n in enumerate(g.randint(1, 400, size=B - 1))]
+    _decode_case(4, 1, 64, BF16, INT8, 16, lens, seed=B)
+    _decode_case(2, 1, 128, F16, E4M3, 32, lens[:3], seed=B, bound=most)
+
+
 def test_kv8_decode_attention_bounds_and_scales(cuda):
     _decode_case(8, 2, 128, BF16, INT8, 16, [500, 90, 3], bound=100)
     _decode_case(4, 2, 64, BF16, INT8, 16, [0, 0], bound=16)
@@ -394,6 +435,8 @@ def test_kv8_decode_attention_of_many_requests(cuda, B, most):
     g = np.random.RandomState(B)
     lens = [0 if i % 7 == 3 else int(n) for i, n in enumerate(g.randint(1, most, size=B))]
     lens[0], lens[-1], lens[5] = 0, 0, most
+    _decode_case(2, 1, 64, BF16, INT8, 16, lens, seed=B)
+    lens[7] = 2300  # more than a workgroup takes: in parts
     _decode_case(2, 1, 64, BF16, INT8, 16, lens, seed=B)
 
 
