@@ -646,6 +646,7 @@ extern "C" int ll_linear_w4(const void* x, int64_t ldx, const void* packed, int 
                "32, 64 or 128)", fn, (long long)N, (long long)K, (long long)group);
   LL_CHECK_ARG(M > 0 && M <= 1 << 19, "%s: %lld rows (max 2^19)", fn, (long long)M);
   LL_CHECK_ARG(dtype == LL_BF16 || dtype == LL_F16, "%s: bf16 and fp16 only", fn);
+  LL_CHECK_ARG((uintptr_t)packed % 16 == 0, "%s: the packed weight is not 16 B aligned", fn);
   LL_CHECK_ARG(ldx >= 0 && (ldy >= N || M == 1), "%s: row strides %lld, %lld", fn, (long long)ldx,
                (long long)ldy);
   const PackedW4 l = layout_w4(N, K, group, has_zero != 0);

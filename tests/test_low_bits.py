@@ -158,6 +158,9 @@ def test_kv8_entry_points_refuse_bad_arguments():
         assert _decode(L, scale=scale) == -1 and "sm_scale" in _err(L)
     for kw in ({"ob": 0}, {"oh": 0}):
         assert _decode(L, **kw) == -1 and "stride 0" in _err(L)
+    assert _decode(L, most=4096) == -1 and "workspace needs" in _err(L)
+    assert _decode(L, most=4096, ws=256, wsn=64) == -1 and "workspace needs" in _err(L)
+    assert _decode(L, most=4096, ws=264, wsn=1 << 30) == -1 and "aligned" in _err(L)
     for B, H, KVH in ((1 << 24, 256, 256), (1 << 24, 16, 2), (1 << 24, 65535, 1)):
         for D in (64, 80, 128):
             assert _decode(L, B=B, H=H, KVH=KVH, D=D, most=1 << 30) == -1, _err(L)
@@ -180,8 +183,8 @@ def test_w4_entry_points_refuse_bad_arguments():
     def pack(codes=p, N=16, K=128, group=64, n=1 << 20, out=p, zero=p):
         return L.ll_w4_pack(codes, K // 2, p, 2, zero, 2, N, K, group, out, n, None)
 
-    def lin(x=p, N=16, K=128, group=64, M=2, dtype=2, ldy=16, ldx=128):
-        return L.ll_linear_w4(x, ldx, p, 1, group, None, p, ldy, M, N, K, dtype, None, 0, None)
+    def lin(x=p, N=16, K=128, group=64, M=2, dtype=2, ldy=16, ldx=128, w=p):
+        return L.ll_linear_w4(x, ldx, w, 1, group, None, p, ldy, M, N, K, dtype, None, 0, None)
 
     assert pack(codes=None) == -1 and "null" in _err(L)
     assert lin(x=None) == -1 and "null" in _err(L)
@@ -198,6 +201,9 @@ def test_w4_entry_points_refuse_bad_arguments():
     assert pack(N=1 << 26, K=1 << 26, n=1 << 60) == -1 and "too large" in _err(L)
     assert lin(M=0) == 0 and lin(M=-1) == -1 and lin(M=(1 << 19) + 1) == -1
     assert lin(dtype=0) == -1 and "bf16" in _err(L)
+    assert lin(w=264) == -1 and "aligned" in _err(L)
+    long = {"N": 32, "K": 11008, "M": 40, "ldx": 11008, "ldy": 32, "group": 128}
+    assert lin(**long) == -1 and "workspace needs" in _err(L)
     assert lin(ldy=15) == -1 and "strides" in _err(L)
     assert lin(ldx=-8) == -1 and "strides" in _err(L)
 
