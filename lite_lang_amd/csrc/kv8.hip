@@ -1199,8 +1199,8 @@ bool plan8(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, i
   // 1000 of 2: 14.1, 12.9).
   p->whole = steps <= 6 || (steps <= 16 && batch * p->heads >= 64);
   p->W = batch;
-  if (!p->whole)
-    p->W = std::min(std::max(kPlaces / p->heads, batch / 4), batch * steps);
+  if (!p->whole)  // (at least one, where the head blocks alone are more than the places)
+    p->W = std::min(std::max<int64_t>({kPlaces / p->heads, batch / 4, 1}), batch * steps);
   p->bytes = p->whole ? 0 : (p->W + batch) * q_heads * (head_dim * 4 + 8) + batch * 8;
   return (p->W + 7) / 8 * 8 * p->heads <= kMaxGrid8 && batch * steps <= INT32_MAX &&
          batch * ((q_heads * head_dim + 255) / 256) <= kMaxGrid8;
@@ -1210,7 +1210,8 @@ template <typename T, int CODE, int D>
 int launch_decode(const DecodeArgs8& a, unsigned grid, hipStream_t stream) {
   hipLaunchKernelGGL((decode_mfma_kernel<T, CODE, D>), dim3(grid), dim3(kWaves8 * 64), 0, stream,
                      a);
-  if (!a.whole) {
+  // (no merge of what a launch that failed has not written)
+  if (!a.whole && hipPeekAtLastError() == hipSuccess) {
     // few requests have many parts each: more threads along those
     if (a.B <= 8)
       hipLaunchKernelGGL((merge_kernel<T, D, 8>), dim3((unsigned)(a.B * ((a.H * D + 31) / 32))),

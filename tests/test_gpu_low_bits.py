@@ -392,6 +392,50 @@ def test_kv8_decode_attention_around_the_plans_border(cuda, B, most):
     _decode_case(2, 1, 128, F16, E4M3, 32, lens[:3], seed=B, bound=most)
 
 
+@pytest.mark.parametrize("B,H,kvh", [(1, 520, 520), (3, 513, 513), (2, 8200, 1)])
+def test_kv8_decode_attention_of_more_head_blocks_than_places(cuda, B, H, kvh):
+    """More head blocks than workgroups run at a time: one workgroup to each. Some
+    heads against the oracle, the others against calls of those heads alone."""
+    d, n = 64, 2100
+    print(f"case: {B} requests of {H}/{kvh} heads", flush=True)
+    need = _ops()._kv8_decode_bytes(B, H, kvh, d, n)
+    assert need == (1 + B) * H * (d * 4 + 8) + B * 8, "one workgroup to a head block"
+    _ops().workspace(cuda, "kv8_decode", need).fill_(255)
+    g = torch.Generator().manual_seed(B)
+    lens = [n, 1, 700][:B]
+    pool = torch.randint(-127, 128, (n, 2 * kvh, d), generator=g, dtype=torch.int8)
+    scale = torch.rand(-(-n // 16), 2 * kvh, generator=g) * 0.01 + 0.001
+    q = torch.randn(B, H, d, generator=g).to(BF16)
+    table = torch.stack([torch.randperm(n, generator=g) for _ in range(B)]).int()
+    pd, sd, qd, td, rows, ln = pool.cuda(), scale.cuda(), q.cuda(), table.cuda(), _i32(range(B)), _i32(lens)
+    out = torch.full_like(qd, 7.0)
+    _ops().kv8_decode_attention(qd, td, rows, ln, n, pd[:, :kvh], pd[:, kvh:], sd[:, :kvh],
+                                sd[:, kvh:], 16, out)
+    torch.cuda.synchronize()
+    G = H // kvh
+    few = [0, kvh // 2, kvh - 1] if kvh > 1 else [0]
+    for kh in few:
+        heads = list(range(kh * G, kh * G + min(G, 16)))
+        vals = O.kv8_values(pool.double(), scale.double(), 16)
+        want = O.kv8_decode(q[:, heads], vals[:, [kh]], vals[:, [kvh + kh]], table, range(B), lens, n)
+        _inside(out[:, heads], want[0], O.bound_kv8_decode(*want, BF16, d), f"head {kh}")
+    # 64 KV heads (or 1,024 query heads) at a time, dealt out over more workgroups.
+    # Each output is off by half a bf16 step; the sums before it by 2^-16 of the
+    # values' mean magnitude (0.35) each, and fp32's roundings.
+    step = 64 if kvh > 1 else 1
+    for k0 in range(0, kvh, step):
+        k1, h0, h1 = min(k0 + step, kvh), k0 * G, min(k0 + step, kvh) * G
+        for a in range(h0, h1, 1024 if kvh == 1 else h1):
+            b = min(a + 1024, h1) if kvh == 1 else h1
+            ref = torch.empty(B, b - a, d, dtype=BF16, device="cuda")
+            _ops().kv8_decode_attention(qd[:, a:b], td, rows, ln, n, pd[:, k0:k1],
+                                        pd[:, kvh + k0:kvh + k1], sd[:, k0:k1],
+                                        sd[:, kvh + k0:kvh + k1], 16, ref)
+            off = (out[:, a:b].float() - ref.float()).abs()
+            top = torch.maximum(out[:, a:b].float().abs(), ref.float().abs())
+            assert bool((off <= 2.0 ** -7 * top + 2e-5).all()), (a, float(off.max()))
+
+
 def test_kv8_decode_attention_bounds_and_scales(cuda):
     _decode_case(8, 2, 128, BF16, INT8, 16, [500, 90, 3], bound=100)
     _decode_case(4, 2, 64, BF16, INT8, 16, [0, 0], bound=16)

@@ -176,6 +176,22 @@ def test_kv8_workspace_query_takes_any_counts():
         assert fn(*a) == 0, a
 
 
+def test_kv8_workspace_holds_a_part_of_every_workgroup():
+    """Head blocks below and above the 512 workgroups that run at a time: each has
+    one at least, so that W + batch parts of W >= 1 fit (fp32 sums, a maximum and a
+    sum for each query head, two words for each request)."""
+    from lite_lang_amd import _lib
+    fn = _lib.load().ll_kv8_decode_attention_workspace_size
+    for D in (64, 128, 256):
+        for B in (1, 2, 3, 4, 5, 9):
+            for H, KVH in ((511, 511), (512, 512), (513, 513), (520, 520), (1024, 1024), (8192, 1),
+                           (8200, 1), (16400, 2), (65535, 65535), (65535, 1)):
+                for most in (2049, 4096, 1 << 20):
+                    need = fn(B, H, KVH, D, most)
+                    w = max(512 // (KVH * -(-H // KVH // 16)), B // 4, 1)
+                    assert need == (w + B) * H * (D * 4 + 8) + B * 8, (B, H, KVH, D, most)
+
+
 def test_w4_entry_points_refuse_bad_arguments():
     from lite_lang_amd import _lib
     L, p = _lib.load(), 256
