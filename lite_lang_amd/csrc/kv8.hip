@@ -441,7 +441,7 @@ __global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
   const int64_t row = ll_load_idx(a.req, b, a.req64), len = ll_load_idx(a.len, b, a.len64);
   const int64_t base = ll_load_idx(a.start, b, a.start64);
   if (row < 0 || row >= a.r2t_rows) return;
-  const int n = (int)min(len, (int64_t)a.max_len);
+  const int n = (int)min(max(len, (int64_t)0), (int64_t)a.max_len);
   const int32_t* table = a.r2t + row * a.r2t_s;
   const int places = 2 * a.KVH * a.pieces;
   const int here = min(places, kLoadThreads), tokens = kLoadThreads / here;  // of the workgroup

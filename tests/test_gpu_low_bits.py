@@ -292,6 +292,26 @@ def test_kv8_load_bounds_and_strides(cuda):
         assert bool((wide[:, 0] == 7.0).all()) and bool((wide[..., d:] == 7.0).all())
 
 
+def test_kv8_lengths_below_zero(cuda):
+    """Lengths below 0 are of empty requests, in 64 bits too: those whose low 32
+    bits are a small, and the largest, positive number."""
+    g = torch.Generator().manual_seed(5)
+    c, table, rids = _filled(g, [20, 30], 2, 64, INT8, 8, BF16)
+    rids = rids[:1] * 5 + rids[1:]
+    lens = [-1, -2 ** 31, -2 ** 33 + 5, -2 ** 32 + 2 ** 31 - 1, -2 ** 63, 30]
+    i64 = lambda v: _i32(v, dtype=torch.int64)  # noqa: E731
+    out = [torch.full((40, 2, 64), 7.0, dtype=BF16, device="cuda") for _ in range(2)]
+    _ops().kv8_load(*c.args, table.cuda(), i64(rids), i64([0, 1, 2, 3, 4, 5]), i64(lens), 30, *out)
+    for got, val in zip(out, c.values()):
+        want = torch.full((40, 2, 64), 7.0, dtype=torch.float64)
+        want[5:35] = val[table[rids[5], :30].long()]
+        _inside(got, want, O.bound_value(want, BF16), "values")
+    q = torch.randn(6, 4, 64, generator=g).to(BF16).cuda()
+    o = torch.full_like(q, 7.0)
+    _ops().kv8_decode_attention(q, table.cuda(), i64(rids), i64(lens), 30, *c.args, o)
+    assert bool((o[:5] == 0).all()) and bool((o[5] != 0).any())
+
+
 # ---------------------------------------------------------------- attention
 ATT = [(16, 2, 128, BF16, INT8, 16), (12, 2, 128, BF16, E4M3, 64), (28, 4, 128, F16, INT8, 1),
        (32, 8, 64, F16, E4M3, 16), (8, 2, 64, BF16, INT8, 32), (4, 4, 128, F32, INT8, 16),
