@@ -118,19 +118,48 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs a) {
   }
   if (nb > 0) {
     __syncthreads();
-    for (int i = tid; i < nb; i += THREADS) {
-      const int32_t id = ids[i];
-      const uint32_t at = (uint32_t)id - (uint32_t)v0;
-      if (at >= (uint32_t)n) continue;
-      float s = vals[i];
-      if (twice) {  // a token with several: its first entry's thread adds them up
-        bool first = true;
-        for (int j = 0; j < i; ++j) first &= ids[j] != id;
-        if (!first) continue;
-        for (int j = i + 1; j < nb; ++j)
-          if (ids[j] == id) s = s + vals[j];
+    if (!twice) {
+      for (int i = tid; i < nb; i += THREADS) {
+        const uint32_t at = (uint32_t)ids[i] - (uint32_t)v0;
+        if (at < (uint32_t)n) bias[at] = vals[i];
       }
-      bias[at] = s;
+    } else {
+      // Tokens with several: a wave goes through the list in its order and adds up
+      // those of its 64 kEach tokens, so that the time grows with the list alone
+      // (2^20 entries for 151,936 tokens: 3.0 ms, all of them for one: 38; 300 for
+      // 50 tokens: 26 us).
+      const int lane = tid & 63, first = (tid >> 6) * (64 * kEach);
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) bias[first + k * 64 + lane] = -0.f;  // (-0 + v is v)
+      constexpr int kAhead = 4;
+      for (int i0 = 0; i0 < nb; i0 += kAhead * 64) {
+        uint32_t at[kAhead];
+        float v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = min(i0 + k * 64 + lane, nb - 1);
+          at[k] = (uint32_t)ids[i] - (uint32_t)v0;
+          v[k] = vals[i];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          uint64_t todo = __ballot(i0 + k * 64 + lane < nb && at[k] < (uint32_t)n &&
+                                   at[k] - (uint32_t)first < 64u * kEach);
+          while (todo) {
+            const int one = __builtin_amdgcn_readlane((int)at[k], __builtin_ctzll(todo));
+            uint64_t same = __ballot(at[k] == (uint32_t)one) & todo;
+            todo &= ~same;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            float s = bias[one];
+            for (; same; same &= same - 1)
+              s = s + __builtin_bit_cast(
+                          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v[k]),
+                                                           __builtin_ctzll(same)));
+            if (lane == 0) bias[one] = s;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
+      }
     }
   }
   __syncthreads();

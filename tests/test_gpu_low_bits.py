@@ -730,6 +730,34 @@ def test_adjust_logits_of_no_history(cuda):
     assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("V,nb,kind", [(151936, 1 << 20, "random"), (5000, 1 << 20, "one"),
+                                       (3000, 1000, "random"), (3000, 257, "two"),
+                                       (70000, 40000, "random"), (2048, 64, "one")])
+def test_adjust_logits_many_biases_of_a_token(cuda, V, nb, kind):
+    """Lists that name tokens again and again, up to the longest: each token's sum
+    is added up in the list's order, bit for bit."""
+    print(f"case: {nb} biases ({kind}) of {V} tokens", flush=True)
+    g = np.random.RandomState(nb % 1000)
+    B = 2
+    ids = {"random": g.randint(-3, V + 3, size=(B, nb)), "one": np.full((B, nb), V - 1),
+           "two": g.randint(0, 2, size=(B, nb)) * (V - 1)}[kind].astype(np.int32)
+    vals = (g.randn(B, nb) * 10.0 ** g.randint(-3, 4, size=(B, nb))).astype(np.float32)
+    x = g.randn(B, V).astype(np.float32)
+    want = x.copy()
+    for b in range(B):
+        total = np.full(V, -0.0, np.float32)
+        ok = (ids[b] >= 0) & (ids[b] < V)
+        np.add.at(total, ids[b][ok], vals[b][ok])  # entry after entry, each addition rounded
+        hit = np.zeros(V, bool)
+        hit[ids[b][ok]] = True
+        want[b] = np.where(hit, x[b] + total, x[b])
+    for pieces in (1, 2):  # rows of biases next to each other, and apart
+        di = torch.from_numpy(np.tile(ids, (1, pieces))).cuda()[:, :nb]
+        dv = torch.from_numpy(np.tile(vals, (1, pieces))).cuda()[:, :nb]
+        y = _ops().adjust_logits(torch.from_numpy(x).cuda(), bias_ids=di, bias_values=dv)
+        assert torch.equal(y.cpu(), torch.from_numpy(want)), f"rows of {pieces}"
+
+
 def test_adjust_logits_infinities(cuda):
     """-inf stays -inf under a penalty and a bias, a mask rules NaN out."""
     inf = float("inf")
