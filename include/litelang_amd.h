@@ -811,7 +811,8 @@ int64_t ll_linear_w4_workspace_size(int64_t M, int64_t N, int64_t K);
  *   x / repetition[b] (x > 0) or x * repetition[b], where v is in either;
  *   x - frequency[b] * (count of v in the answer);
  *   x - presence[b] where v is in the answer;
- *   x + every bias_values[b, i] with bias_ids[b, i] == v, added up in order;
+ *   x + the sum of the bias_values[b, i] with bias_ids[b, i] == v (in fp32, in
+ *   their order, before x is added);
  *   -inf where bit v % 32 of mask[b, v / 32] is 0.
  * Any of repetition, frequency, presence, the biases (n_bias 0) and the mask may
  * be null; without penalties tokens too. Ids outside [0, vocab) and rows outside

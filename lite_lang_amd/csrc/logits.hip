@@ -6,7 +6,7 @@
 //   count: how often v is among tokens[prompt_len .. seq_len)   (the answer)
 //   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
 //   x = x - frequency * count - (count > 0 ? presence : 0)
-//   x = x + the biases of v, in their order
+//   x = x + w, w the sum of the biases of v, added up in their order
 //   x = -inf where the mask's bit v is 0
 // in fp32, each operation rounded, and one rounding to the logits' type.
 //

@@ -916,9 +916,9 @@ def adjust_logits(logits, tokens=None, b_req_idx=None, b_prompt_len=None, b_seq_
       positive, multiplied else;
     * frequency [B]: times the token's count in the answer, subtracted;
     * presence [B]: subtracted from the answer's tokens;
-    * bias_values [B, n] fp32, added to the tokens bias_ids [B, n] int32 (a token
-      with several gets their sum; ids outside the vocabulary, such as -1, are
-      unused);
+    * bias_values [B, n] fp32, added to the tokens bias_ids [B, n] int32 (several of
+      a token are summed in their order, and the sum is added once; ids outside the
+      vocabulary, such as -1, are unused);
     * mask [B, at least V / 32] int32: tokens whose bit v % 32 of word v / 32 is 0
       become -inf (a row of zeros leaves none; argmax then gives token 0).
 

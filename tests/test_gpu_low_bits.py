@@ -758,6 +758,17 @@ def test_adjust_logits_many_biases_of_a_token(cuda, V, nb, kind):
         assert torch.equal(y.cpu(), torch.from_numpy(want)), f"rows of {pieces}"
 
 
+def test_adjust_logits_sums_biases_first(cuda):
+    """Two biases of 4 on 1e8, whose neighbours are 8 apart: their sum is added, not
+    one after the other (which would leave 1e8)."""
+    x = torch.full((1, 70), 1e8, device="cuda")
+    y = _ops().adjust_logits(x, bias_ids=_i32([[3, 5, 3, -1]]),
+                             bias_values=torch.tensor([[4.0, 4.0, 4.0, 9.0]], device="cuda"))
+    want = torch.full((1, 70), 1e8)
+    want[0, 3] = 1e8 + 8
+    assert torch.equal(y.cpu(), want)
+
+
 def test_adjust_logits_infinities(cuda):
     """-inf stays -inf under a penalty and a bias, a mask rules NaN out."""
     inf = float("inf")
