@@ -934,9 +934,9 @@ def adjust_logits(logits, tokens=None, b_req_idx=None, b_prompt_len=None, b_seq_
     devs = [out.get_device()]
     f32, i32 = torch.float32, torch.int32
     tok, pen = [0] * 10, [0, 0, 0]
-    if tokens is not None and tokens.shape[1] > 0:  # (no column: nothing to count)
+    if tokens is not None:
         (rows, cols), ts = tokens.shape, tokens.stride()
-        assert tokens.dtype == i32 and ts[1] == 1
+        assert tokens.dtype == i32 and (cols < 2 or ts[1] == 1)
         tok = [tokens.data_ptr(), ts[0], rows, cols]
         devs.append(tokens.get_device())
         for t, name in ((b_req_idx, "b_req_idx"), (b_prompt_len, "b_prompt_len"),
@@ -949,7 +949,9 @@ def adjust_logits(logits, tokens=None, b_req_idx=None, b_prompt_len=None, b_seq_
                 assert t.shape == (B,) and t.dtype == f32 and t.is_contiguous()
                 pen[i] = t.data_ptr()
                 devs.append(t.get_device())
-    elif tokens is None and not (repetition is None and frequency is None and presence is None):
+        if rows == 0 or cols == 0:  # nothing to count, and no address
+            tok, pen = [0] * 10, [0, 0, 0]
+    elif not (repetition is None and frequency is None and presence is None):
         raise ValueError("repetition, frequency and presence penalties need the tokens")
     bias = [0] * 5
     if bias_ids is not None:

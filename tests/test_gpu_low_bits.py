@@ -769,6 +769,22 @@ def test_adjust_logits_sums_biases_first(cuda):
     assert torch.equal(y.cpu(), want)
 
 
+def test_adjust_logits_of_an_empty_table(cuda):
+    """Tables of no row or no column count nothing, other controls go on."""
+    x = torch.randn(2, 50, device="cuda")
+    two, bias = torch.full((2,), 2.0, device="cuda"), torch.ones(2, 1, device="cuda")
+    for rows, cols in ((3, 0), (0, 5), (0, 0)):
+        t = torch.empty(rows, cols, dtype=torch.int32, device="cuda")
+        y = _ops().adjust_logits(x, t, _i32([0, 1]), _i32([0, 0]), _i32([3, 3]), repetition=two,
+                                 frequency=two, presence=two, bias_ids=_i32([[7], [-1]]),
+                                 bias_values=bias)
+        want = x.clone()
+        want[0, 7] += 1.0
+        assert torch.equal(y, want)
+        with pytest.raises(ValueError, match="CPU"):
+            _ops().adjust_logits(x, t, _i32([0, 1]), _i32([0, 0]), _i32([3, 3]), repetition=two.cpu())
+
+
 def test_adjust_logits_infinities(cuda):
     """-inf stays -inf under a penalty and a bias, a mask rules NaN out."""
     inf = float("inf")

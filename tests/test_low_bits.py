@@ -317,3 +317,22 @@ def test_python_w4_and_logits_refuse_bad_arguments():
                   ((), {"out": x[:1]}), ((), {"out": x.half()})):
         with pytest.raises(AssertionError):
             ops.adjust_logits(x, *a, **kw)
+
+
+def test_a_history_of_no_columns_is_checked_like_any_other():
+    """The arguments that a table of five columns would have refused, with none."""
+    ops = _ops()
+    x = torch.zeros(2, 9)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    for cols in (0, 5):
+        hist = (i(4, cols), i(2), i(2), i(2))
+        with pytest.raises(ValueError, match="CPU"):
+            ops.adjust_logits(x, *hist, repetition=torch.ones(2))
+        with pytest.raises(TypeError, match="int32 or int64"):
+            ops.adjust_logits(x, hist[0], i(2).float(), i(2), i(2))
+        for a, kw in ((hist[:1], {}), (hist[:3], {}), ((hist[0], i(3), i(2), i(2)), {}),
+                      ((hist[0].long(), *hist[1:]), {}), ((hist[0].float(), *hist[1:]), {}),
+                      (hist, {"repetition": torch.ones(3)}), (hist, {"frequency": torch.ones(2, 1)}),
+                      (hist, {"presence": torch.ones(2).half()})):
+            with pytest.raises(AssertionError):
+                ops.adjust_logits(x, *a, **kw)
