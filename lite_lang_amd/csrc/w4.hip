@@ -7,9 +7,9 @@
 // tile is 16 rows of 128 inputs, 1 KB, in which lane l holds 16 bytes: row
 // l % 16, and in dword j the inputs 32 j + 8 (l / 16) + 0 .. 7. Nibble i of a
 // dword is input 2 i and nibble i + 4 input 2 i + 1, so that a shift, an `and`
-// and an `or` make two 16-bit floats at once: 0x4300 | c is 128 + c in bf16,
-// 0x6400 | c is 1024 + c in fp16. For bf16 the 128 stays in and leaves with the
-// zero point: a group's sum is
+// and an `or` make two 16-bit floats at once: 128 + c (times a power of two) in
+// bf16, 0x6400 | c, 1024 + c, in fp16. For bf16 the 128 stays in and leaves with
+// the zero point: a group's sum is
 //   sum x (128 + c) - (128 + z) sum x,
 // the second sum taken by the same instruction from a tile of ones (it loses
 // 128 / 15 times fp32's rounding, 2^-20 of the result's terms). In fp16 1024 is
@@ -91,9 +91,15 @@ template <typename T> struct W4Type;
 template <> struct W4Type<__bf16> {
   typedef bf16x8 V;
   typedef __bf16 V2 __attribute__((ext_vector_type(2)));
-  static constexpr uint32_t base = 0x43004300u, one = 0x3f803f80u;
-  // what a converted code is more than the weight, of zero point z
-  static constexpr float off(bool) { return 128.f; }
+  // 128 + c and the ones of the sums of x are held small by powers of two, so that
+  // no sum passes fp32's range where the result does not: 0x3b00 | c is 2^-16 (128 +
+  // c), and the sums are 2^-8 of themselves.
+  static constexpr uint32_t base = 0x3b003b00u, one = 0x3b803b80u;
+  static constexpr float back = 0x1p16f;  // an accumulator is the result by 1 / back
+  // what a converted code is more than the weight, of zero point z, by 2^-8
+  static __device__ __forceinline__ float off(float z) {
+    return __builtin_fmaf(z, 0x1p-8f, 0.5f);
+  }
   static constexpr bool summed(bool) { return true; }  // whether it takes sums of x
   static __device__ __forceinline__ uint32_t pair(uint32_t w, W4Bits b, bool) {
     return (w & b.mask) | b.base;
@@ -110,7 +116,8 @@ template <> struct W4Type<_Float16> {
   typedef f16x8 V;
   typedef _Float16 V2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t base = 0x64006400u, one = 0x3c003c00u;
-  static constexpr float off(bool) { return 0.f; }
+  static constexpr float back = 1.f;
+  static __device__ __forceinline__ float off(float z) { return z; }
   static constexpr bool summed(bool zero) { return zero; }  // (without, 8 is taken off in pair())
   static __device__ __forceinline__ uint32_t pair(uint32_t w, W4Bits b, bool zero) {
     const _Float16 o = zero ? (_Float16)1024.f : (_Float16)1032.f;
@@ -191,7 +198,7 @@ __device__ __forceinline__ void multiply(const Stretch<GROUP, ZERO, R>& f, W4Bit
       for (int e = 0; e < 4; ++e) {
         const uint16_t sb = (uint16_t)((e < 2 ? f.s[r][gi].x : f.s[r][gi].y) >> (16 * (e & 1)));
         const float s = ll_to_f32(__builtin_bit_cast(T, sb));
-        const float z = W::off(ZERO) + (ZERO ? (float)((f.z[r][gi] >> (8 * e)) & 255u) : 8.f);
+        const float z = W::off(ZERO ? (float)((f.z[r][gi] >> (8 * e)) & 255u) : 8.f);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           float v = part[r][mb][e];
@@ -273,6 +280,7 @@ __global__ __launch_bounds__(WAVES * 64) void w4_stream_kernel(W4Args a) {
     f32x4 y = red[0][i][lane];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) y += red[v][i][lane];
+    y *= W4Type<T>::back;
     const int m = m0 + i % MB * 16 + c16, n = (nt0 + i / MB) * 16 + g * 4;
     if (m >= a.M) continue;
     T* o = (T*)a.y + (int64_t)m * a.ldy + n;
@@ -317,6 +325,7 @@ __global__ __launch_bounds__(kWavesW4 * 64) void w4_any_kernel(W4Args a) {
   f32x4 y = red[0][lane];
 #pragma unroll
   for (int v = 1; v < kWavesW4; ++v) y += red[v][lane];
+  y *= W4Type<T>::back;
   const int m = m0 + c16;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -476,6 +485,7 @@ __global__ __launch_bounds__(kWavesW4 * 64 * KG, KG == 4 ? 4 : 2) void w4_tile_k
         }
         continue;
       }
+      y *= W4Type<T>::back;
       T* o = (T*)a.y + (int64_t)m * a.ldy + n;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -499,6 +509,7 @@ __global__ __launch_bounds__(256) void w4_finish_kernel(W4Args a) {
     f32x4 y = *(const f32x4*)p;
 #pragma unroll 4
     for (int s = 1; s < a.splits; ++s) y += *(const f32x4*)(p + s * a.M * a.N);
+    y *= W4Type<T>::back;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (a.bias) y[e] += ll_to_f32(((const T*)a.bias)[n + e]);
@@ -508,6 +519,7 @@ __global__ __launch_bounds__(256) void w4_finish_kernel(W4Args a) {
     for (int e = 0; e < 4 && n + e < a.N; ++e) {
       float y = p[e];
       for (int s = 1; s < a.splits; ++s) y += p[s * a.M * a.N + e];
+      y *= W4Type<T>::back;
       if (a.bias) y += ll_to_f32(((const T*)a.bias)[n + e]);
       o[e] = ll_from_f32<T>(y);
     }

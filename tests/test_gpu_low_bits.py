@@ -625,6 +625,36 @@ def test_linear_w4_zero_bytes_count_by_four_bits(cuda):
     assert torch.equal(_ops().linear_w4(x, w), _ops().linear_w4(x, w2))
 
 
+@pytest.mark.parametrize("N,K,group,zero", [(100, 160, 32, False), (333, 256, 128, True),
+                                            (48, 11008, 128, False), (32800, 256, 64, True),
+                                            (9000, 192, 64, False)])
+def test_linear_w4_of_the_largest_and_smallest_inputs(cuda, N, K, group, zero):
+    """bf16 inputs up to the type's largest, with scales that keep the results finite,
+    and down to its smallest: no sum leaves fp32's range where the result does not."""
+    g = torch.Generator().manual_seed(N + K)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    z = torch.randint(0, 16, (N, K // group), generator=g, dtype=torch.uint8) if zero else None
+    unit = torch.rand(N, K // group, generator=g) + 0.5
+    # the largest: 3.39e38 in every input; of one sign and of both
+    for mag, size, sign in ((3.38e38, 1e-7, False), (3.38e38, 1e-7, True), (1e34, 1e-3, False),
+                            (2e36, 1e-3, True), (1e-30, 0.05, True), (1e-36, 0.05, True),
+                            (3e-38, 0.05, True)):
+        scale = (unit * size).to(BF16)
+        w = _ops().W4Weight(codes.cuda(), scale.cuda(), None if z is None else z.cuda())
+        for M in (1, 16, 20, 40, 70):
+            print(f"case: w4 {M}x{N}x{K} group {group} zero={zero} of {mag}", flush=True)
+            x = (1 - torch.rand(M, K, generator=g) * 0.2) * mag
+            x = (x * (torch.randint(0, 2, (M, K), generator=g) * 2 - 1) if sign else x).to(BF16)
+            assert bool(torch.isfinite(x).all())
+            y, m = O.linear_w4(x, codes, scale, z)
+            bound = O.bound_linear_w4(y, m, BF16, K)
+            assert float(y.abs().max()) < 3e38
+            _inside(_ops().linear_w4(x.cuda(), w), y, bound, "y")
+            wide = torch.zeros(M, K + 1, dtype=BF16, device="cuda")
+            wide[:, 1:] = x.cuda()
+            _inside(_ops().linear_w4(wide[:, 1:], w), y, bound, "y, rows of any address")
+
+
 def test_linear_w4_rows_do_not_mix(cuda):
     """Infinities and NaN in one row of x leave the other rows' bits."""
     g = torch.Generator().manual_seed(6)
