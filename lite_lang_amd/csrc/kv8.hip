@@ -534,7 +534,15 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
   int64_t row;
   const int n = decode_len(a, b, &row);
   const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh;
-  for (int d = lane; d < a.D; d += 64) sq[d] = ll_to_f32(q[d]);
+  float top = 0.f;
+  for (int d = lane; d < a.D; d += 64) {
+    sq[d] = ll_to_f32(q[d]);
+    top = fmaxf(top, fabsf(sq[d]));
+  }
+  // (queries beyond 2^50 as in the matrix form)
+  const int e = max(__builtin_amdgcn_frexp_expf(ll_wave_max(top)) - 50, 0);
+  const float more = __builtin_ldexpf(1.f, e);
+  for (int d = lane; d < a.D; d += 64) sq[d] = __builtin_ldexpf(sq[d], -e);
   __syncthreads();
   const int32_t* table = a.r2t + (n > 0 ? row : 0) * a.r2t_s;
   float m = -INFINITY, l = 0.f, acc[kAnyMaxD / 64] = {};
@@ -547,7 +555,7 @@ __global__ __launch_bounds__(64) void decode_any_kernel(DecodeArgs8 a) {
       const uint8_t* k = a.c[0] + slot * a.c_st[0] + kvh * a.c_sh[0];
       float dot = 0.f;
       for (int d = 0; d < a.D; ++d) dot = __builtin_fmaf(sq[d], CodeOf<CODE>::decode(k[d], 0), dot);
-      x = dot * a.s[0][(slot >> a.shift) * a.s_sb[0] + kvh * a.s_sh[0]] * a.scale_log2;
+      x = dot * a.s[0][(slot >> a.shift) * a.s_sb[0] + kvh * a.s_sh[0]] * a.scale_log2 * more;
     }
     const float mt = fmaxf(m, ll_wave_max(x));
     const float ms = mt == -INFINITY ? 0.f : mt;
@@ -723,6 +731,7 @@ template <typename T, int CODE, int D>
 __global__ __launch_bounds__(kWaves8 * 64, D == 256 || __is_same(T, float) ? 1 : 2)
 void decode_mfma_kernel(DecodeArgs8 a) {
   constexpr bool BIAS = CODE == KV8_INT8 && !__is_same(T, float);
+  constexpr bool FAR = !__is_same(T, _Float16);  // whether a query may be beyond 2^50
   constexpr int NQ = kQParts<T>, NP = kPParts<T>, NK = D / 64, NV = D / 16;
   typedef typename BytesOf<NV>::V VBytes;
   __shared__ int64_t s_off[kWaves8][2][kTile8];
@@ -870,7 +879,10 @@ void decode_mfma_kernel(DecodeArgs8 a) {
         fetch(f[s], t + s * kStep, entry[s]);
       int32_t next = kStages > 1 ? entry[kStages - 1] : entry_of(t + kStep);
       bf16x8 qf[NK * 2][NQ];
-      float cq = a.scale_log2;  // of a score's sum
+      // of a score's sum; of queries beyond 2^50, which are held smaller so that no sum
+      // passes fp32's range before its scales are applied: what takes that back
+      float cq = a.scale_log2, more = 1.f;
+      bool far = false;
       f32x4 qoff = {0.f, 0.f, 0.f, 0.f};
       {
         float v[NK * 2][8];
@@ -883,12 +895,20 @@ void decode_mfma_kernel(DecodeArgs8 a) {
           top = fmaxf(top, fabsf(v[i][e]));
         }
         float up = 1.f;
-        if constexpr (BIAS) {
+        if constexpr (BIAS || FAR) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const int e = min(max(__builtin_amdgcn_frexp_expf(top), -50), 50);
-          up = __builtin_ldexpf(1.f, kUp - e);
-          cq *= __builtin_ldexpf(1.f, 133 - kUp + e);
+          const int e = max(__builtin_amdgcn_frexp_expf(top), -50);
+          if constexpr (BIAS) {
+            up = __builtin_ldexpf(1.f, kUp - e);
+            cq *= __builtin_ldexpf(1.f, 133 - kUp + min(e, 50));
+          } else {
+            up = __builtin_ldexpf(1.f, min(50 - e, 0));
+          }
+          if constexpr (FAR) {
+            more = __builtin_ldexpf(1.f, max(e - 50, 0));
+            far = __ballot(e > 50) != 0;
+          }
         }
 #pragma unroll
         for (int i = 0; i < NK * 2; ++i) {
@@ -951,12 +971,13 @@ void decode_mfma_kernel(DecodeArgs8 a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[grp * 4 + r] = s[r] * cq * ks[r];
         }
-        const bool part = f.see != 0xffffffffu;  // the last tile, or slots that are none
+        // the last tile, slots that are none, or queries that were held smaller
+        const bool part = f.see != 0xffffffffu || far;
         if (part) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const bool is = f.see >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1u;
-            x[j] = is ? x[j] : -INFINITY;
+            x[j] = is ? x[j] * more : -INFINITY;
             if constexpr (CODE == KV8_E4M3) {  // (what is in no token's row may be NaN)
 #pragma unroll
               for (int i = 0; i < NK; ++i) f.vw[i][j] = is ? f.vw[i][j] : 0u;

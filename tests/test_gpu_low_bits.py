@@ -528,6 +528,35 @@ def test_kv8_decode_attention_of_scales_far_apart(cuda, code, dtype):
             _inside(out, want[0], O.bound_kv8_decode(*want, dtype, d), "out")
 
 
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_kv8_decode_attention_of_the_largest_queries(cuda, code, d, dtype):
+    """Queries up to the type's largest, over keys that keep the scores small; heads
+    of ordinary queries, of zeros and of the smallest beside them."""
+    g = torch.Generator().manual_seed(d)
+    n = 300
+    for mag in (2.0 ** 49, 2.0 ** 52, 2.0 ** 100, 2.0 ** 117, 2.0 ** 118, 2.0 ** 124, 3e38):
+        # (of 2^-80 and more in the scale: the smallest that a block has)
+        size = max(1.0 / mag, 2.0 ** -70)
+        print(f"case: queries of {mag:.3g}, keys of {size:.3g} {code} {dtype} D={d}", flush=True)
+        c = Cache(n, 1, d, code, 16)
+        k = (torch.randn(n, 1, d, generator=g) * size).to(BF16)
+        c.store(k, torch.randn(n, 1, d, generator=g).to(BF16), list(range(n)))
+        q = ((0.5 + torch.rand(2, 4, d, generator=g) * 0.49) * mag).to(dtype)
+        q[:, 1] = torch.randn(2, d, generator=g)
+        q[:, 2] = 0.0
+        q[:, 3] = 1e-37
+        assert bool(torch.isfinite(q).all())
+        table = torch.arange(n, dtype=torch.int32).view(1, n)
+        out = torch.empty(2, 4, d, dtype=dtype, device="cuda")
+        scale = 1.0 / max(mag * size, 1.0) / d ** 0.5
+        _ops().kv8_decode_attention(q.cuda(), table.cuda(), _i32([0, 0]), _i32([n, 129]), n,
+                                    *c.args, out, sm_scale=scale)
+        want = O.kv8_decode(q, *c.values(), table, [0, 0], [n, 129], n, scale)
+        _inside(out, want[0], O.bound_kv8_decode(*want, dtype, d), "out")
+
+
 # ---------------------------------------------------------------- 4-bit products
 def _weight(g, N, K, group, dtype, zero):
     codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
