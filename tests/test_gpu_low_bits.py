@@ -684,6 +684,64 @@ def test_linear_w4_of_the_largest_and_smallest_inputs(cuda, N, K, group, zero):
             _inside(_ops().linear_w4(wide[:, 1:], w), y, bound, "y, rows of any address")
 
 
+W4_EXACT = [(48, 11008, 128, (1, 16, 17, 40, 64, 65, 150)), (130, 8960, 64, (2, 16, 33, 100)),
+            (17, 160, 32, (1, 3, 16, 20, 70)), (333, 1536, 128, (5, 48, 600)),
+            (9000, 384, 64, (1, 16, 20, 64)), (33000, 192, 32, (5, 16, 40, 130)),
+            (70, 1152, 128, (2000,))]
+
+
+@pytest.mark.parametrize("N,K,group,rows", W4_EXACT)
+@pytest.mark.parametrize("dtype,zero", [(BF16, False), (BF16, True), (F16, False), (F16, True)])
+def test_linear_w4_counts_every_input_once(cuda, N, K, group, rows, dtype, zero):
+    """Rows of x of seven entries of 1 and -1, each input of the weight in one of them,
+    and scales of 1 and 2: sums below 7 * 15 * 2 + 1, which every type holds exactly,
+    so that an input that is lost, taken twice or met with another group's scale or
+    zero point shows in the bits."""
+    g = torch.Generator().manual_seed(N + K)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    scale = torch.randint(1, 3, (N, K // group), generator=g).to(dtype)
+    z = torch.randint(0, 16, scale.shape, generator=g, dtype=torch.uint8) if zero else None
+    w = _ops().W4Weight(codes.cuda(), scale.cuda(), None if z is None else z.cuda())
+    full = O.w4_weight(codes, scale, z).to(torch.float32).cuda()
+    bias = torch.randint(-1, 2, (N,), generator=g).to(dtype).cuda()
+    for M in rows:
+        print(f"case: w4 exact {M}x{N}x{K} group {group} {dtype} zero={zero}", flush=True)
+        order = torch.cat([torch.randperm(K, generator=g) for _ in range(-(-7 * M // K))])
+        for at in range(0, len(order) if 7 * M <= K else 1, 7 * M):
+            pos = order[at:at + 7 * M]
+            pos = torch.cat([pos, order[:7 * M - len(pos)]]).view(M, 7).cuda()
+            sign = (torch.randint(0, 2, (M, 7), generator=g) * 2 - 1).float().cuda()
+            x = torch.zeros(M, K, device="cuda").scatter_add_(1, pos, sign)
+            want = torch.zeros(M, N, device="cuda")
+            for i in range(7):
+                want += full[:, pos[:, i]].t() * sign[:, i, None]
+            want = (want + bias).to(dtype)
+            got = _ops().linear_w4(x.to(dtype), w, bias)
+            assert torch.equal(got, want), f"inputs from {at} on"
+            if at == 0:
+                wide = torch.zeros(M, K + 1, dtype=dtype, device="cuda")
+                wide[:, 1:] = x
+                assert torch.equal(_ops().linear_w4(wide[:, 1:], w, bias), want), "rows of any address"
+
+
+@pytest.mark.parametrize("dtype,zero", [(BF16, False), (BF16, True), (F16, False), (F16, True)])
+def test_linear_w4_of_small_whole_numbers_is_exact(cuda, dtype, zero):
+    """Full rows of -1, 0 and 1: every sum, of x (128 + c) too, is a whole number below
+    2^24 (11,008 * 143), so the result is the exact one, rounded once."""
+    g = torch.Generator().manual_seed(3)
+    for N, K, group in ((130, 11008, 128), (48, 8960, 64), (9000, 1536, 32), (33000, 512, 128)):
+        codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+        scale = torch.full((N, K // group), 0.125).to(dtype)
+        z = torch.randint(0, 16, scale.shape, generator=g, dtype=torch.uint8) if zero else None
+        w = _ops().W4Weight(codes.cuda(), scale.cuda(), None if z is None else z.cuda())
+        full = O.w4_weight(codes, scale, z).cuda()
+        for M in (1, 16, 17, 40, 70):
+            print(f"case: w4 whole {M}x{N}x{K} group {group} {dtype} zero={zero}", flush=True)
+            x = torch.randint(-1, 2, (M, K), generator=g).cuda()
+            want = (x.double() @ full.t()).to(dtype)
+            assert torch.equal(_ops().linear_w4(x.to(dtype), w), want)
+
+
 def test_linear_w4_rows_do_not_mix(cuda):
     """Infinities and NaN in one row of x leave the other rows' bits."""
     g = torch.Generator().manual_seed(6)
@@ -989,6 +1047,49 @@ def test_threads_with_streams_of_their_own(cuda):
 
     torch.cuda.synchronize()
     ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_threads_whose_calls_hand_on_parts(cuda, shared):
+    """Four threads' decodes and products in parts, which a second launch adds up from
+    the stream's workspace: on streams of their own, and on one that all share."""
+    ops, work = _ops(), []
+    for i in range(4):
+        g = torch.Generator().manual_seed(30 + i)
+        lens = [2500 + 100 * i, 900, 2100]
+        c, table, rids = _filled(g, lens, 2, 64, INT8, 16, BF16)
+        q = torch.randn(3, 4, 64, generator=g).to(BF16).cuda()
+        w = _weight(g, 130, 11008, 128, BF16, True)[3]
+        x = torch.randn(40, 11008, generator=g).to(BF16).cuda()
+        assert ops._kv8_decode_bytes(3, 4, 2, 64, max(lens)) > 0
+        assert ops._linear_w4_bytes(40, 130, 11008) > 0
+        work.append((c, q, table.cuda(), _i32(rids), _i32(lens), max(lens), x, w))
+
+    def call(i):
+        c, q, table, rids, lens, most, x, w = work[i]
+        out = torch.empty_like(q)
+        ops.kv8_decode_attention(q, table, rids, lens, most, *c.args, out)
+        return out, ops.linear_w4(x, w)
+
+    alone = [call(i) for i in range(4)]
+    torch.cuda.synchronize()
+    one, bad = torch.cuda.Stream(), []
+
+    def run(i):
+        st = one if shared else torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            outs = [call(i) for _ in range(50)]
+            st.synchronize()
+            for o, y in outs:
+                if not (torch.equal(o, alone[i][0]) and torch.equal(y, alone[i][1])):
+                    bad.append(i)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(4)]
     for t in ts:
         t.start()
     for t in ts:
