@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs 
 // 4 x 128 behind prefixes: 26 us in one wave, 18.8). Rows are read past the L2 (-2).
 template <typename T, int CODE, bool VEC, int TEAM>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
-  constexpr int kHold = 4, kWindow = 1;
+  constexpr int kHold = 4;
   __shared__ float s_top[2][TEAM];
   const int lane = threadIdx.x & 63, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int team = (blockIdx.x * kStoreWaves + me) / TEAM, units = 2 * a.KVH, unit = team % units;
@@ -294,15 +294,13 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
   const auto valid = [&](int32_t s) { return s >= 0 && s < a.nslots; };
 
   const int64_t t1 = min(t0 + (int64_t)a.per, a.T);
-  // the slots from t0 on, and of the 64 tokens before (no run starts beyond the
-  // first 64 of them)
-  int32_t sl[kWindow];
-#pragma unroll
-  for (int k = 0; k < kWindow; ++k) sl[k] = a.slots[min(t0 + k * 64 + lane, a.T - 1)];
+  // the slots of the 64 tokens from t0 on (no run of this wave's starts behind them),
+  // and of the 64 before
+  const int32_t sl = a.slots[min(t0 + lane, a.T - 1)];
   const int32_t back = a.slots[max(t0 - 1 - lane, (int64_t)0)];
   bool ours = false;  // whether the next token stored begins a run (known behind the first run)
   for (int64_t t = t0; t < t1;) {
-    const int32_t first = __builtin_amdgcn_readlane(sl[0], (int)(t - t0));
+    const int32_t first = __builtin_amdgcn_readlane(sl, (int)(t - t0));
     if (!valid(first)) {
       ++t;
       continue;
@@ -311,10 +309,10 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
     // the run's end (the first token of another block; padded ones among the
     // run's belong to no block) and its last token
     int64_t end = -1, last = t + 1;
-    const auto look = [&](int32_t s, int64_t base) {
-      const bool in = base + lane < a.T, here = valid(s) && s >> a.shift == blk;
-      uint64_t other = __ballot(!in || (valid(s) && !here)), same = __ballot(in && here);
-      if (end >= 0) return;
+    int32_t here = sl;
+    for (int64_t base = t0; end < 0; base += 64) {
+      const bool in = base + lane < a.T, its = valid(here) && here >> a.shift == blk;
+      uint64_t other = __ballot(!in || (valid(here) && !its)), same = __ballot(in && its);
       if (base <= t) {  // (the tokens up to t are behind)
         const uint64_t ahead = t - base == 63 ? 0 : ~(uint64_t)0 << (t - base + 1);
         other &= ahead;
@@ -324,13 +322,11 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
         const int cut = __builtin_ctzll(other);
         same &= ((uint64_t)1 << cut) - 1;
         end = base + cut;
+      } else {
+        here = a.slots[min(base + 64 + lane, a.T - 1)];
       }
       if (same) last = base + 64 - __builtin_clzll(same);
-    };
-#pragma unroll
-    for (int k = 0; k < kWindow; ++k) look(sl[k], t0 + k * 64);
-    for (int64_t base = t0 + kWindow * 64; end < 0; base += 64)
-      look(a.slots[min(base + lane, a.T - 1)], base);
+    }
     if (!ours) {  // a run that began before this wave's tokens is another wave's
       bool theirs = false;
       int32_t s = back;
@@ -440,8 +436,8 @@ __global__ __launch_bounds__(kLoadThreads) void load_kernel(LoadArgs a) {
   const int b = blockIdx.y;
   const int64_t row = ll_load_idx(a.req, b, a.req64), len = ll_load_idx(a.len, b, a.len64);
   const int64_t base = ll_load_idx(a.start, b, a.start64);
-  if (row < 0 || row >= a.r2t_rows) return;
-  const int n = (int)min(max(len, (int64_t)0), (int64_t)a.max_len);
+  if (row < 0 || row >= a.r2t_rows || len <= 0) return;
+  const int n = (int)min(len, (int64_t)a.max_len);
   const int32_t* table = a.r2t + row * a.r2t_s;
   const int places = 2 * a.KVH * a.pieces;
   const int here = min(places, kLoadThreads), tokens = kLoadThreads / here;  // of the workgroup

@@ -363,7 +363,7 @@ template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {
 // MFMAs take a third of the time each and overlap only between workgroups (22,016 x
 // 2048, 40 rows: 14.8 us; 17,920 x 1536, 333 rows: 45 us, 411 TFLOP/s).
 template <typename T, int GROUP, bool ZERO, int R, int MB, int KG>
-__global__ __launch_bounds__(kWavesW4 * 64 * KG, KG == 4 ? 4 : 2) void w4_tile_kernel(W4Args a) {
+__global__ __launch_bounds__(kWavesW4 * 64 * KG, 2) void w4_tile_kernel(W4Args a) {
   typedef typename W4Type<T>::V V;
   constexpr int kGpt = kTileK / GROUP, kDeep = 2;
   constexpr bool kSum = W4Type<T>::summed(ZERO);
