@@ -732,14 +732,17 @@ int ll_dequant_splitk(const int32_t* part, int splits, const float* s_tok, const
 /* k, v [ntok, kv_heads, head_dim] in `dtype`, quantised on their way to their
  * slots. Tokens that follow each other in one block (padded ones among them
  * aside) are a run; a run that starts at the block's first slot begins the block
- * anew, any other continues it. The scale is max(fl32(max |x| / top), 2^-80) over the run, top 127 or 448,
- * and where the run continues a block no less than the block's: where it grows,
- * the codes of the slots in front of the run are rounded again. Codes are the
- * nearest to x / scale, ties to even. An infinity or NaN among a head's elements
- * of a run makes that block and head's scale NaN (until the block begins anew)
- * and the run's codes 0. The slots of a call differ, and those of one block
- * stand next to each other in ascending order (ll_build_slot_maps lists them
- * so). No output may overlap an input. head_dim at most 1024, 2^24 tokens. */
+ * anew, any other continues it. The scale is max(fl32(max |x| / top), 2^-80) over
+ * the run, top 127 or 448, and where the run continues a block no less than the
+ * block's: where it grows, the codes of the slots in front of the run are rounded
+ * again. Codes are the nearest to x / scale, ties to even. An infinity or NaN
+ * among a head's elements of a run makes that block and head's scale NaN (until
+ * the block begins anew) and the run's codes 0. The slots of a call differ, and
+ * those of one block stand next to each other in ascending order
+ * (ll_build_slot_maps lists them so); nothing checks that, and where it does not
+ * hold, the blocks concerned hold some mixture of their tokens. Slots that are
+ * handed out one by one (a stack of free slots) need blocks of one. No output may
+ * overlap an input. head_dim at most 1024, 2^24 tokens. */
 int ll_kv8_store(const void* k, int64_t k_stride_tok, int64_t k_stride_h, const void* v,
                  int64_t v_stride_tok, int64_t v_stride_h, const int32_t* slots, int64_t ntok,
                  int64_t kv_heads, int64_t head_dim, void* k_codes, int64_t kc_stride_tok,
@@ -768,7 +771,11 @@ int ll_kv8_load(const void* k_codes, int64_t kc_stride_tok, int64_t kc_stride_h,
 
 /* ll_decode_attention over this cache: q, out [batch, q_heads, head_dim] in
  * `dtype`. Requests of length 0 give zero rows. head_dim at most 512. The
- * workspace needs no initialisation. */
+ * workspace needs no initialisation. Scores, and sums of probabilities times V
+ * before the division by the probabilities' sum, are fp32 numbers. With int8 codes
+ * and q of 16 bits each addition to those sums may be off by 2^-76 of the largest V
+ * scale among a request's tokens, so that outputs that come from tokens of V scales
+ * below 2^-50 of another token's alone have fewer bits. */
 int64_t ll_kv8_decode_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                int64_t head_dim, int64_t max_len_in_batch);
 int ll_kv8_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_h,

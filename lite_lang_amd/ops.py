@@ -376,10 +376,12 @@ def kv8_store(k, v, slots, cache_k, cache_v, k_scale, v_scale, block):
     float8_e4m3fn) at slots [T] int32, with an fp32 scale per block of `block`
     slots (a power of two up to 128) and head in k_scale, v_scale [blocks, KVH].
 
-    The tokens of one block stand next to each other, in ascending slots. Those
+    The tokens of one block stand next to each other, in ascending slots (nothing
+    checks that; a block of which it does not hold ends as some mixture). Those
     that start at a block's first slot begin it anew; others continue it: the
     scale grows where they need it and the codes in front of them are rounded
-    again. A slot outside the cache (-1) is a padded token. An infinity or NaN
+    again. So whole pages belong to one request (build_slot_maps); slots that
+    are handed out one by one (models.cache.PageCache) need block = 1. A slot outside the cache (-1) is a padded token. An infinity or NaN
     makes its block and head NaN."""
     cache, (P, block, code), dev, (KVH, D) = _kv8_cache(cache_k, cache_v, k_scale, v_scale, block)
     shape, dt = k.shape, k.dtype

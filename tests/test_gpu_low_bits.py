@@ -202,6 +202,43 @@ def test_kv8_store_of_a_long_prompt(cuda):
             c.check()
 
 
+@pytest.mark.parametrize("code", [INT8, E4M3])
+def test_kv8_store_on_a_cache_of_single_slots(cuda, code):
+    """PageCache's slots, freed and handed out again in another order, with a scale for
+    each: prompts, steps and new requests on the slots of former ones."""
+    from types import SimpleNamespace
+
+    from lite_lang_amd.models.cache import PageCache
+    g = torch.Generator().manual_seed(4)
+    pc = PageCache(6, 64, 0.0, 1, 64, 2, torch_dtype=BF16, kv_max_size=120, device=cuda)
+    c = Cache(120, 2, 64, code, 1)
+    live, lens = [], {}
+
+    def add(rids, new):
+        slots = pc.alloc_token_idxs(rids, [lens[r] for r in rids], new)
+        x = torch.randn(len(slots), 2, 64, generator=g).to(BF16)
+        c.store(x, x.flip(0) * 3, slots.tolist())
+        for r, n in zip(rids, new):
+            lens[r] += n
+
+    for step in range(12):
+        fresh = [pc.alloc_req() for _ in range((3, 0, 1, 2)[step % 4])]
+        lens.update({r: 0 for r in fresh})
+        if fresh:
+            add(fresh, [5 + 3 * i + step % 3 for i in range(len(fresh))])
+        live += fresh
+        add(live, [1] * len(live))
+        c.check()
+        while len(live) > 3:  # the oldest go, its slots to the next
+            r = live.pop(step % 2)
+            pc.free_req(SimpleNamespace(rid=r, length=lens.pop(r) + 1))
+    q = torch.randn(len(live), 4, 64, generator=g).to(BF16)
+    out, n = torch.empty_like(q, device="cuda"), [lens[r] for r in live]
+    _ops().kv8_decode_attention(q.cuda(), pc.req_to_tokens_, _i32(live), _i32(n), max(n), *c.args, out)
+    want = O.kv8_decode(q, *c.values(), pc.req_to_tokens_.cpu(), live, n, c.P)
+    _inside(out, want[0], O.bound_kv8_decode(*want, BF16, 64), "out")
+
+
 def test_kv8_far_slots(cuda):
     """Slots whose rows lie beyond 2^31 and 2^32 bytes."""
     kvh, d, block = 8, 128, 16
@@ -526,6 +563,31 @@ def test_kv8_decode_attention_of_scales_far_apart(cuda, code, dtype):
                                         *c.args, out)
             want = O.kv8_decode(q, *c.values(), table, [0, 0], [n, 200], n)
             _inside(out, want[0], O.bound_kv8_decode(*want, dtype, d), "out")
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("first", [False, True])
+def test_kv8_decode_attention_of_tokens_beside_far_larger_ones(cuda, code, first):
+    """Tokens of V scales 2^-50 of others' that no query looks at (their scores are 200
+    below): the outputs are the small ones' to the usual bound."""
+    g = torch.Generator().manual_seed(12)
+    n, d = 480, 64
+    for big in (160, 16):
+        c = Cache(n, 1, d, code, 16)
+        far = torch.zeros(n, dtype=torch.bool)
+        far[:big if first else 0] = True
+        if not first:
+            far[n - big:] = True
+        k = torch.where(far[:, None, None], -5.0, 0.5) * torch.ones(n, 1, d)
+        v = torch.randn(n, 1, d, generator=g) * torch.where(far, 2.0 ** 50, 1.0)[:, None, None]
+        c.store(k.to(BF16), v.to(BF16), list(range(n)))
+        q = (torch.rand(1, 4, d, generator=g) * 0.2 + 4.5).to(BF16)
+        out = torch.empty(1, 4, d, dtype=BF16, device="cuda")
+        table = torch.arange(n, dtype=torch.int32).view(1, n)
+        _ops().kv8_decode_attention(q.cuda(), table.cuda(), _i32([0]), _i32([n]), n, *c.args, out)
+        want = O.kv8_decode(q, *c.values(), table, [0], [n], n)
+        assert float(want[1].max()) < 4.0, "the far ones do not count"
+        _inside(out, want[0], O.bound_kv8_decode(*want, BF16, d), "out")
 
 
 @pytest.mark.parametrize("code", [INT8, E4M3])
