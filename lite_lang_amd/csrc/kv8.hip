@@ -232,8 +232,9 @@ __device__ __forceinline__ int lanes_of(int D) {
 }
 
 // Blocks of one slot: every row has a scale of its own. A row's elements stay in
-// the registers of its lanes between the maximum and the codes. Bound by memory
-// and its one chain (row, maximum, codes): 24,000 tokens of 2 x 128 in about 15 us.
+// the registers of its lanes between the maximum and the codes. Bound by that one
+// chain (slot, row, maximum, codes), with nothing of a next row in flight: 24,000
+// tokens of 2 x 128 in 15.2 us (2.4 TB/s, half of a copy's rate).
 template <typename T, int CODE, bool VEC>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs a) {
   constexpr int kHold = 2;  // D up to 1024
@@ -273,8 +274,11 @@ __global__ __launch_bounds__(kStoreWaves * 64) void store_rows_kernel(StoreArgs 
 // A run is a chain of round trips (slots, rows, codes), so what counts is how many
 // run at a time: registers for 4 groups of rows leave 28 waves per CU (8 groups: 20
 // waves, 24,000 tokens of 2 x 128 in blocks of 16 16.6 us, now 12.6: 2.9 TB/s),
-// and a run of 64 rows is quicker in four waves (blocks of 64, 8,600 new tokens of
-// 4 x 128 behind prefixes: 26 us in one wave, 18.8). Rows are read past the L2 (-2).
+// and a run of 64 rows is quicker in four waves (blocks of 64, 5,055 new tokens of
+// 4 x 128 behind prefixes: 26 us in one wave, 18.5; 672 of the 5,056 teams have a
+// run there, the others read slots and end). Rows are read past the L2 (-2). Blocks
+// that grow are rounded again code by code: 40 single tokens of 2 x 128, blocks of
+// 16 of random numbers, 10.9 us, and 4.1 where no scale grows.
 template <typename T, int CODE, bool VEC, int TEAM>
 __global__ __launch_bounds__(kStoreWaves * 64) void store_kernel(StoreArgs a) {
   constexpr int kHold = 4;

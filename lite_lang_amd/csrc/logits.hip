@@ -13,8 +13,11 @@
 // A workgroup takes a stretch of the vocabulary of one request, counts in LDS
 // what of the request's tokens falls into it (integer additions: no order
 // changes them), and writes its logits once: bound by memory at 40 requests of
-// 151,936 logits (13.5 us, 3.7 TB/s), by the LDS counters of the frequent tokens'
-// workgroup at one request of 131,072 tokens (18 us).
+// 151,936 logits (13.5 us, 3.7 TB/s). One request of 131,072 tokens takes 17.6 us:
+// every one of its 19 workgroups reads all tokens, 8.8 us (so long with ids that
+// fall into none), and counting those of its stretch takes the rest, whether they
+// are spread evenly (16.0) or as in a text; 115 where all are one token, whose
+// additions to one LDS word follow each other.
 #include <algorithm>
 
 #include "ll_common.h"

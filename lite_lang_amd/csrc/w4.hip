@@ -359,9 +359,10 @@ template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {
 // all banks. A workgroup may take its stretches in KG parts of four waves, added
 // up through LDS; blockIdx.z is a split of them, and with more than one the sums
 // go to `part` [split][M][N] and w4_finish_kernel adds them up. Nothing bounds it
-// alone: conversion, scales and sums on the VALU, the reads of x in LDS and the
-// MFMAs take a third of the time each and overlap only between workgroups (22,016 x
-// 2048, 40 rows: 14.8 us; 17,920 x 1536, 333 rows: 45 us, 411 TFLOP/s).
+// alone: conversion, scales and sums fill the VALU for 29% of the time, the accesses
+// to x in LDS (8 cycles each) theirs for 38% and the MFMAs the matrix pipes for 11%,
+// and they overlap only between workgroups (22,016 x 2048, 40 rows: 14.8 us; 17,920
+// x 1536, 333 rows: 35%, 28%, 17%, 45 us, 411 TFLOP/s; 24,000 rows: 2.1 ms, 626).
 template <typename T, int GROUP, bool ZERO, int R, int MB, int KG>
 __global__ __launch_bounds__(kWavesW4 * 64 * KG, 2) void w4_tile_kernel(W4Args a) {
   typedef typename W4Type<T>::V V;
