@@ -800,7 +800,7 @@ int ll_kv8_decode_attention(const void* q, int64_t q_stride_b, int64_t q_stride_
  * or 128 and divides K. ll_w4_pack lays a weight out as ll_linear_w4 reads it:
  *   Y[m, n] = dtype(sum_k X[m, k] (c[n, k] - zero) scale + bias[n])
  * with fp32 sums (bf16 / fp16; M at most 2^19). An infinity or NaN in X makes
- * its row of Y NaN or infinite. */
+ * its row of Y NaN or infinite; finite ones of any size do not. */
 int64_t ll_w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zero);
 int ll_w4_pack(const uint8_t* codes, int64_t ldc, const void* scale, int64_t ld_scale,
                const uint8_t* zero, int64_t ld_zero, int64_t N, int64_t K, int64_t group,
