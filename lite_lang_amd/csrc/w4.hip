@@ -362,7 +362,7 @@ template <int LANES> __device__ __forceinline__ float sum_lanes(float v) {
 // alone: conversion, scales and sums fill the VALU for 29% of the time, the accesses
 // to x in LDS (8 cycles each) theirs for 38% and the MFMAs the matrix pipes for 11%,
 // and they overlap only between workgroups (22,016 x 2048, 40 rows: 14.8 us; 17,920
-// x 1536, 333 rows: 35%, 28%, 17%, 45 us, 411 TFLOP/s; 24,000 rows: 2.1 ms, 626).
+// x 1536, 333 rows: 35%, 28%, 17%, 45 us, 411 TFLOP/s; 24,000 rows: 2.1 ms, 625).
 template <typename T, int GROUP, bool ZERO, int R, int MB, int KG>
 __global__ __launch_bounds__(kWavesW4 * 64 * KG, 2) void w4_tile_kernel(W4Args a) {
   typedef typename W4Type<T>::V V;
